@@ -3,8 +3,9 @@
 Drop-in replacement for the reference's three attention TensorRT plugins
 (``parakeet_relative_attention``, ``zipformer_relative_attention``,
 ``zipformer_attention_value``) and its two convolution-module plugins
-(``parakeet_conformer_convolution``, ``zipformer_convolution``): hand-written CUDA
-kernels behind the C ABI in ``include/fga_attention.h`` and ``include/fga_convolution.h``,
+(``parakeet_conformer_convolution``, ``zipformer_convolution``), and, beside the convolutions,
+group norm with an activation and a gated linear recurrence with their gradients: hand-written
+CUDA kernels behind the C ABI in ``include/fga_attention.h`` and ``include/fga_convolution.h``,
 the same plugin identities for TensorRT, and a data-parallel batch-sharding launcher.
 """
 
@@ -17,6 +18,14 @@ from .attention import (  # noqa: F401
 from .convolution import (  # noqa: F401
     parakeet_conformer_convolution,
     zipformer_convolution,
+)
+from .normalization import (  # noqa: F401
+    group_norm_activation,
+    group_norm_activation_backward,
+)
+from .recurrence import (  # noqa: F401
+    gated_linear_recurrence,
+    gated_linear_recurrence_backward,
 )
 from .constants import (  # noqa: F401
     PARAKEET_CONFORMER_CONVOLUTION_PLUGIN_NAME,

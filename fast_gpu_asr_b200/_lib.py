@@ -22,6 +22,10 @@ FGA_INT32 = 3
 FGA_BOOL = 4
 FGA_BF16 = 7
 
+# enum fga_activation
+ACTIVATIONS = {"none": 0, "silu": 1, "swoosh_r": 2}
+RECURRENCE_STATE_FRAMES = 64  # FGA_RECURRENCE_STATE_FRAMES
+
 STATUS_NAMES = {
     0: "FGA_SUCCESS",
     1: "FGA_ERROR_NULL_POINTER",
@@ -104,6 +108,36 @@ SYMBOLS = {
         ctypes.c_int32, (_P, ctypes.c_int32, _P, ctypes.c_int32)),
     "fga_zipformer_convolution_workspace_size": (ctypes.c_size_t, (_P, ctypes.c_int32)),
     "fga_zipformer_convolution_enqueue": (
+        ctypes.c_int32,
+        (_P, _P, ctypes.POINTER(_VP), ctypes.POINTER(_VP), _VP, ctypes.c_size_t, _VP)),
+    "fga_group_norm_activation_check": (
+        ctypes.c_int32, (_P, ctypes.c_int32, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_float,
+                         ctypes.c_int32)),
+    "fga_group_norm_activation_workspace_size": (
+        ctypes.c_size_t, (_P, ctypes.c_int32, ctypes.c_int32)),
+    "fga_group_norm_activation_enqueue": (
+        ctypes.c_int32,
+        (_P, _P, ctypes.POINTER(_VP), ctypes.POINTER(_VP), ctypes.c_int32, ctypes.c_float,
+         ctypes.c_int32, _VP, ctypes.c_size_t, _VP)),
+    "fga_group_norm_activation_backward_check": (
+        ctypes.c_int32, (_P, ctypes.c_int32, _P, ctypes.c_int32, ctypes.c_int32)),
+    "fga_group_norm_activation_backward_workspace_size": (
+        ctypes.c_size_t, (_P, ctypes.c_int32)),
+    "fga_group_norm_activation_backward_enqueue": (
+        ctypes.c_int32,
+        (_P, _P, ctypes.POINTER(_VP), ctypes.POINTER(_VP), ctypes.c_int32, _VP,
+         ctypes.c_size_t, _VP)),
+    "fga_gated_linear_recurrence_check": (
+        ctypes.c_int32, (_P, ctypes.c_int32, _P, ctypes.c_int32)),
+    "fga_gated_linear_recurrence_workspace_size": (ctypes.c_size_t, (_P, ctypes.c_int32)),
+    "fga_gated_linear_recurrence_enqueue": (
+        ctypes.c_int32,
+        (_P, _P, ctypes.POINTER(_VP), ctypes.POINTER(_VP), _VP, ctypes.c_size_t, _VP)),
+    "fga_gated_linear_recurrence_backward_check": (
+        ctypes.c_int32, (_P, ctypes.c_int32, _P, ctypes.c_int32)),
+    "fga_gated_linear_recurrence_backward_workspace_size": (
+        ctypes.c_size_t, (_P, ctypes.c_int32)),
+    "fga_gated_linear_recurrence_backward_enqueue": (
         ctypes.c_int32,
         (_P, _P, ctypes.POINTER(_VP), ctypes.POINTER(_VP), _VP, ctypes.c_size_t, _VP)),
     "fga_abi_version": (ctypes.c_int32, ()),

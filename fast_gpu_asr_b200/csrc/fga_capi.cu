@@ -306,6 +306,214 @@ int32_t convolution_enqueue(const fga_tensor_desc* in, const fga_tensor_desc* ou
     return FGA_SUCCESS;
 }
 
+// ---- group norm with activation, gated linear recurrence ---------------------------------
+
+bool same_dims(const fga_tensor_desc& a, const fga_tensor_desc& b) {
+    if (a.nb_dims != b.nb_dims) return false;
+    for (int i = 0; i < a.nb_dims; ++i)
+        if (a.dims[i] != b.dims[i]) return false;
+    return true;
+}
+
+bool has_dims(const fga_tensor_desc& d, int64_t d0, int64_t d1) {
+    return d.dims[0] == d0 && d.dims[1] == d1;
+}
+
+// Rank and type of every binding (a type of -1 stands for x's), then its size.
+struct Binding {
+    const fga_tensor_desc* desc;
+    int32_t rank, type;
+};
+
+int32_t check_bindings(const Binding* b, int count, int32_t type) {
+    if (!is_float_type(type)) return FGA_ERROR_BAD_DESCRIPTOR;
+    for (int i = 0; i < count; ++i)
+        if (b[i].desc->nb_dims != b[i].rank ||
+            b[i].desc->type != (b[i].type < 0 ? type : b[i].type))
+            return FGA_ERROR_BAD_DESCRIPTOR;
+    for (int i = 0; i < count; ++i)
+        if (!addressable(*b[i].desc, true)) return FGA_ERROR_OVERFLOW;
+    return FGA_SUCCESS;
+}
+
+// The kernels count frames and channels of the whole batch in 32 bits.
+bool rows_in_range(const fga_tensor_desc& x) {
+    return x.dims[0] <= kInt32Max / x.dims[1] && x.dims[0] <= kInt32Max / x.dims[2];
+}
+
+bool activation_ok(int32_t a) {
+    return a == FGA_ACTIVATION_NONE || a == FGA_ACTIVATION_SILU || a == FGA_ACTIVATION_SWOOSH_R;
+}
+
+int64_t state_chunks(int64_t length) {
+    return (length + FGA_RECURRENCE_STATE_FRAMES - 1) / FGA_RECURRENCE_STATE_FRAMES;
+}
+
+int32_t check_group_norm(const fga_tensor_desc* in, int32_t nin, const fga_tensor_desc* out,
+                         int32_t nout, int32_t groups, float eps, int32_t activation,
+                         fga::GroupNormProblem* prob) {
+    if (in == nullptr || out == nullptr) return FGA_ERROR_NULL_POINTER;
+    if (nin != 4 || nout != 3) return FGA_ERROR_BAD_DESCRIPTOR;
+    if (groups < 1 || !std::isfinite(eps) || eps <= 0.0f || !activation_ok(activation))
+        return FGA_ERROR_BAD_FIELD;
+    const fga_tensor_desc& x = in[0];
+    const Binding b[] = {{&x, 3, -1},      {&in[1], 1, FGA_INT32}, {&in[2], 1, -1},
+                         {&in[3], 1, -1},  {&out[0], 3, -1},       {&out[1], 2, FGA_FLOAT},
+                         {&out[2], 2, FGA_FLOAT}};
+    const int32_t st = check_bindings(b, 7, x.type);
+    if (st != FGA_SUCCESS) return st;
+    const int64_t n = x.dims[0], c = x.dims[2];
+    if (in[1].dims[0] != n || in[2].dims[0] != c || in[3].dims[0] != c ||
+        !same_dims(out[0], x) || !has_dims(out[1], n, groups) || !has_dims(out[2], n, groups) ||
+        c % groups != 0)
+        return FGA_ERROR_BAD_SHAPE;
+    if (!rows_in_range(x)) return FGA_ERROR_OVERFLOW;
+    if (prob != nullptr) {
+        prob->batch = static_cast<int32_t>(n);
+        prob->length = static_cast<int32_t>(x.dims[1]);
+        prob->channels = static_cast<int32_t>(c);
+        prob->groups = groups;
+        prob->eps = eps;
+        prob->activation = activation;
+        prob->dtype = x.type;
+    }
+    return FGA_SUCCESS;
+}
+
+int32_t check_group_norm_backward(const fga_tensor_desc* in, int32_t nin,
+                                  const fga_tensor_desc* out, int32_t nout, int32_t activation,
+                                  fga::GroupNormBackwardProblem* prob) {
+    if (in == nullptr || out == nullptr) return FGA_ERROR_NULL_POINTER;
+    if (nin != 7 || nout != 3) return FGA_ERROR_BAD_DESCRIPTOR;
+    if (!activation_ok(activation)) return FGA_ERROR_BAD_FIELD;
+    const fga_tensor_desc& x = in[1];
+    const Binding b[] = {{&in[0], 3, -1},       {&x, 3, -1},           {&in[2], 1, FGA_INT32},
+                         {&in[3], 1, -1},       {&in[4], 1, -1},       {&in[5], 2, FGA_FLOAT},
+                         {&in[6], 2, FGA_FLOAT}, {&out[0], 3, -1},     {&out[1], 1, -1},
+                         {&out[2], 1, -1}};
+    const int32_t st = check_bindings(b, 10, x.type);
+    if (st != FGA_SUCCESS) return st;
+    const int64_t n = x.dims[0], c = x.dims[2], groups = in[5].dims[1];
+    if (!same_dims(in[0], x) || in[2].dims[0] != n || in[3].dims[0] != c || in[4].dims[0] != c ||
+        in[5].dims[0] != n || !same_dims(in[5], in[6]) || !same_dims(out[0], x) ||
+        out[1].dims[0] != c || out[2].dims[0] != c || c % groups != 0)
+        return FGA_ERROR_BAD_SHAPE;
+    if (!rows_in_range(x)) return FGA_ERROR_OVERFLOW;
+    if (prob != nullptr) {
+        prob->batch = static_cast<int32_t>(n);
+        prob->length = static_cast<int32_t>(x.dims[1]);
+        prob->channels = static_cast<int32_t>(c);
+        prob->groups = static_cast<int32_t>(groups);
+        prob->activation = activation;
+        prob->dtype = x.type;
+    }
+    return FGA_SUCCESS;
+}
+
+int32_t check_recurrence(const fga_tensor_desc* in, int32_t nin, const fga_tensor_desc* out,
+                         int32_t nout, fga::RecurrenceProblem* prob) {
+    if (in == nullptr || out == nullptr) return FGA_ERROR_NULL_POINTER;
+    if (nin != 4 || nout != 3) return FGA_ERROR_BAD_DESCRIPTOR;
+    const fga_tensor_desc& x = in[0];
+    const Binding b[] = {{&x, 3, -1},      {&in[1], 3, -1},         {&in[2], 1, FGA_INT32},
+                         {&in[3], 2, FGA_FLOAT}, {&out[0], 3, -1},  {&out[1], 2, FGA_FLOAT},
+                         {&out[2], 3, FGA_FLOAT}};
+    const int32_t st = check_bindings(b, 7, x.type);
+    if (st != FGA_SUCCESS) return st;
+    const int64_t n = x.dims[0], c = x.dims[2], chunks = state_chunks(x.dims[1]);
+    if (!same_dims(in[1], x) || in[2].dims[0] != n || !has_dims(in[3], n, c) ||
+        !same_dims(out[0], x) || !has_dims(out[1], n, c) || !has_dims(out[2], n, chunks) ||
+        out[2].dims[2] != c)
+        return FGA_ERROR_BAD_SHAPE;
+    if (!rows_in_range(x)) return FGA_ERROR_OVERFLOW;
+    if (prob != nullptr) {
+        prob->batch = static_cast<int32_t>(n);
+        prob->length = static_cast<int32_t>(x.dims[1]);
+        prob->channels = static_cast<int32_t>(c);
+        prob->chunks = static_cast<int32_t>(chunks);
+        prob->dtype = x.type;
+    }
+    return FGA_SUCCESS;
+}
+
+int32_t check_recurrence_backward(const fga_tensor_desc* in, int32_t nin,
+                                  const fga_tensor_desc* out, int32_t nout,
+                                  fga::RecurrenceBackwardProblem* prob) {
+    if (in == nullptr || out == nullptr) return FGA_ERROR_NULL_POINTER;
+    if (nin != 6 || nout != 3) return FGA_ERROR_BAD_DESCRIPTOR;
+    const fga_tensor_desc& x = in[1];
+    const Binding b[] = {{&in[0], 3, -1},        {&x, 3, -1},      {&in[2], 3, -1},
+                         {&in[3], 1, FGA_INT32}, {&in[4], 3, FGA_FLOAT},
+                         {&in[5], 2, FGA_FLOAT}, {&out[0], 3, -1}, {&out[1], 3, -1},
+                         {&out[2], 2, FGA_FLOAT}};
+    const int32_t st = check_bindings(b, 9, x.type);
+    if (st != FGA_SUCCESS) return st;
+    const int64_t n = x.dims[0], c = x.dims[2], chunks = state_chunks(x.dims[1]);
+    if (!same_dims(in[0], x) || !same_dims(in[2], x) || in[3].dims[0] != n ||
+        !has_dims(in[4], n, chunks) || in[4].dims[2] != c || !has_dims(in[5], n, c) ||
+        !same_dims(out[0], x) || !same_dims(out[1], x) || !has_dims(out[2], n, c))
+        return FGA_ERROR_BAD_SHAPE;
+    if (!rows_in_range(x)) return FGA_ERROR_OVERFLOW;
+    if (prob != nullptr) {
+        prob->batch = static_cast<int32_t>(n);
+        prob->length = static_cast<int32_t>(x.dims[1]);
+        prob->channels = static_cast<int32_t>(c);
+        prob->chunks = static_cast<int32_t>(chunks);
+        prob->dtype = x.type;
+    }
+    return FGA_SUCCESS;
+}
+
+int64_t desc_bytes(const fga_tensor_desc& d) {
+    int64_t bytes = type_bytes(d.type);
+    for (int i = 0; i < d.nb_dims; ++i) bytes *= d.dims[i];
+    return bytes;
+}
+
+// Pointers of validated bindings: present unless optional, aligned to their element, and no
+// output on top of an input or another output. `may_alias_in` / `may_alias_out` name one
+// pair that may be the same buffer (-1: none).
+int32_t check_buffers(const fga_tensor_desc* in, const void* const* inputs, int nin,
+                      uint32_t optional_in, const fga_tensor_desc* out, void* const* outputs,
+                      int nout, uint32_t optional_out, int may_alias_in, int may_alias_out) {
+    if (inputs == nullptr || outputs == nullptr) return FGA_ERROR_NULL_POINTER;
+    for (int i = 0; i < nin; ++i)
+        if (inputs[i] == nullptr && !(optional_in >> i & 1u)) return FGA_ERROR_NULL_POINTER;
+    for (int i = 0; i < nout; ++i)
+        if (outputs[i] == nullptr && !(optional_out >> i & 1u)) return FGA_ERROR_NULL_POINTER;
+    auto aligned = [](const void* p, const fga_tensor_desc& d) {
+        return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(type_bytes(d.type)) == 0;
+    };
+    for (int i = 0; i < nin; ++i)
+        if (!aligned(inputs[i], in[i])) return FGA_ERROR_UNSUPPORTED;
+    for (int i = 0; i < nout; ++i)
+        if (!aligned(outputs[i], out[i])) return FGA_ERROR_UNSUPPORTED;
+    auto overlap = [](const void* p, const fga_tensor_desc& d, const void* q,
+                      const fga_tensor_desc& e) {
+        if (p == nullptr || q == nullptr) return false;
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+        return a < b + static_cast<uintptr_t>(desc_bytes(e)) &&
+               b < a + static_cast<uintptr_t>(desc_bytes(d));
+    };
+    for (int o = 0; o < nout; ++o) {
+        for (int i = 0; i < nin; ++i)
+            if (overlap(outputs[o], out[o], inputs[i], in[i]) &&
+                !(o == may_alias_out && i == may_alias_in && outputs[o] == inputs[i]))
+                return FGA_ERROR_UNSUPPORTED;
+        for (int q = 0; q < o; ++q)
+            if (overlap(outputs[o], out[o], outputs[q], out[q])) return FGA_ERROR_UNSUPPORTED;
+    }
+    return FGA_SUCCESS;
+}
+
+int32_t check_workspace(const void* workspace, size_t bytes, size_t needed) {
+    if (needed == 0) return FGA_SUCCESS;
+    if (workspace == nullptr || bytes < needed ||
+        (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+        return FGA_ERROR_WORKSPACE;
+    return FGA_SUCCESS;
+}
+
 }  // namespace
 
 namespace fga {
@@ -565,6 +773,177 @@ int32_t fga_zipformer_convolution_enqueue(const fga_tensor_desc* in, const fga_t
                                           void*, size_t, void* stream) {
     return convolution_enqueue(in, out, inputs, outputs, fga::ConvolutionProblem::kZipformer,
                                stream);
+}
+
+// ---- group norm with activation -----------------------------------------------------------
+
+int32_t fga_group_norm_activation_check(const fga_tensor_desc* in, int32_t nin,
+                                        const fga_tensor_desc* out, int32_t nout,
+                                        int32_t num_groups, float eps, int32_t activation) {
+    return check_group_norm(in, nin, out, nout, num_groups, eps, activation, nullptr);
+}
+
+size_t fga_group_norm_activation_workspace_size(const fga_tensor_desc* in, int32_t nin,
+                                                int32_t num_groups) {
+    if (in == nullptr || nin < 1 || num_groups < 1) return 0;
+    fga_tensor_desc out[3] = {in[0], {FGA_FLOAT, 2, {in[0].dims[0], num_groups}},
+                              {FGA_FLOAT, 2, {in[0].dims[0], num_groups}}};
+    fga::GroupNormProblem p{};
+    if (check_group_norm(in, nin, out, 3, num_groups, 1.0f, FGA_ACTIVATION_NONE, &p) !=
+        FGA_SUCCESS)
+        return 0;
+    return fga::group_norm_workspace(p);
+}
+
+int32_t fga_group_norm_activation_enqueue(const fga_tensor_desc* in, const fga_tensor_desc* out,
+                                          const void* const* inputs, void* const* outputs,
+                                          int32_t num_groups, float eps, int32_t activation,
+                                          void* workspace, size_t workspace_bytes,
+                                          void* stream) {
+    fga::GroupNormProblem p{};
+    int32_t st = check_group_norm(in, 4, out, 3, num_groups, eps, activation, &p);
+    if (st != FGA_SUCCESS) return st;
+    st = check_buffers(in, inputs, 4, 0u, out, outputs, 3, 6u, -1, -1);
+    if (st != FGA_SUCCESS) return st;
+    st = check_workspace(workspace, workspace_bytes, fga::group_norm_workspace(p));
+    if (st != FGA_SUCCESS) return st;
+    if ((st = prior_error_status()) != FGA_SUCCESS) return st;
+    if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
+    p.x = inputs[0];
+    p.valid_lengths = static_cast<const int32_t*>(inputs[1]);
+    p.weight = inputs[2];
+    p.bias = inputs[3];
+    p.output = outputs[0];
+    p.mean = static_cast<float*>(outputs[1]);
+    p.rstd = static_cast<float*>(outputs[2]);
+    p.workspace = workspace;
+    const char* variant = "none";
+    if (fga::launch_group_norm(p, static_cast<cudaStream_t>(stream), &variant) != cudaSuccess)
+        return FGA_ERROR_LAUNCH;
+    t_last_variant = variant;
+    return FGA_SUCCESS;
+}
+
+int32_t fga_group_norm_activation_backward_check(const fga_tensor_desc* in, int32_t nin,
+                                                 const fga_tensor_desc* out, int32_t nout,
+                                                 int32_t activation) {
+    return check_group_norm_backward(in, nin, out, nout, activation, nullptr);
+}
+
+size_t fga_group_norm_activation_backward_workspace_size(const fga_tensor_desc* in,
+                                                         int32_t nin) {
+    if (in == nullptr || nin != 7) return 0;
+    const fga_tensor_desc out[3] = {in[1], in[3], in[4]};
+    fga::GroupNormBackwardProblem p{};
+    if (check_group_norm_backward(in, nin, out, 3, FGA_ACTIVATION_NONE, &p) != FGA_SUCCESS)
+        return 0;
+    return fga::group_norm_backward_workspace(p);
+}
+
+int32_t fga_group_norm_activation_backward_enqueue(const fga_tensor_desc* in,
+                                                   const fga_tensor_desc* out,
+                                                   const void* const* inputs,
+                                                   void* const* outputs, int32_t activation,
+                                                   void* workspace, size_t workspace_bytes,
+                                                   void* stream) {
+    fga::GroupNormBackwardProblem p{};
+    int32_t st = check_group_norm_backward(in, 7, out, 3, activation, &p);
+    if (st != FGA_SUCCESS) return st;
+    st = check_buffers(in, inputs, 7, 0u, out, outputs, 3, 0u, -1, -1);
+    if (st != FGA_SUCCESS) return st;
+    st = check_workspace(workspace, workspace_bytes, fga::group_norm_backward_workspace(p));
+    if (st != FGA_SUCCESS) return st;
+    if ((st = prior_error_status()) != FGA_SUCCESS) return st;
+    if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
+    p.grad_output = inputs[0];
+    p.x = inputs[1];
+    p.valid_lengths = static_cast<const int32_t*>(inputs[2]);
+    p.weight = inputs[3];
+    p.bias = inputs[4];
+    p.mean = static_cast<const float*>(inputs[5]);
+    p.rstd = static_cast<const float*>(inputs[6]);
+    p.grad_x = outputs[0];
+    p.grad_weight = outputs[1];
+    p.grad_bias = outputs[2];
+    p.workspace = workspace;
+    const char* variant = "none";
+    if (fga::launch_group_norm_backward(p, static_cast<cudaStream_t>(stream), &variant) !=
+        cudaSuccess)
+        return FGA_ERROR_LAUNCH;
+    t_last_variant = variant;
+    return FGA_SUCCESS;
+}
+
+// ---- gated linear recurrence --------------------------------------------------------------
+
+int32_t fga_gated_linear_recurrence_check(const fga_tensor_desc* in, int32_t nin,
+                                          const fga_tensor_desc* out, int32_t nout) {
+    return check_recurrence(in, nin, out, nout, nullptr);
+}
+
+size_t fga_gated_linear_recurrence_workspace_size(const fga_tensor_desc*, int32_t) { return 0; }
+
+int32_t fga_gated_linear_recurrence_enqueue(const fga_tensor_desc* in,
+                                            const fga_tensor_desc* out,
+                                            const void* const* inputs, void* const* outputs,
+                                            void*, size_t, void* stream) {
+    fga::RecurrenceProblem p{};
+    int32_t st = check_recurrence(in, 4, out, 3, &p);
+    if (st != FGA_SUCCESS) return st;
+    st = check_buffers(in, inputs, 4, 8u, out, outputs, 3, 4u, 3, 1);
+    if (st != FGA_SUCCESS) return st;
+    if ((st = prior_error_status()) != FGA_SUCCESS) return st;
+    if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
+    p.x = inputs[0];
+    p.gate = inputs[1];
+    p.valid_lengths = static_cast<const int32_t*>(inputs[2]);
+    p.initial_state = static_cast<const float*>(inputs[3]);
+    p.output = outputs[0];
+    p.final_state = static_cast<float*>(outputs[1]);
+    p.states = static_cast<float*>(outputs[2]);
+    const char* variant = "none";
+    if (fga::launch_recurrence(p, static_cast<cudaStream_t>(stream), &variant) != cudaSuccess)
+        return FGA_ERROR_LAUNCH;
+    t_last_variant = variant;
+    return FGA_SUCCESS;
+}
+
+int32_t fga_gated_linear_recurrence_backward_check(const fga_tensor_desc* in, int32_t nin,
+                                                   const fga_tensor_desc* out, int32_t nout) {
+    return check_recurrence_backward(in, nin, out, nout, nullptr);
+}
+
+size_t fga_gated_linear_recurrence_backward_workspace_size(const fga_tensor_desc*, int32_t) {
+    return 0;
+}
+
+int32_t fga_gated_linear_recurrence_backward_enqueue(const fga_tensor_desc* in,
+                                                     const fga_tensor_desc* out,
+                                                     const void* const* inputs,
+                                                     void* const* outputs, void*, size_t,
+                                                     void* stream) {
+    fga::RecurrenceBackwardProblem p{};
+    int32_t st = check_recurrence_backward(in, 6, out, 3, &p);
+    if (st != FGA_SUCCESS) return st;
+    st = check_buffers(in, inputs, 6, 32u, out, outputs, 3, 0u, -1, -1);
+    if (st != FGA_SUCCESS) return st;
+    if ((st = prior_error_status()) != FGA_SUCCESS) return st;
+    if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
+    p.grad_output = inputs[0];
+    p.x = inputs[1];
+    p.gate = inputs[2];
+    p.valid_lengths = static_cast<const int32_t*>(inputs[3]);
+    p.states = static_cast<const float*>(inputs[4]);
+    p.grad_final_state = static_cast<const float*>(inputs[5]);
+    p.grad_x = outputs[0];
+    p.grad_gate = outputs[1];
+    p.grad_initial_state = static_cast<float*>(outputs[2]);
+    const char* variant = "none";
+    if (fga::launch_recurrence_backward(p, static_cast<cudaStream_t>(stream), &variant) !=
+        cudaSuccess)
+        return FGA_ERROR_LAUNCH;
+    t_last_variant = variant;
+    return FGA_SUCCESS;
 }
 
 }  // extern "C"

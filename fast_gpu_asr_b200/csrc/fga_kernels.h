@@ -70,6 +70,64 @@ struct ConvolutionProblem {
     int32_t kind;
 };
 
+// Group norm with activation over [N, T, C] (act: fga_activation).
+struct GroupNormProblem {
+    const void* x;                 // [N, T, C]
+    const int32_t* valid_lengths;  // [N]
+    const void* weight;            // [C]
+    const void* bias;              // [C]
+    void* output;                  // [N, T, C]
+    float* mean;                   // [N, G] or null
+    float* rstd;                   // [N, G] or null
+    void* workspace;
+    int32_t batch, length, channels, groups;
+    float eps;
+    int32_t activation, dtype;
+};
+
+struct GroupNormBackwardProblem {
+    const void* grad_output;       // [N, T, C]
+    const void* x;                 // [N, T, C]
+    const int32_t* valid_lengths;  // [N]
+    const void* weight;            // [C]
+    const void* bias;              // [C]
+    const float* mean;             // [N, G]
+    const float* rstd;             // [N, G]
+    void* grad_x;                  // [N, T, C]
+    void* grad_weight;             // [C]
+    void* grad_bias;               // [C]
+    void* workspace;
+    int32_t batch, length, channels, groups;
+    int32_t activation, dtype;
+};
+
+// Gated linear recurrence over [N, T, C]; chunks = ceil(T / FGA_RECURRENCE_STATE_FRAMES).
+struct RecurrenceProblem {
+    const void* x;                 // [N, T, C]
+    const void* gate;              // [N, T, C]
+    const int32_t* valid_lengths;  // [N]
+    const float* initial_state;    // [N, C] or null
+    void* output;                  // [N, T, C]
+    float* final_state;            // [N, C]; may be initial_state
+    float* states;                 // [N, chunks, C] or null
+    int32_t batch, length, channels, chunks;
+    int32_t dtype;
+};
+
+struct RecurrenceBackwardProblem {
+    const void* grad_output;        // [N, T, C]
+    const void* x;                  // [N, T, C]
+    const void* gate;               // [N, T, C]
+    const int32_t* valid_lengths;   // [N]
+    const float* states;            // [N, chunks, C]
+    const float* grad_final_state;  // [N, C] or null
+    void* grad_x;                   // [N, T, C]
+    void* grad_gate;                // [N, T, C]
+    float* grad_initial_state;      // [N, C]
+    int32_t batch, length, channels, chunks;
+    int32_t dtype;
+};
+
 // Each launcher returns cudaSuccess or the launch error, and records the variant.
 cudaError_t launch_parakeet(const ParakeetProblem& p, cudaStream_t stream, const char** variant);
 cudaError_t launch_zipformer_weights(const ZipformerWeightsProblem& p, cudaStream_t stream,
@@ -78,6 +136,17 @@ cudaError_t launch_zipformer_value(const ZipformerValueProblem& p, cudaStream_t 
                                    const char** variant);
 cudaError_t launch_convolution(const ConvolutionProblem& p, cudaStream_t stream,
                                const char** variant);
+cudaError_t launch_group_norm(const GroupNormProblem& p, cudaStream_t stream,
+                              const char** variant);
+cudaError_t launch_group_norm_backward(const GroupNormBackwardProblem& p, cudaStream_t stream,
+                                       const char** variant);
+cudaError_t launch_recurrence(const RecurrenceProblem& p, cudaStream_t stream,
+                              const char** variant);
+cudaError_t launch_recurrence_backward(const RecurrenceBackwardProblem& p, cudaStream_t stream,
+                                       const char** variant);
+// Workspace of the group norm launchers: from the shape and type alone.
+size_t group_norm_workspace(const GroupNormProblem& p);
+size_t group_norm_backward_workspace(const GroupNormBackwardProblem& p);
 // Tensor cores only: cudaErrorNotSupported outside the envelope (f16/bf16, qd = 32,
 // T <= 768, vd a multiple of 4 up to 16, H*vd a multiple of 8, aligned buffers).
 cudaError_t launch_zipformer_fused(const ZipformerFusedProblem& p, cudaStream_t stream);

@@ -1,0 +1,96 @@
+"""Gated linear recurrence over ``[N, T, C]`` and its gradients, called on torch CUDA tensors
+through the C ABI (``include/fga_convolution.h``).
+
+A time mixer beside the depthwise convolution, with unbounded left context and a state of one
+value per channel::
+
+    f = sigmoid(gate);  h[t] = f[t] * h[t-1] + (1 - f[t]) * x[t];  out[t] = h[t]
+
+The state is float32 and passes from call to call, so a recording may be cut anywhere; ``T =
+1`` is the streaming step. ``valid_lengths`` is int32 ``[N]`` as in the convolutions, clamped
+to ``[0, T]``: padded frames are not read and leave the state as it is, and padded frames of
+the outputs are zeros. No reference plugin.
+
+The operators record no autograd graph: a call on tensors that require grad is refused while
+grad mode is on. The two functions are the halves of a ``torch.autograd.Function``.
+
+Tensors must be contiguous and live on the current CUDA device. Work is enqueued on
+``stream`` (default: torch's current stream), outputs are allocated on it, and nothing is
+synchronised.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._call import Absent, enqueue, launch_stream, require
+
+STATE_FRAMES = _lib.RECURRENCE_STATE_FRAMES
+
+
+def gated_linear_recurrence_check(input_descs, output_descs) -> int:
+    """Status of the shape and type checks (no device needed)."""
+    return _lib.library().fga_gated_linear_recurrence_check(
+        _lib.desc_array(input_descs), len(input_descs), _lib.desc_array(output_descs),
+        len(output_descs))
+
+
+def gated_linear_recurrence_backward_check(input_descs, output_descs) -> int:
+    return _lib.library().fga_gated_linear_recurrence_backward_check(
+        _lib.desc_array(input_descs), len(input_descs), _lib.desc_array(output_descs),
+        len(output_descs))
+
+
+def gated_linear_recurrence(x: torch.Tensor, gate: torch.Tensor, valid_lengths: torch.Tensor,
+                            initial_state: torch.Tensor | None = None, *,
+                            return_states: bool = False, out: torch.Tensor | None = None,
+                            final_state: torch.Tensor | None = None, stream=None):
+    """``(out, final_state)``, or ``(out, final_state, states)`` with ``return_states``.
+
+    ``gate`` holds logits; ``initial_state`` is float32 ``[N, C]`` (default zeros).
+    ``final_state`` is the state after the last valid frame; a buffer may be passed for it,
+    ``initial_state`` itself for an update in place. ``states`` (float32 ``[N, ceil(T / 64),
+    C]``, the state before every 64th frame, zero where that frame is padding) is what the
+    backward call takes."""
+    require("x", x, 3)
+    n, t, c = x.shape
+    handle, context = launch_stream(stream)
+    state, saved = (n, c), (n, -(-t // STATE_FRAMES), c)
+    with context:
+        if out is None:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        if final_state is None:
+            final_state = torch.empty(state, dtype=torch.float32, device=x.device)
+        states = (torch.empty(saved, dtype=torch.float32, device=x.device) if return_states
+                  else Absent(torch.float32, saved))
+    if initial_state is None:
+        initial_state = Absent(torch.float32, state)
+    enqueue("gated_linear_recurrence", (x, gate, valid_lengths, initial_state),
+            ("x", "gate", "valid_lengths", "initial_state"), (out, final_state, states),
+            ("out", "final_state", "states"), (), None, handle, context)
+    return (out, final_state, states) if return_states else (out, final_state)
+
+
+def gated_linear_recurrence_backward(grad_out: torch.Tensor, x: torch.Tensor,
+                                     gate: torch.Tensor, valid_lengths: torch.Tensor,
+                                     states: torch.Tensor,
+                                     grad_final_state: torch.Tensor | None = None, *,
+                                     stream=None):
+    """``(grad_x, grad_gate, grad_initial_state)`` from the forward call's inputs and its
+    ``states``. ``grad_final_state`` is float32 ``[N, C]`` (default zeros), and so is
+    ``grad_initial_state``."""
+    require("x", x, 3)
+    n, _, c = x.shape
+    handle, context = launch_stream(stream)
+    with context:
+        outputs = (torch.empty_like(x, memory_format=torch.contiguous_format),
+                   torch.empty_like(x, memory_format=torch.contiguous_format),
+                   torch.empty((n, c), dtype=torch.float32, device=x.device))
+    if grad_final_state is None:
+        grad_final_state = Absent(torch.float32, (n, c))
+    enqueue("gated_linear_recurrence_backward",
+            (grad_out, x, gate, valid_lengths, states, grad_final_state),
+            ("grad_out", "x", "gate", "valid_lengths", "states", "grad_final_state"), outputs,
+            ("grad_x", "grad_gate", "grad_initial_state"), (), None, handle, context)
+    return outputs
