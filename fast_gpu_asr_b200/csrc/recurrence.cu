@@ -4,18 +4,16 @@
 //   dx[t] = p[t] G[t], dgate[t] = f[t] p[t] (h[t-1] - x[t]) G[t], dinitial = f[0] G[0].
 //
 // A run of frames takes h to A h + B, with A the product of its f and B what it makes of
-// h = 0, and runs compose: that is the scan. A warp holds kFrames consecutive frames of 32
-// lanes' channels (one 128-byte row a frame) in registers, finds its (A, B), learns the state
-// before its first frame from the warps before it through shared memory, and walks its frames
-// a second time from there; no element is read twice. A block's warps cover one tile, a block
-// walks the tiles of its utterance and channels in turn. Where utterances and channels are too
-// few to fill the GPU, a cluster of blocks takes consecutive tiles and passes (A, B) on
-// through distributed shared memory. The backward pass runs the same scan from the last tile
-// to the first for the carry c[t] = f[t] G[t], and recomputes h within 64 frames of the states
-// that the forward pass saved.
-//
-// Both are bound by HBM; arithmetic is fp32, of which the sigmoid's two special functions and
-// about 20 instructions an element leave the issue slots about half free.
+// h = 0, and runs compose: that is the scan. A warp takes kFrames consecutive frames of one
+// 128-byte row's channels (a lane one value of f32, two of a 16-bit type), finds its (A, B),
+// learns the state before its first frame from the warps before it through shared memory, and
+// walks its frames again from there, so that no element is read twice. A block's warps cover
+// one tile; a block walks the tiles of its utterance and channels in turn, with the next
+// tile's rows on their way to shared memory meanwhile. Where utterances and channels are too
+// few to fill the GPU, a cluster of blocks takes consecutive tiles and passes (A, B) on through
+// distributed shared memory. The backward pass runs the same scan from the last tile to the
+// first for the carry c[t] = f[t] G[t], and recomputes h from the states that the forward pass
+// saved every 64 frames.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -35,16 +33,15 @@ namespace cg = cooperative_groups;
 
 constexpr int kChunk = FGA_RECURRENCE_STATE_FRAMES;
 constexpr int kMaxCluster = 16;
+constexpr int kRow = 128;  // bytes of a row that a warp takes
+constexpr int kFrames = 8, kWarps = 8;
+constexpr int kTile = kFrames * kWarps;
+constexpr int kForwardBlocks = 4, kBackwardBlocks = 3;  // on a multiprocessor
+static_assert(kTile == kChunk, "a tile starts at a saved state");
 
-// ---- a lane's channels: a pair of a 16-bit type in one register, or one value --------------
-template <typename T, int kVec> struct Lane;
-template <typename T> struct Lane<T, 1> {
-    using Raw = T;
-    static __device__ __forceinline__ void unpack(Raw r, float* v) { v[0] = to_f32<T>(r); }
-    static __device__ __forceinline__ Raw pack(const float* v) { return from_f32<T>(v[0]); }
-    static __device__ __forceinline__ void keep_packed(Raw&) {}
-};
-template <typename T> struct Lane<T, 2> {
+// ---- a lane's four bytes of a row ----------------------------------------------------------
+template <typename T> struct Lane {
+    static constexpr int kVec = 2;
     using Raw = uint32_t;
     static __device__ __forceinline__ void unpack(Raw r, float* v) {
         float2 f;
@@ -62,419 +59,532 @@ template <typename T> struct Lane<T, 2> {
             return *reinterpret_cast<const uint32_t*>(&h);
         }
     }
-    // Hides from the compiler that a pair was unpacked before: it would keep the two floats
-    // from one pass over the frames to the next, at twice the registers.
-    static __device__ __forceinline__ void keep_packed(Raw& r) { asm("" : "+r"(r)); }
+    static constexpr uint32_t kInfinity = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
 };
-template <typename T, int kVec> __device__ __forceinline__ typename Lane<T, kVec>::Raw splat(float v) {
-    const float two[2] = {v, v};
-    return Lane<T, kVec>::pack(two);
+template <> struct Lane<float> {
+    static constexpr int kVec = 1;
+    using Raw = float;
+    static __device__ __forceinline__ void unpack(Raw r, float* v) { v[0] = r; }
+    static __device__ __forceinline__ Raw pack(const float* v) { return v[0]; }
+    static constexpr uint32_t kInfinity = 0x7f800000u;
+};
+
+// f and p = 1 - f, both with all their bits: e = exp(-gate), f = 1 / (1 + e), p = e f. The
+// exponent stops at 126, where f is the smallest normal number and p is 1; a NaN stays one. The
+// special functions flush subnormals: otherwise each costs three more instructions.
+__device__ __forceinline__ void gates(float g, float& f, float& p) {
+    float e;
+    asm("min.NaN.f32 %0, %1, 0f42fc0000;" : "=f"(e) : "f"(g * -kLog2e));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(1.0f + e));
+    p = e * f;
 }
 
-// ---- the step ------------------------------------------------------------------------------
-// Of f and p, the one below 1/2 has all its bits and the other is one minus it. `signed_gate`
-// holds the small one, with its sign for which it is: f >= 0, or -p (so -0 keeps the state
-// exactly and +0 takes x exactly).
-__device__ __forceinline__ float signed_gate(float g) {
-    const float e = __expf(-fabsf(g));
-    const float small = e * __fdividef(1.0f, 1.0f + e);
-    return __uint_as_float(__float_as_uint(small) | (~__float_as_uint(g) & 0x80000000u));
+// ---- rows between global and shared memory -------------------------------------------------
+// A warp moves its kFrames rows in units of kUnit bytes, which every row's address is a
+// multiple of. `from` and `to` are the same for the whole block; `offset` is the warp's first
+// row and the slab's first channel, in bytes.
+struct Rows {
+    uint32_t offset, pitch;
+    int bytes;  // of the slab's row: less than kRow in the last slab
+};
+
+template <int kUnit> __device__ __forceinline__ void copy_unit(char* to, const char* from) {
+    if constexpr (kUnit == 2) {
+        *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+    } else {
+        const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+        if constexpr (kUnit == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+        else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(from) : "memory");
+    }
 }
-__device__ __forceinline__ bool keeps(float s) { return __float_as_int(s) < 0; }  // s is -p
-// f h + p x, from the larger of the two: h + p (x - h) or x + f (h - x); d = h - x.
-__device__ __forceinline__ float step(float s, float d, float h, float x) {
-    return fmaf(s, d, keeps(s) ? h : x);
+
+// The first `rows` rows; the others hold `fill`.
+template <int kUnit>
+__device__ __forceinline__ void fetch(char* to, const void* from, const Rows& at, int rows,
+                                      uint32_t fill, int lane) {
+    constexpr int kPerRow = kRow / kUnit;
+#pragma unroll
+    for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
+        const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
+        if (row < rows) {
+            if (byte < at.bytes)
+                copy_unit<kUnit>(to + u * kUnit, static_cast<const char*>(from) +
+                                                     (at.offset + row * at.pitch + byte));
+        } else if constexpr (kUnit == 16) {
+            *reinterpret_cast<uint4*>(to + u * kUnit) = make_uint4(fill, fill, fill, fill);
+        } else if constexpr (kUnit == 4) {
+            *reinterpret_cast<uint32_t*>(to + u * kUnit) = fill;
+        } else {
+            *reinterpret_cast<uint16_t*>(to + u * kUnit) = static_cast<uint16_t>(fill);
+        }
+    }
 }
-__device__ __forceinline__ float forget(float s) { return keeps(s) ? 1.0f + s : s; }  // f
-__device__ __forceinline__ float take(float s) { return keeps(s) ? -s : 1.0f - s; }   // p
-// f a
-__device__ __forceinline__ float fade(float s, float a) {
-    return fmaf(s, a, keeps(s) ? a : 0.0f);
+
+template <int kUnit>
+__device__ __forceinline__ void store(void* to, const char* from, const Rows& at, int rows,
+                                      int lane) {
+    constexpr int kPerRow = kRow / kUnit;
+    using Unit = std::conditional_t<kUnit == 16, uint4,
+                                    std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
+#pragma unroll
+    for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
+        const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
+        if (row < rows && byte < at.bytes)
+            *reinterpret_cast<Unit*>(static_cast<char*>(to) +
+                                     (at.offset + row * at.pitch + byte)) =
+                *reinterpret_cast<const Unit*>(from + u * kUnit);
+    }
+}
+
+// Zeros in rows [from, to) of an utterance, of which this warp takes every `by`-th run of rows
+// that one access of the warp covers.
+template <int kUnit>
+__device__ __forceinline__ void zero_rows(void* utterance, uint32_t slab, int64_t pitch, int bytes,
+                                          int from, int to, int warp, int by, int lane) {
+    constexpr int kPerRow = kRow / kUnit, kRun = kPerRow < kWarp ? kWarp / kPerRow : 1;
+    using Unit = std::conditional_t<kUnit == 16, uint4,
+                                    std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
+    for (int t = from + warp * kRun; t < to; t += by * kRun) {
+#pragma unroll
+        for (int u = lane; u < kRun * kPerRow; u += kWarp) {
+            const int row = t + u / kPerRow, byte = u % kPerRow * kUnit;
+            if (row < to && byte < bytes)
+                *reinterpret_cast<Unit*>(static_cast<char*>(utterance) + row * pitch + slab + byte) =
+                    Unit{};
+        }
+    }
+}
+
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest group have arrived, for every lane of the warp.
+__device__ __forceinline__ void arrived() {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
 }
 
 struct Geometry {
     int length, channels, chunks;
-    int slabs;    // channel slabs of 32 lanes
+    int slabs;    // of kRow bytes
     int cluster;  // blocks that share an utterance's slab
 };
 
-// What a block works on.
-template <int kVec> struct Place {
-    int n, m, channel, rank, warp, lane, warps;
-    bool active;
+// What a thread works on.
+template <typename T> struct Place {
+    int n, m, channel, slab, rank, warp, lane;
+    Rows rows;
     __device__ Place(const Geometry& g, const int32_t* lengths) {
         warp = threadIdx.x / kWarp;
         lane = threadIdx.x % kWarp;
-        warps = blockDim.x / kWarp;
         rank = blockIdx.x % g.cluster;
         const int unit = blockIdx.x / g.cluster;
         n = unit / g.slabs;
-        channel = (unit % g.slabs * kWarp + lane) * kVec;
-        active = channel < g.channels;
+        slab = unit % g.slabs * (kRow / static_cast<int>(sizeof(T)));
+        channel = slab + lane * Lane<T>::kVec;
         m = min(max(lengths[n], 0), g.length);
+        rows.pitch = static_cast<uint32_t>(g.channels) * sizeof(T);
+        rows.offset = (rank * kTile + warp * kFrames) * rows.pitch + slab * sizeof(T);
+        rows.bytes = min(kRow, (g.channels - slab) * static_cast<int>(sizeof(T)));
     }
 };
 
-// kFrames rows from frame t0 on; rows at or past `limit` are `fill`.
-template <typename Raw, int kFrames>
-__device__ __forceinline__ void load_rows(Raw (&r)[kFrames], const Raw* p, int64_t stride, int t0,
-                                          int limit, Raw fill) {
-    if (t0 + kFrames <= limit) {
+// A lane's values of an [.., C] f32 row at the slab; channels past the last are skipped.
+template <int kVec>
+__device__ __forceinline__ void read_state(float* v, const float* row, int channel, int channels) {
 #pragma unroll
-        for (int i = 0; i < kFrames; ++i, p += stride) r[i] = *p;
-    } else {
+    for (int i = 0; i < kVec; ++i) v[i] = row != nullptr && channel + i < channels ? row[channel + i] : 0.0f;
+}
+template <int kVec>
+__device__ __forceinline__ void write_state(float* row, const float* v, int channel, int channels) {
 #pragma unroll
-        for (int i = 0; i < kFrames; ++i, p += stride) r[i] = t0 + i < limit ? *p : fill;
-    }
+    for (int i = 0; i < kVec; ++i)
+        if (channel + i < channels) row[channel + i] = v[i];
 }
 
-template <typename Raw>
-__device__ __forceinline__ void zero_rows(Raw* p, int64_t stride, int from, int to, int by,
-                                          Raw zero) {
-    for (int t = from; t < to; t += by) p[t * stride] = zero;
+// What the warps of a block and the blocks of a cluster tell one another. Two of each in turn,
+// so that one barrier a tile is enough.
+struct Runs {
+    float2 warp[2][kWarps][2 * kWarp];  // (A, B)
+    float back[2][kWarps][2 * kWarp];   // B of the carry (backward)
+    float behind[2][2 * kWarp];         // the state (forward) or carry (backward) after the tile
+};
+struct ClusterRuns {
+    float2 block[2][kMaxCluster][2 * kWarp];
+};
+
+// Dynamic shared memory: each warp's stages of rows, Runs, and in a cluster ClusterRuns.
+constexpr int kForwardStage = 2 * kFrames * kRow, kBackwardStage = 3 * kFrames * kRow;
+constexpr int smem_bytes(int stage, bool cluster) {
+    return 2 * kWarps * stage + static_cast<int>(sizeof(Runs)) +
+           (cluster ? static_cast<int>(sizeof(ClusterRuns)) : 0);
 }
 
-template <typename T, int kVec, int kFrames, int kWarps>
-__global__ void __launch_bounds__(kWarps* kWarp, 3) recurrence_kernel(
+template <typename T, int kUnit>
+__global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks) recurrence_kernel(
     const T* __restrict__ x, const T* __restrict__ gate, const int32_t* __restrict__ lengths,
     const float* initial, T* __restrict__ out, float* final_state, float* __restrict__ states,
     Geometry geo) {
-    using L = Lane<T, kVec>;
+    using L = Lane<T>;
     using Raw = typename L::Raw;
-    // Of each warp of the block and of each block of the cluster; two of them in turn, so that
-    // one barrier a tile is enough.
-    __shared__ float2 warp_run[2][kWarps][kWarp * kVec];
-    __shared__ float2 block_run[2][kMaxCluster][kWarp * kVec];
+    constexpr int kVec = L::kVec;
+    extern __shared__ __align__(16) char smem[];
+    Runs& runs = *reinterpret_cast<Runs*>(smem + 2 * kWarps * kForwardStage);
+    ClusterRuns& others = *reinterpret_cast<ClusterRuns*>(&runs + 1);
 
-    const Place<kVec> at(geo, lengths);
-    const int limit = at.active ? at.m : 0;
-    const int64_t stride = geo.channels / kVec;  // in Raw
-    const int64_t base =
-        static_cast<int64_t>(at.n) * geo.length * geo.channels + at.channel;
-    const int64_t state_at = static_cast<int64_t>(at.n) * geo.channels + at.channel;
+    const Place<T> at(geo, lengths);
+    char* stage = smem + at.warp * 2 * kForwardStage;
+    const int last_warp = blockDim.x / kWarp - 1, state = at.lane * kVec;
+    const int64_t first_row = static_cast<int64_t>(at.n) * geo.length * geo.channels;
+    const int64_t state_row = static_cast<int64_t>(at.n) * geo.channels;
     float* saved = states == nullptr
                        ? nullptr
-                       : states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels + at.channel;
+                       : states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels;
+    const int round = kTile * geo.cluster, in_round = at.rank * kTile + at.warp * kFrames;
 
-    float carry[kVec];
+    auto fetch_tile = [&](int start, int which) {
+        const int64_t here = first_row + start * static_cast<int64_t>(geo.channels);
+        const int rows = at.m - start - in_round;
+        char* to = stage + which * kForwardStage;
+        fetch<kUnit>(to, x + here, at.rows, rows, 0u, at.lane);
+        // An infinite gate keeps the state.
+        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, rows, L::kInfinity, at.lane);
+    };
+    if (at.m > 0) fetch_tile(0, 0);
+    commit();
+
+    float h[kVec];
+    read_state<kVec>(h, initial == nullptr ? nullptr : initial + state_row, at.channel,
+                     geo.channels);
+    if (at.warp == 0)
 #pragma unroll
-    for (int v = 0; v < kVec; ++v)
-        carry[v] = at.active && initial != nullptr ? initial[state_at + v] : 0.0f;
+        for (int v = 0; v < kVec; ++v) runs.behind[1][state + v] = h[v];
     // Every block of the cluster runs, and has read its state, before any writes to another.
     if (geo.cluster > 1) cg::this_cluster().sync();
 
-    const int tile = at.warps * kFrames;
     int turn = 0;
-    for (int start = 0; start < at.m; start += tile * geo.cluster, turn ^= 1) {
-        const int t0 = start + at.rank * tile + at.warp * kFrames;
-        const int64_t row = base + t0 * static_cast<int64_t>(geo.channels);
-        Raw xr[kFrames];
-        float s[kFrames][kVec];
-        float a[kVec], b[kVec];
-        {
-            Raw gr[kFrames];
-            load_rows(xr, reinterpret_cast<const Raw*>(x + row), stride, t0, limit,
-                      splat<T, kVec>(0.0f));
-            // An infinite gate keeps the state.
-            load_rows(gr, reinterpret_cast<const Raw*>(gate + row), stride, t0, limit,
-                      splat<T, kVec>(__int_as_float(0x7f800000)));
+    for (int start = 0; start < at.m; start += round, turn ^= 1) {
+        if (start + round < at.m) fetch_tile(start + round, turn ^ 1);
+        commit();
+        arrived();
+        char* rows = stage + turn * kForwardStage;
+        // After each frame: the product of f, and h from 0.
+        float a[kFrames][kVec], b[kFrames][kVec];
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
+        for (int i = 0; i < kFrames; ++i) {
+            float xv[kVec], gv[kVec];
+            L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
+            L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
 #pragma unroll
-            for (int i = 0; i < kFrames; ++i) {
-                float xv[kVec];
-                L::unpack(gr[i], s[i]);
-                L::unpack(xr[i], xv);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    s[i][v] = signed_gate(s[i][v]);
-                    a[v] = fade(s[i][v], a[v]);
-                    b[v] = step(s[i][v], b[v] - xv[v], b[v], xv[v]);
-                }
+            for (int v = 0; v < kVec; ++v) {
+                float f, p;
+                gates(gv[v], f, p);
+                a[i][v] = i == 0 ? f : a[i - 1][v] * f;
+                b[i][v] = i == 0 ? p * xv[v] : fmaf(f, b[i - 1][v], p * xv[v]);
             }
         }
 #pragma unroll
         for (int v = 0; v < kVec; ++v)
-            warp_run[turn][at.warp][at.lane * kVec + v] = make_float2(a[v], b[v]);
+            runs.warp[turn][at.warp][state + v] =
+                make_float2(a[kFrames - 1][v], b[kFrames - 1][v]);
         __syncthreads();
-        if (geo.cluster > 1) {
-            // Every warp finds the block's run; it tells its share of the cluster.
-            auto cluster = cg::this_cluster();
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
-            for (int w = 0; w < at.warps; ++w)
+        for (int v = 0; v < kVec; ++v) h[v] = runs.behind[turn ^ 1][state + v];
+        if (geo.cluster > 1) {
+            // Every warp finds the block's run and tells its share of the cluster.
+            auto cluster = cg::this_cluster();
+            float all_a[kVec], all_b[kVec];
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) all_a[v] = 1.0f, all_b[v] = 0.0f;
+            for (int w = 0; w <= last_warp; ++w)
 #pragma unroll
                 for (int v = 0; v < kVec; ++v) {
-                    const float2 r = warp_run[turn][w][at.lane * kVec + v];
-                    b[v] = fmaf(r.x, b[v], r.y);
-                    a[v] *= r.x;
+                    const float2 r = runs.warp[turn][w][state + v];
+                    all_b[v] = fmaf(r.x, all_b[v], r.y);
+                    all_a[v] *= r.x;
                 }
-            for (int q = at.warp; q < geo.cluster; q += at.warps) {
-                float2* there = cluster.map_shared_rank(&block_run[turn][at.rank][0], q);
+            for (int q = at.warp; q < geo.cluster; q += last_warp + 1) {
+                float2* there = cluster.map_shared_rank(&others.block[turn][at.rank][0], q);
 #pragma unroll
-                for (int v = 0; v < kVec; ++v)
-                    there[at.lane * kVec + v] = make_float2(a[v], b[v]);
+                for (int v = 0; v < kVec; ++v) there[state + v] = make_float2(all_a[v], all_b[v]);
             }
             cluster.sync();
-        }
-        float h[kVec];
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) h[v] = carry[v];
-        if (geo.cluster > 1) {
-            for (int q = 0; q < geo.cluster; ++q)
+            for (int q = 0; q < at.rank; ++q)
 #pragma unroll
                 for (int v = 0; v < kVec; ++v) {
-                    const float2 r = block_run[turn][q][at.lane * kVec + v];
-                    if (q == at.rank) h[v] = carry[v];
-                    carry[v] = fmaf(r.x, carry[v], r.y);
-                }
-            for (int w = 0; w < at.warp; ++w)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = warp_run[turn][w][at.lane * kVec + v];
+                    const float2 r = others.block[turn][q][state + v];
                     h[v] = fmaf(r.x, h[v], r.y);
                 }
-        } else {
-            for (int w = 0; w < at.warps; ++w)
+            if (at.warp == last_warp) {
+                float behind[kVec];
 #pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = warp_run[turn][w][at.lane * kVec + v];
-                    if (w == at.warp) h[v] = carry[v];
-                    carry[v] = fmaf(r.x, carry[v], r.y);
-                }
+                for (int v = 0; v < kVec; ++v) behind[v] = h[v];
+                for (int q = at.rank; q < geo.cluster; ++q)
+#pragma unroll
+                    for (int v = 0; v < kVec; ++v) {
+                        const float2 r = others.block[turn][q][state + v];
+                        behind[v] = fmaf(r.x, behind[v], r.y);
+                    }
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = behind[v];
+            }
         }
-        if (saved != nullptr && t0 % kChunk == 0 && t0 < limit) {
+        // The tile starts at a saved state.
+        if (saved != nullptr && at.warp == 0 && start + in_round < at.m)
+            write_state<kVec>(saved + (start + in_round) / kChunk * static_cast<int64_t>(geo.channels),
+                              h, at.channel, geo.channels);
+        for (int w = 0; w < at.warp; ++w)
 #pragma unroll
-            for (int v = 0; v < kVec; ++v)
-                saved[static_cast<int64_t>(t0 / kChunk) * geo.channels + v] = h[v];
+            for (int v = 0; v < kVec; ++v) {
+                const float2 r = runs.warp[turn][w][state + v];
+                h[v] = fmaf(r.x, h[v], r.y);
+            }
+        // The outputs take the place of x.
+        float hv[kVec];
+#pragma unroll
+        for (int i = 0; i < kFrames; ++i) {
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) hv[v] = fmaf(a[i][v], h[v], b[i][v]);
+            reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(hv);
         }
-        Raw* to = reinterpret_cast<Raw*>(out + row);
+        if (geo.cluster == 1 && at.warp == last_warp) {
 #pragma unroll
-        for (int i = 0; i < kFrames; ++i, to += stride) {
-            float xv[kVec];
-            L::keep_packed(xr[i]);
-            L::unpack(xr[i], xv);
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) h[v] = step(s[i][v], h[v] - xv[v], h[v], xv[v]);
-            if (t0 + i < limit) *to = L::pack(h);
+            for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = hv[v];
         }
+        __syncwarp();
+        store<kUnit>(out + first_row + start * static_cast<int64_t>(geo.channels), rows, at.rows,
+                     at.m - start - in_round, at.lane);
+        __syncwarp();
     }
-    if (!at.active) return;
-    if (at.rank == 0 && at.warp == 0) {
+    if (at.rank == 0 && at.warp == last_warp) {
+        if (at.m > 0)  // this warp wrote it
 #pragma unroll
-        for (int v = 0; v < kVec; ++v) final_state[state_at + v] = carry[v];
+            for (int v = 0; v < kVec; ++v) h[v] = runs.behind[turn ^ 1][state + v];
+        write_state<kVec>(final_state + state_row, h, at.channel, geo.channels);
     }
-    const int first = at.rank * at.warps + at.warp, by = geo.cluster * at.warps;
-    zero_rows(reinterpret_cast<Raw*>(out + base), stride, at.m + first, geo.length, by,
-              splat<T, kVec>(0.0f));
-    if (saved != nullptr)
+    const int first = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
+    zero_rows<kUnit>(out + first_row, at.slab * static_cast<uint32_t>(sizeof(T)), at.rows.pitch,
+                     at.rows.bytes, at.m, geo.length, first, by, at.lane);
+    if (saved != nullptr) {
+        const float zero[2] = {0.0f, 0.0f};
         for (int j = (at.m + kChunk - 1) / kChunk + first; j < geo.chunks; j += by)
-#pragma unroll
-            for (int v = 0; v < kVec; ++v)
-                saved[static_cast<int64_t>(j) * geo.channels + v] = 0.0f;
+            write_state<kVec>(saved + j * static_cast<int64_t>(geo.channels), zero, at.channel,
+                              geo.channels);
+    }
 }
 
-template <typename T, int kVec, int kFrames, int kWarps>
-__global__ void __launch_bounds__(kWarps* kWarp, 2) recurrence_backward_kernel(
+template <typename T, int kUnit>
+__global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks) recurrence_backward_kernel(
     const T* __restrict__ dout, const T* __restrict__ x, const T* __restrict__ gate,
     const int32_t* __restrict__ lengths, const float* __restrict__ states,
     const float* __restrict__ dfinal, T* __restrict__ dx, T* __restrict__ dgate,
     float* __restrict__ dinitial, Geometry geo) {
-    using L = Lane<T, kVec>;
+    using L = Lane<T>;
     using Raw = typename L::Raw;
-    // (A, B of h) of a warp; B of the carry; (A, B of the carry) of a block.
-    __shared__ float2 warp_run[2][kWarps][kWarp * kVec];
-    __shared__ float warp_back[2][kWarps][kWarp * kVec];
-    __shared__ float2 block_run[2][kMaxCluster][kWarp * kVec];
+    constexpr int kVec = L::kVec;
+    extern __shared__ __align__(16) char smem[];
+    Runs& runs = *reinterpret_cast<Runs*>(smem + 2 * kWarps * kBackwardStage);
+    ClusterRuns& others = *reinterpret_cast<ClusterRuns*>(&runs + 1);
 
-    const Place<kVec> at(geo, lengths);
-    const int limit = at.active ? at.m : 0;
-    const int64_t stride = geo.channels / kVec;
-    const int64_t base =
-        static_cast<int64_t>(at.n) * geo.length * geo.channels + at.channel;
-    const int64_t state_at = static_cast<int64_t>(at.n) * geo.channels + at.channel;
-    const float* saved =
-        states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels + at.channel;
+    const Place<T> at(geo, lengths);
+    char* stage = smem + at.warp * 2 * kBackwardStage;
+    const int last_warp = blockDim.x / kWarp - 1, state = at.lane * kVec;
+    const int64_t first_row = static_cast<int64_t>(at.n) * geo.length * geo.channels;
+    const int64_t state_row = static_cast<int64_t>(at.n) * geo.channels;
+    const float* saved = states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels;
+    const int round = kTile * geo.cluster, in_round = at.rank * kTile + at.warp * kFrames;
 
-    float carry[kVec];
+    auto fetch_tile = [&](int start, int which) {
+        const int64_t here = first_row + start * static_cast<int64_t>(geo.channels);
+        const int rows = at.m - start - in_round;
+        char* to = stage + which * kBackwardStage;
+        fetch<kUnit>(to, x + here, at.rows, rows, 0u, at.lane);
+        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, rows, L::kInfinity, at.lane);
+        fetch<kUnit>(to + 2 * kFrames * kRow, dout + here, at.rows, rows, 0u, at.lane);
+    };
+    const int last = (at.m - 1) / round * round;
+    if (at.m > 0) fetch_tile(last, 0);
+    commit();
+
+    float c[kVec];
+    read_state<kVec>(c, dfinal == nullptr ? nullptr : dfinal + state_row, at.channel,
+                     geo.channels);
+    if (at.warp == 0)
 #pragma unroll
-    for (int v = 0; v < kVec; ++v)
-        carry[v] = at.active && dfinal != nullptr ? dfinal[state_at + v] : 0.0f;
+        for (int v = 0; v < kVec; ++v) runs.behind[1][state + v] = c[v];
     if (geo.cluster > 1) cg::this_cluster().sync();
 
-    const int tile = at.warps * kFrames, round = tile * geo.cluster;
     int turn = 0;
-    for (int start = (at.m + round - 1) / round * round - round; start >= 0;
-         start -= round, turn ^= 1) {
-        const int t0 = start + at.rank * tile + at.warp * kFrames;
-        const int64_t row = base + t0 * static_cast<int64_t>(geo.channels);
-        Raw xr[kFrames], dr[kFrames];
-        float s[kFrames][kVec];
-        float a[kVec], b[kVec], c[kVec], h[kVec];
-        {
-            Raw gr[kFrames];
-            load_rows(xr, reinterpret_cast<const Raw*>(x + row), stride, t0, limit,
-                      splat<T, kVec>(0.0f));
-            load_rows(gr, reinterpret_cast<const Raw*>(gate + row), stride, t0, limit,
-                      splat<T, kVec>(__int_as_float(0x7f800000)));
-            load_rows(dr, reinterpret_cast<const Raw*>(dout + row), stride, t0, limit,
-                      splat<T, kVec>(0.0f));
-            // The saved state at or before this warp's frames.
-            const int64_t chunk = static_cast<int64_t>(t0 / kChunk) * geo.channels;
+    for (int start = at.m > 0 ? last : -1; start >= 0; start -= round, turn ^= 1) {
+        float h[kVec];  // the saved state before the tile
+        read_state<kVec>(h, start + at.rank * kTile < at.m
+                                ? saved + (start / kChunk + at.rank) * static_cast<int64_t>(geo.channels)
+                                : nullptr, at.channel, geo.channels);
+        if (start >= round) fetch_tile(start - round, turn ^ 1);
+        commit();
+        arrived();
+        char* rows = stage + turn * kBackwardStage;
+        float f[kFrames][kVec], p[kFrames][kVec];
+        float a[kVec], b[kVec], back[kVec];
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f, back[v] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFrames; ++i) {
+            float xv[kVec], gv[kVec];
+            L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
+            L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
-                h[v] = t0 < limit ? saved[chunk + v] : 0.0f;
-                a[v] = 1.0f, b[v] = 0.0f, c[v] = 0.0f;
+                gates(gv[v], f[i][v], p[i][v]);
+                a[v] *= f[i][v];
+                b[v] = fmaf(f[i][v], b[v], p[i][v] * xv[v]);
             }
+        }
 #pragma unroll
-            for (int i = 0; i < kFrames; ++i) {
-                float xv[kVec];
-                L::unpack(gr[i], s[i]);
-                L::unpack(xr[i], xv);
+        for (int i = kFrames - 1; i >= 0; --i) {
+            float dv[kVec];
+            L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], dv);
 #pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    s[i][v] = signed_gate(s[i][v]);
-                    a[v] = fade(s[i][v], a[v]);
-                    b[v] = step(s[i][v], b[v] - xv[v], b[v], xv[v]);
-                }
-            }
-#pragma unroll
-            for (int i = kFrames - 1; i >= 0; --i) {
-                float dv[kVec];
-                L::unpack(dr[i], dv);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) c[v] = fade(s[i][v], dv[v] + c[v]);
-            }
+            for (int v = 0; v < kVec; ++v) back[v] = f[i][v] * (dv[v] + back[v]);
         }
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
-            warp_run[turn][at.warp][at.lane * kVec + v] = make_float2(a[v], b[v]);
-            warp_back[turn][at.warp][at.lane * kVec + v] = c[v];
+            runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
+            runs.back[turn][at.warp][state + v] = back[v];
         }
         __syncthreads();
-        // h before this warp's frames: the saved state through the warps since.
-        for (int w = at.warp - t0 % kChunk / kFrames; w < at.warp; ++w)
+        for (int w = 0; w < at.warp; ++w)
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
-                const float2 r = warp_run[turn][w][at.lane * kVec + v];
+                const float2 r = runs.warp[turn][w][state + v];
                 h[v] = fmaf(r.x, h[v], r.y);
             }
-        // The carry behind them.
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) c[v] = runs.behind[turn ^ 1][state + v];
         if (geo.cluster > 1) {
             auto cluster = cg::this_cluster();
+            float all_a[kVec], all_c[kVec];
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, c[v] = 0.0f;
-            for (int w = at.warps - 1; w >= 0; --w)
+            for (int v = 0; v < kVec; ++v) all_a[v] = 1.0f, all_c[v] = 0.0f;
+            for (int w = last_warp; w >= 0; --w)
 #pragma unroll
                 for (int v = 0; v < kVec; ++v) {
-                    const float r = warp_run[turn][w][at.lane * kVec + v].x;
-                    c[v] = fmaf(r, c[v], warp_back[turn][w][at.lane * kVec + v]);
-                    a[v] *= r;
+                    const float r = runs.warp[turn][w][state + v].x;
+                    all_c[v] = fmaf(r, all_c[v], runs.back[turn][w][state + v]);
+                    all_a[v] *= r;
                 }
-            for (int q = at.warp; q < geo.cluster; q += at.warps) {
-                float2* there = cluster.map_shared_rank(&block_run[turn][at.rank][0], q);
+            for (int q = at.warp; q < geo.cluster; q += last_warp + 1) {
+                float2* there = cluster.map_shared_rank(&others.block[turn][at.rank][0], q);
 #pragma unroll
-                for (int v = 0; v < kVec; ++v)
-                    there[at.lane * kVec + v] = make_float2(a[v], c[v]);
+                for (int v = 0; v < kVec; ++v) there[state + v] = make_float2(all_a[v], all_c[v]);
             }
             cluster.sync();
-            for (int q = geo.cluster - 1; q >= 0; --q)
+            for (int q = geo.cluster - 1; q > at.rank; --q)
 #pragma unroll
                 for (int v = 0; v < kVec; ++v) {
-                    const float2 r = block_run[turn][q][at.lane * kVec + v];
-                    if (q == at.rank) c[v] = carry[v];
-                    carry[v] = fmaf(r.x, carry[v], r.y);
+                    const float2 r = others.block[turn][q][state + v];
+                    c[v] = fmaf(r.x, c[v], r.y);
                 }
-            for (int w = at.warps - 1; w > at.warp; --w)
+            if (at.warp == 0) {
+                float behind[kVec];
 #pragma unroll
-                for (int v = 0; v < kVec; ++v)
-                    c[v] = fmaf(warp_run[turn][w][at.lane * kVec + v].x, c[v],
-                                warp_back[turn][w][at.lane * kVec + v]);
-        } else {
-            for (int w = at.warps - 1; w >= 0; --w)
+                for (int v = 0; v < kVec; ++v) behind[v] = c[v];
+                for (int q = at.rank; q >= 0; --q)
 #pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    if (w == at.warp) c[v] = carry[v];
-                    carry[v] = fmaf(warp_run[turn][w][at.lane * kVec + v].x, carry[v],
-                                    warp_back[turn][w][at.lane * kVec + v]);
-                }
+                    for (int v = 0; v < kVec; ++v) {
+                        const float2 r = others.block[turn][q][state + v];
+                        behind[v] = fmaf(r.x, behind[v], r.y);
+                    }
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = behind[v];
+            }
         }
+        for (int w = last_warp; w > at.warp; --w)
+#pragma unroll
+            for (int v = 0; v < kVec; ++v)
+                c[v] = fmaf(runs.warp[turn][w][state + v].x, c[v], runs.back[turn][w][state + v]);
         float away[kFrames][kVec];  // h[t-1] - x[t]
 #pragma unroll
         for (int i = 0; i < kFrames; ++i) {
             float xv[kVec];
-            L::keep_packed(xr[i]);
-            L::unpack(xr[i], xv);
+            L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
                 away[i][v] = h[v] - xv[v];
-                h[v] = step(s[i][v], away[i][v], h[v], xv[v]);
+                h[v] = fmaf(f[i][v], h[v], p[i][v] * xv[v]);
             }
         }
-        const int64_t end = row + (kFrames - 1) * static_cast<int64_t>(geo.channels);
-        Raw* to_x = reinterpret_cast<Raw*>(dx + end);
-        Raw* to_g = reinterpret_cast<Raw*>(dgate + end);
+        // dx takes the place of x, dgate that of gate.
 #pragma unroll
-        for (int i = kFrames - 1; i >= 0; --i, to_x -= stride, to_g -= stride) {
+        for (int i = kFrames - 1; i >= 0; --i) {
             float gx[kVec], gg[kVec];
-            L::keep_packed(dr[i]);
-            L::unpack(dr[i], gx);
+            L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], gx);
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
-                const float total = gx[v] + c[v], f = forget(s[i][v]);
-                gx[v] = take(s[i][v]) * total;
-                gg[v] = f * gx[v] * away[i][v];
-                c[v] = f * total;
+                const float total = gx[v] + c[v];
+                gx[v] = p[i][v] * total;
+                gg[v] = f[i][v] * gx[v] * away[i][v];
+                c[v] = f[i][v] * total;
             }
-            if (t0 + i < limit) {
-                *to_x = L::pack(gx);
-                *to_g = L::pack(gg);
-            }
+            reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(gx);
+            reinterpret_cast<Raw*>(rows + (kFrames + i) * kRow)[at.lane] = L::pack(gg);
         }
-    }
-    if (!at.active) return;
-    if (at.rank == 0 && at.warp == 0) {
+        if (geo.cluster == 1 && at.warp == 0) {
 #pragma unroll
-        for (int v = 0; v < kVec; ++v) dinitial[state_at + v] = carry[v];
+            for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = c[v];
+        }
+        __syncwarp();
+        const int64_t here = first_row + start * static_cast<int64_t>(geo.channels);
+        store<kUnit>(dx + here, rows, at.rows, at.m - start - in_round, at.lane);
+        store<kUnit>(dgate + here, rows + kFrames * kRow, at.rows, at.m - start - in_round, at.lane);
+        __syncwarp();
     }
-    const int first = at.m + at.rank * at.warps + at.warp, by = geo.cluster * at.warps;
-    const Raw zero = splat<T, kVec>(0.0f);
-    zero_rows(reinterpret_cast<Raw*>(dx + base), stride, first, geo.length, by, zero);
-    zero_rows(reinterpret_cast<Raw*>(dgate + base), stride, first, geo.length, by, zero);
+    if (at.rank == 0 && at.warp == 0) {
+        if (at.m > 0)  // this warp wrote it
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) c[v] = runs.behind[turn ^ 1][state + v];
+        write_state<kVec>(dinitial + state_row, c, at.channel, geo.channels);
+    }
+    const int first = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
+    for (T* grad : {dx, dgate})
+        zero_rows<kUnit>(grad + first_row, at.slab * static_cast<uint32_t>(sizeof(T)),
+                         at.rows.pitch, at.rows.bytes, at.m, geo.length, first, by, at.lane);
 }
 
 // ---- launch --------------------------------------------------------------------------------
-
-constexpr int kFrames = 16, kWarps = 8;
 
 struct Shape {
     Geometry geo;
     int blocks, threads;
 };
 
-template <int kVec> Shape shape_of(int batch, int length, int channels, int chunks) {
+Shape shape_of(int batch, int length, int channels, int chunks, int row_channels) {
     Shape s{};
-    const int slabs = (channels + kWarp * kVec - 1) / (kWarp * kVec);
-    const int warps = std::min(kWarps, (length + kFrames - 1) / kFrames);
+    const int slabs = (channels + row_channels - 1) / row_channels;
     const int64_t units = static_cast<int64_t>(batch) * slabs;
-    const int tiles = (length + kWarps * kFrames - 1) / (kWarps * kFrames);
     // Blocks for three on every multiprocessor, in rounds of the same number of tiles.
     const int64_t wanted = (3LL * sm_count() + units - 1) / units;
     int cluster = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>(wanted, std::min(tiles, kMaxCluster))));
-    const int rounds = (tiles + cluster - 1) / cluster;
-    cluster = (tiles + rounds - 1) / rounds;
+        1, std::min<int64_t>(wanted, std::min(chunks, kMaxCluster))));
+    const int rounds = (chunks + cluster - 1) / cluster;
+    cluster = (chunks + rounds - 1) / rounds;
     s.geo = {length, channels, chunks, slabs, cluster};
     s.blocks = static_cast<int>(units * cluster);
-    s.threads = warps * kWarp;
+    s.threads = std::min(kWarps, (length + kFrames - 1) / kFrames) * kWarp;
     return s;
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch(void (*kernel)(Params...), const Shape& s, cudaStream_t stream, Args... args) {
+cudaError_t launch(SmemAttr& attribute, void (*kernel)(Params...), const Shape& s, int stage,
+                   cudaStream_t stream, Args... args) {
+    const void* entry = reinterpret_cast<const void*>(kernel);
+    cudaError_t e = attribute.ensure(entry, smem_bytes(stage, true));
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(s.blocks));
     cfg.blockDim = dim3(static_cast<unsigned>(s.threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem_bytes(stage, s.geo.cluster > 1));
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -483,55 +593,70 @@ cudaError_t launch(void (*kernel)(Params...), const Shape& s, cudaStream_t strea
     cfg.attrs = attr;
     cfg.numAttrs = s.geo.cluster > 1 ? 1 : 0;
     if (s.geo.cluster > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(
-            reinterpret_cast<const void*>(kernel),
-            cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        e = cudaFuncSetAttribute(entry, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
     }
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-bool pairs(int channels, std::initializer_list<const void*> buffers) {
-    if (channels % 2 != 0) return false;
-    for (const void* b : buffers)
-        if (reinterpret_cast<uintptr_t>(b) % 4 != 0) return false;
-    return true;
+// The widest unit that divides every row's address: 16 bytes, 4, or an element.
+int unit_of(int64_t pitch, std::initializer_list<const void*> buffers) {
+    uintptr_t all = static_cast<uintptr_t>(pitch);
+    for (const void* b : buffers) all |= reinterpret_cast<uintptr_t>(b);
+    return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
 }
 
-template <typename T, int kVec> cudaError_t forward(const RecurrenceProblem& p, cudaStream_t s) {
-    const Shape shape = shape_of<kVec>(p.batch, p.length, p.channels, p.chunks);
-    return launch(recurrence_kernel<T, kVec, kFrames, kWarps>, shape, s,
+template <typename T, int kUnit> cudaError_t forward(const RecurrenceProblem& p, cudaStream_t s) {
+    static SmemAttr attribute;
+    const Shape shape = shape_of(p.batch, p.length, p.channels, p.chunks, kRow / sizeof(T));
+    return launch(attribute, recurrence_kernel<T, kUnit>, shape, kForwardStage, s,
                   static_cast<const T*>(p.x), static_cast<const T*>(p.gate), p.valid_lengths,
                   p.initial_state, static_cast<T*>(p.output), p.final_state, p.states, shape.geo);
 }
 
-template <typename T, int kVec>
+template <typename T, int kUnit>
 cudaError_t backward(const RecurrenceBackwardProblem& p, cudaStream_t s) {
-    const Shape shape = shape_of<kVec>(p.batch, p.length, p.channels, p.chunks);
-    return launch(recurrence_backward_kernel<T, kVec, kFrames, kWarps>, shape, s,
+    static SmemAttr attribute;
+    const Shape shape = shape_of(p.batch, p.length, p.channels, p.chunks, kRow / sizeof(T));
+    return launch(attribute, recurrence_backward_kernel<T, kUnit>, shape, kBackwardStage, s,
                   static_cast<const T*>(p.grad_output), static_cast<const T*>(p.x),
                   static_cast<const T*>(p.gate), p.valid_lengths, p.states, p.grad_final_state,
                   static_cast<T*>(p.grad_x), static_cast<T*>(p.grad_gate), p.grad_initial_state,
                   shape.geo);
 }
 
+template <typename T> cudaError_t forward(const RecurrenceProblem& p, cudaStream_t s) {
+    const int unit = unit_of(p.channels * static_cast<int64_t>(sizeof(T)), {p.x, p.gate, p.output});
+    if (unit == 16) return forward<T, 16>(p, s);
+    if constexpr (sizeof(T) == 2)
+        if (unit == 2) return forward<T, 2>(p, s);
+    return forward<T, 4>(p, s);
+}
+
+template <typename T> cudaError_t backward(const RecurrenceBackwardProblem& p, cudaStream_t s) {
+    const int unit = unit_of(p.channels * static_cast<int64_t>(sizeof(T)),
+                             {p.grad_output, p.x, p.gate, p.grad_x, p.grad_gate});
+    if (unit == 16) return backward<T, 16>(p, s);
+    if constexpr (sizeof(T) == 2)
+        if (unit == 2) return backward<T, 2>(p, s);
+    return backward<T, 4>(p, s);
+}
+
 }  // namespace
 
 cudaError_t launch_recurrence(const RecurrenceProblem& p, cudaStream_t s, const char** variant) {
     *variant = "recurrence";
-    const bool two = pairs(p.channels, {p.x, p.gate, p.output});
-    if (p.dtype == FGA_FLOAT) return forward<float, 1>(p, s);
-    if (p.dtype == FGA_HALF) return two ? forward<__half, 2>(p, s) : forward<__half, 1>(p, s);
-    return two ? forward<__nv_bfloat16, 2>(p, s) : forward<__nv_bfloat16, 1>(p, s);
+    if (p.dtype == FGA_FLOAT) return forward<float>(p, s);
+    if (p.dtype == FGA_HALF) return forward<__half>(p, s);
+    return forward<__nv_bfloat16>(p, s);
 }
 
 cudaError_t launch_recurrence_backward(const RecurrenceBackwardProblem& p, cudaStream_t s,
                                        const char** variant) {
     *variant = "recurrence-backward";
-    const bool two = pairs(p.channels, {p.grad_output, p.x, p.gate, p.grad_x, p.grad_gate});
-    if (p.dtype == FGA_FLOAT) return backward<float, 1>(p, s);
-    if (p.dtype == FGA_HALF) return two ? backward<__half, 2>(p, s) : backward<__half, 1>(p, s);
-    return two ? backward<__nv_bfloat16, 2>(p, s) : backward<__nv_bfloat16, 1>(p, s);
+    if (p.dtype == FGA_FLOAT) return backward<float>(p, s);
+    if (p.dtype == FGA_HALF) return backward<__half>(p, s);
+    return backward<__nv_bfloat16>(p, s);
 }
 
 }  // namespace fga

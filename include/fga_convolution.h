@@ -75,8 +75,8 @@ FGA_API int32_t fga_zipformer_convolution_enqueue(const fga_tensor_desc* input_d
  * zeros. Conventions that all four entry points share:
  * - "type" is f32, f16 or bf16; arithmetic, statistics, sums and states are fp32, each
  *   output is rounded once.
- * - T is at most 2^30, N*T and N*C at most INT32_MAX (N*T*C may be larger), else
- *   FGA_ERROR_OVERFLOW.
+ * - T is at most 2^30, C at most 2^18, N*T and N*C at most INT32_MAX (N*T*C may be
+ *   larger), else FGA_ERROR_OVERFLOW.
  * - Buffers are aligned to their element size and outputs overlap neither inputs nor one
  *   another (one exception is named below), else FGA_ERROR_UNSUPPORTED. 16-byte aligned
  *   buffers with C a multiple of 16 bytes are the fast case.
