@@ -9,11 +9,14 @@
 // learns the state before its first frame from the warps before it through shared memory, and
 // walks its frames again from there, so that no element is read twice. A block's warps cover
 // one tile; a block walks the tiles of its utterance and channels in turn, with the next
-// tile's rows on their way to shared memory meanwhile. Where utterances and channels are too
-// few to fill the GPU, a cluster of blocks takes consecutive tiles and passes (A, B) on through
-// distributed shared memory. The backward pass runs the same scan from the last tile to the
-// first for the carry c[t] = f[t] G[t], and recomputes h from the states that the forward pass
-// saved every 64 frames.
+// tile's rows on their way to shared memory meanwhile. The backward pass runs the same scan
+// from the last tile to the first for the carry c[t] = f[t] G[t], and recomputes h from the
+// states that the forward pass saved every 64 frames.
+//
+// Where utterances and channels are too few to fill the GPU, a cluster of blocks divides the
+// frames: each block first finds the (A, B) of its whole range, reading it once more (the
+// second time from L2), the blocks exchange them through distributed shared memory, and each
+// walks its tiles from the state that it now knows.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -81,11 +84,10 @@ __device__ __forceinline__ void gates(float g, float& f, float& p) {
 }
 
 // ---- rows between global and shared memory -------------------------------------------------
-// A warp moves its kFrames rows in units of kUnit bytes, which every row's address is a
-// multiple of. `from` and `to` are the same for the whole block; `offset` is the warp's first
-// row and the slab's first channel, in bytes.
+// A warp moves kFrames rows in units of kUnit bytes, which every row's address is a multiple
+// of. `from` and `to` are the first row's slab.
 struct Rows {
-    uint32_t offset, pitch;
+    uint32_t pitch;
     int bytes;  // of the slab's row: less than kRow in the last slab
 };
 
@@ -106,13 +108,13 @@ template <int kUnit>
 __device__ __forceinline__ void fetch(char* to, const void* from, const Rows& at, int rows,
                                       uint32_t fill, int lane) {
     constexpr int kPerRow = kRow / kUnit;
-#pragma unroll
+#pragma unroll 2
     for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
         const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
         if (row < rows) {
             if (byte < at.bytes)
-                copy_unit<kUnit>(to + u * kUnit, static_cast<const char*>(from) +
-                                                     (at.offset + row * at.pitch + byte));
+                copy_unit<kUnit>(to + u * kUnit,
+                                 static_cast<const char*>(from) + (row * at.pitch + byte));
         } else if constexpr (kUnit == 16) {
             *reinterpret_cast<uint4*>(to + u * kUnit) = make_uint4(fill, fill, fill, fill);
         } else if constexpr (kUnit == 4) {
@@ -129,12 +131,11 @@ __device__ __forceinline__ void store(void* to, const char* from, const Rows& at
     constexpr int kPerRow = kRow / kUnit;
     using Unit = std::conditional_t<kUnit == 16, uint4,
                                     std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
-#pragma unroll
+#pragma unroll 2
     for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
         const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
         if (row < rows && byte < at.bytes)
-            *reinterpret_cast<Unit*>(static_cast<char*>(to) +
-                                     (at.offset + row * at.pitch + byte)) =
+            *reinterpret_cast<Unit*>(static_cast<char*>(to) + (row * at.pitch + byte)) =
                 *reinterpret_cast<const Unit*>(from + u * kUnit);
     }
 }
@@ -142,8 +143,8 @@ __device__ __forceinline__ void store(void* to, const char* from, const Rows& at
 // Zeros in rows [from, to) of an utterance, of which this warp takes every `by`-th run of rows
 // that one access of the warp covers.
 template <int kUnit>
-__device__ __forceinline__ void zero_rows(void* utterance, uint32_t slab, int64_t pitch, int bytes,
-                                          int from, int to, int warp, int by, int lane) {
+__device__ __forceinline__ void zero_rows(void* utterance, const Rows& at, int from, int to,
+                                          int warp, int by, int lane) {
     constexpr int kPerRow = kRow / kUnit, kRun = kPerRow < kWarp ? kWarp / kPerRow : 1;
     using Unit = std::conditional_t<kUnit == 16, uint4,
                                     std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
@@ -151,9 +152,9 @@ __device__ __forceinline__ void zero_rows(void* utterance, uint32_t slab, int64_
 #pragma unroll
         for (int u = lane; u < kRun * kPerRow; u += kWarp) {
             const int row = t + u / kPerRow, byte = u % kPerRow * kUnit;
-            if (row < to && byte < bytes)
-                *reinterpret_cast<Unit*>(static_cast<char*>(utterance) + row * pitch + slab + byte) =
-                    Unit{};
+            if (row < to && byte < at.bytes)
+                *reinterpret_cast<Unit*>(static_cast<char*>(utterance) +
+                                         row * static_cast<int64_t>(at.pitch) + byte) = Unit{};
         }
     }
 }
@@ -169,11 +170,13 @@ struct Geometry {
     int length, channels, chunks;
     int slabs;    // of kRow bytes
     int cluster;  // blocks that share an utterance's slab
+    int tiles;    // consecutive tiles of a block in a round of the cluster
 };
 
 // What a thread works on.
 template <typename T> struct Place {
-    int n, m, channel, slab, rank, warp, lane;
+    int n, m, channel, rank, warp, lane;
+    int64_t first;  // the utterance's first row at the slab, in elements
     Rows rows;
     __device__ Place(const Geometry& g, const int32_t* lengths) {
         warp = threadIdx.x / kWarp;
@@ -181,11 +184,11 @@ template <typename T> struct Place {
         rank = blockIdx.x % g.cluster;
         const int unit = blockIdx.x / g.cluster;
         n = unit / g.slabs;
-        slab = unit % g.slabs * (kRow / static_cast<int>(sizeof(T)));
+        const int slab = unit % g.slabs * (kRow / static_cast<int>(sizeof(T)));
         channel = slab + lane * Lane<T>::kVec;
         m = min(max(lengths[n], 0), g.length);
         rows.pitch = static_cast<uint32_t>(g.channels) * sizeof(T);
-        rows.offset = (rank * kTile + warp * kFrames) * rows.pitch + slab * sizeof(T);
+        first = static_cast<int64_t>(n) * g.length * g.channels + slab;
         rows.bytes = min(kRow, (g.channels - slab) * static_cast<int>(sizeof(T)));
     }
 };
@@ -204,7 +207,7 @@ __device__ __forceinline__ void write_state(float* row, const float* v, int chan
 }
 
 // What the warps of a block and the blocks of a cluster tell one another. Two of each in turn,
-// so that one barrier a tile is enough.
+// so that one barrier a tile (or a round) is enough.
 struct Runs {
     float2 warp[2][kWarps][2 * kWarp];  // (A, B)
     float back[2][kWarps][2 * kWarp];   // B of the carry (backward)
@@ -219,6 +222,47 @@ constexpr int kForwardStage = 2 * kFrames * kRow, kBackwardStage = 3 * kFrames *
 constexpr int smem_bytes(int stage, bool cluster) {
     return 2 * kWarps * stage + static_cast<int>(sizeof(Runs)) +
            (cluster ? static_cast<int>(sizeof(ClusterRuns)) : 0);
+}
+
+// This block's share of a round of the cluster, in frames.
+struct Range {
+    int begin, end;
+    __device__ Range(const Geometry& g, int m, int rank, int round_start) {
+        if (g.cluster == 1) {
+            begin = 0;
+            end = m;
+        } else {
+            begin = round_start + rank * g.tiles * kTile;
+            end = max(begin, min(m, begin + g.tiles * kTile));
+        }
+    }
+};
+
+// (A, B) of this block's frames to every block of the cluster, from those of its warps'
+// consecutive parts in runs.warp[turn]: in the order of time, or against it. Returns once all
+// have arrived in others.block[which].
+template <int kVec, bool kBack>
+__device__ __forceinline__ void exchange(const Runs& runs, ClusterRuns& others, int turn,
+                                         int which, int rank, int warp, int state,
+                                         int cluster_size) {
+    auto cluster = cg::this_cluster();
+    __syncthreads();
+    float a[kVec], b[kVec];
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
+    for (int i = 0; i < kWarps; ++i)
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+            const float2 r = runs.warp[turn][kBack ? kWarps - 1 - i : i][state + v];
+            b[v] = fmaf(r.x, b[v], r.y);
+            a[v] *= r.x;
+        }
+    for (int q = warp; q < cluster_size; q += kWarps) {
+        float2* there = cluster.map_shared_rank(&others.block[which][rank][0], q);
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) there[state + v] = make_float2(a[v], b[v]);
+    }
+    cluster.sync();
 }
 
 template <typename T, int kUnit>
@@ -236,139 +280,148 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks) recurrence_kern
     const Place<T> at(geo, lengths);
     char* stage = smem + at.warp * 2 * kForwardStage;
     const int last_warp = blockDim.x / kWarp - 1, state = at.lane * kVec;
-    const int64_t first_row = static_cast<int64_t>(at.n) * geo.length * geo.channels;
     const int64_t state_row = static_cast<int64_t>(at.n) * geo.channels;
     float* saved = states == nullptr
                        ? nullptr
                        : states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels;
-    const int round = kTile * geo.cluster, in_round = at.rank * kTile + at.warp * kFrames;
 
-    auto fetch_tile = [&](int start, int which) {
-        const int64_t here = first_row + start * static_cast<int64_t>(geo.channels);
-        const int rows = at.m - start - in_round;
+    // Rows [t, end) to a stage.
+    auto fetch_rows = [&](int t, int end, int which) {
+        const int64_t here = at.first + t * static_cast<int64_t>(geo.channels);
         char* to = stage + which * kForwardStage;
-        fetch<kUnit>(to, x + here, at.rows, rows, 0u, at.lane);
+        fetch<kUnit>(to, x + here, at.rows, end - t, 0u, at.lane);
         // An infinite gate keeps the state.
-        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, rows, L::kInfinity, at.lane);
+        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, end - t, L::kInfinity, at.lane);
     };
-    if (at.m > 0) fetch_tile(0, 0);
-    commit();
-
-    float h[kVec];
-    read_state<kVec>(h, initial == nullptr ? nullptr : initial + state_row, at.channel,
+    float carry[kVec];  // before the round
+    read_state<kVec>(carry, initial == nullptr ? nullptr : initial + state_row, at.channel,
                      geo.channels);
-    if (at.warp == 0)
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) runs.behind[1][state + v] = h[v];
     // Every block of the cluster runs, and has read its state, before any writes to another.
     if (geo.cluster > 1) cg::this_cluster().sync();
 
-    int turn = 0;
-    for (int start = 0; start < at.m; start += round, turn ^= 1) {
-        if (start + round < at.m) fetch_tile(start + round, turn ^ 1);
-        commit();
-        arrived();
-        char* rows = stage + turn * kForwardStage;
-        // After each frame: the product of f, and h from 0.
-        float a[kFrames][kVec], b[kFrames][kVec];
-#pragma unroll
-        for (int i = 0; i < kFrames; ++i) {
-            float xv[kVec], gv[kVec];
-            L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
-            L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                float f, p;
-                gates(gv[v], f, p);
-                a[i][v] = i == 0 ? f : a[i - 1][v] * f;
-                b[i][v] = i == 0 ? p * xv[v] : fmaf(f, b[i - 1][v], p * xv[v]);
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < kVec; ++v)
-            runs.warp[turn][at.warp][state + v] =
-                make_float2(a[kFrames - 1][v], b[kFrames - 1][v]);
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) h[v] = runs.behind[turn ^ 1][state + v];
+    int turn = 0, which = 0;
+    const int round = geo.cluster == 1 ? geo.length : geo.cluster * geo.tiles * kTile;
+    for (int round_start = 0; round_start < at.m; round_start += round, which ^= 1) {
+        const Range range(geo, at.m, at.rank, round_start);
+        float h[kVec];
         if (geo.cluster > 1) {
-            // Every warp finds the block's run and tells its share of the cluster.
-            auto cluster = cg::this_cluster();
-            float all_a[kVec], all_b[kVec];
+            // This warp's part of the range, for its (A, B) alone.
+            const int part = geo.tiles * kFrames, from = range.begin + at.warp * part;
+            const int to = min(range.end, from + part);
+            float a[kVec], b[kVec];
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) all_a[v] = 1.0f, all_b[v] = 0.0f;
-            for (int w = 0; w <= last_warp; ++w)
+            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
+            if (from < to) fetch_rows(from, to, 0);
+            commit();
+            for (int t = from, s = 0; t < to; t += kFrames, s ^= 1) {
+                if (t + kFrames < to) fetch_rows(t + kFrames, to, s ^ 1);
+                commit();
+                arrived();
+                const char* rows = stage + s * kForwardStage;
+#pragma unroll
+                for (int i = 0; i < kFrames; ++i) {
+                    float xv[kVec], gv[kVec];
+                    L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
+                    L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
+#pragma unroll
+                    for (int v = 0; v < kVec; ++v) {
+                        float f, p;
+                        gates(gv[v], f, p);
+                        a[v] *= f;
+                        b[v] = fmaf(f, b[v], p * xv[v]);
+                    }
+                }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int v = 0; v < kVec; ++v)
+                runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
+            exchange<kVec, false>(runs, others, turn, which, at.rank, at.warp, state, geo.cluster);
+            for (int q = 0; q < geo.cluster; ++q)
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) {
+                    const float2 r = others.block[which][q][state + v];
+                    if (q == at.rank) h[v] = carry[v];
+                    carry[v] = fmaf(r.x, carry[v], r.y);
+                }
+        } else {
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) h[v] = carry[v];
+        }
+        if (at.warp == 0)
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) runs.behind[turn ^ 1][state + v] = h[v];
+
+        const int mine = range.begin + at.warp * kFrames;
+        if (mine < range.end) fetch_rows(mine, range.end, turn);
+        else fetch_rows(0, 0, turn);
+        commit();
+        for (int start = range.begin; start < range.end; start += kTile, turn ^= 1) {
+            const int t0 = start + at.warp * kFrames;
+            if (start + kTile < range.end) fetch_rows(t0 + kTile, range.end, turn ^ 1);
+            commit();
+            arrived();
+            char* rows = stage + turn * kForwardStage;
+            // After each frame: the product of f, and h from 0.
+            float a[kFrames][kVec], b[kFrames][kVec];
+#pragma unroll
+            for (int i = 0; i < kFrames; ++i) {
+                float xv[kVec], gv[kVec];
+                L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
+                L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) {
+                    float f, p;
+                    gates(gv[v], f, p);
+                    a[i][v] = i == 0 ? f : a[i - 1][v] * f;
+                    b[i][v] = i == 0 ? p * xv[v] : fmaf(f, b[i - 1][v], p * xv[v]);
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < kVec; ++v)
+                runs.warp[turn][at.warp][state + v] =
+                    make_float2(a[kFrames - 1][v], b[kFrames - 1][v]);
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) h[v] = runs.behind[turn ^ 1][state + v];
+            // The tile starts at a saved state.
+            if (saved != nullptr && at.warp == 0)
+                write_state<kVec>(saved + start / kChunk * static_cast<int64_t>(geo.channels), h,
+                                  at.channel, geo.channels);
+            for (int w = 0; w < at.warp; ++w)
 #pragma unroll
                 for (int v = 0; v < kVec; ++v) {
                     const float2 r = runs.warp[turn][w][state + v];
-                    all_b[v] = fmaf(r.x, all_b[v], r.y);
-                    all_a[v] *= r.x;
-                }
-            for (int q = at.warp; q < geo.cluster; q += last_warp + 1) {
-                float2* there = cluster.map_shared_rank(&others.block[turn][at.rank][0], q);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) there[state + v] = make_float2(all_a[v], all_b[v]);
-            }
-            cluster.sync();
-            for (int q = 0; q < at.rank; ++q)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = others.block[turn][q][state + v];
                     h[v] = fmaf(r.x, h[v], r.y);
                 }
+            // The outputs take the place of x.
+            float hv[kVec];
+#pragma unroll
+            for (int i = 0; i < kFrames; ++i) {
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) hv[v] = fmaf(a[i][v], h[v], b[i][v]);
+                reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(hv);
+            }
             if (at.warp == last_warp) {
-                float behind[kVec];
 #pragma unroll
-                for (int v = 0; v < kVec; ++v) behind[v] = h[v];
-                for (int q = at.rank; q < geo.cluster; ++q)
+                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = hv[v];
+                if (geo.cluster == 1)
 #pragma unroll
-                    for (int v = 0; v < kVec; ++v) {
-                        const float2 r = others.block[turn][q][state + v];
-                        behind[v] = fmaf(r.x, behind[v], r.y);
-                    }
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = behind[v];
+                    for (int v = 0; v < kVec; ++v) carry[v] = hv[v];
             }
+            __syncwarp();
+            store<kUnit>(out + at.first + t0 * static_cast<int64_t>(geo.channels), rows, at.rows,
+                         range.end - t0, at.lane);
+            __syncwarp();
         }
-        // The tile starts at a saved state.
-        if (saved != nullptr && at.warp == 0 && start + in_round < at.m)
-            write_state<kVec>(saved + (start + in_round) / kChunk * static_cast<int64_t>(geo.channels),
-                              h, at.channel, geo.channels);
-        for (int w = 0; w < at.warp; ++w)
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                const float2 r = runs.warp[turn][w][state + v];
-                h[v] = fmaf(r.x, h[v], r.y);
-            }
-        // The outputs take the place of x.
-        float hv[kVec];
-#pragma unroll
-        for (int i = 0; i < kFrames; ++i) {
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) hv[v] = fmaf(a[i][v], h[v], b[i][v]);
-            reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(hv);
-        }
-        if (geo.cluster == 1 && at.warp == last_warp) {
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = hv[v];
-        }
-        __syncwarp();
-        store<kUnit>(out + first_row + start * static_cast<int64_t>(geo.channels), rows, at.rows,
-                     at.m - start - in_round, at.lane);
-        __syncwarp();
     }
-    if (at.rank == 0 && at.warp == last_warp) {
-        if (at.m > 0)  // this warp wrote it
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) h[v] = runs.behind[turn ^ 1][state + v];
-        write_state<kVec>(final_state + state_row, h, at.channel, geo.channels);
-    }
-    const int first = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
-    zero_rows<kUnit>(out + first_row, at.slab * static_cast<uint32_t>(sizeof(T)), at.rows.pitch,
-                     at.rows.bytes, at.m, geo.length, first, by, at.lane);
+    if (at.rank == 0 && at.warp == last_warp)
+        write_state<kVec>(final_state + state_row, carry, at.channel, geo.channels);
+    const int index = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
+    zero_rows<kUnit>(out + at.first, at.rows, at.m, geo.length, index, by, at.lane);
     if (saved != nullptr) {
         const float zero[2] = {0.0f, 0.0f};
-        for (int j = (at.m + kChunk - 1) / kChunk + first; j < geo.chunks; j += by)
+        for (int j = (at.m + kChunk - 1) / kChunk + index; j < geo.chunks; j += by)
             write_state<kVec>(saved + j * static_cast<int64_t>(geo.channels), zero, at.channel,
                               geo.channels);
     }
@@ -390,169 +443,185 @@ __global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks) recurrence_bac
     const Place<T> at(geo, lengths);
     char* stage = smem + at.warp * 2 * kBackwardStage;
     const int last_warp = blockDim.x / kWarp - 1, state = at.lane * kVec;
-    const int64_t first_row = static_cast<int64_t>(at.n) * geo.length * geo.channels;
     const int64_t state_row = static_cast<int64_t>(at.n) * geo.channels;
     const float* saved = states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels;
-    const int round = kTile * geo.cluster, in_round = at.rank * kTile + at.warp * kFrames;
 
-    auto fetch_tile = [&](int start, int which) {
-        const int64_t here = first_row + start * static_cast<int64_t>(geo.channels);
-        const int rows = at.m - start - in_round;
+    // Rows [t, end) to a stage: x, gate, dout; the scan for (A, B) alone needs no x.
+    auto fetch_rows = [&](int t, int end, int which, bool with_x) {
+        const int64_t here = at.first + t * static_cast<int64_t>(geo.channels);
         char* to = stage + which * kBackwardStage;
-        fetch<kUnit>(to, x + here, at.rows, rows, 0u, at.lane);
-        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, rows, L::kInfinity, at.lane);
-        fetch<kUnit>(to + 2 * kFrames * kRow, dout + here, at.rows, rows, 0u, at.lane);
+        if (with_x) fetch<kUnit>(to, x + here, at.rows, end - t, 0u, at.lane);
+        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, end - t, L::kInfinity, at.lane);
+        fetch<kUnit>(to + 2 * kFrames * kRow, dout + here, at.rows, end - t, 0u, at.lane);
     };
-    const int last = (at.m - 1) / round * round;
-    if (at.m > 0) fetch_tile(last, 0);
-    commit();
-
-    float c[kVec];
-    read_state<kVec>(c, dfinal == nullptr ? nullptr : dfinal + state_row, at.channel,
+    float carry[kVec];  // behind the round
+    read_state<kVec>(carry, dfinal == nullptr ? nullptr : dfinal + state_row, at.channel,
                      geo.channels);
-    if (at.warp == 0)
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) runs.behind[1][state + v] = c[v];
     if (geo.cluster > 1) cg::this_cluster().sync();
 
-    int turn = 0;
-    for (int start = at.m > 0 ? last : -1; start >= 0; start -= round, turn ^= 1) {
-        float h[kVec];  // the saved state before the tile
-        read_state<kVec>(h, start + at.rank * kTile < at.m
-                                ? saved + (start / kChunk + at.rank) * static_cast<int64_t>(geo.channels)
-                                : nullptr, at.channel, geo.channels);
-        if (start >= round) fetch_tile(start - round, turn ^ 1);
-        commit();
-        arrived();
-        char* rows = stage + turn * kBackwardStage;
-        float f[kFrames][kVec], p[kFrames][kVec];
-        float a[kVec], b[kVec], back[kVec];
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f, back[v] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kFrames; ++i) {
-            float xv[kVec], gv[kVec];
-            L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
-            L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                gates(gv[v], f[i][v], p[i][v]);
-                a[v] *= f[i][v];
-                b[v] = fmaf(f[i][v], b[v], p[i][v] * xv[v]);
-            }
-        }
-#pragma unroll
-        for (int i = kFrames - 1; i >= 0; --i) {
-            float dv[kVec];
-            L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], dv);
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) back[v] = f[i][v] * (dv[v] + back[v]);
-        }
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-            runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
-            runs.back[turn][at.warp][state + v] = back[v];
-        }
-        __syncthreads();
-        for (int w = 0; w < at.warp; ++w)
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                const float2 r = runs.warp[turn][w][state + v];
-                h[v] = fmaf(r.x, h[v], r.y);
-            }
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) c[v] = runs.behind[turn ^ 1][state + v];
+    int turn = 0, which = 0;
+    const int round = geo.cluster == 1 ? geo.length : geo.cluster * geo.tiles * kTile;
+    for (int round_start = at.m > 0 ? (at.m - 1) / round * round : -1; round_start >= 0;
+         round_start -= round, which ^= 1) {
+        const Range range(geo, at.m, at.rank, round_start);
+        float c[kVec];
         if (geo.cluster > 1) {
-            auto cluster = cg::this_cluster();
-            float all_a[kVec], all_c[kVec];
+            const int part = geo.tiles * kFrames, from = range.begin + at.warp * part;
+            const int to = min(range.end, from + part);
+            float a[kVec], b[kVec];
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) all_a[v] = 1.0f, all_c[v] = 0.0f;
-            for (int w = last_warp; w >= 0; --w)
+            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
+            const int last = from + (to - from - 1) / kFrames * kFrames;
+            if (from < to) fetch_rows(last, to, 0, false);
+            commit();
+            for (int t = from < to ? last : from - 1, s = 0; t >= from; t -= kFrames, s ^= 1) {
+                if (t > from) fetch_rows(t - kFrames, to, s ^ 1, false);
+                commit();
+                arrived();
+                const char* rows = stage + s * kBackwardStage;
 #pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float r = runs.warp[turn][w][state + v].x;
-                    all_c[v] = fmaf(r, all_c[v], runs.back[turn][w][state + v]);
-                    all_a[v] *= r;
-                }
-            for (int q = at.warp; q < geo.cluster; q += last_warp + 1) {
-                float2* there = cluster.map_shared_rank(&others.block[turn][at.rank][0], q);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) there[state + v] = make_float2(all_a[v], all_c[v]);
-            }
-            cluster.sync();
-            for (int q = geo.cluster - 1; q > at.rank; --q)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = others.block[turn][q][state + v];
-                    c[v] = fmaf(r.x, c[v], r.y);
-                }
-            if (at.warp == 0) {
-                float behind[kVec];
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) behind[v] = c[v];
-                for (int q = at.rank; q >= 0; --q)
+                for (int i = kFrames - 1; i >= 0; --i) {
+                    float gv[kVec], dv[kVec];
+                    L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
+                    L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane],
+                              dv);
 #pragma unroll
                     for (int v = 0; v < kVec; ++v) {
-                        const float2 r = others.block[turn][q][state + v];
-                        behind[v] = fmaf(r.x, behind[v], r.y);
+                        float f, p;
+                        gates(gv[v], f, p);
+                        a[v] *= f;
+                        b[v] = f * (dv[v] + b[v]);
                     }
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = behind[v];
+                }
+                __syncwarp();
             }
-        }
-        for (int w = last_warp; w > at.warp; --w)
 #pragma unroll
             for (int v = 0; v < kVec; ++v)
-                c[v] = fmaf(runs.warp[turn][w][state + v].x, c[v], runs.back[turn][w][state + v]);
-        float away[kFrames][kVec];  // h[t-1] - x[t]
+                runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
+            exchange<kVec, true>(runs, others, turn, which, at.rank, at.warp, state, geo.cluster);
+            for (int q = geo.cluster - 1; q >= 0; --q)
 #pragma unroll
-        for (int i = 0; i < kFrames; ++i) {
-            float xv[kVec];
-            L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
+                for (int v = 0; v < kVec; ++v) {
+                    const float2 r = others.block[which][q][state + v];
+                    if (q == at.rank) c[v] = carry[v];
+                    carry[v] = fmaf(r.x, carry[v], r.y);
+                }
+        } else {
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) c[v] = carry[v];
+        }
+        if (at.warp == 0)
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) runs.behind[turn ^ 1][state + v] = c[v];
+
+        const int tiles = (range.end - range.begin + kTile - 1) / kTile;
+        const int last = range.begin + (tiles - 1) * kTile;
+        if (tiles > 0 && last + at.warp * kFrames < range.end)
+            fetch_rows(last + at.warp * kFrames, range.end, turn, true);
+        else
+            fetch_rows(0, 0, turn, true);
+        commit();
+        for (int i = 0, start = last; i < tiles; ++i, start -= kTile, turn ^= 1) {
+            const int t0 = start + at.warp * kFrames;
+            float h[kVec];  // the saved state before the tile
+            read_state<kVec>(h, saved + start / kChunk * static_cast<int64_t>(geo.channels),
+                             at.channel, geo.channels);
+            if (i + 1 < tiles) fetch_rows(t0 - kTile, range.end, turn ^ 1, true);
+            commit();
+            arrived();
+            char* rows = stage + turn * kBackwardStage;
+            float f[kFrames][kVec], p[kFrames][kVec];
+            float a[kVec], b[kVec], back[kVec];
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f, back[v] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFrames; ++i) {
+                float xv[kVec], gv[kVec];
+                L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
+                L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) {
+                    gates(gv[v], f[i][v], p[i][v]);
+                    a[v] *= f[i][v];
+                    b[v] = fmaf(f[i][v], b[v], p[i][v] * xv[v]);
+                }
+            }
+#pragma unroll
+            for (int i = kFrames - 1; i >= 0; --i) {
+                float dv[kVec];
+                L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], dv);
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) back[v] = f[i][v] * (dv[v] + back[v]);
+            }
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
-                away[i][v] = h[v] - xv[v];
-                h[v] = fmaf(f[i][v], h[v], p[i][v] * xv[v]);
+                runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
+                runs.back[turn][at.warp][state + v] = back[v];
             }
-        }
-        // dx takes the place of x, dgate that of gate.
+            __syncthreads();
+            for (int w = 0; w < at.warp; ++w)
 #pragma unroll
-        for (int i = kFrames - 1; i >= 0; --i) {
-            float gx[kVec], gg[kVec];
-            L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], gx);
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                const float total = gx[v] + c[v];
-                gx[v] = p[i][v] * total;
-                gg[v] = f[i][v] * gx[v] * away[i][v];
-                c[v] = f[i][v] * total;
-            }
-            reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(gx);
-            reinterpret_cast<Raw*>(rows + (kFrames + i) * kRow)[at.lane] = L::pack(gg);
-        }
-        if (geo.cluster == 1 && at.warp == 0) {
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = c[v];
-        }
-        __syncwarp();
-        const int64_t here = first_row + start * static_cast<int64_t>(geo.channels);
-        store<kUnit>(dx + here, rows, at.rows, at.m - start - in_round, at.lane);
-        store<kUnit>(dgate + here, rows + kFrames * kRow, at.rows, at.m - start - in_round, at.lane);
-        __syncwarp();
-    }
-    if (at.rank == 0 && at.warp == 0) {
-        if (at.m > 0)  // this warp wrote it
+                for (int v = 0; v < kVec; ++v) {
+                    const float2 r = runs.warp[turn][w][state + v];
+                    h[v] = fmaf(r.x, h[v], r.y);
+                }
 #pragma unroll
             for (int v = 0; v < kVec; ++v) c[v] = runs.behind[turn ^ 1][state + v];
-        write_state<kVec>(dinitial + state_row, c, at.channel, geo.channels);
+            for (int w = last_warp; w > at.warp; --w)
+#pragma unroll
+                for (int v = 0; v < kVec; ++v)
+                    c[v] = fmaf(runs.warp[turn][w][state + v].x, c[v],
+                                runs.back[turn][w][state + v]);
+            float away[kFrames][kVec];  // h[t-1] - x[t]
+#pragma unroll
+            for (int i = 0; i < kFrames; ++i) {
+                float xv[kVec];
+                L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) {
+                    away[i][v] = h[v] - xv[v];
+                    h[v] = fmaf(f[i][v], h[v], p[i][v] * xv[v]);
+                }
+            }
+            // dx takes the place of x, dgate that of gate.
+#pragma unroll
+            for (int i = kFrames - 1; i >= 0; --i) {
+                float gx[kVec], gg[kVec];
+                L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], gx);
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) {
+                    const float total = gx[v] + c[v];
+                    gx[v] = p[i][v] * total;
+                    gg[v] = f[i][v] * gx[v] * away[i][v];
+                    c[v] = f[i][v] * total;
+                }
+                reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(gx);
+                reinterpret_cast<Raw*>(rows + (kFrames + i) * kRow)[at.lane] = L::pack(gg);
+            }
+            if (at.warp == 0) {
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = c[v];
+                if (geo.cluster == 1)
+#pragma unroll
+                    for (int v = 0; v < kVec; ++v) carry[v] = c[v];
+            }
+            __syncwarp();
+            const int64_t here = at.first + t0 * static_cast<int64_t>(geo.channels);
+            store<kUnit>(dx + here, rows, at.rows, range.end - t0, at.lane);
+            store<kUnit>(dgate + here, rows + kFrames * kRow, at.rows, range.end - t0, at.lane);
+            __syncwarp();
+        }
     }
-    const int first = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
+    if (at.rank == 0 && at.warp == 0)
+        write_state<kVec>(dinitial + state_row, carry, at.channel, geo.channels);
+    const int index = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
     for (T* grad : {dx, dgate})
-        zero_rows<kUnit>(grad + first_row, at.slab * static_cast<uint32_t>(sizeof(T)),
-                         at.rows.pitch, at.rows.bytes, at.m, geo.length, first, by, at.lane);
+        zero_rows<kUnit>(grad + at.first, at.rows, at.m, geo.length, index, by, at.lane);
 }
 
 // ---- launch --------------------------------------------------------------------------------
+
+constexpr int64_t kClusterBlocks = 1, kRoundBytes = 32 << 20;
 
 struct Shape {
     Geometry geo;
@@ -563,13 +632,14 @@ Shape shape_of(int batch, int length, int channels, int chunks, int row_channels
     Shape s{};
     const int slabs = (channels + row_channels - 1) / row_channels;
     const int64_t units = static_cast<int64_t>(batch) * slabs;
-    // Blocks for three on every multiprocessor, in rounds of the same number of tiles.
-    const int64_t wanted = (3LL * sm_count() + units - 1) / units;
+    const int64_t wanted = (kClusterBlocks * sm_count() + units - 1) / units;
     int cluster = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>(wanted, std::min(chunks, kMaxCluster))));
-    const int rounds = (chunks + cluster - 1) / cluster;
-    cluster = (chunks + rounds - 1) / rounds;
-    s.geo = {length, channels, chunks, slabs, cluster};
+    // Rounds whose rows stay in L2 from the first reading to the second.
+    const int64_t most = std::max<int64_t>(1, kRoundBytes / (units * cluster * kTile * kRow));
+    const int64_t each = (chunks + cluster - 1) / cluster, rounds = (each + most - 1) / most;
+    const int tiles = static_cast<int>((each + rounds - 1) / rounds);
+    s.geo = {length, channels, chunks, slabs, cluster, tiles};
     s.blocks = static_cast<int>(units * cluster);
     s.threads = std::min(kWarps, (length + kFrames - 1) / kFrames) * kWarp;
     return s;
