@@ -1,203 +1,312 @@
-// Group norm with activation over [N, T, C] (channels last), forward and backward.
+// Group norm with activation over [N, T, C] (channels last).
 //
 // Over the M valid frames of an utterance and the Cg channels of a group:
 //   mean = sum x / (M Cg), var = sum (x - mean)^2 / (M Cg), rstd = (var + eps)^-1/2,
-//   xhat = (x - mean) rstd, z = weight xhat + bias, out = act(z);
-//   dz = dout act'(z), dbias = sum dz, dweight = sum dz xhat (over every valid frame),
-//   dx = rstd (weight dz - (s1 + xhat s2) / (M Cg)),
-//   s1 = sum weight dz, s2 = sum weight dz xhat (over the group).
+//   out = act((x - mean) rstd weight + bias).
 //
-// One block per utterance and group, one thread per element in turn; the parameters'
-// gradients by one block per channel.
-#include <cstdint>
-
-#include "../../include/fga_convolution.h"
-#include "fga_common.cuh"
+// The rows of an utterance's slab stay on chip between the statistics and the output: a block
+// keeps them in shared memory, a cluster of up to 16 blocks where one is not enough. Every
+// thread reads only vectors that it copied itself, so the tile needs no barrier. A thread
+// takes mean and sum of squares about it over its own values (two passes over shared memory),
+// and pairs of (mean, squares) merge exactly as the two-pass formula would have it:
+//   mean = sum n_i mean_i / sum n_i, squares = sum (squares_i + n_i (mean_i - mean)^2);
+// no difference of large sums is taken. What no cluster holds is done in two launches, the
+// first of which leaves each block's (mean, squares) in the workspace.
 #include "fga_kernels.h"
+#include "group_norm.cuh"
 
 namespace fga {
 namespace {
 
-constexpr int kThreads = 256;
+using namespace group_norm;
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+constexpr int kTileBytes = 48 << 10;
 
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == FGA_ACTIVATION_SILU) return z * sigmoid(z);
-    if (act == FGA_ACTIVATION_SWOOSH_R) {
-        const float v = z - 1.0f;
-        return fmaxf(v, 0.0f) + log1pf(__expf(-fabsf(v))) - 0.08f * z - 0.313261687f;
-    }
-    return z;
-}
-
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == FGA_ACTIVATION_SILU) {
-        const float s = sigmoid(z);
-        return s * (1.0f + z * (1.0f - s));
-    }
-    if (act == FGA_ACTIVATION_SWOOSH_R) return sigmoid(z - 1.0f) - 0.08f;
-    return 1.0f;
-}
-
-// Sum over the block, the same value in every thread; `red` holds one float per warp.
-__device__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
-    __syncthreads();
-    if (threadIdx.x % kWarp == 0) red[threadIdx.x / kWarp] = v;
-    __syncthreads();
-    float total = 0.0f;
-    for (int i = 0; i < kThreads / kWarp; ++i) total += red[i];
-    return total;
-}
-
-__device__ __forceinline__ int valid_frames(const int32_t* lengths, int n, int length) {
-    return min(max(lengths[n], 0), length);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) group_norm_kernel(
-    const T* __restrict__ x, const int32_t* __restrict__ lengths, const T* __restrict__ weight,
-    const T* __restrict__ bias, T* __restrict__ out, float* __restrict__ mean_out,
-    float* __restrict__ rstd_out, int length, int channels, int groups, float eps, int act) {
-    __shared__ float red[kThreads / kWarp];
-    const int n = blockIdx.x / groups, g = blockIdx.x % groups, cg = channels / groups;
-    const int m = valid_frames(lengths, n, length);
-    const int64_t base = static_cast<int64_t>(n) * length * channels + g * cg;
-    const int64_t count = static_cast<int64_t>(m) * cg, all = static_cast<int64_t>(length) * cg;
-    const float inv = count > 0 ? 1.0f / static_cast<float>(count) : 0.0f;
+// Merges (mean, squares) over `items` entries by one warp; entry(i) gives the count, mean and
+// squares of item i. Every lane returns the whole's.
+template <typename Entry>
+__device__ __forceinline__ float2 merge(int items, float total, Entry entry) {
+    const int lane = threadIdx.x % kWarp;
     float sum = 0.0f;
-    for (int64_t i = threadIdx.x; i < count; i += kThreads)
-        sum += to_f32<T>(x[base + i / cg * channels + i % cg]);
-    const float mean = block_sum(sum, red) * inv;
-    float square = 0.0f;
-    for (int64_t i = threadIdx.x; i < count; i += kThreads) {
-        const float d = to_f32<T>(x[base + i / cg * channels + i % cg]) - mean;
-        square += d * d;
+    for (int i = lane; i < items; i += kWarp) {
+        const float3 v = entry(i);
+        sum = fmaf(v.x, v.y, sum);
     }
-    const float rstd = 1.0f / sqrtf(block_sum(square, red) * inv + eps);
-    if (threadIdx.x == 0) {
-        if (mean_out != nullptr) mean_out[blockIdx.x] = mean;
-        if (rstd_out != nullptr) rstd_out[blockIdx.x] = rstd;
+    const float mean = total > 0.0f ? warp_sum(sum) / total : 0.0f;
+    float squares = 0.0f;
+    for (int i = lane; i < items; i += kWarp) {
+        const float3 v = entry(i);
+        const float d = v.y - mean;
+        squares += fmaf(v.x * d, d, v.z);
     }
-    for (int64_t i = threadIdx.x; i < all; i += kThreads) {
-        const int64_t at = base + i / cg * channels + i % cg;
-        const int c = g * cg + static_cast<int>(i % cg);
-        float v = 0.0f;
-        if (i < count)
-            v = activate((to_f32<T>(x[at]) - mean) * rstd * to_f32<T>(weight[c]) +
-                             to_f32<T>(bias[c]), act);
-        out[at] = from_f32<T>(v);
-    }
+    return make_float2(mean, warp_sum(squares));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) group_norm_backward_kernel(
-    const T* __restrict__ dout, const T* __restrict__ x, const int32_t* __restrict__ lengths,
-    const T* __restrict__ weight, const T* __restrict__ bias, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, T* __restrict__ dx, int length, int channels, int groups,
-    int act) {
-    __shared__ float red[kThreads / kWarp];
-    const int n = blockIdx.x / groups, g = blockIdx.x % groups, cg = channels / groups;
-    const int m = valid_frames(lengths, n, length);
-    const int64_t base = static_cast<int64_t>(n) * length * channels + g * cg;
-    const int64_t count = static_cast<int64_t>(m) * cg, all = static_cast<int64_t>(length) * cg;
-    const float inv = count > 0 ? 1.0f / static_cast<float>(count) : 0.0f;
-    const float mean = mean_in[blockIdx.x], rstd = rstd_in[blockIdx.x];
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int64_t i = threadIdx.x; i < count; i += kThreads) {
-        const int64_t at = base + i / cg * channels + i % cg;
-        const int c = g * cg + static_cast<int>(i % cg);
-        const float w = to_f32<T>(weight[c]), xhat = (to_f32<T>(x[at]) - mean) * rstd;
-        const float d = w * to_f32<T>(dout[at]) * slope(xhat * w + to_f32<T>(bias[c]), act);
-        s1 += d;
-        s2 += d * xhat;
-    }
-    s1 = block_sum(s1, red) * inv;
-    s2 = block_sum(s2, red) * inv;
-    for (int64_t i = threadIdx.x; i < all; i += kThreads) {
-        const int64_t at = base + i / cg * channels + i % cg;
-        const int c = g * cg + static_cast<int>(i % cg);
-        float v = 0.0f;
-        if (i < count) {
-            const float w = to_f32<T>(weight[c]), xhat = (to_f32<T>(x[at]) - mean) * rstd;
-            const float d = w * to_f32<T>(dout[at]) * slope(xhat * w + to_f32<T>(bias[c]), act);
-            v = rstd * (d - s1 - xhat * s2);
+// (mean, squares) of every group of the slab over this block's rows, which its threads have in
+// `tile`, to moments[group]. `part` holds an entry per thread (and channel, if not kWhole).
+template <typename T, bool kWhole>
+__device__ __forceinline__ void block_moments(const uint4* tile, float2* part, float2* moments,
+                                              const Place<T>& p, const Geometry& g) {
+    constexpr int kValues = kWhole ? 1 : kVec<T>;
+    const int mine = p.rows_of(p.row);
+    float mean[kValues], squares[kValues];
+#pragma unroll
+    for (int e = 0; e < kValues; ++e) mean[e] = 0.0f, squares[e] = 0.0f;
+    if (mine > 0) {
+        const uint4* at = tile + p.row * p.lanes + p.lane;
+        const int pitch = p.step * p.lanes;
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i) {
+            float v[kVec<T>];
+            unpack<T>(at[i * pitch], v);
+            if constexpr (kWhole) {
+                float s = 0.0f;
+#pragma unroll
+                for (int e = 0; e < kVec<T>; ++e) s += v[e];
+                mean[0] += s;
+            } else {
+#pragma unroll
+                for (int e = 0; e < kVec<T>; ++e) mean[e] += v[e];
+            }
         }
-        dx[at] = from_f32<T>(v);
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) group_norm_parameters_kernel(
-    const T* __restrict__ dout, const T* __restrict__ x, const int32_t* __restrict__ lengths,
-    const T* __restrict__ weight, const T* __restrict__ bias, const float* __restrict__ mean,
-    const float* __restrict__ rstd, T* __restrict__ dweight, T* __restrict__ dbias, int batch,
-    int length, int channels, int groups, int act) {
-    __shared__ float red[kThreads / kWarp];
-    const int c = blockIdx.x, g = c / (channels / groups);
-    const float w = to_f32<T>(weight[c]), b = to_f32<T>(bias[c]);
-    float sw = 0.0f, sb = 0.0f;
-    for (int n = 0; n < batch; ++n) {
-        const int m = valid_frames(lengths, n, length);
-        const float mu = mean[static_cast<int64_t>(n) * groups + g];
-        const float r = rstd[static_cast<int64_t>(n) * groups + g];
-        for (int t = threadIdx.x; t < m; t += kThreads) {
-            const int64_t at = (static_cast<int64_t>(n) * length + t) * channels + c;
-            const float xhat = (to_f32<T>(x[at]) - mu) * r;
-            const float d = to_f32<T>(dout[at]) * slope(xhat * w + b, act);
-            sb += d;
-            sw += d * xhat;
+        const float inv = 1.0f / static_cast<float>(mine * (kWhole ? kVec<T> : 1));
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) mean[e] *= inv;
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i) {
+            float v[kVec<T>];
+            unpack<T>(at[i * pitch], v);
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e) {
+                const float d = v[e] - mean[kWhole ? 0 : e];
+                squares[kWhole ? 0 : e] = fmaf(d, d, squares[kWhole ? 0 : e]);
+            }
         }
     }
-    sw = block_sum(sw, red);
-    sb = block_sum(sb, red);
-    if (threadIdx.x == 0) {
-        dweight[c] = from_f32<T>(sw);
-        dbias[c] = from_f32<T>(sb);
+    const int columns = p.lanes * kValues;
+    if (p.row < p.step)
+#pragma unroll
+        for (int e = 0; e < kValues; ++e)
+            part[p.row * columns + p.lane * kValues + e] = make_float2(mean[e], squares[e]);
+    __syncthreads();
+    // A warp per group: its columns of every row of threads.
+    const int per_group = kWhole ? p.channels / p.groups / kVec<T> : p.channels / p.groups;
+    const int items = min(p.step, p.rows) * per_group;
+    const float total = static_cast<float>(p.rows) * static_cast<float>(p.channels / p.groups);
+    for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+        const float2 r = merge(items, total, [&](int i) {
+            const int row = i / per_group;
+            const float2 v = part[row * columns + j * per_group + i % per_group];
+            return make_float3(static_cast<float>(p.rows_of(row) * (kWhole ? kVec<T> : 1)), v.x, v.y);
+        });
+        if (threadIdx.x % kWarp == 0) moments[j] = r;
     }
 }
 
-template <typename T>
-cudaError_t forward(const GroupNormProblem& p, cudaStream_t s) {
-    group_norm_kernel<T><<<p.batch * p.groups, kThreads, 0, s>>>(
-        static_cast<const T*>(p.x), p.valid_lengths, static_cast<const T*>(p.weight),
-        static_cast<const T*>(p.bias), static_cast<T*>(p.output), p.mean, p.rstd, p.length,
-        p.channels, p.groups, p.eps, p.activation);
-    return cudaGetLastError();
+// A column's parameters: out = act((x - mean) scale + bias).
+template <typename T, bool kWhole> struct Column {
+    static constexpr int kMeans = kWhole ? 1 : kVec<T>;
+    float mean[kMeans], scale[kVec<T>], bias[kVec<T>];
+    // `stats`: (mean, rstd) of the slab's groups.
+    template <bool kAligned>
+    __device__ __forceinline__ void read(const T* w, const T* b, const float2* stats,
+                                         const Place<T>& p, const Geometry& g) {
+        unpack<T>(load<T, kAligned>(w + p.channel(), p.count), scale);
+        unpack<T>(load<T, kAligned>(b + p.channel(), p.count), bias);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e) {
+            const float2 s = stats[p.group_of(kWhole ? 0 : e, g)];
+            mean[kWhole ? 0 : e] = s.x;
+            scale[e] *= s.y;
+        }
+    }
+    __device__ __forceinline__ uint4 apply(const uint4& r, int act) const {
+        float v[kVec<T>];
+        unpack<T>(r, v);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e)
+            v[e] = fmaf(v[e] - mean[kWhole ? 0 : e], scale[e], bias[e]);
+        activate(v, act);
+        return pack<T>(v);
+    }
+};
+
+__device__ __forceinline__ float2 to_stats(float2 moments, float total, float eps) {
+    return make_float2(moments.x, 1.0f / sqrtf((total > 0.0f ? moments.y / total : 0.0f) + eps));
 }
 
-template <typename T>
-cudaError_t backward(const GroupNormBackwardProblem& p, cudaStream_t s) {
-    const T *dout = static_cast<const T*>(p.grad_output), *x = static_cast<const T*>(p.x),
-            *w = static_cast<const T*>(p.weight), *b = static_cast<const T*>(p.bias);
-    group_norm_backward_kernel<T><<<p.batch * p.groups, kThreads, 0, s>>>(
-        dout, x, p.valid_lengths, w, b, p.mean, p.rstd, static_cast<T*>(p.grad_x), p.length,
-        p.channels, p.groups, p.activation);
-    group_norm_parameters_kernel<T><<<p.channels, kThreads, 0, s>>>(
-        dout, x, p.valid_lengths, w, b, p.mean, p.rstd, static_cast<T*>(p.grad_weight),
-        static_cast<T*>(p.grad_bias), p.batch, p.length, p.channels, p.groups, p.activation);
-    return cudaGetLastError();
+template <typename T> struct Tensors {
+    const T* x;
+    const int32_t* lengths;
+    const T* weight;
+    const T* bias;
+    T* out;
+    float* mean;  // [N, G] or null
+    float* rstd;
+};
+
+// kPartial: leaves the blocks' moments in `partial` [N, G, parts * blocks], nothing else.
+template <typename T, bool kAligned, bool kWhole, bool kPartial>
+__global__ void __launch_bounds__(kThreads, 4)
+    group_norm_kernel(Tensors<T> t, float2* __restrict__ partial, Geometry g, float eps, int act) {
+    extern __shared__ __align__(16) uint4 tile[];
+    __shared__ float2 part[kWhole ? kThreads : kThreads * kVec<T>];
+    __shared__ float2 moments[kMaxSlabGroups];
+    __shared__ float2 gathered[kPartial ? 1 : kMaxCluster][kMaxSlabGroups];
+    const Place<T> p = Place<T>::template make<kPartial>(g, t.lengths);
+    const int mine = p.rows_of(p.row), pitch = p.step * p.lanes;
+    uint4* at = tile + p.row * p.lanes + p.lane;
+    const int64_t stride = static_cast<int64_t>(p.step) * g.channels;
+    {
+        const T* from = t.x + p.at(g, p.begin + p.row);
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i, from += stride)
+            stage<T, kAligned>(at + i * pitch, from, p.count);
+    }
+    arrived();
+    block_moments<T, kWhole>(tile, part, moments, p, g);
+    __syncthreads();
+    const float width = static_cast<float>(g.group_channels);
+    if constexpr (kPartial) {
+        const int slots = g.parts * g.blocks;
+        if (threadIdx.x < p.groups)
+            partial[(static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x) * slots +
+                    p.slab % g.parts * g.blocks + p.block] = moments[threadIdx.x];
+    } else {
+        const float total = static_cast<float>(p.m) * width;
+        if (g.blocks > 1) {
+            auto cluster = cg::this_cluster();
+            cluster.sync();  // every block runs, and may be written to
+            for (int i = threadIdx.x; i < g.blocks * p.groups; i += kThreads)
+                *cluster.map_shared_rank(&gathered[p.block][i % p.groups], i / p.groups) =
+                    moments[i % p.groups];
+            cluster.sync();
+            const int each = (p.m + g.blocks - 1) / g.blocks;
+            for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+                const float2 r = merge(g.blocks, total, [&](int i) {
+                    const float2 v = gathered[i][j];
+                    return make_float3(static_cast<float>(max(0, min(each, p.m - i * each))) * width,
+                                       v.x, v.y);
+                });
+                if (threadIdx.x % kWarp == 0) moments[j] = r;
+            }
+            __syncthreads();
+        }
+        if (threadIdx.x < p.groups) {
+            const float2 s = to_stats(moments[threadIdx.x], total, eps);
+            moments[threadIdx.x] = s;
+            if (p.block == 0) {
+                const int64_t i = static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x;
+                if (t.mean != nullptr) t.mean[i] = s.x;
+                if (t.rstd != nullptr) t.rstd[i] = s.y;
+            }
+        }
+        __syncthreads();
+        if (mine > 0) {
+            Column<T, kWhole> column;
+            column.template read<kAligned>(t.weight, t.bias, moments, p, g);
+            T* to = t.out + p.at(g, p.begin + p.row);
+#pragma unroll 2
+            for (int i = 0; i < mine; ++i, to += stride)
+                store<T, kAligned>(to, column.apply(at[i * pitch], act), p.count);
+        }
+        zero_padding<T, kAligned>(t.out, p, g);
+    }
+}
+
+// The second launch: merges the partial moments and applies them.
+template <typename T, bool kAligned, bool kWhole>
+__global__ void __launch_bounds__(kThreads, 4)
+    group_norm_apply_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g, float eps,
+                            int act) {
+    __shared__ float2 stats[kMaxSlabGroups];
+    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
+    const int slots = g.parts * g.blocks;
+    const float total = static_cast<float>(p.m) * static_cast<float>(g.group_channels);
+    for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+        const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group + j;
+        const float2* mine = partial + group * slots;
+        const float2 r = merge(slots, total, [&](int i) {
+            const int rows = max(0, min(g.rows, p.m - i % g.blocks * g.rows));
+            const int wide = g.parts > 1 ? min(g.part_channels,
+                                               g.group_channels - i / g.blocks * g.part_channels)
+                                         : g.group_channels;
+            const float2 v = mine[i];
+            return make_float3(static_cast<float>(rows) * static_cast<float>(wide), v.x, v.y);
+        });
+        if (threadIdx.x % kWarp == 0) {
+            const float2 s = to_stats(r, total, eps);
+            stats[j] = s;
+            if (p.block == 0 && p.slab % g.parts == 0) {
+                if (t.mean != nullptr) t.mean[group] = s.x;
+                if (t.rstd != nullptr) t.rstd[group] = s.y;
+            }
+        }
+    }
+    __syncthreads();
+    const int mine = p.rows_of(p.row);
+    if (mine > 0) {
+        Column<T, kWhole> column;
+        column.template read<kAligned>(t.weight, t.bias, stats, p, g);
+        const int64_t stride = static_cast<int64_t>(p.step) * g.channels;
+        const int64_t first = p.at(g, p.begin + p.row);
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i)
+            store<T, kAligned>(t.out + first + i * stride,
+                               column.apply(load<T, kAligned>(t.x + first + i * stride, p.count), act),
+                               p.count);
+    }
+    zero_padding<T, kAligned>(t.out, p, g);
+}
+
+template <typename T, bool kAligned, bool kWhole>
+cudaError_t run(const GroupNormProblem& p, const Shape& s, cudaStream_t stream) {
+    static SmemAttr resident, partial, apply;
+    const Tensors<T> t{static_cast<const T*>(p.x), p.valid_lengths, static_cast<const T*>(p.weight),
+                       static_cast<const T*>(p.bias), static_cast<T*>(p.output), p.mean, p.rstd};
+    const Geometry& g = s.geo;
+    const int lanes = (std::min(g.group_channels * g.slab_groups, g.part_channels) + kVec<T> - 1) /
+                      kVec<T>;
+    const int smem = g.rows * lanes * 16, most = kTileBytes + kThreads * 16;
+    float2* ws = static_cast<float2*>(p.workspace);
+    if (!s.split)
+        return launch(resident, group_norm_kernel<T, kAligned, kWhole, false>, s, true, smem, most,
+                      stream, t, ws, g, p.eps, p.activation);
+    const cudaError_t e = launch(partial, group_norm_kernel<T, kAligned, kWhole, true>, s, false,
+                                 smem, most, stream, t, ws, g, p.eps, p.activation);
+    if (e != cudaSuccess) return e;
+    return launch(apply, group_norm_apply_kernel<T, kAligned, kWhole>, s, false, 0, 0, stream, t,
+                  static_cast<const float2*>(ws), g, p.eps, p.activation);
+}
+
+Shape shape_of(const GroupNormProblem& p, bool aligned) {
+    return group_norm::shape_of(p.batch, p.length, p.channels, p.groups,
+                                p.dtype == FGA_FLOAT ? 4 : 2, aligned, 16, kTileBytes);
+}
+
+template <typename T> cudaError_t run(const GroupNormProblem& p, cudaStream_t stream) {
+    const Shape s = shape_of(p, aligned16({p.x, p.weight, p.bias, p.output}));
+    if (!s.aligned) return run<T, false, false>(p, s, stream);
+    return s.whole ? run<T, true, true>(p, s, stream) : run<T, true, false>(p, s, stream);
 }
 
 }  // namespace
 
-size_t group_norm_workspace(const GroupNormProblem&) { return 0; }
-size_t group_norm_backward_workspace(const GroupNormBackwardProblem&) { return 0; }
+size_t group_norm_workspace(const GroupNormProblem& p) {
+    size_t most = 0;
+    for (bool aligned : {true, false}) {
+        const Shape s = shape_of(p, aligned);
+        if (s.split)
+            most = std::max(most, sizeof(float2) * p.batch * p.groups * s.geo.parts * s.geo.blocks);
+    }
+    return most;
+}
 
 cudaError_t launch_group_norm(const GroupNormProblem& p, cudaStream_t s, const char** variant) {
     *variant = "group-norm";
-    if (p.dtype == FGA_FLOAT) return forward<float>(p, s);
-    if (p.dtype == FGA_HALF) return forward<__half>(p, s);
-    return forward<__nv_bfloat16>(p, s);
-}
-
-cudaError_t launch_group_norm_backward(const GroupNormBackwardProblem& p, cudaStream_t s,
-                                       const char** variant) {
-    *variant = "group-norm-backward";
-    if (p.dtype == FGA_FLOAT) return backward<float>(p, s);
-    if (p.dtype == FGA_HALF) return backward<__half>(p, s);
-    return backward<__nv_bfloat16>(p, s);
+    if (p.dtype == FGA_FLOAT) return run<float>(p, s);
+    if (p.dtype == FGA_HALF) return run<__half>(p, s);
+    return run<__nv_bfloat16>(p, s);
 }
 
 }  // namespace fga

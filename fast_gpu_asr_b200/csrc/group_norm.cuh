@@ -1,0 +1,332 @@
+// What the forward and backward kernels of group norm with activation share: how [N, T, C] is
+// cut into slabs of whole groups, a thread's vectors, the activations, and the launch shape.
+//
+// A block works on some rows of one utterance's slab: the channels of whole groups, at least
+// 128 bytes a row where there are so many (or, for a group wider than a block's threads, a part
+// of one). Its threads stand in `rows` x `lanes`, a lane one 16-byte vector of channels, and
+// keep their column from row to row, so that a column's parameters stay in registers.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <initializer_list>
+#include <numeric>
+
+#include "../../include/fga_convolution.h"
+#include "fga_common.cuh"
+#include "host_util.h"
+
+namespace fga {
+namespace group_norm {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256, kBlockWarps = kThreads / kWarp;
+constexpr int kMaxCluster = 16;
+constexpr int kMaxSlabGroups = 64;
+constexpr int kSlabBytes = 128;
+
+template <typename T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+// ---- vectors -------------------------------------------------------------------------------
+__device__ __forceinline__ void unpack(const uint4& r, float (&v)[4], float) {
+    v[0] = __uint_as_float(r.x);
+    v[1] = __uint_as_float(r.y);
+    v[2] = __uint_as_float(r.z);
+    v[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], __half) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(h[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], __nv_bfloat16) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+}
+template <typename T> __device__ __forceinline__ void unpack(const uint4& r, float (&v)[kVec<T>]) {
+    unpack(r, v, T{});
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[4], float) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                      __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[8], __half) {
+    uint4 r;
+    __half2* h = reinterpret_cast<__half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    return r;
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[8], __nv_bfloat16) {
+    uint4 r;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[kVec<T>]) {
+    return pack(v, T{});
+}
+
+// `count` channels at p, which need only be aligned to their type unless kAligned; the others
+// are zero.
+template <typename T, bool kAligned>
+__device__ __forceinline__ uint4 load(const T* p, int count) {
+    if constexpr (kAligned) {
+        return *reinterpret_cast<const uint4*>(p);
+    } else {
+        uint4 r = make_uint4(0, 0, 0, 0);
+        T* v = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e)
+            if (e < count) v[e] = p[e];
+        return r;
+    }
+}
+template <typename T, bool kAligned>
+__device__ __forceinline__ void store(T* p, const uint4& r, int count) {
+    if constexpr (kAligned) {
+        *reinterpret_cast<uint4*>(p) = r;
+    } else {
+        const T* v = reinterpret_cast<const T*>(&r);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e)
+            if (e < count) p[e] = v[e];
+    }
+}
+// The same into shared memory, to be read by the same thread after `arrived`.
+template <typename T, bool kAligned>
+__device__ __forceinline__ void stage(uint4* to, const T* p, int count) {
+    if constexpr (kAligned)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                     "l"(p)
+                     : "memory");
+    else
+        *to = load<T, false>(p, count);
+}
+__device__ __forceinline__ void arrived() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// ---- activations ---------------------------------------------------------------------------
+// The special functions flush subnormals: otherwise each costs three more instructions.
+__device__ __forceinline__ float exp_of(float v) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * kLog2e));
+    return e;
+}
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float sigmoid(float v) { return reciprocal(1.0f + exp_of(-v)); }
+
+template <int kCount> __device__ __forceinline__ void activate(float (&z)[kCount], int act) {
+    if (act == FGA_ACTIVATION_SILU) {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) z[e] *= sigmoid(z[e]);
+    } else if (act == FGA_ACTIVATION_SWOOSH_R) {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            const float v = z[e] - 1.0f;
+            // softplus(v) = max(v, 0) + log(1 + exp(-|v|)); the logarithm's argument is in
+            // [1, 2], where a log2 of absolute error 2^-22 is as good as log1p next to the sum.
+            float l;
+            asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(l) : "f"(1.0f + exp_of(-fabsf(v))));
+            z[e] = fmaxf(v, 0.0f) + 0.69314718f * l - 0.08f * z[e] - 0.313261687f;
+        }
+    }
+}
+
+// act'(z)
+__device__ __forceinline__ float slope(float z, int act) {
+    if (act == FGA_ACTIVATION_SILU) {
+        const float s = sigmoid(z);
+        return s * fmaf(z, 1.0f - s, 1.0f);
+    }
+    if (act == FGA_ACTIVATION_SWOOSH_R) return sigmoid(z - 1.0f) - 0.08f;
+    return 1.0f;
+}
+
+// ---- geometry ------------------------------------------------------------------------------
+struct Geometry {
+    int length, channels, groups, group_channels;
+    int slab_groups;  // whole groups of a slab
+    int parts;        // slabs of a group that is wider than one (then slab_groups is 1)
+    int part_channels;
+    int slabs;        // of a row
+    int blocks;       // of an utterance's slab: a cluster, or the chunks of a split launch
+    int rows;         // most rows of a block
+};
+
+template <typename T> struct Place {
+    int n, m, slab, block;
+    int first_group, groups;        // of the slab
+    int first_channel, channels;    // of the slab
+    int lanes, step;                // threads of a row, rows of the block's threads
+    int lane, row;                  // of this thread; row >= step: no work
+    int count;                      // valid channels of this thread's vector
+    int begin, rows;                // rows of the block
+
+    // kChunks: blocks take g.rows rows each; else they divide the valid rows evenly.
+    template <bool kChunks>
+    __device__ static Place make(const Geometry& g, const int32_t* lengths) {
+        Place p;
+        p.block = blockIdx.x % g.blocks;
+        const int unit = blockIdx.x / g.blocks;
+        p.n = unit / g.slabs;
+        p.slab = unit % g.slabs;
+        p.m = min(max(lengths[p.n], 0), g.length);
+        if (g.parts > 1) {
+            p.first_group = p.slab / g.parts;
+            p.groups = 1;
+            const int at = p.slab % g.parts * g.part_channels;
+            p.first_channel = p.first_group * g.group_channels + at;
+            p.channels = min(g.part_channels, g.group_channels - at);
+        } else {
+            p.first_group = p.slab * g.slab_groups;
+            p.groups = min(g.slab_groups, g.groups - p.first_group);
+            p.first_channel = p.first_group * g.group_channels;
+            p.channels = p.groups * g.group_channels;
+        }
+        p.lanes = (p.channels + kVec<T> - 1) / kVec<T>;
+        p.step = kThreads / p.lanes;
+        p.lane = threadIdx.x % p.lanes;
+        p.row = threadIdx.x / p.lanes;
+        p.count = min(kVec<T>, p.channels - p.lane * kVec<T>);
+        const int each = kChunks ? g.rows : (p.m + g.blocks - 1) / g.blocks;
+        p.begin = min(p.m, p.block * each);
+        p.rows = min(p.m - p.begin, each);
+        return p;
+    }
+    // Rows of the block in the threads of row r.
+    __device__ int rows_of(int r) const {
+        return r < step && r < rows ? (rows - r + step - 1) / step : 0;
+    }
+    // The group, within the slab, of this thread's channel e.
+    __device__ int group_of(int e, const Geometry& g) const {
+        return min((lane * kVec<T> + e) / g.group_channels, groups - 1);
+    }
+    __device__ int channel() const { return first_channel + lane * kVec<T>; }
+    // Element offset of this thread's vector in row t.
+    __device__ int64_t at(const Geometry& g, int t) const {
+        return (static_cast<int64_t>(n) * g.length + t) * g.channels + channel();
+    }
+};
+
+// Zeros in the rows past the valid ones, of which the unit's blocks take turns.
+template <typename T, bool kAligned>
+__device__ __forceinline__ void zero_padding(T* out, const Place<T>& p, const Geometry& g) {
+    if (p.row >= p.step) return;
+    const int64_t stride = static_cast<int64_t>(g.blocks) * p.step;
+    for (int64_t t = p.m + static_cast<int64_t>(p.block) * p.step + p.row; t < g.length; t += stride)
+        store<T, kAligned>(out + p.at(g, static_cast<int>(t)), make_uint4(0, 0, 0, 0), p.count);
+}
+
+// ---- launch shape --------------------------------------------------------------------------
+struct Shape {
+    Geometry geo;
+    bool aligned;  // vectors are 16-byte aligned in global memory, and full
+    bool whole;    // a vector's channels are of one group
+    bool split;    // too large for a cluster: several launches with a workspace between them
+    int64_t units; // utterances x slabs
+};
+
+// `bytes_per_vector`: of shared memory that a block keeps for a vector of its rows;
+// `tile_bytes`: what it should hold at most.
+inline Shape shape_of(int batch, int length, int channels, int groups, int element, bool aligned,
+                      int bytes_per_vector, int tile_bytes) {
+    Shape s{};
+    const int vec = 16 / element, width = channels / groups;
+    Geometry& g = s.geo;
+    g.length = length;
+    g.channels = channels;
+    g.groups = groups;
+    g.group_channels = width;
+    g.parts = 1;
+    g.part_channels = kThreads * vec;
+    const int64_t group_bytes = static_cast<int64_t>(width) * element;
+    // Slabs that start at a multiple of 16 bytes, if that takes no more than the threads.
+    int64_t step = 16 / std::gcd<int64_t>(group_bytes, 16);
+    if (step > groups) step = groups;  // one slab: the row
+    aligned = aligned && channels % vec == 0 && (step == 1 || step * group_bytes <= kThreads * 16);
+    if (!aligned) step = 1;
+    int64_t slab = step * std::max<int64_t>(1, kSlabBytes / (step * group_bytes));
+    slab = std::min<int64_t>({slab, groups, kMaxSlabGroups});
+    g.slab_groups = static_cast<int>(slab);
+    g.slabs = (groups + g.slab_groups - 1) / g.slab_groups;
+    if (width > g.part_channels) {
+        // (A group this wide has a step of 1, so parts of full vectors if aligned at all.)
+        g.slab_groups = 1;
+        g.parts = (width + g.part_channels - 1) / g.part_channels;
+        g.slabs = groups * g.parts;
+    }
+    s.aligned = aligned;
+    s.whole = g.slab_groups == 1 ? aligned : aligned && width % vec == 0;
+    s.units = static_cast<int64_t>(batch) * g.slabs;
+    const int64_t lanes =
+        (std::min(width * g.slab_groups, g.part_channels) + vec - 1) / vec;
+    const int64_t row_bytes = lanes * bytes_per_vector, rows_in_step = kThreads / lanes;
+    const int64_t fit = std::max<int64_t>(1, tile_bytes / row_bytes);  // rows of a block
+    // Enough blocks for two on every multiprocessor, as long as each has rows for its threads.
+    const int64_t fill = std::min<int64_t>((2LL * sm_count() + s.units - 1) / s.units,
+                                           (length + 2 * rows_in_step - 1) / (2 * rows_in_step));
+    const int64_t blocks = std::max<int64_t>({(length + fit - 1) / fit, fill, 1});
+    s.split = g.parts > 1 || (length + fit - 1) / fit > kMaxCluster;
+    if (s.split) {
+        const int64_t rows = (length + blocks - 1) / blocks;
+        g.rows = static_cast<int>(rows);
+        g.blocks = static_cast<int>((length + rows - 1) / rows);
+    } else {
+        g.blocks = static_cast<int>(std::min<int64_t>(blocks, kMaxCluster));
+        g.rows = (length + g.blocks - 1) / g.blocks;
+    }
+    return s;
+}
+
+inline bool aligned16(std::initializer_list<const void*> buffers) {
+    uintptr_t all = 0;
+    for (const void* b : buffers) all |= reinterpret_cast<uintptr_t>(b);
+    return all % 16 == 0;
+}
+
+// One launch of `units` x geo.blocks blocks, as clusters of geo.blocks if `cluster`.
+template <typename... Params, typename... Args>
+cudaError_t launch(SmemAttr& attribute, void (*kernel)(Params...), const Shape& s, bool cluster,
+                   int smem, int most_smem, cudaStream_t stream, Args... args) {
+    const void* entry = reinterpret_cast<const void*>(kernel);
+    cudaError_t e = attribute.ensure(entry, most_smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(s.units * s.geo.blocks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(s.geo.blocks);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster && s.geo.blocks > 1 ? 1 : 0;
+    if (cluster && s.geo.blocks > 8) {
+        e = cudaFuncSetAttribute(entry, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace group_norm
+}  // namespace fga
