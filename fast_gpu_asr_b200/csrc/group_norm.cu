@@ -7,8 +7,8 @@
 // The rows of an utterance's slab stay on chip between the statistics and the output: a block
 // keeps them in shared memory, a cluster of up to 16 blocks where one is not enough. Every
 // thread reads only vectors that it copied itself, so the tile needs no barrier. A thread
-// takes mean and sum of squares about it over its own values (two passes over shared memory),
-// and pairs of (mean, squares) merge exactly as the two-pass formula would have it:
+// takes the mean and the sum of squares about it over its own values, and pairs of (mean,
+// squares) merge exactly as the two-pass formula would have it:
 //   mean = sum n_i mean_i / sum n_i, squares = sum (squares_i + n_i (mean_i - mean)^2);
 // no difference of large sums is taken. What no cluster holds is done in two launches, the
 // first of which leaves each block's (mean, squares) in the workspace.
@@ -21,111 +21,109 @@ namespace {
 using namespace group_norm;
 
 constexpr int kTileBytes = 48 << 10;
+constexpr int kGatherBytes = kMaxCluster * kMaxSlabGroups * static_cast<int>(sizeof(float2));
 
-// Merges (mean, squares) over `items` entries by one warp; entry(i) gives the count, mean and
-// squares of item i. Every lane returns the whole's.
-template <typename Entry>
-__device__ __forceinline__ float2 merge(int items, float total, Entry entry) {
-    const int lane = threadIdx.x % kWarp;
+// Merges (mean, squares) pairs: visit(add) calls add(count, pair) for each of this lane's, and
+// is called twice. Every lane returns the whole's.
+template <typename Visit> __device__ __forceinline__ float2 merge(float total, Visit visit) {
     float sum = 0.0f;
-    for (int i = lane; i < items; i += kWarp) {
-        const float3 v = entry(i);
-        sum = fmaf(v.x, v.y, sum);
-    }
+    visit([&](float count, float2 v) { sum = fmaf(count, v.x, sum); });
     const float mean = total > 0.0f ? warp_sum(sum) / total : 0.0f;
     float squares = 0.0f;
-    for (int i = lane; i < items; i += kWarp) {
-        const float3 v = entry(i);
-        const float d = v.y - mean;
-        squares += fmaf(v.x * d, d, v.z);
-    }
+    visit([&](float count, float2 v) {
+        const float d = v.x - mean;
+        squares += fmaf(count * d, d, v.y);
+    });
     return make_float2(mean, warp_sum(squares));
 }
 
 // (mean, squares) of every group of the slab over this block's rows, which its threads have in
 // `tile`, to moments[group]. `part` holds an entry per thread (and channel, if not kWhole).
+//
+// A thread takes both in one pass, about a pivot: the mean of its own first vector (the first
+// value of each channel). With n values and the first q of them in the pivot, squares about
+// the mean are at least q (pivot - mean)^2, so the n (pivot - mean)^2 taken off the squares
+// about the pivot is at most n / q times what is left: with at most kTileBytes / 4096 rows a
+// thread, a factor of 12 on a rounding error.
 template <typename T, bool kWhole>
 __device__ __forceinline__ void block_moments(const uint4* tile, float2* part, float2* moments,
                                               const Place<T>& p, const Geometry& g) {
     constexpr int kValues = kWhole ? 1 : kVec<T>;
-    const int mine = p.rows_of(p.row);
-    float mean[kValues], squares[kValues];
-#pragma unroll
-    for (int e = 0; e < kValues; ++e) mean[e] = 0.0f, squares[e] = 0.0f;
+    const int mine = p.own_rows(), columns = g.lanes * kValues;
     if (mine > 0) {
-        const uint4* at = tile + p.row * p.lanes + p.lane;
-        const int pitch = p.step * p.lanes;
+        const uint4* at = tile + p.row * g.lanes + p.lane;
+        const int pitch = g.step * g.lanes;
+        float pivot[kValues], sum[kValues], squares[kValues], v[kVec<T>];
+        unpack<T>(at[0], v);
+        if constexpr (kWhole) {
+            float s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e) s += v[e];
+            pivot[0] = s * (1.0f / kVec<T>);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e) pivot[e] = v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < kValues; ++e) sum[e] = 0.0f, squares[e] = 0.0f;
 #pragma unroll 4
         for (int i = 0; i < mine; ++i) {
-            float v[kVec<T>];
             unpack<T>(at[i * pitch], v);
-            if constexpr (kWhole) {
-                float s = 0.0f;
 #pragma unroll
-                for (int e = 0; e < kVec<T>; ++e) s += v[e];
-                mean[0] += s;
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec<T>; ++e) mean[e] += v[e];
+            for (int e = 0; e < kVec<T>; ++e) {
+                constexpr bool kOne = kWhole;
+                const int k = kOne ? 0 : e;
+                const float d = v[e] - pivot[k];
+                sum[k] += d;
+                squares[k] = fmaf(d, d, squares[k]);
             }
         }
         const float inv = 1.0f / static_cast<float>(mine * (kWhole ? kVec<T> : 1));
 #pragma unroll
-        for (int e = 0; e < kValues; ++e) mean[e] *= inv;
-#pragma unroll 4
-        for (int i = 0; i < mine; ++i) {
-            float v[kVec<T>];
-            unpack<T>(at[i * pitch], v);
-#pragma unroll
-            for (int e = 0; e < kVec<T>; ++e) {
-                const float d = v[e] - mean[kWhole ? 0 : e];
-                squares[kWhole ? 0 : e] = fmaf(d, d, squares[kWhole ? 0 : e]);
-            }
+        for (int e = 0; e < kValues; ++e) {
+            const float off = sum[e] * inv;  // mean - pivot
+            part[p.row * columns + p.lane * kValues + e] =
+                make_float2(pivot[e] + off, fmaxf(fmaf(-sum[e], off, squares[e]), 0.0f));
         }
     }
-    const int columns = p.lanes * kValues;
-    if (p.row < p.step)
-#pragma unroll
-        for (int e = 0; e < kValues; ++e)
-            part[p.row * columns + p.lane * kValues + e] = make_float2(mean[e], squares[e]);
     __syncthreads();
     // A warp per group: its columns of every row of threads.
-    const int per_group = kWhole ? p.channels / p.groups / kVec<T> : p.channels / p.groups;
-    const int items = min(p.step, p.rows) * per_group;
+    const int width = kWhole ? p.channels / p.groups / kVec<T> : p.channels / p.groups;
+    const int used = min(g.step, p.rows);
     const float total = static_cast<float>(p.rows) * static_cast<float>(p.channels / p.groups);
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
-        const float2 r = merge(items, total, [&](int i) {
-            const int row = i / per_group;
-            const float2 v = part[row * columns + j * per_group + i % per_group];
-            return make_float3(static_cast<float>(p.rows_of(row) * (kWhole ? kVec<T> : 1)), v.x, v.y);
+        const float2 r = merge(total, [&](auto add) {
+            for (Items i(width); i.row < used; i.next())
+                add(static_cast<float>(p.rows_of(i.row) * (kWhole ? kVec<T> : 1)),
+                    part[i.row * columns + j * width + i.column]);
         });
         if (threadIdx.x % kWarp == 0) moments[j] = r;
     }
 }
 
-// A column's parameters: out = act((x - mean) scale + bias).
-template <typename T, bool kWhole> struct Column {
-    static constexpr int kMeans = kWhole ? 1 : kVec<T>;
-    float mean[kMeans], scale[kVec<T>], bias[kVec<T>];
+// A column's parameters: out = act(x scale + shift), scale = rstd weight, shift = bias - mean
+// scale. Next to (x - mean) scale + bias this costs two roundings of mean * scale, what the
+// rounding of the mean to fp32 costs in either form, and saves an instruction an element.
+template <typename T> struct Column {
+    float scale[kVec<T>], shift[kVec<T>];
     // `stats`: (mean, rstd) of the slab's groups.
-    template <bool kAligned>
+    template <bool kAligned, bool kWhole>
     __device__ __forceinline__ void read(const T* w, const T* b, const float2* stats,
                                          const Place<T>& p, const Geometry& g) {
         unpack<T>(load<T, kAligned>(w + p.channel(), p.count), scale);
-        unpack<T>(load<T, kAligned>(b + p.channel(), p.count), bias);
+        unpack<T>(load<T, kAligned>(b + p.channel(), p.count), shift);
 #pragma unroll
         for (int e = 0; e < kVec<T>; ++e) {
             const float2 s = stats[p.group_of(kWhole ? 0 : e, g)];
-            mean[kWhole ? 0 : e] = s.x;
             scale[e] *= s.y;
+            shift[e] = fmaf(-s.x, scale[e], shift[e]);
         }
     }
     __device__ __forceinline__ uint4 apply(const uint4& r, int act) const {
         float v[kVec<T>];
         unpack<T>(r, v);
 #pragma unroll
-        for (int e = 0; e < kVec<T>; ++e)
-            v[e] = fmaf(v[e] - mean[kWhole ? 0 : e], scale[e], bias[e]);
+        for (int e = 0; e < kVec<T>; ++e) v[e] = fmaf(v[e], scale[e], shift[e]);
         activate(v, act);
         return pack<T>(v);
     }
@@ -152,11 +150,10 @@ __global__ void __launch_bounds__(kThreads, 4)
     extern __shared__ __align__(16) uint4 tile[];
     __shared__ float2 part[kWhole ? kThreads : kThreads * kVec<T>];
     __shared__ float2 moments[kMaxSlabGroups];
-    __shared__ float2 gathered[kPartial ? 1 : kMaxCluster][kMaxSlabGroups];
     const Place<T> p = Place<T>::template make<kPartial>(g, t.lengths);
-    const int mine = p.rows_of(p.row), pitch = p.step * p.lanes;
-    uint4* at = tile + p.row * p.lanes + p.lane;
-    const int64_t stride = static_cast<int64_t>(p.step) * g.channels;
+    const int mine = p.own_rows(), pitch = g.step * g.lanes;
+    uint4* at = tile + p.row * g.lanes + p.lane;
+    const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
     {
         const T* from = t.x + p.at(g, p.begin + p.row);
 #pragma unroll 4
@@ -175,18 +172,20 @@ __global__ void __launch_bounds__(kThreads, 4)
     } else {
         const float total = static_cast<float>(p.m) * width;
         if (g.blocks > 1) {
+            // Behind the tile: [block][group].
+            float2* gathered = reinterpret_cast<float2*>(tile + g.rows * g.lanes);
             auto cluster = cg::this_cluster();
             cluster.sync();  // every block runs, and may be written to
-            for (int i = threadIdx.x; i < g.blocks * p.groups; i += kThreads)
-                *cluster.map_shared_rank(&gathered[p.block][i % p.groups], i / p.groups) =
-                    moments[i % p.groups];
+            for (int q = threadIdx.x / kWarp; q < g.blocks; q += kBlockWarps)
+                for (int j = threadIdx.x % kWarp; j < p.groups; j += kWarp)
+                    *cluster.map_shared_rank(gathered + p.block * g.slab_groups + j, q) = moments[j];
             cluster.sync();
-            const int each = (p.m + g.blocks - 1) / g.blocks;
+            const int each = g.by_blocks.quotient(p.m + g.blocks - 1);
             for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
-                const float2 r = merge(g.blocks, total, [&](int i) {
-                    const float2 v = gathered[i][j];
-                    return make_float3(static_cast<float>(max(0, min(each, p.m - i * each))) * width,
-                                       v.x, v.y);
+                const float2 r = merge(total, [&](auto add) {
+                    for (int i = threadIdx.x % kWarp; i < g.blocks; i += kWarp)
+                        add(static_cast<float>(max(0, min(each, p.m - i * each))) * width,
+                            gathered[i * g.slab_groups + j]);
                 });
                 if (threadIdx.x % kWarp == 0) moments[j] = r;
             }
@@ -203,8 +202,8 @@ __global__ void __launch_bounds__(kThreads, 4)
         }
         __syncthreads();
         if (mine > 0) {
-            Column<T, kWhole> column;
-            column.template read<kAligned>(t.weight, t.bias, moments, p, g);
+            Column<T> column;
+            column.template read<kAligned, kWhole>(t.weight, t.bias, moments, p, g);
             T* to = t.out + p.at(g, p.begin + p.row);
 #pragma unroll 2
             for (int i = 0; i < mine; ++i, to += stride)
@@ -226,13 +225,13 @@ __global__ void __launch_bounds__(kThreads, 4)
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
         const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group + j;
         const float2* mine = partial + group * slots;
-        const float2 r = merge(slots, total, [&](int i) {
-            const int rows = max(0, min(g.rows, p.m - i % g.blocks * g.rows));
-            const int wide = g.parts > 1 ? min(g.part_channels,
-                                               g.group_channels - i / g.blocks * g.part_channels)
-                                         : g.group_channels;
-            const float2 v = mine[i];
-            return make_float3(static_cast<float>(rows) * static_cast<float>(wide), v.x, v.y);
+        const float2 r = merge(total, [&](auto add) {
+            for (int i = threadIdx.x % kWarp; i < slots; i += kWarp) {
+                const int q = g.by_blocks.quotient(i), chunk = i - q * g.blocks;
+                const int rows = max(0, min(g.rows, p.m - chunk * g.rows));
+                const int wide = min(g.part_channels, g.group_channels - q * g.part_channels);
+                add(static_cast<float>(rows) * static_cast<float>(wide), mine[i]);
+            }
         });
         if (threadIdx.x % kWarp == 0) {
             const float2 s = to_stats(r, total, eps);
@@ -244,11 +243,11 @@ __global__ void __launch_bounds__(kThreads, 4)
         }
     }
     __syncthreads();
-    const int mine = p.rows_of(p.row);
+    const int mine = p.own_rows();
     if (mine > 0) {
-        Column<T, kWhole> column;
-        column.template read<kAligned>(t.weight, t.bias, stats, p, g);
-        const int64_t stride = static_cast<int64_t>(p.step) * g.channels;
+        Column<T> column;
+        column.template read<kAligned, kWhole>(t.weight, t.bias, stats, p, g);
+        const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
         const int64_t first = p.at(g, p.begin + p.row);
 #pragma unroll 4
         for (int i = 0; i < mine; ++i)
@@ -265,13 +264,12 @@ cudaError_t run(const GroupNormProblem& p, const Shape& s, cudaStream_t stream) 
     const Tensors<T> t{static_cast<const T*>(p.x), p.valid_lengths, static_cast<const T*>(p.weight),
                        static_cast<const T*>(p.bias), static_cast<T*>(p.output), p.mean, p.rstd};
     const Geometry& g = s.geo;
-    const int lanes = (std::min(g.group_channels * g.slab_groups, g.part_channels) + kVec<T> - 1) /
-                      kVec<T>;
-    const int smem = g.rows * lanes * 16, most = kTileBytes + kThreads * 16;
+    const int smem = g.rows * g.lanes * 16, most = kTileBytes + kThreads * 16 + kGatherBytes;
+    const int gather = g.blocks > 1 ? g.blocks * g.slab_groups * static_cast<int>(sizeof(float2)) : 0;
     float2* ws = static_cast<float2*>(p.workspace);
     if (!s.split)
-        return launch(resident, group_norm_kernel<T, kAligned, kWhole, false>, s, true, smem, most,
-                      stream, t, ws, g, p.eps, p.activation);
+        return launch(resident, group_norm_kernel<T, kAligned, kWhole, false>, s, true,
+                      smem + gather, most, stream, t, ws, g, p.eps, p.activation);
     const cudaError_t e = launch(partial, group_norm_kernel<T, kAligned, kWhole, true>, s, false,
                                  smem, most, stream, t, ws, g, p.eps, p.activation);
     if (e != cudaSuccess) return e;

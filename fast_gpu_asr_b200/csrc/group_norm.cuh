@@ -162,6 +162,22 @@ __device__ __forceinline__ float slope(float z, int act) {
 }
 
 // ---- geometry ------------------------------------------------------------------------------
+// Division by a number that the host knows, for dividends below 2^31: a block of a few
+// microseconds would otherwise spend a third of its instructions on dividing indexes.
+struct Divisor {
+    uint32_t d, multiplier, shift;
+    Divisor() = default;
+    explicit Divisor(uint32_t divisor) : d(divisor), multiplier(0), shift(0) {
+        if (d == 1) return;
+        while ((1ull << shift) < d) ++shift;  // ceil(log2 d)
+        multiplier = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
+        --shift;
+    }
+    __device__ __forceinline__ int quotient(int n) const {
+        return d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), multiplier) >> shift);
+    }
+};
+
 struct Geometry {
     int length, channels, groups, group_channels;
     int slab_groups;  // whole groups of a slab
@@ -170,25 +186,27 @@ struct Geometry {
     int slabs;        // of a row
     int blocks;       // of an utterance's slab: a cluster, or the chunks of a split launch
     int rows;         // most rows of a block
+    int lanes, step;  // threads of a row, rows of a block's threads
+    Divisor by_blocks, by_slabs, by_lanes, by_step, by_group;
 };
 
 template <typename T> struct Place {
     int n, m, slab, block;
-    int first_group, groups;        // of the slab
-    int first_channel, channels;    // of the slab
-    int lanes, step;                // threads of a row, rows of the block's threads
-    int lane, row;                  // of this thread; row >= step: no work
-    int count;                      // valid channels of this thread's vector
-    int begin, rows;                // rows of the block
+    int first_group, groups;      // of the slab
+    int first_channel, channels;  // of the slab
+    int lane, row;                // of this thread
+    int count;                    // valid channels of this thread's vector; below 1: no work
+    int begin, rows;              // rows of the block
+    int passes, extra;            // rows of a thread: passes, and one more in the first `extra`
 
     // kChunks: blocks take g.rows rows each; else they divide the valid rows evenly.
     template <bool kChunks>
     __device__ static Place make(const Geometry& g, const int32_t* lengths) {
         Place p;
-        p.block = blockIdx.x % g.blocks;
-        const int unit = blockIdx.x / g.blocks;
-        p.n = unit / g.slabs;
-        p.slab = unit % g.slabs;
+        const int unit = g.by_blocks.quotient(blockIdx.x);
+        p.block = blockIdx.x - unit * g.blocks;
+        p.n = g.by_slabs.quotient(unit);
+        p.slab = unit - p.n * g.slabs;
         p.m = min(max(lengths[p.n], 0), g.length);
         if (g.parts > 1) {
             p.first_group = p.slab / g.parts;
@@ -202,38 +220,61 @@ template <typename T> struct Place {
             p.first_channel = p.first_group * g.group_channels;
             p.channels = p.groups * g.group_channels;
         }
-        p.lanes = (p.channels + kVec<T> - 1) / kVec<T>;
-        p.step = kThreads / p.lanes;
-        p.lane = threadIdx.x % p.lanes;
-        p.row = threadIdx.x / p.lanes;
-        p.count = min(kVec<T>, p.channels - p.lane * kVec<T>);
-        const int each = kChunks ? g.rows : (p.m + g.blocks - 1) / g.blocks;
+        p.row = g.by_lanes.quotient(threadIdx.x);
+        p.lane = threadIdx.x - p.row * g.lanes;
+        p.count = p.row < g.step ? min(kVec<T>, p.channels - p.lane * kVec<T>) : 0;
+        const int each = kChunks ? g.rows : g.by_blocks.quotient(p.m + g.blocks - 1);
         p.begin = min(p.m, p.block * each);
         p.rows = min(p.m - p.begin, each);
+        p.passes = g.by_step.quotient(p.rows);
+        p.extra = p.rows - p.passes * g.step;
         return p;
     }
     // Rows of the block in the threads of row r.
-    __device__ int rows_of(int r) const {
-        return r < step && r < rows ? (rows - r + step - 1) / step : 0;
-    }
+    __device__ __forceinline__ int rows_of(int r) const { return passes + (r < extra ? 1 : 0); }
+    __device__ __forceinline__ int own_rows() const { return count > 0 ? rows_of(row) : 0; }
     // The group, within the slab, of this thread's channel e.
-    __device__ int group_of(int e, const Geometry& g) const {
-        return min((lane * kVec<T> + e) / g.group_channels, groups - 1);
+    __device__ __forceinline__ int group_of(int e, const Geometry& g) const {
+        return g.parts > 1 ? 0 : min(g.by_group.quotient(lane * kVec<T> + e), groups - 1);
     }
-    __device__ int channel() const { return first_channel + lane * kVec<T>; }
+    __device__ __forceinline__ int channel() const { return first_channel + lane * kVec<T>; }
     // Element offset of this thread's vector in row t.
-    __device__ int64_t at(const Geometry& g, int t) const {
+    __device__ __forceinline__ int64_t at(const Geometry& g, int t) const {
         return (static_cast<int64_t>(n) * g.length + t) * g.channels + channel();
+    }
+};
+
+// The items of one group in a matrix of `columns` columns, `width` of them the group's: a warp
+// takes 32 at a time, row by row.
+struct Items {
+    int row, column, rows_by, columns_by, width;
+    __device__ __forceinline__ Items(int width_) : width(width_) {
+        const int lane = threadIdx.x % kWarp;
+        row = lane / width;
+        column = lane - row * width;
+        rows_by = kWarp / width;
+        columns_by = kWarp - rows_by * width;
+    }
+    __device__ __forceinline__ void next() {
+        row += rows_by;
+        column += columns_by;
+        if (column >= width) {
+            column -= width;
+            ++row;
+        }
     }
 };
 
 // Zeros in the rows past the valid ones, of which the unit's blocks take turns.
 template <typename T, bool kAligned>
 __device__ __forceinline__ void zero_padding(T* out, const Place<T>& p, const Geometry& g) {
-    if (p.row >= p.step) return;
-    const int64_t stride = static_cast<int64_t>(g.blocks) * p.step;
-    for (int64_t t = p.m + static_cast<int64_t>(p.block) * p.step + p.row; t < g.length; t += stride)
-        store<T, kAligned>(out + p.at(g, static_cast<int>(t)), make_uint4(0, 0, 0, 0), p.count);
+    if (p.count <= 0) return;
+    const int by = g.blocks * g.step;
+    const int64_t stride = static_cast<int64_t>(by) * g.channels;
+    int t = p.m + p.block * g.step + p.row;
+    T* to = out + p.at(g, t);
+    for (; t < g.length; t += by, to += stride)
+        store<T, kAligned>(to, make_uint4(0, 0, 0, 0), p.count);
 }
 
 // ---- launch shape --------------------------------------------------------------------------
@@ -277,13 +318,13 @@ inline Shape shape_of(int batch, int length, int channels, int groups, int eleme
     s.aligned = aligned;
     s.whole = g.slab_groups == 1 ? aligned : aligned && width % vec == 0;
     s.units = static_cast<int64_t>(batch) * g.slabs;
-    const int64_t lanes =
-        (std::min(width * g.slab_groups, g.part_channels) + vec - 1) / vec;
-    const int64_t row_bytes = lanes * bytes_per_vector, rows_in_step = kThreads / lanes;
+    g.lanes = (std::min(width * g.slab_groups, g.part_channels) + vec - 1) / vec;
+    g.step = kThreads / g.lanes;
+    const int64_t row_bytes = static_cast<int64_t>(g.lanes) * bytes_per_vector;
     const int64_t fit = std::max<int64_t>(1, tile_bytes / row_bytes);  // rows of a block
     // Enough blocks for two on every multiprocessor, as long as each has rows for its threads.
     const int64_t fill = std::min<int64_t>((2LL * sm_count() + s.units - 1) / s.units,
-                                           (length + 2 * rows_in_step - 1) / (2 * rows_in_step));
+                                           (length + 2 * g.step - 1) / (2 * g.step));
     const int64_t blocks = std::max<int64_t>({(length + fit - 1) / fit, fill, 1});
     s.split = g.parts > 1 || (length + fit - 1) / fit > kMaxCluster;
     if (s.split) {
@@ -294,6 +335,11 @@ inline Shape shape_of(int batch, int length, int channels, int groups, int eleme
         g.blocks = static_cast<int>(std::min<int64_t>(blocks, kMaxCluster));
         g.rows = (length + g.blocks - 1) / g.blocks;
     }
+    g.by_blocks = Divisor(g.blocks);
+    g.by_slabs = Divisor(g.slabs);
+    g.by_lanes = Divisor(g.lanes);
+    g.by_step = Divisor(g.step);
+    g.by_group = Divisor(g.group_channels);
     return s;
 }
 
