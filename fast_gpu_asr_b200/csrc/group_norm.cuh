@@ -26,7 +26,6 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256, kBlockWarps = kThreads / kWarp;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSlabGroups = 64;
-constexpr int kSlabBytes = 128;
 
 template <typename T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 
@@ -152,13 +151,13 @@ template <int kCount> __device__ __forceinline__ void activate(float (&z)[kCount
 }
 
 // act'(z)
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == FGA_ACTIVATION_SILU) {
+template <int kAct> __device__ __forceinline__ float slope(float z) {
+    if constexpr (kAct == FGA_ACTIVATION_SILU) {
         const float s = sigmoid(z);
         return s * fmaf(z, 1.0f - s, 1.0f);
+    } else {
+        return sigmoid(z - 1.0f) - 0.08f;
     }
-    if (act == FGA_ACTIVATION_SWOOSH_R) return sigmoid(z - 1.0f) - 0.08f;
-    return 1.0f;
 }
 
 // ---- geometry ------------------------------------------------------------------------------
@@ -286,8 +285,10 @@ struct Shape {
     int64_t units; // utterances x slabs
 };
 
-// `bytes_per_vector`: of shared memory that a block keeps for a vector of its rows;
-// `tile_bytes`: what it should hold at most.
+// `bytes_per_vector`: of shared memory that a block keeps for a vector of its rows; `tile_bytes`:
+// what it should hold at most. Slabs are as wide as that allows for the whole length, since a
+// cluster costs two barriers, but at least 64 bytes a row, and no wider than 128 where that
+// would leave multiprocessors without work.
 inline Shape shape_of(int batch, int length, int channels, int groups, int element, bool aligned,
                       int bytes_per_vector, int tile_bytes) {
     Shape s{};
@@ -305,7 +306,13 @@ inline Shape shape_of(int batch, int length, int channels, int groups, int eleme
     if (step > groups) step = groups;  // one slab: the row
     aligned = aligned && channels % vec == 0 && (step == 1 || step * group_bytes <= kThreads * 16);
     if (!aligned) step = 1;
-    int64_t slab = step * std::max<int64_t>(1, kSlabBytes / (step * group_bytes));
+    const int64_t row_fit = 16LL * tile_bytes / (static_cast<int64_t>(length) * bytes_per_vector);
+    const int64_t wanted = (2LL * sm_count() + batch - 1) / batch;  // slabs for every processor
+    const int64_t spread = std::max<int64_t>(128, channels * static_cast<int64_t>(element) /
+                                                      std::max<int64_t>(1, wanted));
+    const int64_t slab_bytes =
+        std::max<int64_t>(64, std::min<int64_t>({row_fit, spread, kThreads * 16}));
+    int64_t slab = step * std::max<int64_t>(1, slab_bytes / (step * group_bytes));
     slab = std::min<int64_t>({slab, groups, kMaxSlabGroups});
     g.slab_groups = static_cast<int>(slab);
     g.slabs = (groups + g.slab_groups - 1) / g.slab_groups;

@@ -1,141 +1,432 @@
 // The gradients of group norm with activation over [N, T, C] (channels last).
 //
-// Over the M valid frames of an utterance and the Cg channels of a group:
-//   mean = sum x / (M Cg), var = sum (x - mean)^2 / (M Cg), rstd = (var + eps)^-1/2,
-//   xhat = (x - mean) rstd, z = weight xhat + bias, out = act(z);
-//   dz = dout act'(z), dbias = sum dz, dweight = sum dz xhat (over every valid frame),
+// With xhat = (x - mean) rstd, z = weight xhat + bias, dz = dout act'(z):
+//   dbias = sum dz, dweight = sum dz xhat (over every valid frame of the batch),
 //   dx = rstd (weight dz - (s1 + xhat s2) / (M Cg)),
-//   s1 = sum weight dz, s2 = sum weight dz xhat (over the group).
+//   s1 = sum weight dz, s2 = sum weight dz xhat (over the group's M Cg values).
 //
-// One block per utterance and group, one thread per element in turn; the parameters'
-// gradients by one block per channel.
-#include <cstdint>
-
-#include "../../include/fga_convolution.h"
-#include "fga_common.cuh"
+// Every sum is one over a channel's column first: dbias and dweight of this utterance, of which
+// s1 and s2 are sums weighted by `weight`. A block keeps its rows of x on chip, and dz in fp32
+// in the place of dout (which takes 48 bytes for 8 values of a 16-bit type, but evaluating the
+// slope twice would make the kernel bound by instructions), so x and dout are read once; a
+// cluster adds up (s1, s2) where one block cannot hold an utterance's slab. The columns' sums
+// go to the workspace, a row for each block, and a second launch adds the rows in order. What
+// no cluster holds is read twice: one launch for the sums, one for dx.
 #include "fga_kernels.h"
+#include "group_norm.cuh"
 
 namespace fga {
 namespace {
 
-constexpr int kThreads = 256;
+using namespace group_norm;
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+constexpr int kTileBytes = 72 << 10;
+constexpr int kGatherBytes = kMaxCluster * kMaxSlabGroups * static_cast<int>(sizeof(float2));
 
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == FGA_ACTIVATION_SILU) {
-        const float s = sigmoid(z);
-        return s * (1.0f + z * (1.0f - s));
-    }
-    if (act == FGA_ACTIVATION_SWOOSH_R) return sigmoid(z - 1.0f) - 0.08f;
-    return 1.0f;
-}
+// dz as fp32 planes of 16 bytes of each vector, the first of which held dout.
+template <typename T> constexpr int kPlanes = kVec<T> / 4;
+template <typename T> constexpr int kVectorBytes = 16 + 16 * kPlanes<T>;
+// What a thread adds up for each of its channels, in shared memory.
+template <typename T> constexpr int kSumBytes = kThreads * kVec<T> * static_cast<int>(sizeof(float2));
 
-// Sum over the block, the same value in every thread; `red` holds one float per warp.
-__device__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
-    __syncthreads();
-    if (threadIdx.x % kWarp == 0) red[threadIdx.x / kWarp] = v;
-    __syncthreads();
-    float total = 0.0f;
-    for (int i = 0; i < kThreads / kWarp; ++i) total += red[i];
-    return total;
-}
+template <typename T> struct Tensors {
+    const T* dout;
+    const T* x;
+    const int32_t* lengths;
+    const T* weight;
+    const T* bias;
+    const float* mean;  // [N, G]
+    const float* rstd;
+    T* dx;
+};
 
-__device__ __forceinline__ int valid_frames(const int32_t* lengths, int n, int length) {
-    return min(max(lengths[n], 0), length);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) group_norm_backward_kernel(
-    const T* __restrict__ dout, const T* __restrict__ x, const int32_t* __restrict__ lengths,
-    const T* __restrict__ weight, const T* __restrict__ bias, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, T* __restrict__ dx, int length, int channels, int groups,
-    int act) {
-    __shared__ float red[kThreads / kWarp];
-    const int n = blockIdx.x / groups, g = blockIdx.x % groups, cg = channels / groups;
-    const int m = valid_frames(lengths, n, length);
-    const int64_t base = static_cast<int64_t>(n) * length * channels + g * cg;
-    const int64_t count = static_cast<int64_t>(m) * cg, all = static_cast<int64_t>(length) * cg;
-    const float inv = count > 0 ? 1.0f / static_cast<float>(count) : 0.0f;
-    const float mean = mean_in[blockIdx.x], rstd = rstd_in[blockIdx.x];
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int64_t i = threadIdx.x; i < count; i += kThreads) {
-        const int64_t at = base + i / cg * channels + i % cg;
-        const int c = g * cg + static_cast<int>(i % cg);
-        const float w = to_f32<T>(weight[c]), xhat = (to_f32<T>(x[at]) - mean) * rstd;
-        const float d = w * to_f32<T>(dout[at]) * slope(xhat * w + to_f32<T>(bias[c]), act);
-        s1 += d;
-        s2 += d * xhat;
-    }
-    s1 = block_sum(s1, red) * inv;
-    s2 = block_sum(s2, red) * inv;
-    for (int64_t i = threadIdx.x; i < all; i += kThreads) {
-        const int64_t at = base + i / cg * channels + i % cg;
-        const int c = g * cg + static_cast<int>(i % cg);
-        float v = 0.0f;
-        if (i < count) {
-            const float w = to_f32<T>(weight[c]), xhat = (to_f32<T>(x[at]) - mean) * rstd;
-            const float d = w * to_f32<T>(dout[at]) * slope(xhat * w + to_f32<T>(bias[c]), act);
-            v = rstd * (d - s1 - xhat * s2);
+// A column's parameters: z = x scale + shift, xhat = x rstd - centre.
+template <typename T, bool kWhole> struct Column {
+    static constexpr int kStats = kWhole ? 1 : kVec<T>;
+    float scale[kVec<T>], shift[kVec<T>], rstd[kStats], centre[kStats];
+    template <bool kAligned>
+    __device__ __forceinline__ void read(const Tensors<T>& t, const Place<T>& p, const Geometry& g) {
+        unpack<T>(load<T, kAligned>(t.weight + p.channel(), p.count), scale);
+        unpack<T>(load<T, kAligned>(t.bias + p.channel(), p.count), shift);
+        const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group;
+#pragma unroll
+        for (int k = 0; k < kStats; ++k) {
+            rstd[k] = t.rstd[group + p.group_of(k, g)];
+            centre[k] = t.mean[group + p.group_of(k, g)] * rstd[k];
         }
-        dx[at] = from_f32<T>(v);
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) group_norm_parameters_kernel(
-    const T* __restrict__ dout, const T* __restrict__ x, const int32_t* __restrict__ lengths,
-    const T* __restrict__ weight, const T* __restrict__ bias, const float* __restrict__ mean,
-    const float* __restrict__ rstd, T* __restrict__ dweight, T* __restrict__ dbias, int batch,
-    int length, int channels, int groups, int act) {
-    __shared__ float red[kThreads / kWarp];
-    const int c = blockIdx.x, g = c / (channels / groups);
-    const float w = to_f32<T>(weight[c]), b = to_f32<T>(bias[c]);
-    float sw = 0.0f, sb = 0.0f;
-    for (int n = 0; n < batch; ++n) {
-        const int m = valid_frames(lengths, n, length);
-        const float mu = mean[static_cast<int64_t>(n) * groups + g];
-        const float r = rstd[static_cast<int64_t>(n) * groups + g];
-        for (int t = threadIdx.x; t < m; t += kThreads) {
-            const int64_t at = (static_cast<int64_t>(n) * length + t) * channels + c;
-            const float xhat = (to_f32<T>(x[at]) - mu) * r;
-            const float d = to_f32<T>(dout[at]) * slope(xhat * w + b, act);
-            sb += d;
-            sw += d * xhat;
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e) {
+            shift[e] = fmaf(-centre[kWhole ? 0 : e], scale[e], shift[e]);
+            scale[e] *= rstd[kWhole ? 0 : e];
         }
     }
-    sw = block_sum(sw, red);
-    sb = block_sum(sb, red);
-    if (threadIdx.x == 0) {
-        dweight[c] = from_f32<T>(sw);
-        dbias[c] = from_f32<T>(sb);
+    __device__ __forceinline__ float normalised(float x, int e) const {
+        return fmaf(x, rstd[kWhole ? 0 : e], -centre[kWhole ? 0 : e]);
+    }
+    // dout to dz.
+    __device__ __forceinline__ void through(float (&d)[kVec<T>], const float (&x)[kVec<T>],
+                                            int act) const {
+        if (act == FGA_ACTIVATION_SILU) {
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e)
+                d[e] *= slope<FGA_ACTIVATION_SILU>(fmaf(x[e], scale[e], shift[e]));
+        } else if (act == FGA_ACTIVATION_SWOOSH_R) {
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e)
+                d[e] *= slope<FGA_ACTIVATION_SWOOSH_R>(fmaf(x[e], scale[e], shift[e]));
+        }
+    }
+};
+
+// dx = dz scale + x slope + offset, with the group's means m1 = s1 / (M Cg), m2 = s2 / (M Cg):
+// slope = -rstd^2 m2, offset = rstd (centre m2 - m1).
+template <typename T, bool kWhole> struct Final {
+    static constexpr int kStats = kWhole ? 1 : kVec<T>;
+    float slope[kStats], offset[kStats];
+    __device__ __forceinline__ void make(const Column<T, kWhole>& column, const float2* sums,
+                                         float inv, const Place<T>& p, const Geometry& g) {
+#pragma unroll
+        for (int k = 0; k < kStats; ++k) {
+            const float2 m = make_float2(sums[p.group_of(k, g)].x * inv, sums[p.group_of(k, g)].y * inv);
+            slope[k] = -column.rstd[k] * column.rstd[k] * m.y;
+            offset[k] = column.rstd[k] * fmaf(column.centre[k], m.y, -m.x);
+        }
+    }
+    __device__ __forceinline__ float operator()(float dz, float x, float scale, int e) const {
+        return fmaf(dz, scale, fmaf(x, slope[kWhole ? 0 : e], offset[kWhole ? 0 : e]));
+    }
+};
+
+// Adds the threads' column sums: (dbias, dweight) of the block's rows to `sums` (also left in
+// shared memory at part[0..]), and of each group (s1, s2), weighted, to group_sums.
+template <typename T, bool kAligned>
+__device__ __forceinline__ void add_up(float (&db)[kVec<T>], float (&dw)[kVec<T>], float2* part,
+                                       float2* group_sums, float2* __restrict__ sums,
+                                       const T* __restrict__ weight, const Place<T>& p,
+                                       const Geometry& g) {
+    const int columns = g.lanes * kVec<T>;
+    int rows = g.step;
+    if (kWarp % g.lanes == 0) {
+        // Whole rows of threads in a warp: the warp's own sum first.
+        for (int o = g.lanes; o < kWarp; o *= 2)
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e) {
+                db[e] += __shfl_xor_sync(0xffffffffu, db[e], o);
+                dw[e] += __shfl_xor_sync(0xffffffffu, dw[e], o);
+            }
+        rows = kBlockWarps;
+        const int lane = threadIdx.x % kWarp;
+        if (lane < g.lanes)
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e)
+                part[threadIdx.x / kWarp * columns + lane * kVec<T> + e] = make_float2(db[e], dw[e]);
+    } else if (p.row < g.step) {
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e)
+            part[p.row * columns + p.lane * kVec<T> + e] = make_float2(db[e], dw[e]);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.channels; c += kThreads) {
+        float2 s = part[c];
+        for (int r = 1; r < rows; ++r) {
+            const float2 v = part[r * columns + c];
+            s.x += v.x;
+            s.y += v.y;
+        }
+        sums[p.first_channel + c] = s;
+        part[c] = s;
+    }
+    __syncthreads();
+    const int width = p.channels / p.groups;
+    for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int c = j * width + threadIdx.x % kWarp; c < (j + 1) * width; c += kWarp) {
+            const float w = to_f32<T>(weight[p.first_channel + c]);
+            s1 = fmaf(w, part[c].x, s1);
+            s2 = fmaf(w, part[c].y, s2);
+        }
+        s1 = warp_sum(s1);
+        s2 = warp_sum(s2);
+        if (threadIdx.x % kWarp == 0) group_sums[j] = make_float2(s1, s2);
+    }
+    __syncthreads();
+}
+
+// `sums`: [N * blocks, C] (dbias, dweight) of each block's rows.
+template <typename T, bool kAligned, bool kWhole>
+__global__ void __launch_bounds__(kThreads, 2)
+    group_norm_backward_kernel(Tensors<T> t, float2* __restrict__ sums, Geometry g, int act) {
+    extern __shared__ __align__(16) uint4 shared[];
+    __shared__ float2 means[kMaxSlabGroups];
+    const Place<T> p = Place<T>::template make<false>(g, t.lengths);
+    const int vectors = g.rows * g.lanes;
+    uint4* xs = shared;
+    uint4* ds = shared + vectors;
+    float2* part = reinterpret_cast<float2*>(shared + (1 + kPlanes<T>) * vectors);
+    const int mine = p.own_rows(), pitch = g.step * g.lanes, at = p.row * g.lanes + p.lane;
+    const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
+    const int64_t first = p.at(g, p.begin + p.row);
+    if (mine > 0) {
+        const T *x = t.x + first, *d = t.dout + first;
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i, x += stride, d += stride) {
+            stage<T, kAligned>(xs + at + i * pitch, x, p.count);
+            stage<T, kAligned>(ds + at + i * pitch, d, p.count);
+        }
+    }
+    Column<T, kWhole> column;
+    float db[kVec<T>], dw[kVec<T>];
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) db[e] = 0.0f, dw[e] = 0.0f;
+    if (mine > 0) column.template read<kAligned>(t, p, g);
+    arrived();
+#pragma unroll 2
+    for (int i = 0; i < mine; ++i) {
+        float x[kVec<T>], d[kVec<T>];
+        unpack<T>(xs[at + i * pitch], x);
+        unpack<T>(ds[at + i * pitch], d);
+        column.through(d, x, act);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e) {
+            db[e] += d[e];
+            dw[e] = fmaf(d[e], column.normalised(x[e], e), dw[e]);
+        }
+#pragma unroll
+        for (int q = 0; q < kPlanes<T>; ++q)
+            ds[q * vectors + at + i * pitch] =
+                make_uint4(__float_as_uint(d[4 * q]), __float_as_uint(d[4 * q + 1]),
+                           __float_as_uint(d[4 * q + 2]), __float_as_uint(d[4 * q + 3]));
+    }
+    add_up<T, kAligned>(db, dw, part, means,
+                        sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
+                        t.weight, p, g);
+    if (g.blocks > 1) {
+        float2* gathered = part + g.lanes * kVec<T>;  // behind the columns' sums: [block][group]
+        auto cluster = cg::this_cluster();
+        cluster.sync();  // every block runs, and has its sums
+        for (int q = threadIdx.x / kWarp; q < g.blocks; q += kBlockWarps)
+            for (int j = threadIdx.x % kWarp; j < p.groups; j += kWarp)
+                *cluster.map_shared_rank(gathered + p.block * g.slab_groups + j, q) = means[j];
+        cluster.sync();
+        if (threadIdx.x < p.groups) {
+            float2 s = make_float2(0.0f, 0.0f);
+            for (int q = 0; q < g.blocks; ++q) {
+                const float2 v = gathered[q * g.slab_groups + threadIdx.x];
+                s.x += v.x;
+                s.y += v.y;
+            }
+            means[threadIdx.x] = s;
+        }
+        __syncthreads();
+    }
+    if (mine > 0) {
+        const float inv = 1.0f / (static_cast<float>(p.m) * static_cast<float>(g.group_channels));
+        Final<T, kWhole> final_;
+        final_.make(column, means, inv, p, g);
+        T* to = t.dx + first;
+#pragma unroll 2
+        for (int i = 0; i < mine; ++i, to += stride) {
+            float x[kVec<T>], v[kVec<T>];
+            unpack<T>(xs[at + i * pitch], x);
+#pragma unroll
+            for (int q = 0; q < kPlanes<T>; ++q) {
+                float d[4];
+                unpack(ds[q * vectors + at + i * pitch], d, 0.0f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[4 * q + e] = final_(d[e], x[4 * q + e], column.scale[4 * q + e], 4 * q + e);
+            }
+            store<T, kAligned>(to, pack<T>(v), p.count);
+        }
+    }
+    zero_padding<T, kAligned>(t.dx, p, g);
+}
+
+// The two launches for what no cluster holds. The first leaves each block's (s1, s2) in
+// `partial` [N, G, parts * blocks].
+template <typename T, bool kAligned, bool kWhole>
+__global__ void __launch_bounds__(kThreads, 2)
+    group_norm_sums_kernel(Tensors<T> t, float2* __restrict__ sums, float2* __restrict__ partial,
+                           Geometry g, int act) {
+    extern __shared__ __align__(16) uint4 shared[];
+    __shared__ float2 group_sums[kMaxSlabGroups];
+    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
+    const int mine = p.own_rows();
+    float db[kVec<T>], dw[kVec<T>];
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) db[e] = 0.0f, dw[e] = 0.0f;
+    if (mine > 0) {
+        Column<T, kWhole> column;
+        column.template read<kAligned>(t, p, g);
+        const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
+        const int64_t first = p.at(g, p.begin + p.row);
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i) {
+            float x[kVec<T>], d[kVec<T>];
+            unpack<T>(load<T, kAligned>(t.x + first + i * stride, p.count), x);
+            unpack<T>(load<T, kAligned>(t.dout + first + i * stride, p.count), d);
+            column.through(d, x, act);
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e) {
+                db[e] += d[e];
+                dw[e] = fmaf(d[e], column.normalised(x[e], e), dw[e]);
+            }
+        }
+    }
+    add_up<T, kAligned>(db, dw, reinterpret_cast<float2*>(shared), group_sums,
+                        sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
+                        t.weight, p, g);
+    if (threadIdx.x < p.groups)
+        partial[(static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x) * g.parts *
+                    g.blocks +
+                p.slab % g.parts * g.blocks + p.block] = group_sums[threadIdx.x];
+}
+
+template <typename T, bool kAligned, bool kWhole>
+__global__ void __launch_bounds__(kThreads, 2)
+    group_norm_gradient_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g,
+                               int act) {
+    __shared__ float2 means[kMaxSlabGroups];
+    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
+    const int slots = g.parts * g.blocks;
+    for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+        const float2* from =
+            partial + (static_cast<int64_t>(p.n) * g.groups + p.first_group + j) * slots;
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int i = threadIdx.x % kWarp; i < slots; i += kWarp) {
+            s1 += from[i].x;
+            s2 += from[i].y;
+        }
+        s1 = warp_sum(s1);
+        s2 = warp_sum(s2);
+        if (threadIdx.x % kWarp == 0) means[j] = make_float2(s1, s2);
+    }
+    __syncthreads();
+    const int mine = p.own_rows();
+    if (mine > 0) {
+        const float inv = 1.0f / (static_cast<float>(p.m) * static_cast<float>(g.group_channels));
+        Column<T, kWhole> column;
+        column.template read<kAligned>(t, p, g);
+        Final<T, kWhole> final_;
+        final_.make(column, means, inv, p, g);
+        const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
+        const int64_t first = p.at(g, p.begin + p.row);
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i) {
+            float x[kVec<T>], d[kVec<T>];
+            unpack<T>(load<T, kAligned>(t.x + first + i * stride, p.count), x);
+            unpack<T>(load<T, kAligned>(t.dout + first + i * stride, p.count), d);
+            column.through(d, x, act);
+#pragma unroll
+            for (int e = 0; e < kVec<T>; ++e) d[e] = final_(d[e], x[e], column.scale[e], e);
+            store<T, kAligned>(t.dx + first + i * stride, pack<T>(d), p.count);
+        }
+    }
+    zero_padding<T, kAligned>(t.dx, p, g);
+}
+
+// Adds the blocks' rows of column sums, in an order that the launch fixes: a warp every
+// kSumWarps-th row of 32 channels.
+constexpr int kSumWarps = 32;
+template <typename T>
+__global__ void __launch_bounds__(kSumWarps* kWarp)
+    group_norm_parameters_kernel(const float2* __restrict__ sums, T* __restrict__ dweight,
+                                 T* __restrict__ dbias, int rows, int channels) {
+    __shared__ float2 part[kSumWarps][kWarp];
+    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+    const int c = blockIdx.x * kWarp + lane;
+    float2 s = make_float2(0.0f, 0.0f);
+    if (c < channels) {
+#pragma unroll 8
+        for (int r = warp; r < rows; r += kSumWarps) {
+            const float2 v = sums[static_cast<int64_t>(r) * channels + c];
+            s.x += v.x;
+            s.y += v.y;
+        }
+    }
+    part[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < channels) {
+        for (int w = 1; w < kSumWarps; ++w) {
+            s.x += part[w][lane].x;
+            s.y += part[w][lane].y;
+        }
+        dbias[c] = from_f32<T>(s.x);
+        dweight[c] = from_f32<T>(s.y);
     }
 }
 
-template <typename T>
-cudaError_t backward(const GroupNormBackwardProblem& p, cudaStream_t s) {
-    const T *dout = static_cast<const T*>(p.grad_output), *x = static_cast<const T*>(p.x),
-            *w = static_cast<const T*>(p.weight), *b = static_cast<const T*>(p.bias);
-    group_norm_backward_kernel<T><<<p.batch * p.groups, kThreads, 0, s>>>(
-        dout, x, p.valid_lengths, w, b, p.mean, p.rstd, static_cast<T*>(p.grad_x), p.length,
-        p.channels, p.groups, p.activation);
-    group_norm_parameters_kernel<T><<<p.channels, kThreads, 0, s>>>(
-        dout, x, p.valid_lengths, w, b, p.mean, p.rstd, static_cast<T*>(p.grad_weight),
-        static_cast<T*>(p.grad_bias), p.batch, p.length, p.channels, p.groups, p.activation);
+Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
+    const int element = p.dtype == FGA_FLOAT ? 4 : 2;
+    return group_norm::shape_of(p.batch, p.length, p.channels, p.groups, element, aligned,
+                                element == 4 ? kVectorBytes<float> : kVectorBytes<__half>,
+                                kTileBytes);
+}
+
+int64_t sum_rows(const Shape& s, int batch) { return static_cast<int64_t>(batch) * s.geo.blocks; }
+
+template <typename T, bool kAligned, bool kWhole>
+cudaError_t run(const GroupNormBackwardProblem& p, const Shape& s, cudaStream_t stream) {
+    static SmemAttr resident, first, second;
+    const Tensors<T> t{static_cast<const T*>(p.grad_output), static_cast<const T*>(p.x),
+                       p.valid_lengths, static_cast<const T*>(p.weight),
+                       static_cast<const T*>(p.bias), p.mean, p.rstd, static_cast<T*>(p.grad_x)};
+    const Geometry& g = s.geo;
+    float2* sums = static_cast<float2*>(p.workspace);
+    const int64_t rows = sum_rows(s, p.batch);
+    // The sums of a warp's rows of threads, or of each row of threads; behind the first of them
+    // what a cluster gathers.
+    const int columns = g.lanes * kVec<T> * static_cast<int>(sizeof(float2));
+    const int gather = g.blocks * g.slab_groups * static_cast<int>(sizeof(float2));
+    const int part = std::max(columns * (kWarp % g.lanes == 0 ? kBlockWarps : g.step),
+                              s.split ? 0 : columns + gather);
+    cudaError_t e;
+    if (!s.split) {
+        e = launch(resident, group_norm_backward_kernel<T, kAligned, kWhole>, s, true,
+                   g.rows * g.lanes * kVectorBytes<T> + part,
+                   kTileBytes + kThreads * kVectorBytes<T> + kSumBytes<T> + kGatherBytes, stream, t,
+                   sums, g, p.activation);
+    } else {
+        float2* partial = sums + rows * p.channels;
+        e = launch(first, group_norm_sums_kernel<T, kAligned, kWhole>, s, false, part, kSumBytes<T>,
+                   stream, t, sums, partial, g, p.activation);
+        if (e == cudaSuccess)
+            e = launch(second, group_norm_gradient_kernel<T, kAligned, kWhole>, s, false, 0, 0,
+                       stream, t, static_cast<const float2*>(partial), g, p.activation);
+    }
+    if (e != cudaSuccess) return e;
+    group_norm_parameters_kernel<T><<<(p.channels + kWarp - 1) / kWarp, kSumWarps * kWarp, 0, stream>>>(
+        sums, static_cast<T*>(p.grad_weight), static_cast<T*>(p.grad_bias), static_cast<int>(rows),
+        p.channels);
     return cudaGetLastError();
+}
+
+template <typename T> cudaError_t run(const GroupNormBackwardProblem& p, cudaStream_t stream) {
+    const Shape s = shape_of(p, aligned16({p.grad_output, p.x, p.weight, p.bias, p.grad_x}));
+    if (!s.aligned) return run<T, false, false>(p, s, stream);
+    return s.whole ? run<T, true, true>(p, s, stream) : run<T, true, false>(p, s, stream);
 }
 
 }  // namespace
 
-size_t group_norm_backward_workspace(const GroupNormBackwardProblem&) { return 0; }
+size_t group_norm_backward_workspace(const GroupNormBackwardProblem& p) {
+    size_t most = 0;
+    for (bool aligned : {true, false}) {
+        const Shape s = shape_of(p, aligned);
+        size_t values = static_cast<size_t>(sum_rows(s, p.batch)) * p.channels;
+        if (s.split)
+            values += static_cast<size_t>(p.batch) * p.groups * s.geo.parts * s.geo.blocks;
+        most = std::max(most, values * sizeof(float2));
+    }
+    return most;
+}
 
 cudaError_t launch_group_norm_backward(const GroupNormBackwardProblem& p, cudaStream_t s,
                                        const char** variant) {
     *variant = "group-norm-backward";
-    if (p.dtype == FGA_FLOAT) return backward<float>(p, s);
-    if (p.dtype == FGA_HALF) return backward<__half>(p, s);
-    return backward<__nv_bfloat16>(p, s);
+    if (p.dtype == FGA_FLOAT) return run<float>(p, s);
+    if (p.dtype == FGA_HALF) return run<__half>(p, s);
+    return run<__nv_bfloat16>(p, s);
 }
 
 }  // namespace fga
