@@ -154,7 +154,7 @@ __device__ __forceinline__ void add_up(float (&db)[kVec<T>], float (&dw)[kVec<T>
 
 // `sums`: [N * blocks, C] (dbias, dweight) of each block's rows.
 template <typename T, bool kAligned, bool kWhole>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
     group_norm_backward_kernel(Tensors<T> t, float2* __restrict__ sums, Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
     __shared__ float2 means[kMaxSlabGroups];
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 // The two launches for what no cluster holds. The first leaves each block's (s1, s2) in
 // `partial` [N, G, parts * blocks].
 template <typename T, bool kAligned, bool kWhole>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
     group_norm_sums_kernel(Tensors<T> t, float2* __restrict__ sums, float2* __restrict__ partial,
                            Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 template <typename T, bool kAligned, bool kWhole>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
     group_norm_gradient_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g,
                                int act) {
     __shared__ float2 means[kMaxSlabGroups];
