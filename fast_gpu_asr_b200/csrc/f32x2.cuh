@@ -1,0 +1,81 @@
+// Pairs of fp32 in one instruction (sm_100: fma, add and mul on f32x2). The kernels that use
+// them are bound by instruction issue before they are bound by HBM; a pair takes one issue slot
+// instead of two. Each half rounds as its scalar instruction would.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace fga {
+
+__device__ __forceinline__ uint64_t bits_of(float2 v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 pair_of(uint64_t r) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ float2 splat2(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+
+// A pair of a 16-bit type in one register.
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t r);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t r) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&r));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t r) {
+    return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float2 v);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float2 v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The special functions flush subnormals: otherwise each costs three more instructions.
+__device__ __forceinline__ float exp2_approx(float v) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v));
+    return e;
+}
+__device__ __forceinline__ float log2_approx(float v) {
+    float l;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(l) : "f"(v));
+    return l;
+}
+__device__ __forceinline__ float reciprocal_approx(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// 1 / (1 + exp(-v))
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+    const float2 t = mul2(v, splat2(-1.4426950408889634f));
+    const float2 d = add2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), splat2(1.0f));
+    return make_float2(reciprocal_approx(d.x), reciprocal_approx(d.y));
+}
+
+}  // namespace fga

@@ -37,53 +37,58 @@ template <typename Visit> __device__ __forceinline__ float2 merge(float total, V
     return make_float2(mean, warp_sum(squares));
 }
 
-// (mean, squares) of every group of the slab over this block's rows, which its threads have in
-// `tile`, to moments[group]. `part` holds an entry per thread (and channel, if not kWhole).
+// (mean, squares) of every group of the slab over this block's rows to moments[group]; row(i)
+// is this thread's vector of its i-th row. `part` holds an entry per thread (and channel, if
+// not kWhole).
 //
 // A thread takes both in one pass, about a pivot: the mean of its own first vector (the first
 // value of each channel). With n values and the first q of them in the pivot, squares about
 // the mean are at least q (pivot - mean)^2, so the n (pivot - mean)^2 taken off the squares
-// about the pivot is at most n / q times what is left: with at most kTileBytes / 4096 rows a
-// thread, a factor of 12 on a rounding error.
-template <typename T, bool kWhole>
-__device__ __forceinline__ void block_moments(const uint4* tile, float2* part, float2* moments,
+// about the pivot is at most n / q times what is left, a factor on its rounding error: with 12
+// rows of a tile or 64 of a split launch at most, and values that differ like that only where
+// the first vector is an outlier itself.
+template <typename T, bool kWhole, typename Row>
+__device__ __forceinline__ void block_moments(Row row, float2* part, float2* moments,
                                               const Place<T>& p, const Geometry& g) {
-    constexpr int kValues = kWhole ? 1 : kVec<T>;
+    constexpr int kValues = kWhole ? 1 : kVec<T>, kSums = kWhole ? 1 : kPairs<T>;
     const int mine = p.own_rows(), columns = g.lanes * kValues;
     if (mine > 0) {
-        const uint4* at = tile + p.row * g.lanes + p.lane;
-        const int pitch = g.step * g.lanes;
-        float pivot[kValues], sum[kValues], squares[kValues], v[kVec<T>];
-        unpack<T>(at[0], v);
+        float2 pivot[kSums], sum[kSums], squares[kSums], v[kPairs<T>];
+        unpack<T>(row(0), v);
         if constexpr (kWhole) {
-            float s = 0.0f;
+            float2 s = v[0];
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e) s += v[e];
-            pivot[0] = s * (1.0f / kVec<T>);
+            for (int i = 1; i < kPairs<T>; ++i) s = add2(s, v[i]);
+            pivot[0] = splat2((s.x + s.y) * (-1.0f / kVec<T>));  // negative
         } else {
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e) pivot[e] = v[e];
+            for (int i = 0; i < kPairs<T>; ++i) pivot[i] = make_float2(-v[i].x, -v[i].y);
         }
 #pragma unroll
-        for (int e = 0; e < kValues; ++e) sum[e] = 0.0f, squares[e] = 0.0f;
+        for (int k = 0; k < kSums; ++k) sum[k] = squares[k] = splat2(0.0f);
 #pragma unroll 4
         for (int i = 0; i < mine; ++i) {
-            unpack<T>(at[i * pitch], v);
+            unpack<T>(row(i), v);
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e) {
+            for (int e = 0; e < kPairs<T>; ++e) {
                 constexpr bool kOne = kWhole;
                 const int k = kOne ? 0 : e;
-                const float d = v[e] - pivot[k];
-                sum[k] += d;
-                squares[k] = fmaf(d, d, squares[k]);
+                const float2 d = add2(v[e], pivot[k]);
+                sum[k] = add2(sum[k], d);
+                squares[k] = fma2(d, d, squares[k]);
             }
         }
         const float inv = 1.0f / static_cast<float>(mine * (kWhole ? kVec<T> : 1));
 #pragma unroll
         for (int e = 0; e < kValues; ++e) {
-            const float off = sum[e] * inv;  // mean - pivot
+            float s = channel_of(sum, e), q = channel_of(squares, e);
+            if constexpr (kWhole) {
+                s += sum[0].y;
+                q += squares[0].y;
+            }
+            const float off = s * inv;  // mean - pivot
             part[p.row * columns + p.lane * kValues + e] =
-                make_float2(pivot[e] + off, fmaxf(fmaf(-sum[e], off, squares[e]), 0.0f));
+                make_float2(off - channel_of(pivot, e), fmaxf(fmaf(-s, off, q), 0.0f));
         }
     }
     __syncthreads();
@@ -105,7 +110,7 @@ __device__ __forceinline__ void block_moments(const uint4* tile, float2* part, f
 // scale. Next to (x - mean) scale + bias this costs two roundings of mean * scale, what the
 // rounding of the mean to fp32 costs in either form, and saves an instruction an element.
 template <typename T> struct Column {
-    float scale[kVec<T>], shift[kVec<T>];
+    float2 scale[kPairs<T>], shift[kPairs<T>];
     // `stats`: (mean, rstd) of the slab's groups.
     template <bool kAligned, bool kWhole>
     __device__ __forceinline__ void read(const T* w, const T* b, const float2* stats,
@@ -113,17 +118,18 @@ template <typename T> struct Column {
         unpack<T>(load<T, kAligned>(w + p.channel(), p.count), scale);
         unpack<T>(load<T, kAligned>(b + p.channel(), p.count), shift);
 #pragma unroll
-        for (int e = 0; e < kVec<T>; ++e) {
-            const float2 s = stats[p.group_of(kWhole ? 0 : e, g)];
-            scale[e] *= s.y;
-            shift[e] = fmaf(-s.x, scale[e], shift[e]);
+        for (int i = 0; i < kPairs<T>; ++i) {
+            const float2 s = stats[p.group_of(kWhole ? 0 : 2 * i, g)];
+            const float2 t = kWhole ? s : stats[p.group_of(2 * i + 1, g)];
+            scale[i] = mul2(scale[i], make_float2(s.y, t.y));
+            shift[i] = fma2(make_float2(-s.x, -t.x), scale[i], shift[i]);
         }
     }
     __device__ __forceinline__ uint4 apply(const uint4& r, int act) const {
-        float v[kVec<T>];
+        float2 v[kPairs<T>];
         unpack<T>(r, v);
 #pragma unroll
-        for (int e = 0; e < kVec<T>; ++e) v[e] = fmaf(v[e], scale[e], shift[e]);
+        for (int i = 0; i < kPairs<T>; ++i) v[i] = fma2(v[i], scale[i], shift[i]);
         activate(v, act);
         return pack<T>(v);
     }
@@ -143,14 +149,13 @@ template <typename T> struct Tensors {
     float* rstd;
 };
 
-// kPartial: leaves the blocks' moments in `partial` [N, G, parts * blocks], nothing else.
-template <typename T, bool kAligned, bool kWhole, bool kPartial>
+template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 4)
-    group_norm_kernel(Tensors<T> t, float2* __restrict__ partial, Geometry g, float eps, int act) {
+    group_norm_kernel(Tensors<T> t, Geometry g, float eps, int act) {
     extern __shared__ __align__(16) uint4 tile[];
     __shared__ float2 part[kWhole ? kThreads : kThreads * kVec<T>];
     __shared__ float2 moments[kMaxSlabGroups];
-    const Place<T> p = Place<T>::template make<kPartial>(g, t.lengths);
+    const Place<T> p = Place<T>::template make<false>(g, t.lengths);
     const int mine = p.own_rows(), pitch = g.step * g.lanes;
     uint4* at = tile + p.row * g.lanes + p.lane;
     const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
@@ -161,59 +166,70 @@ __global__ void __launch_bounds__(kThreads, 4)
             stage<T, kAligned>(at + i * pitch, from, p.count);
     }
     arrived();
-    block_moments<T, kWhole>(tile, part, moments, p, g);
+    block_moments<T, kWhole>([&](int i) { return at[i * pitch]; }, part, moments, p, g);
     __syncthreads();
     const float width = static_cast<float>(g.group_channels);
-    if constexpr (kPartial) {
-        const int slots = g.parts * g.blocks;
-        if (threadIdx.x < p.groups)
-            partial[(static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x) * slots +
-                    p.slab % g.parts * g.blocks + p.block] = moments[threadIdx.x];
-    } else {
-        const float total = static_cast<float>(p.m) * width;
-        if (g.blocks > 1) {
-            // Behind the tile: [block][group].
-            float2* gathered = reinterpret_cast<float2*>(tile + g.rows * g.lanes);
-            auto cluster = cg::this_cluster();
-            cluster.sync();  // every block runs, and may be written to
-            for (int q = threadIdx.x / kWarp; q < g.blocks; q += kBlockWarps)
-                for (int j = threadIdx.x % kWarp; j < p.groups; j += kWarp)
-                    *cluster.map_shared_rank(gathered + p.block * g.slab_groups + j, q) = moments[j];
-            cluster.sync();
-            const int each = g.by_blocks.quotient(p.m + g.blocks - 1);
-            for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
-                const float2 r = merge(total, [&](auto add) {
-                    for (int i = threadIdx.x % kWarp; i < g.blocks; i += kWarp)
-                        add(static_cast<float>(max(0, min(each, p.m - i * each))) * width,
-                            gathered[i * g.slab_groups + j]);
-                });
-                if (threadIdx.x % kWarp == 0) moments[j] = r;
-            }
-            __syncthreads();
-        }
-        if (threadIdx.x < p.groups) {
-            const float2 s = to_stats(moments[threadIdx.x], total, eps);
-            moments[threadIdx.x] = s;
-            if (p.block == 0) {
-                const int64_t i = static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x;
-                if (t.mean != nullptr) t.mean[i] = s.x;
-                if (t.rstd != nullptr) t.rstd[i] = s.y;
-            }
+    const float total = static_cast<float>(p.m) * width;
+    if (g.blocks > 1) {
+        // Behind the tile: [block][group].
+        float2* gathered = reinterpret_cast<float2*>(tile + g.rows * g.lanes);
+        auto cluster = cg::this_cluster();
+        cluster.sync();  // every block runs, and may be written to
+        for (int q = threadIdx.x / kWarp; q < g.blocks; q += kBlockWarps)
+            for (int j = threadIdx.x % kWarp; j < p.groups; j += kWarp)
+                *cluster.map_shared_rank(gathered + p.block * g.slab_groups + j, q) = moments[j];
+        cluster.sync();
+        const int each = g.by_blocks.quotient(p.m + g.blocks - 1);
+        for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+            const float2 r = merge(total, [&](auto add) {
+                for (int i = threadIdx.x % kWarp; i < g.blocks; i += kWarp)
+                    add(static_cast<float>(max(0, min(each, p.m - i * each))) * width,
+                        gathered[i * g.slab_groups + j]);
+            });
+            if (threadIdx.x % kWarp == 0) moments[j] = r;
         }
         __syncthreads();
-        if (mine > 0) {
-            Column<T> column;
-            column.template read<kAligned, kWhole>(t.weight, t.bias, moments, p, g);
-            T* to = t.out + p.at(g, p.begin + p.row);
-#pragma unroll 2
-            for (int i = 0; i < mine; ++i, to += stride)
-                store<T, kAligned>(to, column.apply(at[i * pitch], act), p.count);
-        }
-        zero_padding<T, kAligned>(t.out, p, g);
     }
+    if (threadIdx.x < p.groups) {
+        const float2 s = to_stats(moments[threadIdx.x], total, eps);
+        moments[threadIdx.x] = s;
+        if (p.block == 0) {
+            const int64_t i = static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x;
+            if (t.mean != nullptr) t.mean[i] = s.x;
+            if (t.rstd != nullptr) t.rstd[i] = s.y;
+        }
+    }
+    __syncthreads();
+    if (mine > 0) {
+        Column<T> column;
+        column.template read<kAligned, kWhole>(t.weight, t.bias, moments, p, g);
+        T* to = t.out + p.at(g, p.begin + p.row);
+#pragma unroll 2
+        for (int i = 0; i < mine; ++i, to += stride)
+            store<T, kAligned>(to, column.apply(at[i * pitch], act), p.count);
+    }
+    zero_padding<T, kAligned>(t.out, p, g);
 }
 
-// The second launch: merges the partial moments and applies them.
+// The two launches for what no cluster holds. The first leaves each block's moments in
+// `partial` [N, G, parts * blocks], the second merges and applies them.
+template <typename T, bool kAligned, bool kWhole>
+__global__ void __launch_bounds__(kThreads, 4)
+    group_norm_moments_kernel(Tensors<T> t, float2* __restrict__ partial, Geometry g) {
+    __shared__ float2 part[kWhole ? kThreads : kThreads * kVec<T>];
+    __shared__ float2 moments[kMaxSlabGroups];
+    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
+    const T* from = t.x + p.at(g, p.begin + p.row);
+    const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
+    block_moments<T, kWhole>([&](int i) { return load<T, kAligned>(from + i * stride, p.count); },
+                             part, moments, p, g);
+    __syncthreads();
+    if (threadIdx.x < p.groups)
+        partial[(static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x) * g.parts *
+                    g.blocks +
+                p.slab % g.parts * g.blocks + p.block] = moments[threadIdx.x];
+}
+
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 4)
     group_norm_apply_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g, float eps,
@@ -264,14 +280,14 @@ cudaError_t run(const GroupNormProblem& p, const Shape& s, cudaStream_t stream) 
     const Tensors<T> t{static_cast<const T*>(p.x), p.valid_lengths, static_cast<const T*>(p.weight),
                        static_cast<const T*>(p.bias), static_cast<T*>(p.output), p.mean, p.rstd};
     const Geometry& g = s.geo;
-    const int smem = g.rows * g.lanes * 16, most = kTileBytes + kThreads * 16 + kGatherBytes;
     const int gather = g.blocks > 1 ? g.blocks * g.slab_groups * static_cast<int>(sizeof(float2)) : 0;
+    const int most = kTileBytes + kThreads * 16 + kGatherBytes;
     float2* ws = static_cast<float2*>(p.workspace);
     if (!s.split)
-        return launch(resident, group_norm_kernel<T, kAligned, kWhole, false>, s, true,
-                      smem + gather, most, stream, t, ws, g, p.eps, p.activation);
-    const cudaError_t e = launch(partial, group_norm_kernel<T, kAligned, kWhole, true>, s, false,
-                                 smem, most, stream, t, ws, g, p.eps, p.activation);
+        return launch(resident, group_norm_kernel<T, kAligned, kWhole>, s, true,
+                      g.rows * g.lanes * 16 + gather, most, stream, t, g, p.eps, p.activation);
+    const cudaError_t e = launch(partial, group_norm_moments_kernel<T, kAligned, kWhole>, s, false,
+                                 0, 0, stream, t, ws, g);
     if (e != cudaSuccess) return e;
     return launch(apply, group_norm_apply_kernel<T, kAligned, kWhole>, s, false, 0, 0, stream, t,
                   static_cast<const float2*>(ws), g, p.eps, p.activation);

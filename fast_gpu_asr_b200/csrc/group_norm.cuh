@@ -15,6 +15,7 @@
 #include <numeric>
 
 #include "../../include/fga_convolution.h"
+#include "f32x2.cuh"
 #include "fga_common.cuh"
 #include "host_util.h"
 
@@ -29,53 +30,30 @@ constexpr int kMaxSlabGroups = 64;
 
 template <typename T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 
+template <typename T> constexpr int kPairs = kVec<T> / 2;
+
 // ---- vectors -------------------------------------------------------------------------------
-__device__ __forceinline__ void unpack(const uint4& r, float (&v)[4], float) {
-    v[0] = __uint_as_float(r.x);
-    v[1] = __uint_as_float(r.y);
-    v[2] = __uint_as_float(r.z);
-    v[3] = __uint_as_float(r.w);
-}
-__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], __half) {
-    const __half2* h = reinterpret_cast<const __half2*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(h[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+template <typename T> __device__ __forceinline__ void unpack(const uint4& r, float2 (&v)[kPairs<T>]) {
+    if constexpr (sizeof(T) == 4) {
+        v[0] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+        v[1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
+    } else {
+        v[0] = unpack2<T>(r.x);
+        v[1] = unpack2<T>(r.y);
+        v[2] = unpack2<T>(r.z);
+        v[3] = unpack2<T>(r.w);
     }
 }
-__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], __nv_bfloat16) {
-    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
+template <typename T> __device__ __forceinline__ uint4 pack(const float2 (&v)[kPairs<T>]) {
+    if constexpr (sizeof(T) == 4)
+        return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
+                          __float_as_uint(v[1].y));
+    else
+        return make_uint4(pack2<T>(v[0]), pack2<T>(v[1]), pack2<T>(v[2]), pack2<T>(v[3]));
 }
-template <typename T> __device__ __forceinline__ void unpack(const uint4& r, float (&v)[kVec<T>]) {
-    unpack(r, v, T{});
-}
-__device__ __forceinline__ uint4 pack(const float (&v)[4], float) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                      __float_as_uint(v[3]));
-}
-__device__ __forceinline__ uint4 pack(const float (&v)[8], __half) {
-    uint4 r;
-    __half2* h = reinterpret_cast<__half2*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    return r;
-}
-__device__ __forceinline__ uint4 pack(const float (&v)[8], __nv_bfloat16) {
-    uint4 r;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    return r;
-}
-template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[kVec<T>]) {
-    return pack(v, T{});
+// Channel e of a vector.
+template <int kCount> __device__ __forceinline__ float& channel_of(float2 (&v)[kCount], int e) {
+    return e % 2 == 0 ? v[e / 2].x : v[e / 2].y;
 }
 
 // `count` channels at p, which need only be aligned to their type unless kAligned; the others
@@ -120,43 +98,34 @@ __device__ __forceinline__ void arrived() {
 }
 
 // ---- activations ---------------------------------------------------------------------------
-// The special functions flush subnormals: otherwise each costs three more instructions.
-__device__ __forceinline__ float exp_of(float v) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * kLog2e));
-    return e;
-}
-__device__ __forceinline__ float reciprocal(float v) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
-__device__ __forceinline__ float sigmoid(float v) { return reciprocal(1.0f + exp_of(-v)); }
-
-template <int kCount> __device__ __forceinline__ void activate(float (&z)[kCount], int act) {
+template <int kCount> __device__ __forceinline__ void activate(float2 (&z)[kCount], int act) {
     if (act == FGA_ACTIVATION_SILU) {
 #pragma unroll
-        for (int e = 0; e < kCount; ++e) z[e] *= sigmoid(z[e]);
+        for (int i = 0; i < kCount; ++i) z[i] = mul2(z[i], sigmoid2(z[i]));
     } else if (act == FGA_ACTIVATION_SWOOSH_R) {
 #pragma unroll
-        for (int e = 0; e < kCount; ++e) {
-            const float v = z[e] - 1.0f;
+        for (int i = 0; i < kCount; ++i) {
             // softplus(v) = max(v, 0) + log(1 + exp(-|v|)); the logarithm's argument is in
             // [1, 2], where a log2 of absolute error 2^-22 is as good as log1p next to the sum.
-            float l;
-            asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(l) : "f"(1.0f + exp_of(-fabsf(v))));
-            z[e] = fmaxf(v, 0.0f) + 0.69314718f * l - 0.08f * z[e] - 0.313261687f;
+            const float2 v = add2(z[i], splat2(-1.0f));
+            const float2 e = make_float2(exp2_approx(fabsf(v.x) * -kLog2e),
+                                         exp2_approx(fabsf(v.y) * -kLog2e));
+            const float2 d = add2(e, splat2(1.0f));
+            const float2 l = make_float2(log2_approx(d.x), log2_approx(d.y));
+            const float2 rest = fma2(z[i], splat2(-0.08f), splat2(-0.313261687f));
+            z[i] = add2(fma2(l, splat2(0.69314718f), make_float2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f))),
+                        rest);
         }
     }
 }
 
 // act'(z)
-template <int kAct> __device__ __forceinline__ float slope(float z) {
+template <int kAct> __device__ __forceinline__ float2 slope(float2 z) {
     if constexpr (kAct == FGA_ACTIVATION_SILU) {
-        const float s = sigmoid(z);
-        return s * fmaf(z, 1.0f - s, 1.0f);
+        const float2 s = sigmoid2(z);
+        return mul2(s, fma2(z, fma2(s, splat2(-1.0f), splat2(1.0f)), splat2(1.0f)));
     } else {
-        return sigmoid(z - 1.0f) - 0.08f;
+        return add2(sigmoid2(add2(z, splat2(-1.0f))), splat2(-0.08f));
     }
 }
 
@@ -332,14 +301,18 @@ inline Shape shape_of(int batch, int length, int channels, int groups, int eleme
     // Enough blocks for two on every multiprocessor, as long as each has rows for its threads.
     const int64_t fill = std::min<int64_t>((2LL * sm_count() + s.units - 1) / s.units,
                                            (length + 2 * g.step - 1) / (2 * g.step));
-    const int64_t blocks = std::max<int64_t>({(length + fit - 1) / fit, fill, 1});
-    s.split = g.parts > 1 || (length + fit - 1) / fit > kMaxCluster;
+    const int64_t needed = (length + fit - 1) / fit;
+    s.split = g.parts > 1 || needed > kMaxCluster;
     if (s.split) {
-        const int64_t rows = (length + blocks - 1) / blocks;
-        g.rows = static_cast<int>(rows);
-        g.blocks = static_cast<int>((length + rows - 1) / rows);
+        // Eight blocks for every multiprocessor, of at least 4 rows a thread (a block's sums
+        // cost as much as some rows) and at most 64.
+        const int64_t share = length * s.units / (8LL * std::max(1, sm_count())) + 1;
+        const int64_t rows = std::max<int64_t>(4 * g.step, std::min<int64_t>(64 * g.step, share));
+        g.rows = static_cast<int>(std::min<int64_t>(rows, length));
+        g.blocks = (length + g.rows - 1) / g.rows;
     } else {
-        g.blocks = static_cast<int>(std::min<int64_t>(blocks, kMaxCluster));
+        g.blocks = static_cast<int>(std::min<int64_t>({std::max(needed, fill), kMaxCluster}));
+        g.blocks = std::max(1, g.blocks);
         g.rows = (length + g.blocks - 1) / g.blocks;
     }
     g.by_blocks = Divisor(g.blocks);

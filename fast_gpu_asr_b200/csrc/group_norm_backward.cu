@@ -40,10 +40,10 @@ template <typename T> struct Tensors {
     T* dx;
 };
 
-// A column's parameters: z = x scale + shift, xhat = x rstd - centre.
+// A column's parameters: z = x scale + shift, xhat = x rstd + centre.
 template <typename T, bool kWhole> struct Column {
-    static constexpr int kStats = kWhole ? 1 : kVec<T>;
-    float scale[kVec<T>], shift[kVec<T>], rstd[kStats], centre[kStats];
+    static constexpr int kStats = kWhole ? 1 : kPairs<T>;
+    float2 scale[kPairs<T>], shift[kPairs<T>], rstd[kStats], centre[kStats];
     template <bool kAligned>
     __device__ __forceinline__ void read(const Tensors<T>& t, const Place<T>& p, const Geometry& g) {
         unpack<T>(load<T, kAligned>(t.weight + p.channel(), p.count), scale);
@@ -51,56 +51,61 @@ template <typename T, bool kWhole> struct Column {
         const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group;
 #pragma unroll
         for (int k = 0; k < kStats; ++k) {
-            rstd[k] = t.rstd[group + p.group_of(k, g)];
-            centre[k] = t.mean[group + p.group_of(k, g)] * rstd[k];
+            const int64_t i = group + p.group_of(2 * k, g);
+            const int64_t j = kWhole ? i : group + p.group_of(2 * k + 1, g);
+            rstd[k] = make_float2(t.rstd[i], t.rstd[j]);
+            centre[k] = mul2(make_float2(-t.mean[i], -t.mean[j]), rstd[k]);
         }
 #pragma unroll
-        for (int e = 0; e < kVec<T>; ++e) {
-            shift[e] = fmaf(-centre[kWhole ? 0 : e], scale[e], shift[e]);
-            scale[e] *= rstd[kWhole ? 0 : e];
+        for (int e = 0; e < kPairs<T>; ++e) {
+            shift[e] = fma2(centre[kWhole ? 0 : e], scale[e], shift[e]);
+            scale[e] = mul2(scale[e], rstd[kWhole ? 0 : e]);
         }
     }
-    __device__ __forceinline__ float normalised(float x, int e) const {
-        return fmaf(x, rstd[kWhole ? 0 : e], -centre[kWhole ? 0 : e]);
+    __device__ __forceinline__ float2 normalised(float2 x, int e) const {
+        return fma2(x, rstd[kWhole ? 0 : e], centre[kWhole ? 0 : e]);
     }
     // dout to dz.
-    __device__ __forceinline__ void through(float (&d)[kVec<T>], const float (&x)[kVec<T>],
+    __device__ __forceinline__ void through(float2 (&d)[kPairs<T>], const float2 (&x)[kPairs<T>],
                                             int act) const {
         if (act == FGA_ACTIVATION_SILU) {
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e)
-                d[e] *= slope<FGA_ACTIVATION_SILU>(fmaf(x[e], scale[e], shift[e]));
+            for (int e = 0; e < kPairs<T>; ++e)
+                d[e] = mul2(d[e], slope<FGA_ACTIVATION_SILU>(fma2(x[e], scale[e], shift[e])));
         } else if (act == FGA_ACTIVATION_SWOOSH_R) {
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e)
-                d[e] *= slope<FGA_ACTIVATION_SWOOSH_R>(fmaf(x[e], scale[e], shift[e]));
+            for (int e = 0; e < kPairs<T>; ++e)
+                d[e] = mul2(d[e], slope<FGA_ACTIVATION_SWOOSH_R>(fma2(x[e], scale[e], shift[e])));
         }
     }
 };
 
 // dx = dz scale + x slope + offset, with the group's means m1 = s1 / (M Cg), m2 = s2 / (M Cg):
-// slope = -rstd^2 m2, offset = rstd (centre m2 - m1).
+// slope = -rstd^2 m2, offset = -rstd (centre m2 + m1).
 template <typename T, bool kWhole> struct Final {
-    static constexpr int kStats = kWhole ? 1 : kVec<T>;
-    float slope[kStats], offset[kStats];
+    static constexpr int kStats = kWhole ? 1 : kPairs<T>;
+    float2 slope[kStats], offset[kStats];
     __device__ __forceinline__ void make(const Column<T, kWhole>& column, const float2* sums,
                                          float inv, const Place<T>& p, const Geometry& g) {
 #pragma unroll
         for (int k = 0; k < kStats; ++k) {
-            const float2 m = make_float2(sums[p.group_of(k, g)].x * inv, sums[p.group_of(k, g)].y * inv);
-            slope[k] = -column.rstd[k] * column.rstd[k] * m.y;
-            offset[k] = column.rstd[k] * fmaf(column.centre[k], m.y, -m.x);
+            const float2 a = sums[p.group_of(2 * k, g)];
+            const float2 b = kWhole ? a : sums[p.group_of(2 * k + 1, g)];
+            const float2 m1 = make_float2(a.x * -inv, b.x * -inv);  // negative
+            const float2 m2 = make_float2(a.y * -inv, b.y * -inv);
+            slope[k] = mul2(mul2(column.rstd[k], column.rstd[k]), m2);
+            offset[k] = mul2(column.rstd[k], fma2(column.centre[k], m2, m1));
         }
     }
-    __device__ __forceinline__ float operator()(float dz, float x, float scale, int e) const {
-        return fmaf(dz, scale, fmaf(x, slope[kWhole ? 0 : e], offset[kWhole ? 0 : e]));
+    __device__ __forceinline__ float2 operator()(float2 dz, float2 x, float2 scale, int e) const {
+        return fma2(dz, scale, fma2(x, slope[kWhole ? 0 : e], offset[kWhole ? 0 : e]));
     }
 };
 
 // Adds the threads' column sums: (dbias, dweight) of the block's rows to `sums` (also left in
 // shared memory at part[0..]), and of each group (s1, s2), weighted, to group_sums.
 template <typename T, bool kAligned>
-__device__ __forceinline__ void add_up(float (&db)[kVec<T>], float (&dw)[kVec<T>], float2* part,
+__device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>], float2* part,
                                        float2* group_sums, float2* __restrict__ sums,
                                        const T* __restrict__ weight, const Place<T>& p,
                                        const Geometry& g) {
@@ -110,20 +115,24 @@ __device__ __forceinline__ void add_up(float (&db)[kVec<T>], float (&dw)[kVec<T>
         // Whole rows of threads in a warp: the warp's own sum first.
         for (int o = g.lanes; o < kWarp; o *= 2)
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e) {
-                db[e] += __shfl_xor_sync(0xffffffffu, db[e], o);
-                dw[e] += __shfl_xor_sync(0xffffffffu, dw[e], o);
+            for (int e = 0; e < kPairs<T>; ++e) {
+                db[e] = add2(db[e], make_float2(__shfl_xor_sync(0xffffffffu, db[e].x, o),
+                                                __shfl_xor_sync(0xffffffffu, db[e].y, o)));
+                dw[e] = add2(dw[e], make_float2(__shfl_xor_sync(0xffffffffu, dw[e].x, o),
+                                                __shfl_xor_sync(0xffffffffu, dw[e].y, o)));
             }
         rows = kBlockWarps;
         const int lane = threadIdx.x % kWarp;
         if (lane < g.lanes)
 #pragma unroll
             for (int e = 0; e < kVec<T>; ++e)
-                part[threadIdx.x / kWarp * columns + lane * kVec<T> + e] = make_float2(db[e], dw[e]);
+                part[threadIdx.x / kWarp * columns + lane * kVec<T> + e] =
+                    make_float2(channel_of(db, e), channel_of(dw, e));
     } else if (p.row < g.step) {
 #pragma unroll
         for (int e = 0; e < kVec<T>; ++e)
-            part[p.row * columns + p.lane * kVec<T> + e] = make_float2(db[e], dw[e]);
+            part[p.row * columns + p.lane * kVec<T> + e] =
+                make_float2(channel_of(db, e), channel_of(dw, e));
     }
     __syncthreads();
     for (int c = threadIdx.x; c < p.channels; c += kThreads) {
@@ -175,27 +184,27 @@ __global__ void __launch_bounds__(kThreads, 3)
         }
     }
     Column<T, kWhole> column;
-    float db[kVec<T>], dw[kVec<T>];
+    float2 db[kPairs<T>], dw[kPairs<T>];
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) db[e] = 0.0f, dw[e] = 0.0f;
+    for (int e = 0; e < kPairs<T>; ++e) db[e] = dw[e] = splat2(0.0f);
     if (mine > 0) column.template read<kAligned>(t, p, g);
     arrived();
 #pragma unroll 2
     for (int i = 0; i < mine; ++i) {
-        float x[kVec<T>], d[kVec<T>];
+        float2 x[kPairs<T>], d[kPairs<T>];
         unpack<T>(xs[at + i * pitch], x);
         unpack<T>(ds[at + i * pitch], d);
         column.through(d, x, act);
 #pragma unroll
-        for (int e = 0; e < kVec<T>; ++e) {
-            db[e] += d[e];
-            dw[e] = fmaf(d[e], column.normalised(x[e], e), dw[e]);
+        for (int e = 0; e < kPairs<T>; ++e) {
+            db[e] = add2(db[e], d[e]);
+            dw[e] = fma2(d[e], column.normalised(x[e], e), dw[e]);
         }
 #pragma unroll
         for (int q = 0; q < kPlanes<T>; ++q)
             ds[q * vectors + at + i * pitch] =
-                make_uint4(__float_as_uint(d[4 * q]), __float_as_uint(d[4 * q + 1]),
-                           __float_as_uint(d[4 * q + 2]), __float_as_uint(d[4 * q + 3]));
+                make_uint4(__float_as_uint(d[2 * q].x), __float_as_uint(d[2 * q].y),
+                           __float_as_uint(d[2 * q + 1].x), __float_as_uint(d[2 * q + 1].y));
     }
     add_up<T, kAligned>(db, dw, part, means,
                         sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
@@ -226,15 +235,15 @@ __global__ void __launch_bounds__(kThreads, 3)
         T* to = t.dx + first;
 #pragma unroll 2
         for (int i = 0; i < mine; ++i, to += stride) {
-            float x[kVec<T>], v[kVec<T>];
+            float2 x[kPairs<T>], v[kPairs<T>];
             unpack<T>(xs[at + i * pitch], x);
 #pragma unroll
             for (int q = 0; q < kPlanes<T>; ++q) {
-                float d[4];
-                unpack(ds[q * vectors + at + i * pitch], d, 0.0f);
+                float2 d[2];
+                unpack<float>(ds[q * vectors + at + i * pitch], d);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[4 * q + e] = final_(d[e], x[4 * q + e], column.scale[4 * q + e], 4 * q + e);
+                for (int e = 0; e < 2; ++e)
+                    v[2 * q + e] = final_(d[e], x[2 * q + e], column.scale[2 * q + e], 2 * q + e);
             }
             store<T, kAligned>(to, pack<T>(v), p.count);
         }
@@ -252,9 +261,9 @@ __global__ void __launch_bounds__(kThreads, 3)
     __shared__ float2 group_sums[kMaxSlabGroups];
     const Place<T> p = Place<T>::template make<true>(g, t.lengths);
     const int mine = p.own_rows();
-    float db[kVec<T>], dw[kVec<T>];
+    float2 db[kPairs<T>], dw[kPairs<T>];
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) db[e] = 0.0f, dw[e] = 0.0f;
+    for (int e = 0; e < kPairs<T>; ++e) db[e] = dw[e] = splat2(0.0f);
     if (mine > 0) {
         Column<T, kWhole> column;
         column.template read<kAligned>(t, p, g);
@@ -262,14 +271,14 @@ __global__ void __launch_bounds__(kThreads, 3)
         const int64_t first = p.at(g, p.begin + p.row);
 #pragma unroll 4
         for (int i = 0; i < mine; ++i) {
-            float x[kVec<T>], d[kVec<T>];
+            float2 x[kPairs<T>], d[kPairs<T>];
             unpack<T>(load<T, kAligned>(t.x + first + i * stride, p.count), x);
             unpack<T>(load<T, kAligned>(t.dout + first + i * stride, p.count), d);
             column.through(d, x, act);
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e) {
-                db[e] += d[e];
-                dw[e] = fmaf(d[e], column.normalised(x[e], e), dw[e]);
+            for (int e = 0; e < kPairs<T>; ++e) {
+                db[e] = add2(db[e], d[e]);
+                dw[e] = fma2(d[e], column.normalised(x[e], e), dw[e]);
             }
         }
     }
@@ -313,12 +322,12 @@ __global__ void __launch_bounds__(kThreads, 3)
         const int64_t first = p.at(g, p.begin + p.row);
 #pragma unroll 4
         for (int i = 0; i < mine; ++i) {
-            float x[kVec<T>], d[kVec<T>];
+            float2 x[kPairs<T>], d[kPairs<T>];
             unpack<T>(load<T, kAligned>(t.x + first + i * stride, p.count), x);
             unpack<T>(load<T, kAligned>(t.dout + first + i * stride, p.count), d);
             column.through(d, x, act);
 #pragma unroll
-            for (int e = 0; e < kVec<T>; ++e) d[e] = final_(d[e], x[e], column.scale[e], e);
+            for (int e = 0; e < kPairs<T>; ++e) d[e] = final_(d[e], x[e], column.scale[e], e);
             store<T, kAligned>(t.dx + first + i * stride, pack<T>(d), p.count);
         }
     }
