@@ -38,23 +38,23 @@ template <typename Visit> __device__ __forceinline__ float2 merge(float total, V
 }
 
 // (mean, squares) of every group of the slab over this block's rows to moments[group]; row(i)
-// is this thread's vector of its i-th row. `part` holds an entry per thread (and channel, if
+// is this thread's vector of its i-th row (asked for in order), `first` that of the first. `part` holds an entry per thread (and channel, if
 // not kWhole).
 //
 // A thread takes both in one pass, about a pivot: the mean of its own first vector (the first
 // value of each channel). With n values and the first q of them in the pivot, squares about
 // the mean are at least q (pivot - mean)^2, so the n (pivot - mean)^2 taken off the squares
 // about the pivot is at most n / q times what is left, a factor on its rounding error: with 12
-// rows of a tile or 64 of a split launch at most, and values that differ like that only where
-// the first vector is an outlier itself.
+// rows of a tile or 64 of a stream at most, and values that differ like that only where the
+// first vector is an outlier itself.
 template <typename T, bool kWhole, typename Row>
-__device__ __forceinline__ void block_moments(Row row, float2* part, float2* moments,
+__device__ __forceinline__ void block_moments(const uint4& first, Row row, float2* part, float2* moments,
                                               const Place<T>& p, const Geometry& g) {
     constexpr int kValues = kWhole ? 1 : kVec<T>, kSums = kWhole ? 1 : kPairs<T>;
     const int mine = p.own_rows(), columns = g.lanes * kValues;
     if (mine > 0) {
         float2 pivot[kSums], sum[kSums], squares[kSums], v[kPairs<T>];
-        unpack<T>(row(0), v);
+        unpack<T>(first, v);
         if constexpr (kWhole) {
             float2 s = v[0];
 #pragma unroll
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     extern __shared__ __align__(16) uint4 tile[];
     __shared__ float2 part[kWhole ? kThreads : kThreads * kVec<T>];
     __shared__ float2 moments[kMaxSlabGroups];
-    const Place<T> p = Place<T>::template make<false>(g, t.lengths);
+    const Place<T> p = Place<T>::make(g, t.lengths, blockIdx.x);
     const int mine = p.own_rows(), pitch = g.step * g.lanes;
     uint4* at = tile + p.row * g.lanes + p.lane;
     const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kThreads, 4)
             stage<T, kAligned>(at + i * pitch, from, p.count);
     }
     arrived();
-    block_moments<T, kWhole>([&](int i) { return at[i * pitch]; }, part, moments, p, g);
+    block_moments<T, kWhole>(mine > 0 ? at[0] : uint4{}, [&](int i) { return at[i * pitch]; }, part,
+                             moments, p, g);
     __syncthreads();
     const float width = static_cast<float>(g.group_channels);
     const float total = static_cast<float>(p.m) * width;
@@ -179,11 +180,10 @@ __global__ void __launch_bounds__(kThreads, 4)
             for (int j = threadIdx.x % kWarp; j < p.groups; j += kWarp)
                 *cluster.map_shared_rank(gathered + p.block * g.slab_groups + j, q) = moments[j];
         cluster.sync();
-        const int each = g.by_blocks.quotient(p.m + g.blocks - 1);
         for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
             const float2 r = merge(total, [&](auto add) {
                 for (int i = threadIdx.x % kWarp; i < g.blocks; i += kWarp)
-                    add(static_cast<float>(max(0, min(each, p.m - i * each))) * width,
+                    add(static_cast<float>(p.rows_of_block(i)) * width,
                         gathered[i * g.slab_groups + j]);
             });
             if (threadIdx.x % kWarp == 0) moments[j] = r;
@@ -211,18 +211,25 @@ __global__ void __launch_bounds__(kThreads, 4)
     zero_padding<T, kAligned>(t.out, p, g);
 }
 
-// The two launches for what no cluster holds. The first leaves each block's moments in
-// `partial` [N, G, parts * blocks], the second merges and applies them.
+// The two launches of a stream. The first leaves each block's moments in `partial` [N, G, parts *
+// blocks], the second merges and applies them. It goes through the rows against the order of
+// the first, so that it begins with those that are still in L2.
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 4)
     group_norm_moments_kernel(Tensors<T> t, float2* __restrict__ partial, Geometry g) {
+    extern __shared__ __align__(16) uint4 slots[];
     __shared__ float2 part[kWhole ? kThreads : kThreads * kVec<T>];
     __shared__ float2 moments[kMaxSlabGroups];
-    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
-    const T* from = t.x + p.at(g, p.begin + p.row);
-    const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
-    block_moments<T, kWhole>([&](int i) { return load<T, kAligned>(from + i * stride, p.count); },
-                             part, moments, p, g);
+    const Place<T> p = Place<T>::make(g, t.lengths, blockIdx.x);
+    Stream<T, kAligned, 1> rows;
+    rows.from[0] = t.x + p.at(g, p.begin + p.row);
+    const uint4 first = p.own_rows() > 0 ? load<T, kAligned>(rows.from[0], p.count) : uint4{};
+    rows.start(slots, p.own_rows(), static_cast<int64_t>(g.step) * g.channels, p.count);
+    block_moments<T, kWhole>(first, [&](int) {
+        uint4 v[1];
+        rows.next(v);
+        return v[0];
+    }, part, moments, p, g);
     __syncthreads();
     if (threadIdx.x < p.groups)
         partial[(static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x) * g.parts *
@@ -234,19 +241,26 @@ template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 4)
     group_norm_apply_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g, float eps,
                             int act) {
+    extern __shared__ __align__(16) uint4 slots[];
     __shared__ float2 stats[kMaxSlabGroups];
-    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
-    const int slots = g.parts * g.blocks;
+    const Place<T> p = Place<T>::make(g, t.lengths, gridDim.x - 1 - blockIdx.x);
+    const int mine = p.own_rows();
+    const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
+    const int64_t from = p.at(g, p.begin + p.row);
+    Stream<T, kAligned, 1> rows;
+    rows.from[0] = t.x + from;
+    rows.start(slots, mine, stride, p.count);
+    const int count = g.parts * g.blocks;
     const float total = static_cast<float>(p.m) * static_cast<float>(g.group_channels);
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
         const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group + j;
-        const float2* mine = partial + group * slots;
+        const float2* moments = partial + group * count;
         const float2 r = merge(total, [&](auto add) {
-            for (int i = threadIdx.x % kWarp; i < slots; i += kWarp) {
-                const int q = g.by_blocks.quotient(i), chunk = i - q * g.blocks;
-                const int rows = max(0, min(g.rows, p.m - chunk * g.rows));
+            for (int i = threadIdx.x % kWarp; i < count; i += kWarp) {
+                const int q = g.by_blocks.quotient(i);
                 const int wide = min(g.part_channels, g.group_channels - q * g.part_channels);
-                add(static_cast<float>(rows) * static_cast<float>(wide), mine[i]);
+                add(static_cast<float>(p.rows_of_block(i - q * g.blocks)) * static_cast<float>(wide),
+                    moments[i]);
             }
         });
         if (threadIdx.x % kWarp == 0) {
@@ -259,17 +273,16 @@ __global__ void __launch_bounds__(kThreads, 4)
         }
     }
     __syncthreads();
-    const int mine = p.own_rows();
     if (mine > 0) {
         Column<T> column;
         column.template read<kAligned, kWhole>(t.weight, t.bias, stats, p, g);
-        const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
-        const int64_t first = p.at(g, p.begin + p.row);
-#pragma unroll 4
-        for (int i = 0; i < mine; ++i)
-            store<T, kAligned>(t.out + first + i * stride,
-                               column.apply(load<T, kAligned>(t.x + first + i * stride, p.count), act),
-                               p.count);
+        T* to = t.out + from;
+#pragma unroll 2
+        for (int i = 0; i < mine; ++i, to += stride) {
+            uint4 v[1];
+            rows.next(v);
+            store<T, kAligned>(to, column.apply(v[0], act), p.count);
+        }
     }
     zero_padding<T, kAligned>(t.out, p, g);
 }
@@ -286,16 +299,18 @@ cudaError_t run(const GroupNormProblem& p, const Shape& s, cudaStream_t stream) 
     if (!s.split)
         return launch(resident, group_norm_kernel<T, kAligned, kWhole>, s, true,
                       g.rows * g.lanes * 16 + gather, most, stream, t, g, p.eps, p.activation);
+    constexpr int kSlots = Stream<T, kAligned, 1>::kBytes;
     const cudaError_t e = launch(partial, group_norm_moments_kernel<T, kAligned, kWhole>, s, false,
-                                 0, 0, stream, t, ws, g);
+                                 kSlots, kSlots, stream, t, ws, g);
     if (e != cudaSuccess) return e;
-    return launch(apply, group_norm_apply_kernel<T, kAligned, kWhole>, s, false, 0, 0, stream, t,
-                  static_cast<const float2*>(ws), g, p.eps, p.activation);
+    return launch(apply, group_norm_apply_kernel<T, kAligned, kWhole>, s, false, kSlots, kSlots,
+                  stream, t, static_cast<const float2*>(ws), g, p.eps, p.activation);
 }
 
 Shape shape_of(const GroupNormProblem& p, bool aligned) {
-    return group_norm::shape_of(p.batch, p.length, p.channels, p.groups,
-                                p.dtype == FGA_FLOAT ? 4 : 2, aligned, 16, kTileBytes);
+    const Problem q{p.batch, p.length, p.channels, p.groups, p.dtype == FGA_FLOAT ? 4 : 2, aligned};
+    const Shape s = resident_shape(q, 16, kTileBytes);
+    return s.geo.blocks > 0 && s.geo.blocks <= kMaxCluster ? s : stream_shape(q);
 }
 
 template <typename T> cudaError_t run(const GroupNormProblem& p, cudaStream_t stream) {

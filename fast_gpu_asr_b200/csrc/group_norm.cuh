@@ -152,7 +152,7 @@ struct Geometry {
     int parts;        // slabs of a group that is wider than one (then slab_groups is 1)
     int part_channels;
     int slabs;        // of a row
-    int blocks;       // of an utterance's slab: a cluster, or the chunks of a split launch
+    int blocks;       // that divide the valid rows of an utterance's slab evenly
     int rows;         // most rows of a block
     int lanes, step;  // threads of a row, rows of a block's threads
     Divisor by_blocks, by_slabs, by_lanes, by_step, by_group;
@@ -164,15 +164,14 @@ template <typename T> struct Place {
     int first_channel, channels;  // of the slab
     int lane, row;                // of this thread
     int count;                    // valid channels of this thread's vector; below 1: no work
-    int begin, rows;              // rows of the block
+    int begin, rows, each;        // rows of the block; of a block of this utterance
     int passes, extra;            // rows of a thread: passes, and one more in the first `extra`
 
-    // kChunks: blocks take g.rows rows each; else they divide the valid rows evenly.
-    template <bool kChunks>
-    __device__ static Place make(const Geometry& g, const int32_t* lengths) {
+    // `index`: of the block in the launch, or against it.
+    __device__ static Place make(const Geometry& g, const int32_t* lengths, int index) {
         Place p;
-        const int unit = g.by_blocks.quotient(blockIdx.x);
-        p.block = blockIdx.x - unit * g.blocks;
+        const int unit = g.by_blocks.quotient(index);
+        p.block = index - unit * g.blocks;
         p.n = g.by_slabs.quotient(unit);
         p.slab = unit - p.n * g.slabs;
         p.m = min(max(lengths[p.n], 0), g.length);
@@ -191,12 +190,15 @@ template <typename T> struct Place {
         p.row = g.by_lanes.quotient(threadIdx.x);
         p.lane = threadIdx.x - p.row * g.lanes;
         p.count = p.row < g.step ? min(kVec<T>, p.channels - p.lane * kVec<T>) : 0;
-        const int each = kChunks ? g.rows : g.by_blocks.quotient(p.m + g.blocks - 1);
-        p.begin = min(p.m, p.block * each);
-        p.rows = min(p.m - p.begin, each);
+        p.each = g.by_blocks.quotient(p.m + g.blocks - 1);
+        p.begin = min(p.m, p.block * p.each);
+        p.rows = min(p.m - p.begin, p.each);
         p.passes = g.by_step.quotient(p.rows);
         p.extra = p.rows - p.passes * g.step;
         return p;
+    }
+    __device__ __forceinline__ int rows_of_block(int b) const {
+        return max(0, min(each, m - b * each));
     }
     // Rows of the block in the threads of row r.
     __device__ __forceinline__ int rows_of(int r) const { return passes + (r < extra ? 1 : 0); }
@@ -233,6 +235,54 @@ struct Items {
     }
 };
 
+// A thread's vectors of its rows, in order, from kSources tensors at once: kDepth of them are on
+// their way through the thread's own slots of shared memory while it works on one, whatever
+// the compiler makes of the loop's registers.
+constexpr int kDepth = 4;
+template <typename T, bool kAligned, int kSources> struct Stream {
+    const T* from[kSources];
+    uint4* slots;  // [kDepth][kSources][kThreads]
+    int64_t stride;
+    int rows, count, at = 0, ahead = 0;
+
+    static constexpr int kBytes = kAligned ? kDepth * kSources * kThreads * 16 : 0;
+
+    __device__ __forceinline__ void request() {
+        if (ahead < rows)
+#pragma unroll
+            for (int k = 0; k < kSources; ++k) {
+                stage<T, true>(slots + (ahead % kDepth * kSources + k) * kThreads, from[k], count);
+                from[k] += stride;
+            }
+        ++ahead;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void start(uint4* shared, int rows_, int64_t stride_, int count_) {
+        slots = shared + threadIdx.x;
+        rows = rows_;
+        stride = stride_;
+        count = count_;
+        if constexpr (kAligned)
+#pragma unroll
+            for (int i = 0; i < kDepth - 1; ++i) request();
+    }
+    __device__ __forceinline__ void next(uint4 (&v)[kSources]) {
+        if constexpr (kAligned) {
+            request();
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+#pragma unroll
+            for (int k = 0; k < kSources; ++k) v[k] = slots[(at % kDepth * kSources + k) * kThreads];
+            ++at;
+        } else {
+#pragma unroll
+            for (int k = 0; k < kSources; ++k) {
+                v[k] = load<T, false>(from[k], count);
+                from[k] += stride;
+            }
+        }
+    }
+};
+
 // Zeros in the rows past the valid ones, of which the unit's blocks take turns.
 template <typename T, bool kAligned>
 __device__ __forceinline__ void zero_padding(T* out, const Place<T>& p, const Geometry& g) {
@@ -246,80 +296,101 @@ __device__ __forceinline__ void zero_padding(T* out, const Place<T>& p, const Ge
 }
 
 // ---- launch shape --------------------------------------------------------------------------
+struct Problem {
+    int batch, length, channels, groups, element;  // element: bytes
+    bool aligned;                                  // the buffers, to 16 bytes
+};
+
 struct Shape {
     Geometry geo;
     bool aligned;  // vectors are 16-byte aligned in global memory, and full
     bool whole;    // a vector's channels are of one group
-    bool split;    // too large for a cluster: several launches with a workspace between them
+    bool split;    // several launches with a workspace between them
     int64_t units; // utterances x slabs
 };
 
-// `bytes_per_vector`: of shared memory that a block keeps for a vector of its rows; `tile_bytes`:
-// what it should hold at most. Slabs are as wide as that allows for the whole length, since a
-// cluster costs two barriers, but at least 64 bytes a row, and no wider than 128 where that
-// would leave multiprocessors without work.
-inline Shape shape_of(int batch, int length, int channels, int groups, int element, bool aligned,
-                      int bytes_per_vector, int tile_bytes) {
+// Slabs of about slab_bytes a row.
+inline Shape slabs_of(const Problem& p, int64_t slab_bytes) {
     Shape s{};
-    const int vec = 16 / element, width = channels / groups;
+    const int vec = 16 / p.element, width = p.channels / p.groups;
     Geometry& g = s.geo;
-    g.length = length;
-    g.channels = channels;
-    g.groups = groups;
+    g.length = p.length;
+    g.channels = p.channels;
+    g.groups = p.groups;
     g.group_channels = width;
     g.parts = 1;
     g.part_channels = kThreads * vec;
-    const int64_t group_bytes = static_cast<int64_t>(width) * element;
+    const int64_t group_bytes = static_cast<int64_t>(width) * p.element;
     // Slabs that start at a multiple of 16 bytes, if that takes no more than the threads.
     int64_t step = 16 / std::gcd<int64_t>(group_bytes, 16);
-    if (step > groups) step = groups;  // one slab: the row
-    aligned = aligned && channels % vec == 0 && (step == 1 || step * group_bytes <= kThreads * 16);
-    if (!aligned) step = 1;
-    const int64_t row_fit = 16LL * tile_bytes / (static_cast<int64_t>(length) * bytes_per_vector);
-    const int64_t wanted = (2LL * sm_count() + batch - 1) / batch;  // slabs for every processor
-    const int64_t spread = std::max<int64_t>(128, channels * static_cast<int64_t>(element) /
-                                                      std::max<int64_t>(1, wanted));
-    const int64_t slab_bytes =
-        std::max<int64_t>(64, std::min<int64_t>({row_fit, spread, kThreads * 16}));
-    int64_t slab = step * std::max<int64_t>(1, slab_bytes / (step * group_bytes));
-    slab = std::min<int64_t>({slab, groups, kMaxSlabGroups});
-    g.slab_groups = static_cast<int>(slab);
-    g.slabs = (groups + g.slab_groups - 1) / g.slab_groups;
+    if (step > p.groups) step = p.groups;  // one slab: the row
+    s.aligned = p.aligned && p.channels % vec == 0 &&
+                (step == 1 || step * group_bytes <= kThreads * 16);
+    if (!s.aligned) step = 1;
+    slab_bytes = std::min<int64_t>(slab_bytes, kThreads * 16);
+    const int64_t most = std::min<int64_t>(p.groups, kMaxSlabGroups);
+    g.slab_groups = static_cast<int>(
+        std::min(step * std::max<int64_t>(1, slab_bytes / (step * group_bytes)),
+                 std::max(step, most / step * step)));
+    g.slabs = (p.groups + g.slab_groups - 1) / g.slab_groups;
     if (width > g.part_channels) {
         // (A group this wide has a step of 1, so parts of full vectors if aligned at all.)
         g.slab_groups = 1;
         g.parts = (width + g.part_channels - 1) / g.part_channels;
-        g.slabs = groups * g.parts;
+        g.slabs = p.groups * g.parts;
     }
-    s.aligned = aligned;
-    s.whole = g.slab_groups == 1 ? aligned : aligned && width % vec == 0;
-    s.units = static_cast<int64_t>(batch) * g.slabs;
+    s.whole = s.aligned && width % vec == 0;
+    s.units = static_cast<int64_t>(p.batch) * g.slabs;
     g.lanes = (std::min(width * g.slab_groups, g.part_channels) + vec - 1) / vec;
     g.step = kThreads / g.lanes;
-    const int64_t row_bytes = static_cast<int64_t>(g.lanes) * bytes_per_vector;
-    const int64_t fit = std::max<int64_t>(1, tile_bytes / row_bytes);  // rows of a block
-    // Enough blocks for two on every multiprocessor, as long as each has rows for its threads.
-    const int64_t fill = std::min<int64_t>((2LL * sm_count() + s.units - 1) / s.units,
-                                           (length + 2 * g.step - 1) / (2 * g.step));
-    const int64_t needed = (length + fit - 1) / fit;
-    s.split = g.parts > 1 || needed > kMaxCluster;
-    if (s.split) {
-        // Eight blocks for every multiprocessor, of at least 4 rows a thread (a block's sums
-        // cost as much as some rows) and at most 64.
-        const int64_t share = length * s.units / (8LL * std::max(1, sm_count())) + 1;
-        const int64_t rows = std::max<int64_t>(4 * g.step, std::min<int64_t>(64 * g.step, share));
-        g.rows = static_cast<int>(std::min<int64_t>(rows, length));
-        g.blocks = (length + g.rows - 1) / g.rows;
-    } else {
-        g.blocks = static_cast<int>(std::min<int64_t>({std::max(needed, fill), kMaxCluster}));
-        g.blocks = std::max(1, g.blocks);
-        g.rows = (length + g.blocks - 1) / g.blocks;
-    }
+    return s;
+}
+
+inline void set_blocks(Shape& s, int64_t blocks) {
+    Geometry& g = s.geo;
+    g.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(blocks, g.length)));
+    g.rows = (g.length + g.blocks - 1) / g.blocks;
     g.by_blocks = Divisor(g.blocks);
     g.by_slabs = Divisor(g.slabs);
     g.by_lanes = Divisor(g.lanes);
     g.by_step = Divisor(g.step);
     g.by_group = Divisor(g.group_channels);
+}
+
+// One launch that keeps its rows on chip, with bytes_per_vector of shared memory for a vector
+// of them and at most tile_bytes a block. Slabs are as wide as that allows for the whole
+// length, since a cluster costs two barriers, but at least 64 bytes a row, and no wider than
+// 128 where that would leave multiprocessors without work. blocks is 0 where no cluster holds
+// the rows.
+inline Shape resident_shape(const Problem& p, int bytes_per_vector, int tile_bytes) {
+    const int64_t row_fit = 16LL * tile_bytes / (static_cast<int64_t>(p.length) * bytes_per_vector);
+    const int64_t wanted = (2LL * sm_count() + p.batch - 1) / p.batch;  // slabs for every processor
+    const int64_t spread = std::max<int64_t>(
+        128, static_cast<int64_t>(p.channels) * p.element / std::max<int64_t>(1, wanted));
+    Shape s = slabs_of(p, std::max<int64_t>(64, std::min(row_fit, spread)));
+    const Geometry& g = s.geo;
+    const int64_t row_bytes = static_cast<int64_t>(g.lanes) * bytes_per_vector;
+    const int64_t fit = std::max<int64_t>(1, tile_bytes / row_bytes);  // rows of a block
+    const int64_t needed = (p.length + fit - 1) / fit;
+    if (g.parts > 1 || needed > kMaxCluster) return s;
+    // Enough blocks for two on every multiprocessor, as long as each has rows for its threads.
+    const int64_t fill = std::min<int64_t>((2LL * sm_count() + s.units - 1) / s.units,
+                                           (p.length + 2 * g.step - 1) / (2 * g.step));
+    set_blocks(s, std::min<int64_t>(std::max(needed, fill), kMaxCluster));
+    return s;
+}
+
+// Several launches that stream the rows: slabs as wide as the threads, and kStreamBlocks blocks
+// for every multiprocessor, of at least 4 rows a thread (a block's sums cost as much as some
+// rows) and at most 64.
+constexpr int kStreamBlocks = 8;
+inline Shape stream_shape(const Problem& p) {
+    Shape s = slabs_of(p, kThreads * 16);
+    s.split = true;
+    const int64_t step = s.geo.step, most = (p.length + 4 * step - 1) / (4 * step);
+    const int64_t least = (p.length + 64 * step - 1) / (64 * step);
+    const int64_t share = (kStreamBlocks * std::max(1, sm_count()) + s.units - 1) / s.units;
+    set_blocks(s, std::max(least, std::min(most, share)));
     return s;
 }
 

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     group_norm_backward_kernel(Tensors<T> t, float2* __restrict__ sums, Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
     __shared__ float2 means[kMaxSlabGroups];
-    const Place<T> p = Place<T>::template make<false>(g, t.lengths);
+    const Place<T> p = Place<T>::make(g, t.lengths, blockIdx.x);
     const int vectors = g.rows * g.lanes;
     uint4* xs = shared;
     uint4* ds = shared + vectors;
@@ -251,29 +251,35 @@ __global__ void __launch_bounds__(kThreads, 3)
     zero_padding<T, kAligned>(t.dx, p, g);
 }
 
-// The two launches for what no cluster holds. The first leaves each block's (s1, s2) in
-// `partial` [N, G, parts * blocks].
+// The two launches of a stream. The first leaves each block's (s1, s2) in `partial` [N, G, parts *
+// blocks]; the second goes through the rows against the order of the first, so that it begins
+// with those that are still in L2.
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 3)
     group_norm_sums_kernel(Tensors<T> t, float2* __restrict__ sums, float2* __restrict__ partial,
                            Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
     __shared__ float2 group_sums[kMaxSlabGroups];
-    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
+    const Place<T> p = Place<T>::make(g, t.lengths, blockIdx.x);
     const int mine = p.own_rows();
+    const int64_t from = p.at(g, p.begin + p.row);
+    Stream<T, kAligned, 2> rows;
+    rows.from[0] = t.x + from;
+    rows.from[1] = t.dout + from;
+    rows.start(shared, mine, static_cast<int64_t>(g.step) * g.channels, p.count);
     float2 db[kPairs<T>], dw[kPairs<T>];
 #pragma unroll
     for (int e = 0; e < kPairs<T>; ++e) db[e] = dw[e] = splat2(0.0f);
     if (mine > 0) {
         Column<T, kWhole> column;
         column.template read<kAligned>(t, p, g);
-        const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
-        const int64_t first = p.at(g, p.begin + p.row);
-#pragma unroll 4
+#pragma unroll 2
         for (int i = 0; i < mine; ++i) {
+            uint4 v[2];
+            rows.next(v);
             float2 x[kPairs<T>], d[kPairs<T>];
-            unpack<T>(load<T, kAligned>(t.x + first + i * stride, p.count), x);
-            unpack<T>(load<T, kAligned>(t.dout + first + i * stride, p.count), d);
+            unpack<T>(v[0], x);
+            unpack<T>(v[1], d);
             column.through(d, x, act);
 #pragma unroll
             for (int e = 0; e < kPairs<T>; ++e) {
@@ -282,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 3)
             }
         }
     }
+    __syncthreads();  // the slots become the threads' sums
     add_up<T, kAligned>(db, dw, reinterpret_cast<float2*>(shared), group_sums,
                         sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
                         t.weight, p, g);
@@ -295,81 +302,86 @@ template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 3)
     group_norm_gradient_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g,
                                int act) {
+    extern __shared__ __align__(16) uint4 shared[];
     __shared__ float2 means[kMaxSlabGroups];
-    const Place<T> p = Place<T>::template make<true>(g, t.lengths);
-    const int slots = g.parts * g.blocks;
+    const Place<T> p = Place<T>::make(g, t.lengths, gridDim.x - 1 - blockIdx.x);
+    const int mine = p.own_rows();
+    const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
+    const int64_t from = p.at(g, p.begin + p.row);
+    Stream<T, kAligned, 2> rows;
+    rows.from[0] = t.x + from;
+    rows.from[1] = t.dout + from;
+    rows.start(shared, mine, stride, p.count);
+    const int count = g.parts * g.blocks;
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
-        const float2* from =
-            partial + (static_cast<int64_t>(p.n) * g.groups + p.first_group + j) * slots;
+        const float2* add =
+            partial + (static_cast<int64_t>(p.n) * g.groups + p.first_group + j) * count;
         float s1 = 0.0f, s2 = 0.0f;
-        for (int i = threadIdx.x % kWarp; i < slots; i += kWarp) {
-            s1 += from[i].x;
-            s2 += from[i].y;
+        for (int i = threadIdx.x % kWarp; i < count; i += kWarp) {
+            s1 += add[i].x;
+            s2 += add[i].y;
         }
         s1 = warp_sum(s1);
         s2 = warp_sum(s2);
         if (threadIdx.x % kWarp == 0) means[j] = make_float2(s1, s2);
     }
     __syncthreads();
-    const int mine = p.own_rows();
     if (mine > 0) {
         const float inv = 1.0f / (static_cast<float>(p.m) * static_cast<float>(g.group_channels));
         Column<T, kWhole> column;
         column.template read<kAligned>(t, p, g);
         Final<T, kWhole> final_;
         final_.make(column, means, inv, p, g);
-        const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
-        const int64_t first = p.at(g, p.begin + p.row);
-#pragma unroll 4
-        for (int i = 0; i < mine; ++i) {
+        T* to = t.dx + from;
+#pragma unroll 2
+        for (int i = 0; i < mine; ++i, to += stride) {
+            uint4 v[2];
+            rows.next(v);
             float2 x[kPairs<T>], d[kPairs<T>];
-            unpack<T>(load<T, kAligned>(t.x + first + i * stride, p.count), x);
-            unpack<T>(load<T, kAligned>(t.dout + first + i * stride, p.count), d);
+            unpack<T>(v[0], x);
+            unpack<T>(v[1], d);
             column.through(d, x, act);
 #pragma unroll
             for (int e = 0; e < kPairs<T>; ++e) d[e] = final_(d[e], x[e], column.scale[e], e);
-            store<T, kAligned>(t.dx + first + i * stride, pack<T>(d), p.count);
+            store<T, kAligned>(to, pack<T>(d), p.count);
         }
     }
     zero_padding<T, kAligned>(t.dx, p, g);
 }
 
-// Adds the blocks' rows of column sums, in an order that the launch fixes: a warp every
-// kSumWarps-th row of 32 channels.
-constexpr int kSumWarps = 32;
+// Adds the blocks' rows of column sums, in an order that the launch fixes: 8 channels a block,
+// a thread every 128th row of one of them.
+constexpr int kSumChannels = 8, kSumRows = 128;
 template <typename T>
-__global__ void __launch_bounds__(kSumWarps* kWarp)
+__global__ void __launch_bounds__(kSumChannels* kSumRows)
     group_norm_parameters_kernel(const float2* __restrict__ sums, T* __restrict__ dweight,
                                  T* __restrict__ dbias, int rows, int channels) {
-    __shared__ float2 part[kSumWarps][kWarp];
-    const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-    const int c = blockIdx.x * kWarp + lane;
+    __shared__ float2 part[kSumRows][kSumChannels];
+    const int row = threadIdx.x / kSumChannels, lane = threadIdx.x % kSumChannels;
+    const int c = blockIdx.x * kSumChannels + lane;
     float2 s = make_float2(0.0f, 0.0f);
     if (c < channels) {
 #pragma unroll 8
-        for (int r = warp; r < rows; r += kSumWarps) {
-            const float2 v = sums[static_cast<int64_t>(r) * channels + c];
-            s.x += v.x;
-            s.y += v.y;
-        }
+        for (int r = row; r < rows; r += kSumRows)
+            s = add2(s, sums[static_cast<int64_t>(r) * channels + c]);
     }
-    part[warp][lane] = s;
-    __syncthreads();
-    if (warp == 0 && c < channels) {
-        for (int w = 1; w < kSumWarps; ++w) {
-            s.x += part[w][lane].x;
-            s.y += part[w][lane].y;
-        }
-        dbias[c] = from_f32<T>(s.x);
-        dweight[c] = from_f32<T>(s.y);
+    part[row][lane] = s;
+    for (int half = kSumRows / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (row < half) part[row][lane] = add2(part[row][lane], part[row + half][lane]);
+    }
+    if (row == 0 && c < channels) {
+        dbias[c] = from_f32<T>(part[0][lane].x);
+        dweight[c] = from_f32<T>(part[0][lane].y);
     }
 }
 
 Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
     const int element = p.dtype == FGA_FLOAT ? 4 : 2;
-    return group_norm::shape_of(p.batch, p.length, p.channels, p.groups, element, aligned,
-                                element == 4 ? kVectorBytes<float> : kVectorBytes<__half>,
-                                kTileBytes);
+    const Problem q{p.batch, p.length, p.channels, p.groups, element, aligned};
+    const Shape s = resident_shape(q, element == 4 ? kVectorBytes<float> : kVectorBytes<__half>,
+                                   kTileBytes);
+    return s.geo.blocks > 0 && s.geo.blocks <= kMaxCluster ? s : stream_shape(q);
 }
 
 int64_t sum_rows(const Shape& s, int batch) { return static_cast<int64_t>(batch) * s.geo.blocks; }
@@ -397,14 +409,16 @@ cudaError_t run(const GroupNormBackwardProblem& p, const Shape& s, cudaStream_t 
                    sums, g, p.activation);
     } else {
         float2* partial = sums + rows * p.channels;
-        e = launch(first, group_norm_sums_kernel<T, kAligned, kWhole>, s, false, part, kSumBytes<T>,
-                   stream, t, sums, partial, g, p.activation);
+        constexpr int kSlots = Stream<T, kAligned, 2>::kBytes, kMost = std::max(kSlots, kSumBytes<T>);
+        e = launch(first, group_norm_sums_kernel<T, kAligned, kWhole>, s, false,
+                   std::max(kSlots, part), kMost, stream, t, sums, partial, g, p.activation);
         if (e == cudaSuccess)
-            e = launch(second, group_norm_gradient_kernel<T, kAligned, kWhole>, s, false, 0, 0,
-                       stream, t, static_cast<const float2*>(partial), g, p.activation);
+            e = launch(second, group_norm_gradient_kernel<T, kAligned, kWhole>, s, false, kSlots,
+                       kMost, stream, t, static_cast<const float2*>(partial), g, p.activation);
     }
     if (e != cudaSuccess) return e;
-    group_norm_parameters_kernel<T><<<(p.channels + kWarp - 1) / kWarp, kSumWarps * kWarp, 0, stream>>>(
+    group_norm_parameters_kernel<T><<<(p.channels + kSumChannels - 1) / kSumChannels,
+                                      kSumChannels * kSumRows, 0, stream>>>(
         sums, static_cast<T*>(p.grad_weight), static_cast<T*>(p.grad_bias), static_cast<int>(rows),
         p.channels);
     return cudaGetLastError();
