@@ -213,13 +213,15 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 // The two launches of a stream. The first leaves each block's moments in `partial` [N, G, parts *
 // blocks], the second merges and applies them. It goes through the rows against the order of
-// the first, so that it begins with those that are still in L2.
+// the first, so that it begins with those that are still in L2, and is launched early
+// (programmatic dependent launch): its rows are on their way by the time the first has ended.
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 4)
     group_norm_moments_kernel(Tensors<T> t, float2* __restrict__ partial, Geometry g) {
     extern __shared__ __align__(16) uint4 slots[];
     __shared__ float2 part[kWhole ? kThreads : kThreads * kVec<T>];
     __shared__ float2 moments[kMaxSlabGroups];
+    cudaTriggerProgrammaticLaunchCompletion();
     const Place<T> p = Place<T>::make(g, t.lengths, blockIdx.x);
     Stream<T, kAligned, 1> rows;
     rows.from[0] = t.x + p.at(g, p.begin + p.row);
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 4)
-    group_norm_apply_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g, float eps,
+    group_norm_apply_kernel(Tensors<T> t, const float2* partial, Geometry g, float eps,
                             int act) {
     extern __shared__ __align__(16) uint4 slots[];
     __shared__ float2 stats[kMaxSlabGroups];
@@ -252,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     rows.start(slots, mine, stride, p.count);
     const int count = g.parts * g.blocks;
     const float total = static_cast<float>(p.m) * static_cast<float>(g.group_channels);
+    cudaGridDependencySynchronize();
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
         const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group + j;
         const float2* moments = partial + group * count;
@@ -296,15 +299,18 @@ cudaError_t run(const GroupNormProblem& p, const Shape& s, cudaStream_t stream) 
     const int gather = g.blocks > 1 ? g.blocks * g.slab_groups * static_cast<int>(sizeof(float2)) : 0;
     const int most = kTileBytes + kThreads * 16 + kGatherBytes;
     float2* ws = static_cast<float2*>(p.workspace);
+    const int64_t blocks = s.units * g.blocks;
     if (!s.split)
-        return launch(resident, group_norm_kernel<T, kAligned, kWhole>, s, true,
-                      g.rows * g.lanes * 16 + gather, most, stream, t, g, p.eps, p.activation);
+        return launch(resident, group_norm_kernel<T, kAligned, kWhole>,
+                      {blocks, g.blocks, false, g.rows * g.lanes * 16 + gather, most}, stream, t, g,
+                      p.eps, p.activation);
     constexpr int kSlots = Stream<T, kAligned, 1>::kBytes;
-    const cudaError_t e = launch(partial, group_norm_moments_kernel<T, kAligned, kWhole>, s, false,
-                                 kSlots, kSlots, stream, t, ws, g);
+    const cudaError_t e = launch(partial, group_norm_moments_kernel<T, kAligned, kWhole>,
+                                 {blocks, 1, false, kSlots, kSlots}, stream, t, ws, g);
     if (e != cudaSuccess) return e;
-    return launch(apply, group_norm_apply_kernel<T, kAligned, kWhole>, s, false, kSlots, kSlots,
-                  stream, t, static_cast<const float2*>(ws), g, p.eps, p.activation);
+    return launch(apply, group_norm_apply_kernel<T, kAligned, kWhole>,
+                  {blocks, 1, true, kSlots, kSlots}, stream, t, static_cast<const float2*>(ws), g,
+                  p.eps, p.activation);
 }
 
 Shape shape_of(const GroupNormProblem& p, bool aligned) {

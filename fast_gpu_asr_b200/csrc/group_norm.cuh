@@ -400,27 +400,40 @@ inline bool aligned16(std::initializer_list<const void*> buffers) {
     return all % 16 == 0;
 }
 
-// One launch of `units` x geo.blocks blocks, as clusters of geo.blocks if `cluster`.
+struct Launch {
+    int64_t blocks;
+    int cluster;  // blocks of a cluster
+    bool early;   // may start before the launch before it ends: the kernel waits for that itself
+    int smem, most_smem;
+};
+
 template <typename... Params, typename... Args>
-cudaError_t launch(SmemAttr& attribute, void (*kernel)(Params...), const Shape& s, bool cluster,
-                   int smem, int most_smem, cudaStream_t stream, Args... args) {
+cudaError_t launch(SmemAttr& attribute, void (*kernel)(Params...), const Launch& l,
+                   cudaStream_t stream, Args... args) {
     const void* entry = reinterpret_cast<const void*>(kernel);
-    cudaError_t e = attribute.ensure(entry, most_smem);
+    cudaError_t e = cudaSuccess;
+    if (l.most_smem > 0) e = attribute.ensure(entry, l.most_smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(s.units * s.geo.blocks));
+    cfg.gridDim = dim3(static_cast<unsigned>(l.blocks));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.dynamicSmemBytes = static_cast<size_t>(l.smem);
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(s.geo.blocks);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = cluster && s.geo.blocks > 1 ? 1 : 0;
-    if (cluster && s.geo.blocks > 8) {
-        e = cudaFuncSetAttribute(entry, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (l.cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(l.cluster);
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+        if (l.cluster > 8)
+            e = cudaFuncSetAttribute(entry, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
+    }
+    if (l.early) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
     }
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }

@@ -102,15 +102,17 @@ template <typename T, bool kWhole> struct Final {
     }
 };
 
-// Adds the threads' column sums: (dbias, dweight) of the block's rows to `sums` (also left in
-// shared memory at part[0..]), and of each group (s1, s2), weighted, to group_sums.
-template <typename T, bool kAligned>
+// Adds the threads' column sums: (dbias, dweight) of the block's rows to `sums`, and of each
+// group (s1, s2), weighted, to group_sums.
+template <typename T>
 __device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>], float2* part,
                                        float2* group_sums, float2* __restrict__ sums,
                                        const T* __restrict__ weight, const Place<T>& p,
                                        const Geometry& g) {
     const int columns = g.lanes * kVec<T>;
     int rows = g.step;
+    // Asked for before the barrier that its use comes after.
+    float w = threadIdx.x < p.channels ? to_f32<T>(weight[p.first_channel + threadIdx.x]) : 0.0f;
     if (kWarp % g.lanes == 0) {
         // Whole rows of threads in a warp: the warp's own sum first.
         for (int o = g.lanes; o < kWarp; o *= 2)
@@ -135,31 +137,75 @@ __device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPa
                 make_float2(channel_of(db, e), channel_of(dw, e));
     }
     __syncthreads();
+    float2 own = splat2(0.0f);
     for (int c = threadIdx.x; c < p.channels; c += kThreads) {
         float2 s = part[c];
-        for (int r = 1; r < rows; ++r) {
-            const float2 v = part[r * columns + c];
-            s.x += v.x;
-            s.y += v.y;
-        }
+        for (int r = 1; r < rows; ++r) s = add2(s, part[r * columns + c]);
         sums[p.first_channel + c] = s;
+        if (c >= kThreads) w = to_f32<T>(weight[p.first_channel + c]);
+        s = mul2(s, splat2(w));
         part[c] = s;
+        own = add2(own, s);
     }
-    __syncthreads();
-    const int width = p.channels / p.groups;
-    for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
-        float s1 = 0.0f, s2 = 0.0f;
-        for (int c = j * width + threadIdx.x % kWarp; c < (j + 1) * width; c += kWarp) {
-            const float w = to_f32<T>(weight[p.first_channel + c]);
-            s1 = fmaf(w, part[c].x, s1);
-            s2 = fmaf(w, part[c].y, s2);
+    if (p.groups == 1) {
+        __shared__ float2 warps[kBlockWarps];
+        own = make_float2(warp_sum(own.x), warp_sum(own.y));
+        if (threadIdx.x % kWarp == 0) warps[threadIdx.x / kWarp] = own;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int i = 1; i < kBlockWarps; ++i) own = add2(own, warps[i]);
+            group_sums[0] = own;
         }
-        s1 = warp_sum(s1);
-        s2 = warp_sum(s2);
-        if (threadIdx.x % kWarp == 0) group_sums[j] = make_float2(s1, s2);
+    } else {
+        __syncthreads();
+        const int width = p.channels / p.groups;
+        for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+            float2 s = splat2(0.0f);
+            for (int c = threadIdx.x % kWarp; c < width; c += kWarp) s = add2(s, part[j * width + c]);
+            s = make_float2(warp_sum(s.x), warp_sum(s.y));
+            if (threadIdx.x % kWarp == 0) group_sums[j] = s;
+        }
     }
     __syncthreads();
 }
+
+// Adds the blocks' rows of column sums, in an order that the launch fixes: kSumChannels channels
+// a block, a thread every kSumRows-th row of one of them.
+constexpr int kSumChannels = 8, kSumRows = kThreads / kSumChannels;
+template <typename T>
+__device__ __forceinline__ void sum_parameters(const float2* sums,
+                                               T* __restrict__ dweight, T* __restrict__ dbias,
+                                               int rows, int channels, int block, float2* part) {
+    const int row = threadIdx.x / kSumChannels, lane = threadIdx.x % kSumChannels;
+    const int c = block * kSumChannels + lane;
+    float2 s = splat2(0.0f);
+    if (c < channels) {
+#pragma unroll 8
+        for (int r = row; r < rows; r += kSumRows)
+            s = add2(s, sums[static_cast<int64_t>(r) * channels + c]);
+    }
+    part[threadIdx.x] = s;
+#pragma unroll
+    for (int half = kSumRows / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (row < half) {
+            s = add2(s, part[threadIdx.x + half * kSumChannels]);
+            part[threadIdx.x] = s;
+        }
+    }
+    if (row == 0 && c < channels) {
+        dbias[c] = from_f32<T>(s.x);
+        dweight[c] = from_f32<T>(s.y);
+    }
+}
+
+template <typename T> struct Parameters {
+    const float2* sums;
+    T* dweight;
+    T* dbias;
+    int rows;
+};
 
 // `sums`: [N * blocks, C] (dbias, dweight) of each block's rows.
 template <typename T, bool kAligned, bool kWhole>
@@ -167,6 +213,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     group_norm_backward_kernel(Tensors<T> t, float2* __restrict__ sums, Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
     __shared__ float2 means[kMaxSlabGroups];
+    cudaTriggerProgrammaticLaunchCompletion();
     const Place<T> p = Place<T>::make(g, t.lengths, blockIdx.x);
     const int vectors = g.rows * g.lanes;
     uint4* xs = shared;
@@ -206,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 3)
                 make_uint4(__float_as_uint(d[2 * q].x), __float_as_uint(d[2 * q].y),
                            __float_as_uint(d[2 * q + 1].x), __float_as_uint(d[2 * q + 1].y));
     }
-    add_up<T, kAligned>(db, dw, part, means,
+    add_up<T>(db, dw, part, means,
                         sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
                         t.weight, p, g);
     if (g.blocks > 1) {
@@ -253,13 +300,16 @@ __global__ void __launch_bounds__(kThreads, 3)
 
 // The two launches of a stream. The first leaves each block's (s1, s2) in `partial` [N, G, parts *
 // blocks]; the second goes through the rows against the order of the first, so that it begins
-// with those that are still in L2.
+// with those that are still in L2, and its last blocks add up the parameters' gradients. It is
+// launched early (programmatic dependent launch): its rows are on their way by the time the
+// first has ended.
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 3)
     group_norm_sums_kernel(Tensors<T> t, float2* __restrict__ sums, float2* __restrict__ partial,
                            Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
     __shared__ float2 group_sums[kMaxSlabGroups];
+    cudaTriggerProgrammaticLaunchCompletion();
     const Place<T> p = Place<T>::make(g, t.lengths, blockIdx.x);
     const int mine = p.own_rows();
     const int64_t from = p.at(g, p.begin + p.row);
@@ -289,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 3)
         }
     }
     __syncthreads();  // the slots become the threads' sums
-    add_up<T, kAligned>(db, dw, reinterpret_cast<float2*>(shared), group_sums,
+    add_up<T>(db, dw, reinterpret_cast<float2*>(shared), group_sums,
                         sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
                         t.weight, p, g);
     if (threadIdx.x < p.groups)
@@ -300,11 +350,18 @@ __global__ void __launch_bounds__(kThreads, 3)
 
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 3)
-    group_norm_gradient_kernel(Tensors<T> t, const float2* __restrict__ partial, Geometry g,
-                               int act) {
+    group_norm_gradient_kernel(Tensors<T> t, const float2* partial, Parameters<T> out, int streams,
+                               Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
+    if (blockIdx.x >= streams) {
+        cudaGridDependencySynchronize();
+        __shared__ float2 part[kThreads];
+        sum_parameters(out.sums, out.dweight, out.dbias, out.rows, g.channels, blockIdx.x - streams,
+                       part);
+        return;
+    }
     __shared__ float2 means[kMaxSlabGroups];
-    const Place<T> p = Place<T>::make(g, t.lengths, gridDim.x - 1 - blockIdx.x);
+    const Place<T> p = Place<T>::make(g, t.lengths, streams - 1 - blockIdx.x);
     const int mine = p.own_rows();
     const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
     const int64_t from = p.at(g, p.begin + p.row);
@@ -313,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     rows.from[1] = t.dout + from;
     rows.start(shared, mine, stride, p.count);
     const int count = g.parts * g.blocks;
+    cudaGridDependencySynchronize();
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
         const float2* add =
             partial + (static_cast<int64_t>(p.n) * g.groups + p.first_group + j) * count;
@@ -349,31 +407,12 @@ __global__ void __launch_bounds__(kThreads, 3)
     zero_padding<T, kAligned>(t.dx, p, g);
 }
 
-// Adds the blocks' rows of column sums, in an order that the launch fixes: 8 channels a block,
-// a thread every 128th row of one of them.
-constexpr int kSumChannels = 8, kSumRows = 128;
 template <typename T>
-__global__ void __launch_bounds__(kSumChannels* kSumRows)
-    group_norm_parameters_kernel(const float2* __restrict__ sums, T* __restrict__ dweight,
-                                 T* __restrict__ dbias, int rows, int channels) {
-    __shared__ float2 part[kSumRows][kSumChannels];
-    const int row = threadIdx.x / kSumChannels, lane = threadIdx.x % kSumChannels;
-    const int c = blockIdx.x * kSumChannels + lane;
-    float2 s = make_float2(0.0f, 0.0f);
-    if (c < channels) {
-#pragma unroll 8
-        for (int r = row; r < rows; r += kSumRows)
-            s = add2(s, sums[static_cast<int64_t>(r) * channels + c]);
-    }
-    part[row][lane] = s;
-    for (int half = kSumRows / 2; half > 0; half /= 2) {
-        __syncthreads();
-        if (row < half) part[row][lane] = add2(part[row][lane], part[row + half][lane]);
-    }
-    if (row == 0 && c < channels) {
-        dbias[c] = from_f32<T>(part[0][lane].x);
-        dweight[c] = from_f32<T>(part[0][lane].y);
-    }
+__global__ void __launch_bounds__(kThreads)
+    group_norm_parameters_kernel(Parameters<T> out, int channels) {
+    __shared__ float2 part[kThreads];
+    cudaGridDependencySynchronize();
+    sum_parameters(out.sums, out.dweight, out.dbias, out.rows, channels, blockIdx.x, part);
 }
 
 Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
@@ -401,27 +440,30 @@ cudaError_t run(const GroupNormBackwardProblem& p, const Shape& s, cudaStream_t 
     const int gather = g.blocks * g.slab_groups * static_cast<int>(sizeof(float2));
     const int part = std::max(columns * (kWarp % g.lanes == 0 ? kBlockWarps : g.step),
                               s.split ? 0 : columns + gather);
+    const Parameters<T> out{sums, static_cast<T*>(p.grad_weight), static_cast<T*>(p.grad_bias),
+                            static_cast<int>(rows)};
+    const int adders = (p.channels + kSumChannels - 1) / kSumChannels;
+    const int64_t blocks = s.units * g.blocks;
     cudaError_t e;
     if (!s.split) {
-        e = launch(resident, group_norm_backward_kernel<T, kAligned, kWhole>, s, true,
-                   g.rows * g.lanes * kVectorBytes<T> + part,
-                   kTileBytes + kThreads * kVectorBytes<T> + kSumBytes<T> + kGatherBytes, stream, t,
-                   sums, g, p.activation);
-    } else {
-        float2* partial = sums + rows * p.channels;
-        constexpr int kSlots = Stream<T, kAligned, 2>::kBytes, kMost = std::max(kSlots, kSumBytes<T>);
-        e = launch(first, group_norm_sums_kernel<T, kAligned, kWhole>, s, false,
-                   std::max(kSlots, part), kMost, stream, t, sums, partial, g, p.activation);
-        if (e == cudaSuccess)
-            e = launch(second, group_norm_gradient_kernel<T, kAligned, kWhole>, s, false, kSlots,
-                       kMost, stream, t, static_cast<const float2*>(partial), g, p.activation);
+        e = launch(resident, group_norm_backward_kernel<T, kAligned, kWhole>,
+                   {blocks, g.blocks, false, g.rows * g.lanes * kVectorBytes<T> + part,
+                    kTileBytes + kThreads * kVectorBytes<T> + kSumBytes<T> + kGatherBytes},
+                   stream, t, sums, g, p.activation);
+        if (e != cudaSuccess) return e;
+        return launch(second, group_norm_parameters_kernel<T>, {adders, 1, true, 0, 0}, stream, out,
+                      p.channels);
     }
+    constexpr int kSlots = Stream<T, kAligned, 2>::kBytes, kMost = std::max(kSlots, kSumBytes<T>);
+    float2* partial = sums + rows * p.channels;
+    e = launch(first, group_norm_sums_kernel<T, kAligned, kWhole>,
+               {blocks, 1, false, std::max(kSlots, part), kMost}, stream, t, sums, partial, g,
+               p.activation);
     if (e != cudaSuccess) return e;
-    group_norm_parameters_kernel<T><<<(p.channels + kSumChannels - 1) / kSumChannels,
-                                      kSumChannels * kSumRows, 0, stream>>>(
-        sums, static_cast<T*>(p.grad_weight), static_cast<T*>(p.grad_bias), static_cast<int>(rows),
-        p.channels);
-    return cudaGetLastError();
+    return launch(second, group_norm_gradient_kernel<T, kAligned, kWhole>,
+                  {blocks + adders, 1, true, kSlots, kSlots}, stream, t,
+                  static_cast<const float2*>(partial), out, static_cast<int>(blocks), g,
+                  p.activation);
 }
 
 template <typename T> cudaError_t run(const GroupNormBackwardProblem& p, cudaStream_t stream) {
