@@ -1,39 +1,30 @@
 """One call of a C ABI entry point on torch CUDA tensors, for the operators whose bindings
 include optional ones and a shape-dependent workspace (``normalization``, ``recurrence``).
 
-A call of a few microseconds of GPU work is bound by what Python does around it, so the
-descriptor arrays of a set of shapes and types are built once and reused; they hold no
-address.
+A call whose GPU work takes a few microseconds is bound by what Python does around it. So what
+follows from the shapes and types alone - the descriptor arrays, the workspace's size - is kept
+for the next call of the same shapes and types; nothing is kept by address or identity.
 """
 
 from __future__ import annotations
 
-import contextlib
-from functools import lru_cache
+import ctypes
+import threading
 
 import torch
 
 from . import _lib
-from .attention import _check, _torch_stream, _workspace, dtype_code
+from .attention import _check, _torch_stream, dtype_code
+
+_VP = ctypes.c_void_p
+_MOST_PLANS = 1024
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-class Absent:
-    """An optional binding that is not given: its descriptor without a buffer."""
-
-    __slots__ = ("dtype", "shape")
-
-    def __init__(self, dtype: torch.dtype, shape):
-        self.dtype, self.shape = dtype, tuple(shape)
-
-
-@lru_cache(maxsize=1024)
-def _descs(spec):
-    return _lib.desc_array([_lib.TensorDesc.make(dtype_code(d), s) for d, s in spec])
-
-
-def descs(tensors):
-    """Descriptor array of tensors, ``Absent`` bindings among them (shared: read only)."""
-    return _descs(tuple([(t.dtype, t.shape) for t in tensors]))
+def _current_stream(device: int) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(device)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def require(name: str, t, rank: int) -> None:
@@ -45,9 +36,8 @@ def require(name: str, t, rank: int) -> None:
                                   f"{name} of rank {t.dim()}")
 
 
-def _pointer(t, name: str, device: int, grad: bool):
-    if isinstance(t, Absent):
-        return None
+def _refuse(name: str, t, device: int, grad: bool) -> None:
+    """Why a binding cannot be launched on."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor (got {type(t).__name__})")
     if not t.is_cuda:
@@ -59,36 +49,99 @@ def _pointer(t, name: str, device: int, grad: bool):
     if grad and t.requires_grad:
         raise ValueError(f"{name} requires grad: this operator records no autograd graph; call "
                          "it under torch.no_grad() and use its backward function")
-    return t.data_ptr()
 
 
-def pointers(tensors, names):
-    device = torch.cuda.current_device()
-    grad = torch.is_grad_enabled()
-    return _lib.pointer_array([_pointer(t, n, device, grad) for t, n in zip(tensors, names)])
+def descs(bindings):
+    """Descriptor array of ``(dtype, shape)`` bindings."""
+    return _lib.desc_array([_lib.TensorDesc.make(dtype_code(d), s) for d, s in bindings])
 
 
-def launch_stream(stream):
-    """``(handle, context)``: the ``cudaStream_t`` of the launch, and the context in which
-    outputs and workspace are allocated, so that they belong to that stream."""
-    if stream is None:
-        return torch.cuda.current_stream().cuda_stream, contextlib.nullcontext()
-    stream = _torch_stream(stream)
-    return stream.cuda_stream, torch.cuda.stream(stream)
+class Operator:
+    """The entry point ``fga_<name>_enqueue`` with its bindings' names."""
 
+    def __init__(self, name: str, inputs: tuple[str, ...], outputs: tuple[str, ...]):
+        self.name, self.inputs, self.outputs = name, inputs, outputs
+        self._in_array, self._out_array = _VP * len(inputs), _VP * len(outputs)
+        self._enqueue = None
+        self._plans: dict = {}
+        self._lock = threading.Lock()
 
-def enqueue(op: str, tensors, names, outputs, out_names, fields, workspace, stream, context,
-            size_fields=()):
-    """Size the workspace and enqueue ``fga_<op>_enqueue``; raise on a nonzero status."""
-    lib = _lib.library()
-    ins, outs = descs(tensors), descs(outputs)
-    in_ptrs, out_ptrs = pointers(tensors, names), pointers(outputs, out_names)
-    size = getattr(lib, f"fga_{op}_workspace_size")(ins, len(tensors), *size_fields)
-    ws, ws_bytes = None, 0
-    if size:
-        with context:
-            ws, ws_bytes = _workspace(size, tensors[0].device, workspace, None)
-    status = getattr(lib, f"fga_{op}_enqueue")(ins, outs, in_ptrs, out_ptrs, *fields, ws,
-                                               ws_bytes, stream)
-    if status:
-        _check(status, op)
+    def __call__(self, tensors, given, allocate, absent, fields=(), size_fields=(), workspace=None,
+                 stream=None):
+        """Enqueue on ``tensors`` (None: an optional binding that is not given) and return the
+        outputs: those ``given``, and ``allocate()``'s where that has None (None there as well:
+        not wanted). ``absent(name)`` is the ``(dtype, shape)`` of a binding without a buffer.
+        Outputs and workspace are allocated with the launch's stream as torch's current one."""
+        device = torch.cuda.current_device()
+        if stream is None:
+            return self._launch(tensors, given, allocate, absent, fields, size_fields, workspace,
+                                device, _current_stream(device))
+        stream = _torch_stream(stream)
+        with torch.cuda.stream(stream):
+            return self._launch(tensors, given, allocate, absent, fields, size_fields, workspace,
+                                device, stream.cuda_stream)
+
+    def _launch(self, tensors, given, allocate, absent, fields, size_fields, workspace, device,
+                handle):
+        grad = torch.is_grad_enabled()
+        key, sources, i = [device, size_fields], [], 0
+        for t in tensors:
+            if t is None:
+                sources.append(None)
+                key.append(None)
+            else:
+                if (not isinstance(t, torch.Tensor) or t.get_device() != device
+                        or not t.is_contiguous() or (grad and t.requires_grad)):
+                    _refuse(self.inputs[i], t, device, grad)
+                sources.append(t.data_ptr())
+                key.append(t.dtype)
+                key.append(t.shape)
+            i += 1
+        i = 0
+        for t in given:
+            if t is None:
+                key.append(None)
+            else:
+                if (not isinstance(t, torch.Tensor) or t.get_device() != device
+                        or not t.is_contiguous() or (grad and t.requires_grad)):
+                    _refuse(self.outputs[i], t, device, grad)
+                key.append(t.dtype)
+                key.append(t.shape)
+            i += 1
+        outputs = allocate()
+        targets = [None if t is None else t.data_ptr() for t in outputs]
+        key = tuple(key)
+        ins, outs, size = self._plans.get(key) or self._plan(key, tensors, outputs, absent,
+                                                             size_fields)
+        address = None
+        if size:
+            if workspace is None:
+                workspace = torch.empty(size, dtype=torch.uint8, device=tensors[0].device)
+            elif (not isinstance(workspace, torch.Tensor) or workspace.get_device() != device
+                  or not workspace.is_contiguous()):
+                raise ValueError("workspace must be a contiguous CUDA tensor on the current device")
+            else:
+                size = workspace.numel() * workspace.element_size()
+            address = workspace.data_ptr()
+        if self._enqueue is None:
+            self._enqueue = getattr(_lib.library(), f"fga_{self.name}_enqueue")
+        status = self._enqueue(ins, outs, self._in_array(*sources), self._out_array(*targets),
+                               *fields, address, size, handle)
+        if status:
+            _check(status, self.name)
+        return outputs
+
+    def _plan(self, key, tensors, outputs, absent, size_fields):
+        """Descriptors and workspace size of a call's shapes and types. The outputs' follow from
+        the key: they are given, or shaped after an input."""
+        def bindings(ts, names):
+            return [absent(n) if t is None else (t.dtype, t.shape) for t, n in zip(ts, names)]
+
+        ins, outs = descs(bindings(tensors, self.inputs)), descs(bindings(outputs, self.outputs))
+        size = getattr(_lib.library(), f"fga_{self.name}_workspace_size")(
+            ins, len(tensors), *size_fields)
+        with self._lock:
+            if len(self._plans) >= _MOST_PLANS:
+                self._plans.clear()
+            plan = self._plans[key] = (ins, outs, size)
+        return plan

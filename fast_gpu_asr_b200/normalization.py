@@ -22,7 +22,13 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._call import Absent, descs, enqueue, launch_stream, require
+from ._call import Operator, descs, require
+
+_FORWARD = Operator("group_norm_activation", ("x", "valid_lengths", "weight", "bias"),
+                    ("out", "mean", "rstd"))
+_BACKWARD = Operator("group_norm_activation_backward",
+                     ("grad_out", "x", "valid_lengths", "weight", "bias", "mean", "rstd"),
+                     ("grad_x", "grad_weight", "grad_bias"))
 
 
 def _activation(name) -> int:
@@ -49,7 +55,7 @@ def group_norm_activation_workspace_size(x: torch.Tensor, valid_lengths: torch.T
                                          num_groups: int) -> int:
     """Bytes of device memory that a call with these bindings takes as ``workspace``."""
     return _lib.library().fga_group_norm_activation_workspace_size(
-        descs((x, valid_lengths, weight, bias)), 4, int(num_groups))
+        descs([(t.dtype, t.shape) for t in (x, valid_lengths, weight, bias)]), 4, int(num_groups))
 
 
 def group_norm_activation(x: torch.Tensor, valid_lengths: torch.Tensor, weight: torch.Tensor,
@@ -65,21 +71,18 @@ def group_norm_activation(x: torch.Tensor, valid_lengths: torch.Tensor, weight: 
     float32 ``[N, num_groups]``, which the backward call takes."""
     require("x", x, 3)
     num_groups = int(num_groups)
-    handle, context = launch_stream(stream)
-    shape = (x.shape[0], num_groups)
-    with context:
-        if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        if return_statistics and num_groups > 0:
-            mean = torch.empty(shape, dtype=torch.float32, device=x.device)
-            rstd = torch.empty(shape, dtype=torch.float32, device=x.device)
-        else:
-            mean = rstd = Absent(torch.float32, shape)
-    enqueue("group_norm_activation", (x, valid_lengths, weight, bias),
-            ("x", "valid_lengths", "weight", "bias"), (out, mean, rstd), ("out", "mean", "rstd"),
-            (num_groups, float(eps), _activation(activation)), workspace, handle, context,
-            size_fields=(num_groups,))
-    return (out, mean, rstd) if return_statistics else out
+
+    def allocate():
+        y = torch.empty_like(x) if out is None else out
+        if not return_statistics or num_groups < 1:
+            return y, None, None
+        shape = (x.shape[0], num_groups)
+        return y, x.new_empty(shape, dtype=torch.float32), x.new_empty(shape, dtype=torch.float32)
+
+    outputs = _FORWARD((x, valid_lengths, weight, bias), (out,), allocate,
+                       lambda name: (torch.float32, (x.shape[0], num_groups)),
+                       (num_groups, eps, _activation(activation)), (num_groups,), workspace, stream)
+    return outputs if return_statistics else outputs[0]
 
 
 def group_norm_activation_backward(grad_out: torch.Tensor, x: torch.Tensor,
@@ -93,13 +96,7 @@ def group_norm_activation_backward(grad_out: torch.Tensor, x: torch.Tensor,
     require("x", x, 3)
     require("weight", weight, 1)
     require("bias", bias, 1)
-    handle, context = launch_stream(stream)
-    with context:
-        outputs = tuple(torch.empty_like(t, memory_format=torch.contiguous_format)
-                        for t in (x, weight, bias))
-    enqueue("group_norm_activation_backward",
-            (grad_out, x, valid_lengths, weight, bias, mean, rstd),
-            ("grad_out", "x", "valid_lengths", "weight", "bias", "mean", "rstd"), outputs,
-            ("grad_x", "grad_weight", "grad_bias"), (_activation(activation),), workspace,
-            handle, context)
-    return outputs
+    return _BACKWARD((grad_out, x, valid_lengths, weight, bias, mean, rstd), (),
+                     lambda: (torch.empty_like(x), torch.empty_like(weight),
+                              torch.empty_like(bias)),
+                     None, (_activation(activation),), (), workspace, stream)

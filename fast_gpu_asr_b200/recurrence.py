@@ -24,7 +24,14 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._call import Absent, enqueue, launch_stream, require
+from ._call import Operator, require
+
+_FORWARD = Operator("gated_linear_recurrence",
+                    ("x", "gate", "valid_lengths", "initial_state"),
+                    ("out", "final_state", "states"))
+_BACKWARD = Operator("gated_linear_recurrence_backward",
+                     ("grad_out", "x", "gate", "valid_lengths", "states", "grad_final_state"),
+                     ("grad_x", "grad_gate", "grad_initial_state"))
 
 STATE_FRAMES = _lib.RECURRENCE_STATE_FRAMES
 
@@ -55,21 +62,17 @@ def gated_linear_recurrence(x: torch.Tensor, gate: torch.Tensor, valid_lengths: 
     backward call takes."""
     require("x", x, 3)
     n, t, c = x.shape
-    handle, context = launch_stream(stream)
-    state, saved = (n, c), (n, -(-t // STATE_FRAMES), c)
-    with context:
-        if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        if final_state is None:
-            final_state = torch.empty(state, dtype=torch.float32, device=x.device)
-        states = (torch.empty(saved, dtype=torch.float32, device=x.device) if return_states
-                  else Absent(torch.float32, saved))
-    if initial_state is None:
-        initial_state = Absent(torch.float32, state)
-    enqueue("gated_linear_recurrence", (x, gate, valid_lengths, initial_state),
-            ("x", "gate", "valid_lengths", "initial_state"), (out, final_state, states),
-            ("out", "final_state", "states"), (), None, handle, context)
-    return (out, final_state, states) if return_states else (out, final_state)
+    saved = (n, -(-t // STATE_FRAMES), c)
+
+    def allocate():
+        return (torch.empty_like(x) if out is None else out,
+                x.new_empty((n, c), dtype=torch.float32) if final_state is None else final_state,
+                x.new_empty(saved, dtype=torch.float32) if return_states else None)
+
+    outputs = _FORWARD((x, gate, valid_lengths, initial_state), (out, final_state), allocate,
+                       lambda name: (torch.float32, saved if name == "states" else (n, c)),
+                       stream=stream)
+    return outputs if return_states else outputs[:2]
 
 
 def gated_linear_recurrence_backward(grad_out: torch.Tensor, x: torch.Tensor,
@@ -82,15 +85,7 @@ def gated_linear_recurrence_backward(grad_out: torch.Tensor, x: torch.Tensor,
     ``grad_initial_state``."""
     require("x", x, 3)
     n, _, c = x.shape
-    handle, context = launch_stream(stream)
-    with context:
-        outputs = (torch.empty_like(x, memory_format=torch.contiguous_format),
-                   torch.empty_like(x, memory_format=torch.contiguous_format),
-                   torch.empty((n, c), dtype=torch.float32, device=x.device))
-    if grad_final_state is None:
-        grad_final_state = Absent(torch.float32, (n, c))
-    enqueue("gated_linear_recurrence_backward",
-            (grad_out, x, gate, valid_lengths, states, grad_final_state),
-            ("grad_out", "x", "gate", "valid_lengths", "states", "grad_final_state"), outputs,
-            ("grad_x", "grad_gate", "grad_initial_state"), (), None, handle, context)
-    return outputs
+    return _BACKWARD((grad_out, x, gate, valid_lengths, states, grad_final_state), (),
+                     lambda: (torch.empty_like(x), torch.empty_like(x),
+                              x.new_empty((n, c), dtype=torch.float32)),
+                     lambda name: (torch.float32, (n, c)), stream=stream)
