@@ -882,16 +882,27 @@ int32_t fga_gated_linear_recurrence_check(const fga_tensor_desc* in, int32_t nin
     return check_recurrence(in, nin, out, nout, nullptr);
 }
 
-size_t fga_gated_linear_recurrence_workspace_size(const fga_tensor_desc*, int32_t) { return 0; }
+size_t fga_gated_linear_recurrence_workspace_size(const fga_tensor_desc* in, int32_t nin) {
+    if (in == nullptr || nin != 4) return 0;
+    const fga_tensor_desc out[3] = {
+        in[0], in[3],
+        {FGA_FLOAT, 3, {in[0].dims[0], state_chunks(in[0].dims[1]), in[0].dims[2]}}};
+    fga::RecurrenceProblem p{};
+    if (check_recurrence(in, nin, out, 3, &p) != FGA_SUCCESS) return 0;
+    return fga::recurrence_workspace(p);
+}
 
 int32_t fga_gated_linear_recurrence_enqueue(const fga_tensor_desc* in,
                                             const fga_tensor_desc* out,
                                             const void* const* inputs, void* const* outputs,
-                                            void*, size_t, void* stream) {
+                                            void* workspace, size_t workspace_bytes,
+                                            void* stream) {
     fga::RecurrenceProblem p{};
     int32_t st = check_recurrence(in, 4, out, 3, &p);
     if (st != FGA_SUCCESS) return st;
     st = check_buffers(in, inputs, 4, 8u, out, outputs, 3, 4u, 3, 1);
+    if (st != FGA_SUCCESS) return st;
+    st = check_workspace(workspace, workspace_bytes, fga::recurrence_workspace(p));
     if (st != FGA_SUCCESS) return st;
     if ((st = prior_error_status()) != FGA_SUCCESS) return st;
     if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
@@ -902,6 +913,7 @@ int32_t fga_gated_linear_recurrence_enqueue(const fga_tensor_desc* in,
     p.output = outputs[0];
     p.final_state = static_cast<float*>(outputs[1]);
     p.states = static_cast<float*>(outputs[2]);
+    p.workspace = workspace;
     const char* variant = "none";
     if (fga::launch_recurrence(p, static_cast<cudaStream_t>(stream), &variant) != cudaSuccess)
         return FGA_ERROR_LAUNCH;
@@ -914,19 +926,26 @@ int32_t fga_gated_linear_recurrence_backward_check(const fga_tensor_desc* in, in
     return check_recurrence_backward(in, nin, out, nout, nullptr);
 }
 
-size_t fga_gated_linear_recurrence_backward_workspace_size(const fga_tensor_desc*, int32_t) {
-    return 0;
+size_t fga_gated_linear_recurrence_backward_workspace_size(const fga_tensor_desc* in,
+                                                           int32_t nin) {
+    if (in == nullptr || nin != 6) return 0;
+    const fga_tensor_desc out[3] = {in[1], in[2], in[5]};
+    fga::RecurrenceBackwardProblem p{};
+    if (check_recurrence_backward(in, nin, out, 3, &p) != FGA_SUCCESS) return 0;
+    return fga::recurrence_backward_workspace(p);
 }
 
 int32_t fga_gated_linear_recurrence_backward_enqueue(const fga_tensor_desc* in,
                                                      const fga_tensor_desc* out,
                                                      const void* const* inputs,
-                                                     void* const* outputs, void*, size_t,
-                                                     void* stream) {
+                                                     void* const* outputs, void* workspace,
+                                                     size_t workspace_bytes, void* stream) {
     fga::RecurrenceBackwardProblem p{};
     int32_t st = check_recurrence_backward(in, 6, out, 3, &p);
     if (st != FGA_SUCCESS) return st;
     st = check_buffers(in, inputs, 6, 32u, out, outputs, 3, 0u, -1, -1);
+    if (st != FGA_SUCCESS) return st;
+    st = check_workspace(workspace, workspace_bytes, fga::recurrence_backward_workspace(p));
     if (st != FGA_SUCCESS) return st;
     if ((st = prior_error_status()) != FGA_SUCCESS) return st;
     if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
@@ -939,6 +958,7 @@ int32_t fga_gated_linear_recurrence_backward_enqueue(const fga_tensor_desc* in,
     p.grad_x = outputs[0];
     p.grad_gate = outputs[1];
     p.grad_initial_state = static_cast<float*>(outputs[2]);
+    p.workspace = workspace;
     const char* variant = "none";
     if (fga::launch_recurrence_backward(p, static_cast<cudaStream_t>(stream), &variant) !=
         cudaSuccess)

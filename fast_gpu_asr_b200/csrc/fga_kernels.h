@@ -110,6 +110,7 @@ struct RecurrenceProblem {
     void* output;                  // [N, T, C]
     float* final_state;            // [N, C]; may be initial_state
     float* states;                 // [N, chunks, C] or null
+    void* workspace;
     int32_t batch, length, channels, chunks;
     int32_t dtype;
 };
@@ -124,6 +125,7 @@ struct RecurrenceBackwardProblem {
     void* grad_x;                   // [N, T, C]
     void* grad_gate;                // [N, T, C]
     float* grad_initial_state;      // [N, C]
+    void* workspace;
     int32_t batch, length, channels, chunks;
     int32_t dtype;
 };
@@ -144,9 +146,11 @@ cudaError_t launch_recurrence(const RecurrenceProblem& p, cudaStream_t stream,
                               const char** variant);
 cudaError_t launch_recurrence_backward(const RecurrenceBackwardProblem& p, cudaStream_t stream,
                                        const char** variant);
-// Workspace of the group norm launchers: from the shape and type alone.
+// Workspace of these four launchers: from the shape and type alone.
 size_t group_norm_workspace(const GroupNormProblem& p);
 size_t group_norm_backward_workspace(const GroupNormBackwardProblem& p);
+size_t recurrence_workspace(const RecurrenceProblem& p);
+size_t recurrence_backward_workspace(const RecurrenceBackwardProblem& p);
 // Tensor cores only: cudaErrorNotSupported outside the envelope (f16/bf16, qd = 32,
 // T <= 768, vd a multiple of 4 up to 16, H*vd a multiple of 8, aligned buffers).
 cudaError_t launch_zipformer_fused(const ZipformerFusedProblem& p, cudaStream_t stream);

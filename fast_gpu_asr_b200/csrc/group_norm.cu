@@ -37,8 +37,8 @@ template <typename Visit> __device__ __forceinline__ float2 merge(float total, V
     return make_float2(mean, warp_sum(squares));
 }
 
-// (mean, squares) of every group of the slab over this block's rows to moments[group]; row(i)
-// is this thread's vector of its i-th row (asked for in order), `first` that of the first. `part` holds an entry per thread (and channel, if
+// (mean, squares) of every group of the slab over this block's rows to moments[group]; each(work)
+// calls work(vector) for every row of this thread, `first` is that of its first. `part` holds an entry per thread (and channel, if
 // not kWhole).
 //
 // A thread takes both in one pass, about a pivot: the mean of its own first vector (the first
@@ -47,8 +47,8 @@ template <typename Visit> __device__ __forceinline__ float2 merge(float total, V
 // about the pivot is at most n / q times what is left, a factor on its rounding error: with 12
 // rows of a tile or 64 of a stream at most, and values that differ like that only where the
 // first vector is an outlier itself.
-template <typename T, bool kWhole, typename Row>
-__device__ __forceinline__ void block_moments(const uint4& first, Row row, float2* part, float2* moments,
+template <typename T, bool kWhole, typename Each>
+__device__ __forceinline__ void block_moments(const uint4& first, Each each, float2* part, float2* moments,
                                               const Place<T>& p, const Geometry& g) {
     constexpr int kValues = kWhole ? 1 : kVec<T>, kSums = kWhole ? 1 : kPairs<T>;
     const int mine = p.own_rows(), columns = g.lanes * kValues;
@@ -66,9 +66,8 @@ __device__ __forceinline__ void block_moments(const uint4& first, Row row, float
         }
 #pragma unroll
         for (int k = 0; k < kSums; ++k) sum[k] = squares[k] = splat2(0.0f);
-#pragma unroll 4
-        for (int i = 0; i < mine; ++i) {
-            unpack<T>(row(i), v);
+        each([&](const uint4& r) {
+            unpack<T>(r, v);
 #pragma unroll
             for (int e = 0; e < kPairs<T>; ++e) {
                 constexpr bool kOne = kWhole;
@@ -77,7 +76,7 @@ __device__ __forceinline__ void block_moments(const uint4& first, Row row, float
                 sum[k] = add2(sum[k], d);
                 squares[k] = fma2(d, d, squares[k]);
             }
-        }
+        });
         const float inv = 1.0f / static_cast<float>(mine * (kWhole ? kVec<T> : 1));
 #pragma unroll
         for (int e = 0; e < kValues; ++e) {
@@ -166,8 +165,10 @@ __global__ void __launch_bounds__(kThreads, 4)
             stage<T, kAligned>(at + i * pitch, from, p.count);
     }
     arrived();
-    block_moments<T, kWhole>(mine > 0 ? at[0] : uint4{}, [&](int i) { return at[i * pitch]; }, part,
-                             moments, p, g);
+    block_moments<T, kWhole>(mine > 0 ? at[0] : uint4{}, [&](auto work) {
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i) work(at[i * pitch]);
+    }, part, moments, p, g);
     __syncthreads();
     const float width = static_cast<float>(g.group_channels);
     const float total = static_cast<float>(p.m) * width;
@@ -227,10 +228,8 @@ __global__ void __launch_bounds__(kThreads, 4)
     rows.from[0] = t.x + p.at(g, p.begin + p.row);
     const uint4 first = p.own_rows() > 0 ? load<T, kAligned>(rows.from[0], p.count) : uint4{};
     rows.start(slots, p.own_rows(), static_cast<int64_t>(g.step) * g.channels, p.count);
-    block_moments<T, kWhole>(first, [&](int) {
-        uint4 v[1];
-        rows.next(v);
-        return v[0];
+    block_moments<T, kWhole>(first, [&](auto work) {
+        rows.each([&](const uint4(&v)[1]) { work(v[0]); });
     }, part, moments, p, g);
     __syncthreads();
     if (threadIdx.x < p.groups)
@@ -280,12 +279,10 @@ __global__ void __launch_bounds__(kThreads, 4)
         Column<T> column;
         column.template read<kAligned, kWhole>(t.weight, t.bias, stats, p, g);
         T* to = t.out + from;
-#pragma unroll 2
-        for (int i = 0; i < mine; ++i, to += stride) {
-            uint4 v[1];
-            rows.next(v);
+        rows.each([&](const uint4(&v)[1]) {
             store<T, kAligned>(to, column.apply(v[0], act), p.count);
-        }
+            to += stride;
+        });
     }
     zero_padding<T, kAligned>(t.out, p, g);
 }

@@ -235,26 +235,25 @@ struct Items {
     }
 };
 
-// A thread's vectors of its rows, in order, from kSources tensors at once: kDepth of them are on
-// their way through the thread's own slots of shared memory while it works on one, whatever
+// A thread's vectors of its rows, in order, from kSources tensors at once: kDepth - 1 of them are
+// on their way through the thread's own slots of shared memory while it works on one, whatever
 // the compiler makes of the loop's registers.
 constexpr int kDepth = 4;
 template <typename T, bool kAligned, int kSources> struct Stream {
     const T* from[kSources];
     uint4* slots;  // [kDepth][kSources][kThreads]
     int64_t stride;
-    int rows, count, at = 0, ahead = 0;
+    int rows, count;
 
     static constexpr int kBytes = kAligned ? kDepth * kSources * kThreads * 16 : 0;
 
-    __device__ __forceinline__ void request() {
-        if (ahead < rows)
+    __device__ __forceinline__ void request(bool wanted, int slot) {
+        if (wanted)
 #pragma unroll
             for (int k = 0; k < kSources; ++k) {
-                stage<T, true>(slots + (ahead % kDepth * kSources + k) * kThreads, from[k], count);
+                stage<T, true>(slots + (slot * kSources + k) * kThreads, from[k], count);
                 from[k] += stride;
             }
-        ++ahead;
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
     __device__ __forceinline__ void start(uint4* shared, int rows_, int64_t stride_, int count_) {
@@ -264,20 +263,28 @@ template <typename T, bool kAligned, int kSources> struct Stream {
         count = count_;
         if constexpr (kAligned)
 #pragma unroll
-            for (int i = 0; i < kDepth - 1; ++i) request();
+            for (int i = 0; i < kDepth - 1; ++i) request(i < rows, i);
     }
-    __device__ __forceinline__ void next(uint4 (&v)[kSources]) {
-        if constexpr (kAligned) {
-            request();
-            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    // work(vectors) for every row.
+    template <typename Work> __device__ __forceinline__ void each(Work work) {
+        for (int i = 0; i < rows; i += kDepth) {
 #pragma unroll
-            for (int k = 0; k < kSources; ++k) v[k] = slots[(at % kDepth * kSources + k) * kThreads];
-            ++at;
-        } else {
+            for (int s = 0; s < kDepth; ++s) {
+                if (i + s >= rows) break;
+                uint4 v[kSources];
+                if constexpr (kAligned) {
+                    request(i + s + kDepth - 1 < rows, (s + kDepth - 1) % kDepth);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
 #pragma unroll
-            for (int k = 0; k < kSources; ++k) {
-                v[k] = load<T, false>(from[k], count);
-                from[k] += stride;
+                    for (int k = 0; k < kSources; ++k) v[k] = slots[(s * kSources + k) * kThreads];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kSources; ++k) {
+                        v[k] = load<T, false>(from[k], count);
+                        from[k] += stride;
+                    }
+                }
+                work(v);
             }
         }
     }

@@ -26,8 +26,9 @@ constexpr int kGatherBytes = kMaxCluster * kMaxSlabGroups * static_cast<int>(siz
 // dz as fp32 planes of 16 bytes of each vector, the first of which held dout.
 template <typename T> constexpr int kPlanes = kVec<T> / 4;
 template <typename T> constexpr int kVectorBytes = 16 + 16 * kPlanes<T>;
-// What a thread adds up for each of its channels, in shared memory.
-template <typename T> constexpr int kSumBytes = kThreads * kVec<T> * static_cast<int>(sizeof(float2));
+// What the threads add up for each of their channels, in shared memory, and the columns' sums.
+template <typename T>
+constexpr int kSumBytes = 2 * kThreads * kVec<T> * static_cast<int>(sizeof(float2));
 
 template <typename T> struct Tensors {
     const T* dout;
@@ -128,23 +129,25 @@ __device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPa
         if (lane < g.lanes)
 #pragma unroll
             for (int e = 0; e < kVec<T>; ++e)
-                part[threadIdx.x / kWarp * columns + lane * kVec<T> + e] =
+                part[threadIdx.x / kWarp * columns + e * g.lanes + lane] =
                     make_float2(channel_of(db, e), channel_of(dw, e));
     } else if (p.row < g.step) {
 #pragma unroll
         for (int e = 0; e < kVec<T>; ++e)
-            part[p.row * columns + p.lane * kVec<T> + e] =
+            part[p.row * columns + e * g.lanes + p.lane] =
                 make_float2(channel_of(db, e), channel_of(dw, e));
     }
     __syncthreads();
+    float2* weighted = part + rows * columns;  // by channel, for the groups' sums
     float2 own = splat2(0.0f);
     for (int c = threadIdx.x; c < p.channels; c += kThreads) {
-        float2 s = part[c];
-        for (int r = 1; r < rows; ++r) s = add2(s, part[r * columns + c]);
+        const float2* column = part + c % kVec<T> * g.lanes + c / kVec<T>;
+        float2 s = column[0];
+        for (int r = 1; r < rows; ++r) s = add2(s, column[r * columns]);
         sums[p.first_channel + c] = s;
         if (c >= kThreads) w = to_f32<T>(weight[p.first_channel + c]);
         s = mul2(s, splat2(w));
-        part[c] = s;
+        if (p.groups > 1) weighted[c] = s;
         own = add2(own, s);
     }
     if (p.groups == 1) {
@@ -162,7 +165,7 @@ __device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPa
         const int width = p.channels / p.groups;
         for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
             float2 s = splat2(0.0f);
-            for (int c = threadIdx.x % kWarp; c < width; c += kWarp) s = add2(s, part[j * width + c]);
+            for (int c = threadIdx.x % kWarp; c < width; c += kWarp) s = add2(s, weighted[j * width + c]);
             s = make_float2(warp_sum(s.x), warp_sum(s.y));
             if (threadIdx.x % kWarp == 0) group_sums[j] = s;
         }
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 3)
                         sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
                         t.weight, p, g);
     if (g.blocks > 1) {
-        float2* gathered = part + g.lanes * kVec<T>;  // behind the columns' sums: [block][group]
+        float2* gathered = part;  // [block][group]
         auto cluster = cg::this_cluster();
         cluster.sync();  // every block runs, and has its sums
         for (int q = threadIdx.x / kWarp; q < g.blocks; q += kBlockWarps)
@@ -323,10 +326,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     if (mine > 0) {
         Column<T, kWhole> column;
         column.template read<kAligned>(t, p, g);
-#pragma unroll 2
-        for (int i = 0; i < mine; ++i) {
-            uint4 v[2];
-            rows.next(v);
+        rows.each([&](const uint4(&v)[2]) {
             float2 x[kPairs<T>], d[kPairs<T>];
             unpack<T>(v[0], x);
             unpack<T>(v[1], d);
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 3)
                 db[e] = add2(db[e], d[e]);
                 dw[e] = fma2(d[e], column.normalised(x[e], e), dw[e]);
             }
-        }
+        });
     }
     __syncthreads();  // the slots become the threads' sums
     add_up<T>(db, dw, reinterpret_cast<float2*>(shared), group_sums,
@@ -391,10 +391,7 @@ __global__ void __launch_bounds__(kThreads, 3)
         Final<T, kWhole> final_;
         final_.make(column, means, inv, p, g);
         T* to = t.dx + from;
-#pragma unroll 2
-        for (int i = 0; i < mine; ++i, to += stride) {
-            uint4 v[2];
-            rows.next(v);
+        rows.each([&](const uint4(&v)[2]) {
             float2 x[kPairs<T>], d[kPairs<T>];
             unpack<T>(v[0], x);
             unpack<T>(v[1], d);
@@ -402,7 +399,8 @@ __global__ void __launch_bounds__(kThreads, 3)
 #pragma unroll
             for (int e = 0; e < kPairs<T>; ++e) d[e] = final_(d[e], x[e], column.scale[e], e);
             store<T, kAligned>(to, pack<T>(d), p.count);
-        }
+            to += stride;
+        });
     }
     zero_padding<T, kAligned>(t.dx, p, g);
 }
@@ -434,12 +432,13 @@ cudaError_t run(const GroupNormBackwardProblem& p, const Shape& s, cudaStream_t 
     const Geometry& g = s.geo;
     float2* sums = static_cast<float2*>(p.workspace);
     const int64_t rows = sum_rows(s, p.batch);
-    // The sums of a warp's rows of threads, or of each row of threads; behind the first of them
-    // what a cluster gathers.
+    // The sums of a warp's rows of threads, or of each row of threads, and the columns' for more
+    // than one group; in their place, what a cluster gathers.
     const int columns = g.lanes * kVec<T> * static_cast<int>(sizeof(float2));
     const int gather = g.blocks * g.slab_groups * static_cast<int>(sizeof(float2));
-    const int part = std::max(columns * (kWarp % g.lanes == 0 ? kBlockWarps : g.step),
-                              s.split ? 0 : columns + gather);
+    const int part = std::max(columns * ((kWarp % g.lanes == 0 ? kBlockWarps : g.step) +
+                                         (g.slab_groups > 1 ? 1 : 0)),
+                              s.split ? 0 : gather);
     const Parameters<T> out{sums, static_cast<T*>(p.grad_weight), static_cast<T*>(p.grad_bias),
                             static_cast<int>(rows)};
     const int adders = (p.channels + kSumChannels - 1) / kSumChannels;

@@ -4,27 +4,26 @@
 //   dx[t] = p[t] G[t], dgate[t] = f[t] p[t] (h[t-1] - x[t]) G[t], dinitial = f[0] G[0].
 //
 // A run of frames takes h to A h + B, with A the product of its f and B what it makes of
-// h = 0, and runs compose: that is the scan. A warp takes kFrames consecutive frames of one
-// 128-byte row's channels (a lane one value of f32, two of a 16-bit type), finds its (A, B),
-// learns the state before its first frame from the warps before it through shared memory, and
-// walks its frames again from there, so that no element is read twice. A block's warps cover
-// one tile; a block walks the tiles of its utterance and channels in turn, with the next
-// tile's rows on their way to shared memory meanwhile. The backward pass runs the same scan
-// from the last tile to the first for the carry c[t] = f[t] G[t], and recomputes h from the
+// h = 0, and runs compose: that is the scan, and the backward pass is the same scan against
+// time for the carry c[t] = f[t] G[t]. A warp works on consecutive frames of a 128-byte row's
+// channels (a lane one value of f32, two of a 16-bit type).
+//
+// A block walks the tiles of one utterance's slab of channels; its warps take kFrames frames of
+// the tile each, find their (A, B), learn the state before their first frame from the warps
+// before them, and finish from registers, so that no element is read twice. The next tile's
+// rows are on their way to shared memory meanwhile. The backward pass recomputes h from the
 // states that the forward pass saved every 64 frames.
 //
-// Where utterances and channels are too few to fill the GPU, a cluster of blocks divides the
-// frames: each block first finds the (A, B) of its whole range, reading it once more (the
-// second time from L2), the blocks exchange them through distributed shared memory, and each
-// walks its tiles from the state that it now knows.
-#include <cooperative_groups.h>
-
+// Where utterances and channels are too few to fill the GPU, several blocks divide an
+// utterance's tiles: a first launch leaves the (A, B) of each block's frames in the workspace,
+// and a block of the second starts from what those before it make of the state.
 #include <algorithm>
 #include <cstdint>
 #include <initializer_list>
 #include <type_traits>
 
 #include "../../include/fga_convolution.h"
+#include "f32x2.cuh"
 #include "fga_common.cuh"
 #include "fga_kernels.h"
 #include "host_util.h"
@@ -32,55 +31,56 @@
 namespace fga {
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int kChunk = FGA_RECURRENCE_STATE_FRAMES;
-constexpr int kMaxCluster = 16;
-constexpr int kRow = 128;  // bytes of a row that a warp takes
-constexpr int kFrames = 8, kWarps = 8;
-constexpr int kTile = kFrames * kWarps;
-constexpr int kForwardBlocks = 4, kBackwardBlocks = 3;  // on a multiprocessor
-static_assert(kTile == kChunk, "a tile starts at a saved state");
+constexpr int kRow = 128;   // bytes of a row that a warp takes
+constexpr int kFrames = 8;  // rows that a warp moves at a time
+constexpr int kRows = kFrames * kRow;
 
 // ---- a lane's four bytes of a row ----------------------------------------------------------
+using fga::add2;
+using fga::fma2;
+using fga::mul2;
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float mul2(float a, float b) { return a * b; }
+__device__ __forceinline__ float add2(float a, float b) { return a + b; }
+
 template <typename T> struct Lane {
     static constexpr int kVec = 2;
+    using Value = float2;
     using Raw = uint32_t;
-    static __device__ __forceinline__ void unpack(Raw r, float* v) {
-        float2 f;
-        if constexpr (std::is_same_v<T, __half>) f = __half22float2(*reinterpret_cast<__half2*>(&r));
-        else f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&r));
-        v[0] = f.x;
-        v[1] = f.y;
-    }
-    static __device__ __forceinline__ Raw pack(const float* v) {
-        if constexpr (std::is_same_v<T, __half>) {
-            const __half2 h = __floats2half2_rn(v[0], v[1]);
-            return *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
-            return *reinterpret_cast<const uint32_t*>(&h);
-        }
-    }
+    static __device__ __forceinline__ Value unpack(Raw r) { return unpack2<T>(r); }
+    static __device__ __forceinline__ Raw pack(Value v) { return pack2<T>(v); }
+    static __device__ __forceinline__ Value all(float v) { return splat2(v); }
     static constexpr uint32_t kInfinity = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
 };
 template <> struct Lane<float> {
     static constexpr int kVec = 1;
+    using Value = float;
     using Raw = float;
-    static __device__ __forceinline__ void unpack(Raw r, float* v) { v[0] = r; }
-    static __device__ __forceinline__ Raw pack(const float* v) { return v[0]; }
+    static __device__ __forceinline__ Value unpack(Raw r) { return r; }
+    static __device__ __forceinline__ Raw pack(Value v) { return v; }
+    static __device__ __forceinline__ Value all(float v) { return v; }
     static constexpr uint32_t kInfinity = 0x7f800000u;
 };
 
 // f and p = 1 - f, both with all their bits: e = exp(-gate), f = 1 / (1 + e), p = e f. The
-// exponent stops at 126, where f is the smallest normal number and p is 1; a NaN stays one. The
-// special functions flush subnormals: otherwise each costs three more instructions.
-__device__ __forceinline__ void gates(float g, float& f, float& p) {
+// exponent stops at 126, where f is the smallest normal number and p is 1; a NaN stays one.
+__device__ __forceinline__ float stop(float exponent) {
     float e;
-    asm("min.NaN.f32 %0, %1, 0f42fc0000;" : "=f"(e) : "f"(g * -kLog2e));
-    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(1.0f + e));
+    asm("min.NaN.f32 %0, %1, 0f42fc0000;" : "=f"(e) : "f"(exponent));
+    return e;
+}
+__device__ __forceinline__ void gates(float g, float& f, float& p) {
+    const float e = exp2_approx(stop(g * -kLog2e));
+    f = reciprocal_approx(1.0f + e);
     p = e * f;
+}
+__device__ __forceinline__ void gates(float2 g, float2& f, float2& p) {
+    const float2 t = mul2(g, splat2(-kLog2e));
+    const float2 e = make_float2(exp2_approx(stop(t.x)), exp2_approx(stop(t.y)));
+    const float2 d = add2(e, splat2(1.0f));
+    f = make_float2(reciprocal_approx(d.x), reciprocal_approx(d.y));
+    p = mul2(e, f);
 }
 
 // ---- rows between global and shared memory -------------------------------------------------
@@ -90,6 +90,9 @@ struct Rows {
     uint32_t pitch;
     int bytes;  // of the slab's row: less than kRow in the last slab
 };
+
+template <int kUnit>
+using Unit = std::conditional_t<kUnit == 16, uint4, std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
 
 template <int kUnit> __device__ __forceinline__ void copy_unit(char* to, const char* from) {
     if constexpr (kUnit == 2) {
@@ -117,10 +120,8 @@ __device__ __forceinline__ void fetch(char* to, const void* from, const Rows& at
                                  static_cast<const char*>(from) + (row * at.pitch + byte));
         } else if constexpr (kUnit == 16) {
             *reinterpret_cast<uint4*>(to + u * kUnit) = make_uint4(fill, fill, fill, fill);
-        } else if constexpr (kUnit == 4) {
-            *reinterpret_cast<uint32_t*>(to + u * kUnit) = fill;
         } else {
-            *reinterpret_cast<uint16_t*>(to + u * kUnit) = static_cast<uint16_t>(fill);
+            *reinterpret_cast<Unit<kUnit>*>(to + u * kUnit) = static_cast<Unit<kUnit>>(fill);
         }
     }
 }
@@ -129,14 +130,12 @@ template <int kUnit>
 __device__ __forceinline__ void store(void* to, const char* from, const Rows& at, int rows,
                                       int lane) {
     constexpr int kPerRow = kRow / kUnit;
-    using Unit = std::conditional_t<kUnit == 16, uint4,
-                                    std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
 #pragma unroll 2
     for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
         const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
         if (row < rows && byte < at.bytes)
-            *reinterpret_cast<Unit*>(static_cast<char*>(to) + (row * at.pitch + byte)) =
-                *reinterpret_cast<const Unit*>(from + u * kUnit);
+            *reinterpret_cast<Unit<kUnit>*>(static_cast<char*>(to) + (row * at.pitch + byte)) =
+                *reinterpret_cast<const Unit<kUnit>*>(from + u * kUnit);
     }
 }
 
@@ -146,526 +145,468 @@ template <int kUnit>
 __device__ __forceinline__ void zero_rows(void* utterance, const Rows& at, int from, int to,
                                           int warp, int by, int lane) {
     constexpr int kPerRow = kRow / kUnit, kRun = kPerRow < kWarp ? kWarp / kPerRow : 1;
-    using Unit = std::conditional_t<kUnit == 16, uint4,
-                                    std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
     for (int t = from + warp * kRun; t < to; t += by * kRun) {
 #pragma unroll
         for (int u = lane; u < kRun * kPerRow; u += kWarp) {
             const int row = t + u / kPerRow, byte = u % kPerRow * kUnit;
             if (row < to && byte < at.bytes)
-                *reinterpret_cast<Unit*>(static_cast<char*>(utterance) +
-                                         row * static_cast<int64_t>(at.pitch) + byte) = Unit{};
+                *reinterpret_cast<Unit<kUnit>*>(static_cast<char*>(utterance) +
+                                                row * static_cast<int64_t>(at.pitch) + byte) =
+                    Unit<kUnit>{};
         }
     }
 }
 
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the newest group have arrived, for every lane of the warp.
-__device__ __forceinline__ void arrived() {
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+// All but the newest kNewer groups have arrived, for every lane of the warp.
+template <int kNewer> __device__ __forceinline__ void arrived() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kNewer) : "memory");
     __syncwarp();
 }
 
 struct Geometry {
     int length, channels, chunks;
-    int slabs;    // of kRow bytes
-    int cluster;  // blocks that share an utterance's slab
-    int tiles;    // consecutive tiles of a block in a round of the cluster
+    int slabs;   // of kRow bytes
+    int blocks;  // that divide an utterance's slab
+    int span;    // frames of a block, whole tiles
 };
 
 // What a thread works on.
 template <typename T> struct Place {
-    int n, m, channel, rank, warp, lane;
+    int n, m, channel, unit, block, warp, lane, warps;
+    int begin, end;  // the block's frames
     int64_t first;  // the utterance's first row at the slab, in elements
+    int64_t state;  // of [N, C] at this lane's channel
     Rows rows;
+    int present;    // how many of the lane's channels exist
     __device__ Place(const Geometry& g, const int32_t* lengths) {
         warp = threadIdx.x / kWarp;
         lane = threadIdx.x % kWarp;
-        rank = blockIdx.x % g.cluster;
-        const int unit = blockIdx.x / g.cluster;
+        warps = blockDim.x / kWarp;
+        unit = blockIdx.x / g.blocks;
+        block = blockIdx.x - unit * g.blocks;
         n = unit / g.slabs;
-        const int slab = unit % g.slabs * (kRow / static_cast<int>(sizeof(T)));
+        const int slab = (unit - n * g.slabs) * (kRow / static_cast<int>(sizeof(T)));
         channel = slab + lane * Lane<T>::kVec;
+        present = g.channels - channel;
         m = min(max(lengths[n], 0), g.length);
+        begin = block * g.span;
+        end = max(begin, min(m, begin + g.span));
         rows.pitch = static_cast<uint32_t>(g.channels) * sizeof(T);
         first = static_cast<int64_t>(n) * g.length * g.channels + slab;
+        state = static_cast<int64_t>(n) * g.channels + channel;
         rows.bytes = min(kRow, (g.channels - slab) * static_cast<int>(sizeof(T)));
     }
-};
-
-// A lane's values of an [.., C] f32 row at the slab; channels past the last are skipped.
-template <int kVec>
-__device__ __forceinline__ void read_state(float* v, const float* row, int channel, int channels) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = row != nullptr && channel + i < channels ? row[channel + i] : 0.0f;
-}
-template <int kVec>
-__device__ __forceinline__ void write_state(float* row, const float* v, int channel, int channels) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
-        if (channel + i < channels) row[channel + i] = v[i];
-}
-
-// What the warps of a block and the blocks of a cluster tell one another. Two of each in turn,
-// so that one barrier a tile (or a round) is enough.
-struct Runs {
-    float2 warp[2][kWarps][2 * kWarp];  // (A, B)
-    float back[2][kWarps][2 * kWarp];   // B of the carry (backward)
-    float behind[2][2 * kWarp];         // the state (forward) or carry (backward) after the tile
-};
-struct ClusterRuns {
-    float2 block[2][kMaxCluster][2 * kWarp];
-};
-
-// Dynamic shared memory: each warp's stages of rows, Runs, and in a cluster ClusterRuns.
-constexpr int kForwardStage = 2 * kFrames * kRow, kBackwardStage = 3 * kFrames * kRow;
-constexpr int smem_bytes(int stage, bool cluster) {
-    return 2 * kWarps * stage + static_cast<int>(sizeof(Runs)) +
-           (cluster ? static_cast<int>(sizeof(ClusterRuns)) : 0);
-}
-
-// This block's share of a round of the cluster, in frames.
-struct Range {
-    int begin, end;
-    __device__ Range(const Geometry& g, int m, int rank, int round_start) {
-        if (g.cluster == 1) {
-            begin = 0;
-            end = m;
-        } else {
-            begin = round_start + rank * g.tiles * kTile;
-            end = max(begin, min(m, begin + g.tiles * kTile));
-        }
+    // The block of the last valid frame, or the first where there is none.
+    __device__ bool last_valid(const Geometry& g) const {
+        return begin < m ? m <= begin + g.span : m == 0 && block == 0;
+    }
+    // Of [N, chunks, C] at this lane's channel.
+    __device__ int64_t saved(const Geometry& g, int chunk) const {
+        return (static_cast<int64_t>(n) * g.chunks + chunk) * g.channels + channel;
     }
 };
 
-// (A, B) of this block's frames to every block of the cluster, from those of its warps'
-// consecutive parts in runs.warp[turn]: in the order of time, or against it. Returns once all
-// have arrived in others.block[which].
-template <int kVec, bool kBack>
-__device__ __forceinline__ void exchange(const Runs& runs, ClusterRuns& others, int turn,
-                                         int which, int rank, int warp, int state,
-                                         int cluster_size) {
-    auto cluster = cg::this_cluster();
+__device__ __forceinline__ void read_state(float2& v, const float* at, int present) {
+    v.x = at != nullptr && present > 0 ? at[0] : 0.0f;
+    v.y = at != nullptr && present > 1 ? at[1] : 0.0f;
+}
+__device__ __forceinline__ void read_state(float& v, const float* at, int present) {
+    v = at != nullptr && present > 0 ? at[0] : 0.0f;
+}
+__device__ __forceinline__ void write_state(float* at, float2 v, int present) {
+    if (present > 0) at[0] = v.x;
+    if (present > 1) at[1] = v.y;
+}
+__device__ __forceinline__ void write_state(float* at, float v, int present) {
+    if (present > 0) at[0] = v;
+}
+
+template <typename V> struct alignas(2 * sizeof(V)) Run {
+    V a, b;  // takes h to a h + b
+    __device__ __forceinline__ V operator()(V h) const { return fma2(a, h, b); }
+    // This one, and then the next.
+    __device__ __forceinline__ void then(const Run& next) {
+        b = next(b);
+        a = mul2(a, next.a);
+    }
+};
+
+template <typename T> struct Forward {
+    const T* x;
+    const T* gate;
+    const int32_t* lengths;
+    const float* initial;  // or null
+    T* out;
+    float* final_state;    // may be `initial`
+    float* states;         // or null
+    void* runs;            // [units, blocks, 32] Run; null for one block
+    float* first;          // the initial state's copy, behind them
+};
+
+template <typename T> struct Backward {
+    const T* dout;
+    const T* x;
+    const T* gate;
+    const int32_t* lengths;
+    const float* states;
+    const float* dfinal;  // or null
+    T* dx;
+    T* dgate;
+    float* dinitial;
+    void* runs;
+};
+
+// Rows [t, end) of a tensor to kRows bytes of shared memory.
+template <int kUnit, typename T>
+__device__ __forceinline__ void fetch_rows(char* to, const T* tensor, const Place<T>& at,
+                                           const Geometry& g, int t, int end, uint32_t fill) {
+    fetch<kUnit>(to, tensor + at.first + t * static_cast<int64_t>(g.channels), at.rows, end - t,
+                 fill, at.lane);
+}
+template <int kUnit, typename T>
+__device__ __forceinline__ void store_rows(T* tensor, const char* from, const Place<T>& at,
+                                           const Geometry& g, int t, int end) {
+    store<kUnit>(tensor + at.first + t * static_cast<int64_t>(g.channels), from, at.rows, end - t,
+                 at.lane);
+}
+template <typename T>
+__device__ __forceinline__ typename Lane<T>::Value value(const char* rows, int i, int lane) {
+    using Raw = typename Lane<T>::Raw;
+    return Lane<T>::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[lane]);
+}
+template <typename T>
+__device__ __forceinline__ void put(char* rows, int i, int lane, typename Lane<T>::Value v) {
+    using Raw = typename Lane<T>::Raw;
+    reinterpret_cast<Raw*>(rows + i * kRow)[lane] = Lane<T>::pack(v);
+}
+
+// The padding of an output and of the saved states; `index` and `by` number all warps that work
+// on the slab.
+template <int kUnit, typename T>
+__device__ __forceinline__ void finish(const Forward<T>& f, const Place<T>& at, const Geometry& g) {
+    const int index = at.block * at.warps + at.warp, by = g.blocks * at.warps;
+    zero_rows<kUnit>(f.out + at.first, at.rows, at.m, g.length, index, by, at.lane);
+    if (f.states != nullptr)
+        for (int j = (at.m + kChunk - 1) / kChunk + index; j < g.chunks; j += by)
+            write_state(f.states + at.saved(g, j), Lane<T>::all(0.0f), at.present);
+}
+template <int kUnit, typename T>
+__device__ __forceinline__ void finish(const Backward<T>& f, const Place<T>& at, const Geometry& g) {
+    const int index = at.block * at.warps + at.warp, by = g.blocks * at.warps;
+    for (T* grad : {f.dx, f.dgate})
+        zero_rows<kUnit>(grad + at.first, at.rows, at.m, g.length, index, by, at.lane);
+}
+
+// ---- the walk ------------------------------------------------------------------------------
+// A tile is 64 frames: 8 warps of 8. More frames a warp need more registers than an SM has for
+// the blocks that hide the memory's latency (16 measured 167 us where 8 take 79, 256 x 375 x
+// 1024 bf16 ragged); fewer spend more on the scan across warps.
+constexpr int kWarps = 8, kTile = kFrames * kWarps;
+constexpr int kForwardBlocks = 4, kBackwardBlocks = 3;  // on a multiprocessor
+static_assert(kTile == kChunk, "a tile starts at a saved state");
+
+// What the warps tell one another, two of each in turn, so that one barrier a tile is enough.
+template <typename V> struct Tile {
+    Run<V> run[2][kWarps][kWarp];
+    V back[2][kWarps][kWarp];  // B of the carry (backward)
+    V behind[2][kWarp];        // the state (forward) or carry (backward) after the tile
+};
+constexpr int kForwardStage = 2 * kRows, kBackwardStage = 3 * kRows;
+template <typename V> constexpr int tile_smem(int stage) {
+    return 2 * kWarps * stage + static_cast<int>(sizeof(Tile<V>));
+}
+
+// What the blocks before this one make of `v`, or (kBack) those behind it: each warp composes a
+// share of their runs, which the warps then compose.
+template <bool kBack, typename V, typename T>
+__device__ __forceinline__ V through_blocks(V v, const void* runs, Tile<V>& tile,
+                                            const Place<T>& at, const Geometry& g) {
+    const Run<V>* all =
+        static_cast<const Run<V>*>(runs) + static_cast<int64_t>(at.unit) * g.blocks * kWarp + at.lane;
+    const int count = kBack ? g.blocks - 1 - at.block : at.block;
+    const int each = (count + kWarps - 1) / kWarps, from = at.warp * each;
+    Run<V> run{Lane<T>::all(1.0f), Lane<T>::all(0.0f)};
+#pragma unroll 4
+    for (int i = from; i < min(count, from + each); ++i)
+        run.then(all[(kBack ? g.blocks - 1 - i : i) * kWarp]);
+    tile.run[1][at.warp][at.lane] = run;
     __syncthreads();
-    float a[kVec], b[kVec];
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
-    for (int i = 0; i < kWarps; ++i)
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-            const float2 r = runs.warp[turn][kBack ? kWarps - 1 - i : i][state + v];
-            b[v] = fmaf(r.x, b[v], r.y);
-            a[v] *= r.x;
-        }
-    for (int q = warp; q < cluster_size; q += kWarps) {
-        float2* there = cluster.map_shared_rank(&others.block[which][rank][0], q);
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) there[state + v] = make_float2(a[v], b[v]);
-    }
-    cluster.sync();
+    for (int w = 0; w < kWarps; ++w) v = tile.run[1][w][at.lane](v);
+    return v;
 }
 
 template <typename T, int kUnit>
-__global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks) recurrence_kernel(
-    const T* __restrict__ x, const T* __restrict__ gate, const int32_t* __restrict__ lengths,
-    const float* initial, T* __restrict__ out, float* final_state, float* __restrict__ states,
-    Geometry geo) {
+__global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
+    recurrence_kernel(Forward<T> f, Geometry geo) {
     using L = Lane<T>;
-    using Raw = typename L::Raw;
-    constexpr int kVec = L::kVec;
+    using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
-    Runs& runs = *reinterpret_cast<Runs*>(smem + 2 * kWarps * kForwardStage);
-    ClusterRuns& others = *reinterpret_cast<ClusterRuns*>(&runs + 1);
-
-    const Place<T> at(geo, lengths);
+    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kForwardStage);
+    const Place<T> at(geo, f.lengths);
     char* stage = smem + at.warp * 2 * kForwardStage;
-    const int last_warp = blockDim.x / kWarp - 1, state = at.lane * kVec;
-    const int64_t state_row = static_cast<int64_t>(at.n) * geo.channels;
-    float* saved = states == nullptr
-                       ? nullptr
-                       : states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels;
+    const int last = at.warps - 1;
 
-    // Rows [t, end) to a stage.
-    auto fetch_rows = [&](int t, int end, int which) {
-        const int64_t here = at.first + t * static_cast<int64_t>(geo.channels);
+    auto fetch_tile = [&](int start, int which) {
+        const int t = start + at.warp * kFrames;
         char* to = stage + which * kForwardStage;
-        fetch<kUnit>(to, x + here, at.rows, end - t, 0u, at.lane);
+        fetch_rows<kUnit>(to, f.x, at, geo, t, at.end, 0u);
         // An infinite gate keeps the state.
-        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, end - t, L::kInfinity, at.lane);
+        fetch_rows<kUnit>(to + kRows, f.gate, at, geo, t, at.end, L::kInfinity);
     };
-    float carry[kVec];  // before the round
-    read_state<kVec>(carry, initial == nullptr ? nullptr : initial + state_row, at.channel,
-                     geo.channels);
-    // Every block of the cluster runs, and has read its state, before any writes to another.
-    if (geo.cluster > 1) cg::this_cluster().sync();
-
-    int turn = 0, which = 0;
-    const int round = geo.cluster == 1 ? geo.length : geo.cluster * geo.tiles * kTile;
-    for (int round_start = 0; round_start < at.m; round_start += round, which ^= 1) {
-        const Range range(geo, at.m, at.rank, round_start);
-        float h[kVec];
-        if (geo.cluster > 1) {
-            // This warp's part of the range, for its (A, B) alone.
-            const int part = geo.tiles * kFrames, from = range.begin + at.warp * part;
-            const int to = min(range.end, from + part);
-            float a[kVec], b[kVec];
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
-            if (from < to) fetch_rows(from, to, 0);
-            commit();
-            for (int t = from, s = 0; t < to; t += kFrames, s ^= 1) {
-                if (t + kFrames < to) fetch_rows(t + kFrames, to, s ^ 1);
-                commit();
-                arrived();
-                const char* rows = stage + s * kForwardStage;
-#pragma unroll
-                for (int i = 0; i < kFrames; ++i) {
-                    float xv[kVec], gv[kVec];
-                    L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
-                    L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
-#pragma unroll
-                    for (int v = 0; v < kVec; ++v) {
-                        float f, p;
-                        gates(gv[v], f, p);
-                        a[v] *= f;
-                        b[v] = fmaf(f, b[v], p * xv[v]);
-                    }
-                }
-                __syncwarp();
-            }
-#pragma unroll
-            for (int v = 0; v < kVec; ++v)
-                runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
-            exchange<kVec, false>(runs, others, turn, which, at.rank, at.warp, state, geo.cluster);
-            for (int q = 0; q < geo.cluster; ++q)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = others.block[which][q][state + v];
-                    if (q == at.rank) h[v] = carry[v];
-                    carry[v] = fmaf(r.x, carry[v], r.y);
-                }
-        } else {
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) h[v] = carry[v];
-        }
-        if (at.warp == 0)
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) runs.behind[turn ^ 1][state + v] = h[v];
-
-        const int mine = range.begin + at.warp * kFrames;
-        if (mine < range.end) fetch_rows(mine, range.end, turn);
-        else fetch_rows(0, 0, turn);
-        commit();
-        for (int start = range.begin; start < range.end; start += kTile, turn ^= 1) {
-            const int t0 = start + at.warp * kFrames;
-            if (start + kTile < range.end) fetch_rows(t0 + kTile, range.end, turn ^ 1);
-            commit();
-            arrived();
-            char* rows = stage + turn * kForwardStage;
-            // After each frame: the product of f, and h from 0.
-            float a[kFrames][kVec], b[kFrames][kVec];
-#pragma unroll
-            for (int i = 0; i < kFrames; ++i) {
-                float xv[kVec], gv[kVec];
-                L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
-                L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    float f, p;
-                    gates(gv[v], f, p);
-                    a[i][v] = i == 0 ? f : a[i - 1][v] * f;
-                    b[i][v] = i == 0 ? p * xv[v] : fmaf(f, b[i - 1][v], p * xv[v]);
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < kVec; ++v)
-                runs.warp[turn][at.warp][state + v] =
-                    make_float2(a[kFrames - 1][v], b[kFrames - 1][v]);
-            __syncthreads();
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) h[v] = runs.behind[turn ^ 1][state + v];
-            // The tile starts at a saved state.
-            if (saved != nullptr && at.warp == 0)
-                write_state<kVec>(saved + start / kChunk * static_cast<int64_t>(geo.channels), h,
-                                  at.channel, geo.channels);
-            for (int w = 0; w < at.warp; ++w)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = runs.warp[turn][w][state + v];
-                    h[v] = fmaf(r.x, h[v], r.y);
-                }
-            // The outputs take the place of x.
-            float hv[kVec];
-#pragma unroll
-            for (int i = 0; i < kFrames; ++i) {
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) hv[v] = fmaf(a[i][v], h[v], b[i][v]);
-                reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(hv);
-            }
-            if (at.warp == last_warp) {
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = hv[v];
-                if (geo.cluster == 1)
-#pragma unroll
-                    for (int v = 0; v < kVec; ++v) carry[v] = hv[v];
-            }
-            __syncwarp();
-            store<kUnit>(out + at.first + t0 * static_cast<int64_t>(geo.channels), rows, at.rows,
-                         range.end - t0, at.lane);
-            __syncwarp();
-        }
+    if (at.begin < at.end) fetch_tile(at.begin, 0);
+    commit();
+    V h;
+    if (geo.blocks > 1) {
+        cudaGridDependencySynchronize();
+        read_state(h, f.first + at.state, at.present);
+        h = through_blocks<false>(h, f.runs, tile, at, geo);
+    } else {
+        read_state(h, f.initial == nullptr ? nullptr : f.initial + at.state, at.present);
     }
-    if (at.rank == 0 && at.warp == last_warp)
-        write_state<kVec>(final_state + state_row, carry, at.channel, geo.channels);
-    const int index = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
-    zero_rows<kUnit>(out + at.first, at.rows, at.m, geo.length, index, by, at.lane);
-    if (saved != nullptr) {
-        const float zero[2] = {0.0f, 0.0f};
-        for (int j = (at.m + kChunk - 1) / kChunk + index; j < geo.chunks; j += by)
-            write_state<kVec>(saved + j * static_cast<int64_t>(geo.channels), zero, at.channel,
-                              geo.channels);
+    if (at.warp == 0) tile.behind[1][at.lane] = h;
+
+    int turn = 0;
+    for (int start = at.begin; start < at.end; start += kTile, turn ^= 1) {
+        if (start + kTile < at.end) fetch_tile(start + kTile, turn ^ 1);
+        commit();
+        arrived<1>();
+        char* rows = stage + turn * kForwardStage;
+        Run<V> run[kFrames];  // from the warp's first frame to each of them
+#pragma unroll
+        for (int i = 0; i < kFrames; ++i) {
+            V keep, take;
+            gates(value<T>(rows + kRows, i, at.lane), keep, take);
+            const V add = mul2(take, value<T>(rows, i, at.lane));
+            run[i].a = i == 0 ? keep : mul2(run[i - 1].a, keep);
+            run[i].b = i == 0 ? add : fma2(keep, run[i - 1].b, add);
+        }
+        tile.run[turn][at.warp][at.lane] = run[kFrames - 1];
+        __syncthreads();
+        h = tile.behind[turn ^ 1][at.lane];
+        if (f.states != nullptr && at.warp == 0)
+            write_state(f.states + at.saved(geo, start / kChunk), h, at.present);
+        for (int w = 0; w < at.warp; ++w) h = tile.run[turn][w][at.lane](h);
+        // The outputs take the place of x.
+        V after;
+#pragma unroll
+        for (int i = 0; i < kFrames; ++i) {
+            after = run[i](h);
+            put<T>(rows, i, at.lane, after);
+        }
+        h = after;
+        if (at.warp == last) tile.behind[turn][at.lane] = h;
+        __syncwarp();
+        store_rows<kUnit>(f.out, rows, at, geo, start + at.warp * kFrames, at.end);
+        __syncwarp();
+    }
+    if (at.warp == last && at.last_valid(geo)) write_state(f.final_state + at.state, h, at.present);
+    finish<kUnit>(f, at, geo);
+}
+
+// The gradients of kFrames frames whose rows are in `rows` (x, gate, dout) from h before them and
+// the carry behind them; dx takes the place of x, dgate that of gate. f and p are the caller's.
+template <typename T, typename V>
+__device__ __forceinline__ void gradients(char* rows, int lane, const V (&keep)[kFrames],
+                                          const V (&take)[kFrames], V h, V& carry) {
+    const V minus = Lane<T>::all(-1.0f);
+    V away[kFrames];  // h[t-1] - x[t]
+#pragma unroll
+    for (int i = 0; i < kFrames; ++i) {
+        const V x = value<T>(rows, i, lane);
+        away[i] = fma2(x, minus, h);
+        h = fma2(keep[i], h, mul2(take[i], x));
+    }
+#pragma unroll
+    for (int i = kFrames - 1; i >= 0; --i) {
+        const V total = add2(value<T>(rows + 2 * kRows, i, lane), carry);
+        const V gx = mul2(take[i], total);
+        carry = mul2(keep[i], total);
+        put<T>(rows, i, lane, gx);
+        put<T>(rows + kRows, i, lane, mul2(mul2(keep[i], gx), away[i]));
     }
 }
 
 template <typename T, int kUnit>
-__global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks) recurrence_backward_kernel(
-    const T* __restrict__ dout, const T* __restrict__ x, const T* __restrict__ gate,
-    const int32_t* __restrict__ lengths, const float* __restrict__ states,
-    const float* __restrict__ dfinal, T* __restrict__ dx, T* __restrict__ dgate,
-    float* __restrict__ dinitial, Geometry geo) {
+__global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks)
+    recurrence_backward_kernel(Backward<T> f, Geometry geo) {
     using L = Lane<T>;
-    using Raw = typename L::Raw;
-    constexpr int kVec = L::kVec;
+    using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
-    Runs& runs = *reinterpret_cast<Runs*>(smem + 2 * kWarps * kBackwardStage);
-    ClusterRuns& others = *reinterpret_cast<ClusterRuns*>(&runs + 1);
-
-    const Place<T> at(geo, lengths);
+    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kBackwardStage);
+    const Place<T> at(geo, f.lengths);
     char* stage = smem + at.warp * 2 * kBackwardStage;
-    const int last_warp = blockDim.x / kWarp - 1, state = at.lane * kVec;
-    const int64_t state_row = static_cast<int64_t>(at.n) * geo.channels;
-    const float* saved = states + static_cast<int64_t>(at.n) * geo.chunks * geo.channels;
+    const int last = at.warps - 1;
 
-    // Rows [t, end) to a stage: x, gate, dout; the scan for (A, B) alone needs no x.
-    auto fetch_rows = [&](int t, int end, int which, bool with_x) {
-        const int64_t here = at.first + t * static_cast<int64_t>(geo.channels);
+    auto fetch_tile = [&](int start, int which) {
+        const int t = start + at.warp * kFrames;
         char* to = stage + which * kBackwardStage;
-        if (with_x) fetch<kUnit>(to, x + here, at.rows, end - t, 0u, at.lane);
-        fetch<kUnit>(to + kFrames * kRow, gate + here, at.rows, end - t, L::kInfinity, at.lane);
-        fetch<kUnit>(to + 2 * kFrames * kRow, dout + here, at.rows, end - t, 0u, at.lane);
+        fetch_rows<kUnit>(to, f.x, at, geo, t, at.end, 0u);
+        fetch_rows<kUnit>(to + kRows, f.gate, at, geo, t, at.end, L::kInfinity);
+        fetch_rows<kUnit>(to + 2 * kRows, f.dout, at, geo, t, at.end, 0u);
     };
-    float carry[kVec];  // behind the round
-    read_state<kVec>(carry, dfinal == nullptr ? nullptr : dfinal + state_row, at.channel,
-                     geo.channels);
-    if (geo.cluster > 1) cg::this_cluster().sync();
-
-    int turn = 0, which = 0;
-    const int round = geo.cluster == 1 ? geo.length : geo.cluster * geo.tiles * kTile;
-    for (int round_start = at.m > 0 ? (at.m - 1) / round * round : -1; round_start >= 0;
-         round_start -= round, which ^= 1) {
-        const Range range(geo, at.m, at.rank, round_start);
-        float c[kVec];
-        if (geo.cluster > 1) {
-            const int part = geo.tiles * kFrames, from = range.begin + at.warp * part;
-            const int to = min(range.end, from + part);
-            float a[kVec], b[kVec];
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f;
-            const int last = from + (to - from - 1) / kFrames * kFrames;
-            if (from < to) fetch_rows(last, to, 0, false);
-            commit();
-            for (int t = from < to ? last : from - 1, s = 0; t >= from; t -= kFrames, s ^= 1) {
-                if (t > from) fetch_rows(t - kFrames, to, s ^ 1, false);
-                commit();
-                arrived();
-                const char* rows = stage + s * kBackwardStage;
-#pragma unroll
-                for (int i = kFrames - 1; i >= 0; --i) {
-                    float gv[kVec], dv[kVec];
-                    L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
-                    L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane],
-                              dv);
-#pragma unroll
-                    for (int v = 0; v < kVec; ++v) {
-                        float f, p;
-                        gates(gv[v], f, p);
-                        a[v] *= f;
-                        b[v] = f * (dv[v] + b[v]);
-                    }
-                }
-                __syncwarp();
-            }
-#pragma unroll
-            for (int v = 0; v < kVec; ++v)
-                runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
-            exchange<kVec, true>(runs, others, turn, which, at.rank, at.warp, state, geo.cluster);
-            for (int q = geo.cluster - 1; q >= 0; --q)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = others.block[which][q][state + v];
-                    if (q == at.rank) c[v] = carry[v];
-                    carry[v] = fmaf(r.x, carry[v], r.y);
-                }
-        } else {
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) c[v] = carry[v];
-        }
-        if (at.warp == 0)
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) runs.behind[turn ^ 1][state + v] = c[v];
-
-        const int tiles = (range.end - range.begin + kTile - 1) / kTile;
-        const int last = range.begin + (tiles - 1) * kTile;
-        if (tiles > 0 && last + at.warp * kFrames < range.end)
-            fetch_rows(last + at.warp * kFrames, range.end, turn, true);
-        else
-            fetch_rows(0, 0, turn, true);
-        commit();
-        for (int i = 0, start = last; i < tiles; ++i, start -= kTile, turn ^= 1) {
-            const int t0 = start + at.warp * kFrames;
-            float h[kVec];  // the saved state before the tile
-            read_state<kVec>(h, saved + start / kChunk * static_cast<int64_t>(geo.channels),
-                             at.channel, geo.channels);
-            if (i + 1 < tiles) fetch_rows(t0 - kTile, range.end, turn ^ 1, true);
-            commit();
-            arrived();
-            char* rows = stage + turn * kBackwardStage;
-            float f[kFrames][kVec], p[kFrames][kVec];
-            float a[kVec], b[kVec], back[kVec];
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) a[v] = 1.0f, b[v] = 0.0f, back[v] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kFrames; ++i) {
-                float xv[kVec], gv[kVec];
-                L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
-                L::unpack(reinterpret_cast<const Raw*>(rows + (kFrames + i) * kRow)[at.lane], gv);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    gates(gv[v], f[i][v], p[i][v]);
-                    a[v] *= f[i][v];
-                    b[v] = fmaf(f[i][v], b[v], p[i][v] * xv[v]);
-                }
-            }
-#pragma unroll
-            for (int i = kFrames - 1; i >= 0; --i) {
-                float dv[kVec];
-                L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], dv);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) back[v] = f[i][v] * (dv[v] + back[v]);
-            }
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                runs.warp[turn][at.warp][state + v] = make_float2(a[v], b[v]);
-                runs.back[turn][at.warp][state + v] = back[v];
-            }
-            __syncthreads();
-            for (int w = 0; w < at.warp; ++w)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float2 r = runs.warp[turn][w][state + v];
-                    h[v] = fmaf(r.x, h[v], r.y);
-                }
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) c[v] = runs.behind[turn ^ 1][state + v];
-            for (int w = last_warp; w > at.warp; --w)
-#pragma unroll
-                for (int v = 0; v < kVec; ++v)
-                    c[v] = fmaf(runs.warp[turn][w][state + v].x, c[v],
-                                runs.back[turn][w][state + v]);
-            float away[kFrames][kVec];  // h[t-1] - x[t]
-#pragma unroll
-            for (int i = 0; i < kFrames; ++i) {
-                float xv[kVec];
-                L::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[at.lane], xv);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    away[i][v] = h[v] - xv[v];
-                    h[v] = fmaf(f[i][v], h[v], p[i][v] * xv[v]);
-                }
-            }
-            // dx takes the place of x, dgate that of gate.
-#pragma unroll
-            for (int i = kFrames - 1; i >= 0; --i) {
-                float gx[kVec], gg[kVec];
-                L::unpack(reinterpret_cast<const Raw*>(rows + (2 * kFrames + i) * kRow)[at.lane], gx);
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) {
-                    const float total = gx[v] + c[v];
-                    gx[v] = p[i][v] * total;
-                    gg[v] = f[i][v] * gx[v] * away[i][v];
-                    c[v] = f[i][v] * total;
-                }
-                reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = L::pack(gx);
-                reinterpret_cast<Raw*>(rows + (kFrames + i) * kRow)[at.lane] = L::pack(gg);
-            }
-            if (at.warp == 0) {
-#pragma unroll
-                for (int v = 0; v < kVec; ++v) runs.behind[turn][state + v] = c[v];
-                if (geo.cluster == 1)
-#pragma unroll
-                    for (int v = 0; v < kVec; ++v) carry[v] = c[v];
-            }
-            __syncwarp();
-            const int64_t here = at.first + t0 * static_cast<int64_t>(geo.channels);
-            store<kUnit>(dx + here, rows, at.rows, range.end - t0, at.lane);
-            store<kUnit>(dgate + here, rows + kFrames * kRow, at.rows, range.end - t0, at.lane);
-            __syncwarp();
-        }
+    const int top = at.begin < at.end ? (at.end - 1) / kTile * kTile : -1;  // the last tile
+    if (top >= 0) fetch_tile(top, 0);
+    commit();
+    V carry;
+    read_state(carry, f.dfinal == nullptr ? nullptr : f.dfinal + at.state, at.present);
+    if (geo.blocks > 1) {
+        cudaGridDependencySynchronize();
+        carry = through_blocks<true>(carry, f.runs, tile, at, geo);
     }
-    if (at.rank == 0 && at.warp == 0)
-        write_state<kVec>(dinitial + state_row, carry, at.channel, geo.channels);
-    const int index = at.rank * (last_warp + 1) + at.warp, by = geo.cluster * (last_warp + 1);
-    for (T* grad : {dx, dgate})
-        zero_rows<kUnit>(grad + at.first, at.rows, at.m, geo.length, index, by, at.lane);
+    if (at.warp == 0) tile.behind[1][at.lane] = carry;
+
+    int turn = 0;
+    for (int start = top; start >= at.begin; start -= kTile, turn ^= 1) {
+        V h;
+        read_state(h, f.states + at.saved(geo, start / kChunk), at.present);
+        if (start > at.begin) fetch_tile(start - kTile, turn ^ 1);
+        commit();
+        arrived<1>();
+        char* rows = stage + turn * kBackwardStage;
+        V keep[kFrames], take[kFrames], back = L::all(0.0f);
+        Run<V> run{L::all(1.0f), L::all(0.0f)};
+#pragma unroll
+        for (int i = 0; i < kFrames; ++i) {
+            gates(value<T>(rows + kRows, i, at.lane), keep[i], take[i]);
+            run.a = mul2(run.a, keep[i]);
+            run.b = fma2(keep[i], run.b, mul2(take[i], value<T>(rows, i, at.lane)));
+            back = fma2(run.a, value<T>(rows + 2 * kRows, i, at.lane), back);
+        }
+        tile.run[turn][at.warp][at.lane] = run;
+        tile.back[turn][at.warp][at.lane] = back;
+        __syncthreads();
+        for (int w = 0; w < at.warp; ++w) h = tile.run[turn][w][at.lane](h);
+        carry = tile.behind[turn ^ 1][at.lane];
+        for (int w = last; w > at.warp; --w)
+            carry = fma2(tile.run[turn][w][at.lane].a, carry, tile.back[turn][w][at.lane]);
+        gradients<T>(rows, at.lane, keep, take, h, carry);
+        if (at.warp == 0) tile.behind[turn][at.lane] = carry;
+        __syncwarp();
+        store_rows<kUnit>(f.dx, rows, at, geo, start + at.warp * kFrames, at.end);
+        store_rows<kUnit>(f.dgate, rows + kRows, at, geo, start + at.warp * kFrames, at.end);
+        __syncwarp();
+    }
+    if (at.warp == 0 && at.block == 0) write_state(f.dinitial + at.state, carry, at.present);
+    finish<kUnit>(f, at, geo);
+}
+
+// ---- the first launch of a divided walk ----------------------------------------------------
+// Each warp streams an eighth of the block's frames, kFrames at a time through a ring of stages,
+// for their run alone: (A, B) of the state from x and gate, or (kBack) of the carry from dout
+// and gate: c[first] = A c + sum over t of (f[first] .. f[t]) dout[t].
+constexpr int kDepth = 3;
+constexpr int kRing = kDepth * 2 * kRows;
+template <typename V> constexpr int runs_smem() {
+    return kWarps * (kRing + kWarp * static_cast<int>(sizeof(Run<V>)));
+}
+
+template <typename T, int kUnit, bool kBack>
+__global__ void __launch_bounds__(kWarps* kWarp, 4)
+    recurrence_runs_kernel(const T* __restrict__ input, const T* __restrict__ gate,
+                           const int32_t* __restrict__ lengths, const float* initial, void* runs,
+                           float* first, Geometry geo) {
+    using L = Lane<T>;
+    using V = typename L::Value;
+    extern __shared__ __align__(16) char smem[];
+    cudaTriggerProgrammaticLaunchCompletion();
+    const Place<T> at(geo, lengths);
+    char* ring = smem + at.warp * kRing;
+    Run<V>* warps = reinterpret_cast<Run<V>*>(smem + kWarps * kRing);
+    const int part = geo.span / kWarps, begin = at.begin + at.warp * part;
+    const int end = min(at.end, begin + part);
+    const int steps = begin < end ? (end - begin + kFrames - 1) / kFrames : 0;
+    auto request = [&](int i) {
+        if (i < steps) {
+            char* to = ring + i % kDepth * 2 * kRows;
+            fetch_rows<kUnit>(to, input, at, geo, begin + i * kFrames, end, 0u);
+            fetch_rows<kUnit>(to + kRows, gate, at, geo, begin + i * kFrames, end, L::kInfinity);
+        }
+        commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kDepth - 1; ++i) request(i);
+    Run<V> run{L::all(1.0f), L::all(0.0f)};
+    for (int i = 0; i < steps; ++i) {
+        request(i + kDepth - 1);
+        arrived<kDepth - 1>();
+        const char* rows = ring + i % kDepth * 2 * kRows;
+#pragma unroll
+        for (int k = 0; k < kFrames; ++k) {
+            V keep, take;
+            gates(value<T>(rows + kRows, k, at.lane), keep, take);
+            const V v = value<T>(rows, k, at.lane);
+            run.a = mul2(run.a, keep);
+            run.b = kBack ? fma2(run.a, v, run.b) : fma2(keep, run.b, mul2(take, v));
+        }
+        __syncwarp();
+    }
+    warps[at.warp * kWarp + at.lane] = run;
+    __syncthreads();
+    if (at.warp == 0) {
+        run = warps[(kBack ? kWarps - 1 : 0) * kWarp + at.lane];
+        for (int w = 1; w < kWarps; ++w)
+            run.then(warps[(kBack ? kWarps - 1 - w : w) * kWarp + at.lane]);
+        static_cast<Run<V>*>(runs)[(static_cast<int64_t>(at.unit) * geo.blocks + at.block) * kWarp +
+                                   at.lane] = run;
+    }
+    // The second launch may write the final state on top of the initial one.
+    if (!kBack && at.warp == 1 && at.block == 0) {
+        V h;
+        read_state(h, initial == nullptr ? nullptr : initial + at.state, at.present);
+        write_state(first + at.state, h, at.present);
+    }
 }
 
 // ---- launch --------------------------------------------------------------------------------
 
-constexpr int64_t kClusterBlocks = 1, kRoundBytes = 32 << 20;
-
 struct Shape {
     Geometry geo;
-    int blocks, threads;
+    int64_t units;
+    int warps;
+    size_t runs_bytes, workspace;
 };
 
-Shape shape_of(int batch, int length, int channels, int chunks, int row_channels) {
+// A walk is divided below three blocks of it for every four multiprocessors: into as many as
+// `resident` blocks on each of them take. (T = 3000, C = 1024, bf16, forward: 4 utterances, 64
+// walks, 30 us divided and 51 not; 8 utterances, 128 walks, 58 and 51; backward 75 and 79.)
+Shape shape_of(int batch, int length, int channels, int chunks, int element, int resident) {
+    const int slab = kRow / element;
     Shape s{};
-    const int slabs = (channels + row_channels - 1) / row_channels;
-    const int64_t units = static_cast<int64_t>(batch) * slabs;
-    const int64_t wanted = (kClusterBlocks * sm_count() + units - 1) / units;
-    int cluster = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>(wanted, std::min(chunks, kMaxCluster))));
-    // Rounds whose rows stay in L2 from the first reading to the second.
-    const int64_t most = std::max<int64_t>(1, kRoundBytes / (units * cluster * kTile * kRow));
-    const int64_t each = (chunks + cluster - 1) / cluster, rounds = (each + most - 1) / most;
-    const int tiles = static_cast<int>((each + rounds - 1) / rounds);
-    s.geo = {length, channels, chunks, slabs, cluster, tiles};
-    s.blocks = static_cast<int>(units * cluster);
-    s.threads = std::min(kWarps, (length + kFrames - 1) / kFrames) * kWarp;
+    s.geo = {length, channels, chunks, (channels + slab - 1) / slab, 1, 0};
+    s.units = static_cast<int64_t>(batch) * s.geo.slabs;
+    int each = chunks;
+    if (4 * s.units < 3 * sm_count()) {
+        const int64_t blocks = std::min<int64_t>(chunks, resident * sm_count() / s.units);
+        each = static_cast<int>((chunks + blocks - 1) / blocks);
+        s.geo.blocks = (chunks + each - 1) / each;
+    }
+    s.geo.span = each * kTile;
+    s.warps = s.geo.blocks > 1 ? kWarps : std::min(kWarps, (length + kFrames - 1) / kFrames);
+    if (s.geo.blocks > 1) {
+        s.runs_bytes = static_cast<size_t>(s.units) * s.geo.blocks * kWarp *
+                       (element == 4 ? sizeof(Run<float>) : sizeof(Run<float2>));
+        s.workspace = s.runs_bytes + sizeof(float) * batch * channels;
+    }
     return s;
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch(SmemAttr& attribute, void (*kernel)(Params...), const Shape& s, int stage,
-                   cudaStream_t stream, Args... args) {
-    const void* entry = reinterpret_cast<const void*>(kernel);
-    cudaError_t e = attribute.ensure(entry, smem_bytes(stage, true));
+cudaError_t launch(SmemAttr& attribute, void (*kernel)(Params...), const Shape& s, int smem,
+                   bool early, cudaStream_t stream, Args... args) {
+    const cudaError_t e = attribute.ensure(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(s.blocks));
-    cfg.blockDim = dim3(static_cast<unsigned>(s.threads));
-    cfg.dynamicSmemBytes = static_cast<size_t>(smem_bytes(stage, s.geo.cluster > 1));
+    cfg.gridDim = dim3(static_cast<unsigned>(s.units * s.geo.blocks));
+    cfg.blockDim = dim3(static_cast<unsigned>(s.warps * kWarp));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
+    // The kernel waits for the launch before it itself, after its first rows are on their way.
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(s.geo.cluster);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = s.geo.cluster > 1 ? 1 : 0;
-    if (s.geo.cluster > 8) {
-        e = cudaFuncSetAttribute(entry, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-    }
+    cfg.numAttrs = early ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -676,23 +617,55 @@ int unit_of(int64_t pitch, std::initializer_list<const void*> buffers) {
     return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
 }
 
+Shape shape_of(const RecurrenceProblem& p) {
+    return shape_of(p.batch, p.length, p.channels, p.chunks, p.dtype == FGA_FLOAT ? 4 : 2,
+                    kForwardBlocks);
+}
+Shape shape_of(const RecurrenceBackwardProblem& p) {
+    return shape_of(p.batch, p.length, p.channels, p.chunks, p.dtype == FGA_FLOAT ? 4 : 2,
+                    kBackwardBlocks);
+}
+
 template <typename T, int kUnit> cudaError_t forward(const RecurrenceProblem& p, cudaStream_t s) {
-    static SmemAttr attribute;
-    const Shape shape = shape_of(p.batch, p.length, p.channels, p.chunks, kRow / sizeof(T));
-    return launch(attribute, recurrence_kernel<T, kUnit>, shape, kForwardStage, s,
-                  static_cast<const T*>(p.x), static_cast<const T*>(p.gate), p.valid_lengths,
-                  p.initial_state, static_cast<T*>(p.output), p.final_state, p.states, shape.geo);
+    using V = typename Lane<T>::Value;
+    static SmemAttr walk, runs;
+    const Shape shape = shape_of(p);
+    Forward<T> f{static_cast<const T*>(p.x), static_cast<const T*>(p.gate), p.valid_lengths,
+                 p.initial_state, static_cast<T*>(p.output), p.final_state, p.states, nullptr,
+                 nullptr};
+    const bool divided = shape.geo.blocks > 1;
+    if (divided) {
+        f.runs = p.workspace;
+        f.first = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + shape.runs_bytes);
+        const cudaError_t e =
+            launch(runs, recurrence_runs_kernel<T, kUnit, false>, shape, runs_smem<V>(), false, s,
+                   f.x, f.gate, f.lengths, f.initial, f.runs, f.first, shape.geo);
+        if (e != cudaSuccess) return e;
+    }
+    return launch(walk, recurrence_kernel<T, kUnit>, shape, tile_smem<V>(kForwardStage), divided, s,
+                  f, shape.geo);
 }
 
 template <typename T, int kUnit>
 cudaError_t backward(const RecurrenceBackwardProblem& p, cudaStream_t s) {
-    static SmemAttr attribute;
-    const Shape shape = shape_of(p.batch, p.length, p.channels, p.chunks, kRow / sizeof(T));
-    return launch(attribute, recurrence_backward_kernel<T, kUnit>, shape, kBackwardStage, s,
-                  static_cast<const T*>(p.grad_output), static_cast<const T*>(p.x),
-                  static_cast<const T*>(p.gate), p.valid_lengths, p.states, p.grad_final_state,
-                  static_cast<T*>(p.grad_x), static_cast<T*>(p.grad_gate), p.grad_initial_state,
-                  shape.geo);
+    using V = typename Lane<T>::Value;
+    static SmemAttr walk, runs;
+    const Shape shape = shape_of(p);
+    const bool divided = shape.geo.blocks > 1;
+    const Backward<T> f{static_cast<const T*>(p.grad_output), static_cast<const T*>(p.x),
+                        static_cast<const T*>(p.gate), p.valid_lengths, p.states,
+                        p.grad_final_state, static_cast<T*>(p.grad_x),
+                        static_cast<T*>(p.grad_gate), p.grad_initial_state,
+                        divided ? p.workspace : nullptr};
+    if (divided) {
+        const cudaError_t e =
+            launch(runs, recurrence_runs_kernel<T, kUnit, true>, shape, runs_smem<V>(), false, s,
+                   f.dout, f.gate, f.lengths, static_cast<const float*>(nullptr), f.runs,
+                   static_cast<float*>(nullptr), shape.geo);
+        if (e != cudaSuccess) return e;
+    }
+    return launch(walk, recurrence_backward_kernel<T, kUnit>, shape, tile_smem<V>(kBackwardStage),
+                  divided, s, f, shape.geo);
 }
 
 template <typename T> cudaError_t forward(const RecurrenceProblem& p, cudaStream_t s) {
@@ -713,6 +686,11 @@ template <typename T> cudaError_t backward(const RecurrenceBackwardProblem& p, c
 }
 
 }  // namespace
+
+size_t recurrence_workspace(const RecurrenceProblem& p) { return shape_of(p).workspace; }
+size_t recurrence_backward_workspace(const RecurrenceBackwardProblem& p) {
+    return shape_of(p).workspace;
+}
 
 cudaError_t launch_recurrence(const RecurrenceProblem& p, cudaStream_t s, const char** variant) {
     *variant = "recurrence";

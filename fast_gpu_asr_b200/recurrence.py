@@ -15,8 +15,9 @@ The operators record no autograd graph: a call on tensors that require grad is r
 grad mode is on. The two functions are the halves of a ``torch.autograd.Function``.
 
 Tensors must be contiguous and live on the current CUDA device. Work is enqueued on
-``stream`` (default: torch's current stream), outputs are allocated on it, and nothing is
-synchronised.
+``stream`` (default: torch's current stream), outputs and workspace are allocated on it, and
+nothing is synchronised. A ``workspace`` passed in must not serve two calls in flight; a few
+long rows need one (``gated_linear_recurrence_workspace_size``), many or short rows none.
 """
 
 from __future__ import annotations
@@ -24,7 +25,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._call import Operator, require
+from ._call import Operator, descs, require
 
 _FORWARD = Operator("gated_linear_recurrence",
                     ("x", "gate", "valid_lengths", "initial_state"),
@@ -49,10 +50,28 @@ def gated_linear_recurrence_backward_check(input_descs, output_descs) -> int:
         len(output_descs))
 
 
+def gated_linear_recurrence_workspace_size(x: torch.Tensor, valid_lengths: torch.Tensor) -> int:
+    """Bytes of device memory that a forward call on ``x`` takes as ``workspace``."""
+    state = (torch.float32, (x.shape[0], x.shape[2]))
+    ins = descs([(x.dtype, x.shape)] * 2 + [(valid_lengths.dtype, valid_lengths.shape), state])
+    return _lib.library().fga_gated_linear_recurrence_workspace_size(ins, 4)
+
+
+def gated_linear_recurrence_backward_workspace_size(x: torch.Tensor,
+                                                    valid_lengths: torch.Tensor) -> int:
+    """Bytes of device memory that a backward call on ``x`` takes as ``workspace``."""
+    n, t, c = x.shape
+    ins = descs([(x.dtype, x.shape)] * 3 + [(valid_lengths.dtype, valid_lengths.shape),
+                                            (torch.float32, (n, -(-t // STATE_FRAMES), c)),
+                                            (torch.float32, (n, c))])
+    return _lib.library().fga_gated_linear_recurrence_backward_workspace_size(ins, 6)
+
+
 def gated_linear_recurrence(x: torch.Tensor, gate: torch.Tensor, valid_lengths: torch.Tensor,
                             initial_state: torch.Tensor | None = None, *,
                             return_states: bool = False, out: torch.Tensor | None = None,
-                            final_state: torch.Tensor | None = None, stream=None):
+                            final_state: torch.Tensor | None = None, stream=None,
+                            workspace: torch.Tensor | None = None):
     """``(out, final_state)``, or ``(out, final_state, states)`` with ``return_states``.
 
     ``gate`` holds logits; ``initial_state`` is float32 ``[N, C]`` (default zeros).
@@ -71,7 +90,7 @@ def gated_linear_recurrence(x: torch.Tensor, gate: torch.Tensor, valid_lengths: 
 
     outputs = _FORWARD((x, gate, valid_lengths, initial_state), (out, final_state), allocate,
                        lambda name: (torch.float32, saved if name == "states" else (n, c)),
-                       stream=stream)
+                       workspace=workspace, stream=stream)
     return outputs if return_states else outputs[:2]
 
 
@@ -79,7 +98,7 @@ def gated_linear_recurrence_backward(grad_out: torch.Tensor, x: torch.Tensor,
                                      gate: torch.Tensor, valid_lengths: torch.Tensor,
                                      states: torch.Tensor,
                                      grad_final_state: torch.Tensor | None = None, *,
-                                     stream=None):
+                                     stream=None, workspace: torch.Tensor | None = None):
     """``(grad_x, grad_gate, grad_initial_state)`` from the forward call's inputs and its
     ``states``. ``grad_final_state`` is float32 ``[N, C]`` (default zeros), and so is
     ``grad_initial_state``."""
@@ -88,4 +107,4 @@ def gated_linear_recurrence_backward(grad_out: torch.Tensor, x: torch.Tensor,
     return _BACKWARD((grad_out, x, gate, valid_lengths, states, grad_final_state), (),
                      lambda: (torch.empty_like(x), torch.empty_like(x),
                               x.new_empty((n, c), dtype=torch.float32)),
-                     lambda name: (torch.float32, (n, c)), stream=stream)
+                     lambda name: (torch.float32, (n, c)), workspace=workspace, stream=stream)

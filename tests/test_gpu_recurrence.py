@@ -65,7 +65,7 @@ def test_channels(c, dtype):
 
 @pytest.mark.parametrize("dtype", cases.DTYPES)
 @pytest.mark.parametrize("n,t,c", [(2, 375, 1024), (1, 1500, 33), (2, 3000, 64), (1, 5000, 16),
-                                   (40, 200, 256), (1, 12000, 66)])
+                                   (40, 200, 256), (1, 12000, 66), (1, 13000, 8)])
 def test_every_split(n, t, c, dtype):
     check(n, t, c, dtype, lengths=[t] if n == 1 else None)
 
