@@ -71,11 +71,5 @@ __device__ __forceinline__ float reciprocal_approx(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// 1 / (1 + exp(-v))
-__device__ __forceinline__ float2 sigmoid2(float2 v) {
-    const float2 t = mul2(v, splat2(-1.4426950408889634f));
-    const float2 d = add2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), splat2(1.0f));
-    return make_float2(reciprocal_approx(d.x), reciprocal_approx(d.y));
-}
 
 }  // namespace fga

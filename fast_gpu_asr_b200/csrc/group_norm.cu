@@ -105,30 +105,35 @@ __device__ __forceinline__ void block_moments(const uint4& first, Each each, flo
     }
 }
 
-// A column's parameters: out = act(x scale + shift), scale = rstd weight, shift = bias - mean
-// scale. Next to (x - mean) scale + bias this costs two roundings of mean * scale, what the
-// rounding of the mean to fp32 costs in either form, and saves an instruction an element.
-template <typename T> struct Column {
-    float2 scale[kPairs<T>], shift[kPairs<T>];
+// A column's parameters: z = (x - mean) scale + shift, scale = rstd weight, shift = bias (scale
+// and shift in the activation's units). The mean is taken off first, not as part of shift: that
+// would round mean * scale, which is hundreds in a group of small variance, and saves an
+// instruction of about 16 a pair.
+template <typename T, bool kWhole> struct Column {
+    static constexpr int kMeans = kWhole ? 1 : kPairs<T>;
+    float2 scale[kPairs<T>], shift[kPairs<T>], minus[kMeans];  // minus the mean
     // `stats`: (mean, rstd) of the slab's groups.
-    template <bool kAligned, bool kWhole>
+    template <bool kAligned>
     __device__ __forceinline__ void read(const T* w, const T* b, const float2* stats,
-                                         const Place<T>& p, const Geometry& g) {
+                                         const Place<T>& p, const Geometry& g, int act) {
+        const float2 unit = splat2(unit_of(act)), origin = splat2(-origin_of(act));
         unpack<T>(load<T, kAligned>(w + p.channel(), p.count), scale);
         unpack<T>(load<T, kAligned>(b + p.channel(), p.count), shift);
 #pragma unroll
         for (int i = 0; i < kPairs<T>; ++i) {
             const float2 s = stats[p.group_of(kWhole ? 0 : 2 * i, g)];
             const float2 t = kWhole ? s : stats[p.group_of(2 * i + 1, g)];
-            scale[i] = mul2(scale[i], make_float2(s.y, t.y));
-            shift[i] = fma2(make_float2(-s.x, -t.x), scale[i], shift[i]);
+            scale[i] = mul2(mul2(scale[i], unit), make_float2(s.y, t.y));
+            shift[i] = mul2(add2(shift[i], origin), unit);
+            minus[kWhole ? 0 : i] = make_float2(-s.x, -t.x);
         }
     }
     __device__ __forceinline__ uint4 apply(const uint4& r, int act) const {
         float2 v[kPairs<T>];
         unpack<T>(r, v);
 #pragma unroll
-        for (int i = 0; i < kPairs<T>; ++i) v[i] = fma2(v[i], scale[i], shift[i]);
+        for (int i = 0; i < kPairs<T>; ++i)
+            v[i] = fma2(add2(v[i], minus[kWhole ? 0 : i]), scale[i], shift[i]);
         activate(v, act);
         return pack<T>(v);
     }
@@ -202,8 +207,8 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     __syncthreads();
     if (mine > 0) {
-        Column<T> column;
-        column.template read<kAligned, kWhole>(t.weight, t.bias, moments, p, g);
+        Column<T, kWhole> column;
+        column.template read<kAligned>(t.weight, t.bias, moments, p, g, act);
         T* to = t.out + p.at(g, p.begin + p.row);
 #pragma unroll 2
         for (int i = 0; i < mine; ++i, to += stride)
@@ -276,8 +281,8 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     __syncthreads();
     if (mine > 0) {
-        Column<T> column;
-        column.template read<kAligned, kWhole>(t.weight, t.bias, stats, p, g);
+        Column<T, kWhole> column;
+        column.template read<kAligned>(t.weight, t.bias, stats, p, g, act);
         T* to = t.out + from;
         rows.each([&](const uint4(&v)[1]) {
             store<T, kAligned>(to, column.apply(v[0], act), p.count);

@@ -98,34 +98,57 @@ __device__ __forceinline__ void arrived() {
 }
 
 // ---- activations ---------------------------------------------------------------------------
-template <int kCount> __device__ __forceinline__ void activate(float2 (&z)[kCount], int act) {
+// The exponentials are base 2, so what the columns' parameters give for x is already in units of
+// their exponent: y = unit (z - origin), which saves a multiplication, and for
+// Swoosh-R an addition, of every value.
+constexpr float kLn2 = 0.69314718f;
+__device__ __forceinline__ float unit_of(int act) {
+    return act == FGA_ACTIVATION_SILU ? -kLog2e : act == FGA_ACTIVATION_SWOOSH_R ? kLog2e : 1.0f;
+}
+__device__ __forceinline__ float origin_of(int act) {
+    return act == FGA_ACTIVATION_SWOOSH_R ? 1.0f : 0.0f;
+}
+__device__ __forceinline__ float2 exp2_of(float2 y) {
+    return make_float2(exp2_approx(y.x), exp2_approx(y.y));
+}
+__device__ __forceinline__ float2 reciprocal_of(float2 y) {
+    return make_float2(reciprocal_approx(y.x), reciprocal_approx(y.y));
+}
+
+// y to act(z).
+template <int kCount> __device__ __forceinline__ void activate(float2 (&y)[kCount], int act) {
     if (act == FGA_ACTIVATION_SILU) {
+        // z / (1 + exp(-z)) = y / (unit (1 + 2^y))
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) z[i] = mul2(z[i], sigmoid2(z[i]));
+        for (int i = 0; i < kCount; ++i)
+            y[i] = mul2(y[i], reciprocal_of(fma2(exp2_of(y[i]), splat2(-kLog2e), splat2(-kLog2e))));
     } else if (act == FGA_ACTIVATION_SWOOSH_R) {
+        // softplus(v) = ln 2 (max(y, 0) + log2(1 + 2^-|y|)) with v = z - 1; the logarithm's
+        // argument is in [1, 2], where an absolute error of 2^-22 is as good as log1p next to
+        // the sum. -0.08 z - 0.313261687 = -0.08 v - 0.393261687.
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
-            // softplus(v) = max(v, 0) + log(1 + exp(-|v|)); the logarithm's argument is in
-            // [1, 2], where a log2 of absolute error 2^-22 is as good as log1p next to the sum.
-            const float2 v = add2(z[i], splat2(-1.0f));
-            const float2 e = make_float2(exp2_approx(fabsf(v.x) * -kLog2e),
-                                         exp2_approx(fabsf(v.y) * -kLog2e));
-            const float2 d = add2(e, splat2(1.0f));
+            const float2 d = add2(make_float2(exp2_approx(-fabsf(y[i].x)), exp2_approx(-fabsf(y[i].y))),
+                                  splat2(1.0f));
             const float2 l = make_float2(log2_approx(d.x), log2_approx(d.y));
-            const float2 rest = fma2(z[i], splat2(-0.08f), splat2(-0.313261687f));
-            z[i] = add2(fma2(l, splat2(0.69314718f), make_float2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f))),
-                        rest);
+            const float2 soft = add2(l, make_float2(fmaxf(y[i].x, 0.0f), fmaxf(y[i].y, 0.0f)));
+            y[i] = fma2(soft, splat2(kLn2),
+                        fma2(y[i], splat2(-0.08f * kLn2), splat2(-0.393261687f)));
         }
     }
 }
 
-// act'(z)
-template <int kAct> __device__ __forceinline__ float2 slope(float2 z) {
+// y to act'(z) / unit.
+template <int kAct> __device__ __forceinline__ float2 slope(float2 y) {
     if constexpr (kAct == FGA_ACTIVATION_SILU) {
-        const float2 s = sigmoid2(z);
-        return mul2(s, fma2(z, fma2(s, splat2(-1.0f), splat2(1.0f)), splat2(1.0f)));
+        // s (1 + z (1 - s)) with z = -ln2 y, all times -ln2.
+        const float2 s = reciprocal_of(add2(exp2_of(y), splat2(1.0f)));
+        const float2 rest = fma2(s, splat2(-kLn2 * kLn2), splat2(kLn2 * kLn2));
+        return mul2(s, fma2(y, rest, splat2(-kLn2)));
     } else {
-        return add2(sigmoid2(add2(z, splat2(-1.0f))), splat2(-0.08f));
+        // sigmoid(v) - 0.08 = 0.92 - 1 / (1 + 2^y), times ln2.
+        const float2 s = reciprocal_of(add2(exp2_of(y), splat2(1.0f)));
+        return fma2(s, splat2(-kLn2), splat2(0.92f * kLn2));
     }
 }
 

@@ -41,12 +41,16 @@ template <typename T> struct Tensors {
     T* dx;
 };
 
-// A column's parameters: z = x scale + shift, xhat = x rstd + centre.
+// A column's parameters: d = x - mean, z = d scale + shift (both in the activation's units), xhat
+// = d rstd. What `through` makes of dout is dz / unit: the sums make up for it at their end, dx
+// in its product with scale.
 template <typename T, bool kWhole> struct Column {
     static constexpr int kStats = kWhole ? 1 : kPairs<T>;
-    float2 scale[kPairs<T>], shift[kPairs<T>], rstd[kStats], centre[kStats];
+    float2 scale[kPairs<T>], shift[kPairs<T>], rstd[kStats], minus[kStats];  // minus the mean
     template <bool kAligned>
-    __device__ __forceinline__ void read(const Tensors<T>& t, const Place<T>& p, const Geometry& g) {
+    __device__ __forceinline__ void read(const Tensors<T>& t, const Place<T>& p, const Geometry& g,
+                                         int act) {
+        const float2 unit = splat2(unit_of(act)), origin = splat2(-origin_of(act));
         unpack<T>(load<T, kAligned>(t.weight + p.channel(), p.count), scale);
         unpack<T>(load<T, kAligned>(t.bias + p.channel(), p.count), shift);
         const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group;
@@ -55,18 +59,20 @@ template <typename T, bool kWhole> struct Column {
             const int64_t i = group + p.group_of(2 * k, g);
             const int64_t j = kWhole ? i : group + p.group_of(2 * k + 1, g);
             rstd[k] = make_float2(t.rstd[i], t.rstd[j]);
-            centre[k] = mul2(make_float2(-t.mean[i], -t.mean[j]), rstd[k]);
+            minus[k] = make_float2(-t.mean[i], -t.mean[j]);
         }
 #pragma unroll
         for (int e = 0; e < kPairs<T>; ++e) {
-            shift[e] = fma2(centre[kWhole ? 0 : e], scale[e], shift[e]);
-            scale[e] = mul2(scale[e], rstd[kWhole ? 0 : e]);
+            shift[e] = mul2(add2(shift[e], origin), unit);
+            scale[e] = mul2(mul2(scale[e], unit), rstd[kWhole ? 0 : e]);
         }
     }
-    __device__ __forceinline__ float2 normalised(float2 x, int e) const {
-        return fma2(x, rstd[kWhole ? 0 : e], centre[kWhole ? 0 : e]);
+    // x to x - mean.
+    __device__ __forceinline__ void centre(float2 (&x)[kPairs<T>]) const {
+#pragma unroll
+        for (int e = 0; e < kPairs<T>; ++e) x[e] = add2(x[e], minus[kWhole ? 0 : e]);
     }
-    // dout to dz.
+    // dout to dz / unit; x is centred.
     __device__ __forceinline__ void through(float2 (&d)[kPairs<T>], const float2 (&x)[kPairs<T>],
                                             int act) const {
         if (act == FGA_ACTIVATION_SILU) {
@@ -79,10 +85,24 @@ template <typename T, bool kWhole> struct Column {
                 d[e] = mul2(d[e], slope<FGA_ACTIVATION_SWOOSH_R>(fma2(x[e], scale[e], shift[e])));
         }
     }
+    // The sums of dz and dz xhat, both without their factors unit and (the second) rstd.
+    __device__ __forceinline__ void add(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>],
+                                        const float2 (&d)[kPairs<T>],
+                                        const float2 (&x)[kPairs<T>]) const {
+#pragma unroll
+        for (int e = 0; e < kPairs<T>; ++e) {
+            db[e] = add2(db[e], d[e]);
+            dw[e] = fma2(d[e], x[e], dw[e]);
+        }
+    }
+    __device__ __forceinline__ void finish(float2 (&dw)[kPairs<T>]) const {
+#pragma unroll
+        for (int e = 0; e < kPairs<T>; ++e) dw[e] = mul2(dw[e], rstd[kWhole ? 0 : e]);
+    }
 };
 
-// dx = dz scale + x slope + offset, with the group's means m1 = s1 / (M Cg), m2 = s2 / (M Cg):
-// slope = -rstd^2 m2, offset = -rstd (centre m2 + m1).
+// dx = dz rstd weight + (x - mean) slope + offset, with the group's means m1 = s1 / (M Cg), m2 =
+// s2 / (M Cg): slope = -rstd^2 m2, offset = -rstd m1.
 template <typename T, bool kWhole> struct Final {
     static constexpr int kStats = kWhole ? 1 : kPairs<T>;
     float2 slope[kStats], offset[kStats];
@@ -92,10 +112,9 @@ template <typename T, bool kWhole> struct Final {
         for (int k = 0; k < kStats; ++k) {
             const float2 a = sums[p.group_of(2 * k, g)];
             const float2 b = kWhole ? a : sums[p.group_of(2 * k + 1, g)];
-            const float2 m1 = make_float2(a.x * -inv, b.x * -inv);  // negative
-            const float2 m2 = make_float2(a.y * -inv, b.y * -inv);
-            slope[k] = mul2(mul2(column.rstd[k], column.rstd[k]), m2);
-            offset[k] = mul2(column.rstd[k], fma2(column.centre[k], m2, m1));
+            const float2 r = mul2(column.rstd[k], splat2(-inv));
+            offset[k] = mul2(r, make_float2(a.x, b.x));
+            slope[k] = mul2(mul2(r, column.rstd[k]), make_float2(a.y, b.y));
         }
     }
     __device__ __forceinline__ float2 operator()(float2 dz, float2 x, float2 scale, int e) const {
@@ -103,13 +122,13 @@ template <typename T, bool kWhole> struct Final {
     }
 };
 
-// Adds the threads' column sums: (dbias, dweight) of the block's rows to `sums`, and of each
-// group (s1, s2), weighted, to group_sums.
+// Adds the threads' column sums, times `unit`: (dbias, dweight) of the block's rows to `sums`,
+// and of each group (s1, s2), weighted, to group_sums.
 template <typename T>
 __device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>], float2* part,
                                        float2* group_sums, float2* __restrict__ sums,
-                                       const T* __restrict__ weight, const Place<T>& p,
-                                       const Geometry& g) {
+                                       const T* __restrict__ weight, float unit,
+                                       const Place<T>& p, const Geometry& g) {
     const int columns = g.lanes * kVec<T>;
     int rows = g.step;
     // Asked for before the barrier that its use comes after.
@@ -144,6 +163,7 @@ __device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPa
         const float2* column = part + c % kVec<T> * g.lanes + c / kVec<T>;
         float2 s = column[0];
         for (int r = 1; r < rows; ++r) s = add2(s, column[r * columns]);
+        s = mul2(s, splat2(unit));
         sums[p.first_channel + c] = s;
         if (c >= kThreads) w = to_f32<T>(weight[p.first_channel + c]);
         s = mul2(s, splat2(w));
@@ -237,28 +257,26 @@ __global__ void __launch_bounds__(kThreads, 3)
     float2 db[kPairs<T>], dw[kPairs<T>];
 #pragma unroll
     for (int e = 0; e < kPairs<T>; ++e) db[e] = dw[e] = splat2(0.0f);
-    if (mine > 0) column.template read<kAligned>(t, p, g);
+    if (mine > 0) column.template read<kAligned>(t, p, g, act);
     arrived();
 #pragma unroll 2
     for (int i = 0; i < mine; ++i) {
         float2 x[kPairs<T>], d[kPairs<T>];
         unpack<T>(xs[at + i * pitch], x);
         unpack<T>(ds[at + i * pitch], d);
+        column.centre(x);
         column.through(d, x, act);
-#pragma unroll
-        for (int e = 0; e < kPairs<T>; ++e) {
-            db[e] = add2(db[e], d[e]);
-            dw[e] = fma2(d[e], column.normalised(x[e], e), dw[e]);
-        }
+        column.add(db, dw, d, x);
 #pragma unroll
         for (int q = 0; q < kPlanes<T>; ++q)
             ds[q * vectors + at + i * pitch] =
                 make_uint4(__float_as_uint(d[2 * q].x), __float_as_uint(d[2 * q].y),
                            __float_as_uint(d[2 * q + 1].x), __float_as_uint(d[2 * q + 1].y));
     }
+    if (mine > 0) column.finish(dw);
     add_up<T>(db, dw, part, means,
                         sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
-                        t.weight, p, g);
+                        t.weight, unit_of(act), p, g);
     if (g.blocks > 1) {
         float2* gathered = part;  // [block][group]
         auto cluster = cg::this_cluster();
@@ -287,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 3)
         for (int i = 0; i < mine; ++i, to += stride) {
             float2 x[kPairs<T>], v[kPairs<T>];
             unpack<T>(xs[at + i * pitch], x);
+            column.centre(x);
 #pragma unroll
             for (int q = 0; q < kPlanes<T>; ++q) {
                 float2 d[2];
@@ -325,23 +344,21 @@ __global__ void __launch_bounds__(kThreads, 3)
     for (int e = 0; e < kPairs<T>; ++e) db[e] = dw[e] = splat2(0.0f);
     if (mine > 0) {
         Column<T, kWhole> column;
-        column.template read<kAligned>(t, p, g);
+        column.template read<kAligned>(t, p, g, act);
         rows.each([&](const uint4(&v)[2]) {
             float2 x[kPairs<T>], d[kPairs<T>];
             unpack<T>(v[0], x);
             unpack<T>(v[1], d);
+            column.centre(x);
             column.through(d, x, act);
-#pragma unroll
-            for (int e = 0; e < kPairs<T>; ++e) {
-                db[e] = add2(db[e], d[e]);
-                dw[e] = fma2(d[e], column.normalised(x[e], e), dw[e]);
-            }
+            column.add(db, dw, d, x);
         });
+        column.finish(dw);
     }
     __syncthreads();  // the slots become the threads' sums
     add_up<T>(db, dw, reinterpret_cast<float2*>(shared), group_sums,
                         sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
-                        t.weight, p, g);
+                        t.weight, unit_of(act), p, g);
     if (threadIdx.x < p.groups)
         partial[(static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x) * g.parts *
                     g.blocks +
@@ -387,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     if (mine > 0) {
         const float inv = 1.0f / (static_cast<float>(p.m) * static_cast<float>(g.group_channels));
         Column<T, kWhole> column;
-        column.template read<kAligned>(t, p, g);
+        column.template read<kAligned>(t, p, g, act);
         Final<T, kWhole> final_;
         final_.make(column, means, inv, p, g);
         T* to = t.dx + from;
@@ -395,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, 3)
             float2 x[kPairs<T>], d[kPairs<T>];
             unpack<T>(v[0], x);
             unpack<T>(v[1], d);
+            column.centre(x);
             column.through(d, x, act);
 #pragma unroll
             for (int e = 0; e < kPairs<T>; ++e) d[e] = final_(d[e], x[e], column.scale[e], e);
@@ -418,7 +436,7 @@ Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
     const Problem q{p.batch, p.length, p.channels, p.groups, element, aligned};
     const Shape s = resident_shape(q, element == 4 ? kVectorBytes<float> : kVectorBytes<__half>,
                                    kTileBytes);
-    return s.geo.blocks > 0 && s.geo.blocks <= kMaxCluster ? s : stream_shape(q);
+    return s.geo.blocks > 0 && s.geo.blocks <= 1 ? s : stream_shape(q);
 }
 
 int64_t sum_rows(const Shape& s, int batch) { return static_cast<int64_t>(batch) * s.geo.blocks; }
