@@ -92,12 +92,13 @@ __device__ __forceinline__ void block_moments(const uint4& first, Each each, flo
     }
     __syncthreads();
     // A warp per group: its columns of every row of threads.
-    const int width = kWhole ? p.channels / p.groups / kVec<T> : p.channels / p.groups;
+    const int width = kWhole ? p.width / kVec<T> : p.width;
+    const Items first_item(width, g);
     const int used = min(g.step, p.rows);
-    const float total = static_cast<float>(p.rows) * static_cast<float>(p.channels / p.groups);
+    const float total = static_cast<float>(p.rows) * static_cast<float>(p.width);
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
         const float2 r = merge(total, [&](auto add) {
-            for (Items i(width); i.row < used; i.next())
+            for (Items i = first_item; i.row < used; i.next())
                 add(static_cast<float>(p.rows_of(i.row) * (kWhole ? kVec<T> : 1)),
                     part[i.row * columns + j * width + i.column]);
         });

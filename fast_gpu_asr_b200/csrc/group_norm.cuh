@@ -178,7 +178,8 @@ struct Geometry {
     int blocks;       // that divide the valid rows of an utterance's slab evenly
     int rows;         // most rows of a block
     int lanes, step;  // threads of a row, rows of a block's threads
-    Divisor by_blocks, by_slabs, by_lanes, by_step, by_group;
+    int item_width, item_rows;  // of Items: a group's columns, and rows of 32 of them
+    Divisor by_blocks, by_slabs, by_lanes, by_step, by_group, by_item;
 };
 
 template <typename T> struct Place {
@@ -187,6 +188,7 @@ template <typename T> struct Place {
     int first_channel, channels;  // of the slab
     int lane, row;                // of this thread
     int count;                    // valid channels of this thread's vector; below 1: no work
+    int width;                    // channels of a group in the slab
     int begin, rows, each;        // rows of the block; of a block of this utterance
     int passes, extra;            // rows of a thread: passes, and one more in the first `extra`
 
@@ -203,12 +205,13 @@ template <typename T> struct Place {
             p.groups = 1;
             const int at = p.slab % g.parts * g.part_channels;
             p.first_channel = p.first_group * g.group_channels + at;
-            p.channels = min(g.part_channels, g.group_channels - at);
+            p.channels = p.width = min(g.part_channels, g.group_channels - at);
         } else {
             p.first_group = p.slab * g.slab_groups;
             p.groups = min(g.slab_groups, g.groups - p.first_group);
             p.first_channel = p.first_group * g.group_channels;
-            p.channels = p.groups * g.group_channels;
+            p.width = g.group_channels;
+            p.channels = p.groups * p.width;
         }
         p.row = g.by_lanes.quotient(threadIdx.x);
         p.lane = threadIdx.x - p.row * g.lanes;
@@ -241,11 +244,12 @@ template <typename T> struct Place {
 // takes 32 at a time, row by row.
 struct Items {
     int row, column, rows_by, columns_by, width;
-    __device__ __forceinline__ Items(int width_) : width(width_) {
+    __device__ __forceinline__ Items(int width_, const Geometry& g) : width(width_) {
         const int lane = threadIdx.x % kWarp;
-        row = lane / width;
+        // (A last part is narrower than the others.)
+        row = width == g.item_width ? g.by_item.quotient(lane) : lane / width;
+        rows_by = width == g.item_width ? g.item_rows : kWarp / width;
         column = lane - row * width;
-        rows_by = kWarp / width;
         columns_by = kWarp - rows_by * width;
     }
     __device__ __forceinline__ void next() {
@@ -371,6 +375,7 @@ inline Shape slabs_of(const Problem& p, int64_t slab_bytes) {
     }
     s.whole = s.aligned && width % vec == 0;
     s.units = static_cast<int64_t>(p.batch) * g.slabs;
+    g.item_width = std::min(width, g.part_channels) / (s.whole ? vec : 1);
     g.lanes = (std::min(width * g.slab_groups, g.part_channels) + vec - 1) / vec;
     g.step = kThreads / g.lanes;
     return s;
@@ -385,6 +390,8 @@ inline void set_blocks(Shape& s, int64_t blocks) {
     g.by_lanes = Divisor(g.lanes);
     g.by_step = Divisor(g.step);
     g.by_group = Divisor(g.group_channels);
+    g.by_item = Divisor(g.item_width);
+    g.item_rows = kWarp / g.item_width;
 }
 
 // One launch that keeps its rows on chip, with bytes_per_vector of shared memory for a vector

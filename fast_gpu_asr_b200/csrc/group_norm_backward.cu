@@ -26,7 +26,7 @@ constexpr int kGatherBytes = kMaxCluster * kMaxSlabGroups * static_cast<int>(siz
 // dz as fp32 planes of 16 bytes of each vector, the first of which held dout.
 template <typename T> constexpr int kPlanes = kVec<T> / 4;
 template <typename T> constexpr int kVectorBytes = 16 + 16 * kPlanes<T>;
-// What the threads add up for each of their channels, in shared memory, and the columns' sums.
+// The most that add_up takes.
 template <typename T>
 constexpr int kSumBytes = 2 * kThreads * kVec<T> * static_cast<int>(sizeof(float2));
 
@@ -85,7 +85,7 @@ template <typename T, bool kWhole> struct Column {
                 d[e] = mul2(d[e], slope<FGA_ACTIVATION_SWOOSH_R>(fma2(x[e], scale[e], shift[e])));
         }
     }
-    // The sums of dz and dz xhat, both without their factors unit and (the second) rstd.
+    // The sums of dz and dz xhat, without their factors: unit, and (the second) rstd.
     __device__ __forceinline__ void add(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>],
                                         const float2 (&d)[kPairs<T>],
                                         const float2 (&x)[kPairs<T>]) const {
@@ -95,9 +95,27 @@ template <typename T, bool kWhole> struct Column {
             dw[e] = fma2(d[e], x[e], dw[e]);
         }
     }
-    __device__ __forceinline__ void finish(float2 (&dw)[kPairs<T>]) const {
+    // This vector's part of (s1, s2), from those sums: scale is weight unit rstd.
+    __device__ __forceinline__ float2 weigh(const float2 (&db)[kPairs<T>],
+                                            const float2 (&dw)[kPairs<T>]) const {
+        float2 s1 = mul2(scale[0], db[0]), s2 = mul2(scale[0], dw[0]);
 #pragma unroll
-        for (int e = 0; e < kPairs<T>; ++e) dw[e] = mul2(dw[e], rstd[kWhole ? 0 : e]);
+        for (int e = 1; e < kPairs<T>; ++e) {
+            s1 = fma2(scale[e], db[e], s1);
+            s2 = fma2(scale[e], dw[e], s2);
+        }
+        // (rstd is 0 where the variance overflowed: then dx is 0 whatever s1 is.)
+        return make_float2(rstd[0].x > 0.0f ? (s1.x + s1.y) * reciprocal_approx(rstd[0].x) : 0.0f, s2.x + s2.y);
+    }
+    // The sums with their factors.
+    __device__ __forceinline__ void finish(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>],
+                                           int act) const {
+        const float2 unit = splat2(unit_of(act));
+#pragma unroll
+        for (int e = 0; e < kPairs<T>; ++e) {
+            db[e] = mul2(db[e], unit);
+            dw[e] = mul2(dw[e], mul2(unit, rstd[kWhole ? 0 : e]));
+        }
     }
 };
 
@@ -122,20 +140,27 @@ template <typename T, bool kWhole> struct Final {
     }
 };
 
-// Adds the threads' column sums, times `unit`: (dbias, dweight) of the block's rows to `sums`,
-// and of each group (s1, s2), weighted, to group_sums.
+// The weight of the channel whose column this thread adds up, asked for early (not kWhole).
 template <typename T>
-__device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>], float2* part,
-                                       float2* group_sums, float2* __restrict__ sums,
-                                       const T* __restrict__ weight, float unit,
+__device__ __forceinline__ float own_weight(const T* weight, const Place<T>& p, const Geometry& g) {
+    const int e = g.by_lanes.quotient(threadIdx.x), c = (threadIdx.x - e * g.lanes) * kVec<T> + e;
+    return e < kVec<T> && c < p.channels ? to_f32<T>(weight[p.first_channel + c]) : 0.0f;
+}
+
+// What the threads of a block add up at their end, in shared memory: (dbias, dweight) of each
+// column, [row][vector's channel][lane] so that neither side of the barrier meets a bank twice,
+// and behind them for the groups' (s1, s2) what each vector contributes, [row][lane] (if not
+// kWhole, the columns' weighted sums).
+template <typename T, bool kWhole>
+__device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPairs<T>],
+                                       float2 weighed, float w, float2* part, float2* group_sums,
+                                       float2* __restrict__ sums, const T* __restrict__ weight,
                                        const Place<T>& p, const Geometry& g) {
     const int columns = g.lanes * kVec<T>;
-    int rows = g.step;
-    // Asked for before the barrier that its use comes after.
-    float w = threadIdx.x < p.channels ? to_f32<T>(weight[p.first_channel + threadIdx.x]) : 0.0f;
+    int rows = g.step, row = p.row;
     if (kWarp % g.lanes == 0) {
         // Whole rows of threads in a warp: the warp's own sum first.
-        for (int o = g.lanes; o < kWarp; o *= 2)
+        for (int o = g.lanes; o < kWarp; o *= 2) {
 #pragma unroll
             for (int e = 0; e < kPairs<T>; ++e) {
                 db[e] = add2(db[e], make_float2(__shfl_xor_sync(0xffffffffu, db[e].x, o),
@@ -143,84 +168,110 @@ __device__ __forceinline__ void add_up(float2 (&db)[kPairs<T>], float2 (&dw)[kPa
                 dw[e] = add2(dw[e], make_float2(__shfl_xor_sync(0xffffffffu, dw[e].x, o),
                                                 __shfl_xor_sync(0xffffffffu, dw[e].y, o)));
             }
+            if (kWhole)
+                weighed = add2(weighed, make_float2(__shfl_xor_sync(0xffffffffu, weighed.x, o),
+                                                    __shfl_xor_sync(0xffffffffu, weighed.y, o)));
+        }
         rows = kBlockWarps;
-        const int lane = threadIdx.x % kWarp;
-        if (lane < g.lanes)
-#pragma unroll
-            for (int e = 0; e < kVec<T>; ++e)
-                part[threadIdx.x / kWarp * columns + e * g.lanes + lane] =
-                    make_float2(channel_of(db, e), channel_of(dw, e));
-    } else if (p.row < g.step) {
+        row = threadIdx.x % kWarp < g.lanes ? threadIdx.x / kWarp : rows;
+    }
+    float2* behind = part + rows * columns;
+    if (row < rows) {
 #pragma unroll
         for (int e = 0; e < kVec<T>; ++e)
-            part[p.row * columns + e * g.lanes + p.lane] =
+            part[row * columns + e * g.lanes + p.lane] =
                 make_float2(channel_of(db, e), channel_of(dw, e));
+        if (kWhole) behind[row * g.lanes + p.lane] = weighed;
     }
     __syncthreads();
-    float2* weighted = part + rows * columns;  // by channel, for the groups' sums
-    float2 own = splat2(0.0f);
-    for (int c = threadIdx.x; c < p.channels; c += kThreads) {
-        const float2* column = part + c % kVec<T> * g.lanes + c / kVec<T>;
-        float2 s = column[0];
-        for (int r = 1; r < rows; ++r) s = add2(s, column[r * columns]);
-        s = mul2(s, splat2(unit));
-        sums[p.first_channel + c] = s;
-        if (c >= kThreads) w = to_f32<T>(weight[p.first_channel + c]);
-        s = mul2(s, splat2(w));
-        if (p.groups > 1) weighted[c] = s;
-        own = add2(own, s);
+    for (int i = threadIdx.x; i < columns; i += kThreads) {
+        float2 s = part[i];
+#pragma unroll 4
+        for (int r = 1; r < rows; ++r) s = add2(s, part[r * columns + i]);
+        sums[i] = s;
+        if (!kWhole) {
+            const int e = g.by_lanes.quotient(i), c = (i - e * g.lanes) * kVec<T> + e;
+            if (i >= kThreads)
+                w = c < p.channels ? to_f32<T>(weight[p.first_channel + c]) : 0.0f;
+            behind[c] = mul2(s, splat2(w));
+        }
     }
-    if (p.groups == 1) {
-        __shared__ float2 warps[kBlockWarps];
-        own = make_float2(warp_sum(own.x), warp_sum(own.y));
-        if (threadIdx.x % kWarp == 0) warps[threadIdx.x / kWarp] = own;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-#pragma unroll
-            for (int i = 1; i < kBlockWarps; ++i) own = add2(own, warps[i]);
-            group_sums[0] = own;
-        }
-    } else {
-        __syncthreads();
-        const int width = p.channels / p.groups;
-        for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
-            float2 s = splat2(0.0f);
-            for (int c = threadIdx.x % kWarp; c < width; c += kWarp) s = add2(s, weighted[j * width + c]);
-            s = make_float2(warp_sum(s.x), warp_sum(s.y));
-            if (threadIdx.x % kWarp == 0) group_sums[j] = s;
-        }
+    if (!kWhole) __syncthreads();
+    const int width = kWhole ? p.width / kVec<T> : p.width;
+    const Items first(width, g);
+    for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
+        float2 s = splat2(0.0f);
+        for (Items i = first; i.row < (kWhole ? rows : 1); i.next())
+            s = add2(s, behind[i.row * g.lanes + j * width + i.column]);
+        s = make_float2(warp_sum(s.x), warp_sum(s.y));
+        if (threadIdx.x % kWarp == 0) group_sums[j] = s;
     }
     __syncthreads();
 }
+// Shared memory of it, in float2.
+template <typename T, bool kWhole> int sum_values(const Geometry& g) {
+    const int columns = g.lanes * kVec<T>;
+    const int rows = kWarp % g.lanes == 0 ? kBlockWarps : g.step;
+    return columns * rows + (kWhole ? rows * g.lanes : columns);
+}
 
-// Adds the blocks' rows of column sums, in an order that the launch fixes: kSumChannels channels
-// a block, a thread every kSumRows-th row of one of them.
-constexpr int kSumChannels = 8, kSumRows = kThreads / kSumChannels;
+// A row of column sums in the workspace: the slabs' columns in the order of add_up.
+template <typename T> __host__ __device__ __forceinline__ int64_t sum_pitch(const Geometry& g) {
+    return static_cast<int64_t>(g.slabs) * g.lanes * kVec<T>;
+}
+// The channel of column i of a row, -1 for the padding of a slab's last vector.
+template <typename T> __device__ __forceinline__ int channel_at(const Geometry& g, int i) {
+    const int columns = g.lanes * kVec<T>, slab = i / columns, at = i - slab * columns;
+    const int c = at % g.lanes * kVec<T> + at / g.lanes;  // in the slab
+    if (g.parts > 1) {
+        const int group = slab / g.parts, from = (slab - group * g.parts) * g.part_channels;
+        return c < min(g.part_channels, g.group_channels - from)
+                   ? group * g.group_channels + from + c
+                   : -1;
+    }
+    const int slab_channels = g.slab_groups * g.group_channels, from = slab * slab_channels;
+    return c < min(slab_channels, g.channels - from) ? from + c : -1;
+}
+
+// Adds the rows of column sums, in an order that the launch fixes: kSumColumns columns a block, a
+// thread every kSumRows-th row of one of them.
+constexpr int kSumColumns = 8, kSumRows = kThreads / kSumColumns;
 template <typename T>
-__device__ __forceinline__ void sum_parameters(const float2* sums,
-                                               T* __restrict__ dweight, T* __restrict__ dbias,
-                                               int rows, int channels, int block, float2* part) {
-    const int row = threadIdx.x / kSumChannels, lane = threadIdx.x % kSumChannels;
-    const int c = block * kSumChannels + lane;
+__device__ __forceinline__ void sum_parameters(const float2* sums, T* __restrict__ dweight,
+                                               T* __restrict__ dbias, int rows, const Geometry& g,
+                                               int block, float2* part) {
+    const int row = threadIdx.x / kSumColumns;
+    const int i = block * kSumColumns + threadIdx.x % kSumColumns;
+    const int64_t pitch = sum_pitch<T>(g);
     float2 s = splat2(0.0f);
-    if (c < channels) {
+    if (i < pitch) {
 #pragma unroll 8
-        for (int r = row; r < rows; r += kSumRows)
-            s = add2(s, sums[static_cast<int64_t>(r) * channels + c]);
+        for (int r = row; r < rows; r += kSumRows) s = add2(s, sums[r * pitch + i]);
     }
     part[threadIdx.x] = s;
 #pragma unroll
     for (int half = kSumRows / 2; half > 0; half /= 2) {
         __syncthreads();
         if (row < half) {
-            s = add2(s, part[threadIdx.x + half * kSumChannels]);
+            s = add2(s, part[threadIdx.x + half * kSumColumns]);
             part[threadIdx.x] = s;
         }
     }
-    if (row == 0 && c < channels) {
-        dbias[c] = from_f32<T>(s.x);
-        dweight[c] = from_f32<T>(s.y);
+    if (row == 0 && i < pitch) {
+        const int c = channel_at<T>(g, i);
+        if (c >= 0) {
+            dbias[c] = from_f32<T>(s.x);
+            dweight[c] = from_f32<T>(s.y);
+        }
     }
+}
+
+// The place of a block's columns in its row of the workspace, a row for each block of each
+// utterance.
+template <typename T>
+__device__ __forceinline__ float2* sums_of(float2* sums, const Place<T>& p, const Geometry& g) {
+    return sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * sum_pitch<T>(g) +
+           static_cast<int64_t>(p.slab) * g.lanes * kVec<T>;
 }
 
 template <typename T> struct Parameters {
@@ -230,7 +281,7 @@ template <typename T> struct Parameters {
     int rows;
 };
 
-// `sums`: [N * blocks, C] (dbias, dweight) of each block's rows.
+// `sums`: a row of column sums for each block of each utterance.
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 3)
     group_norm_backward_kernel(Tensors<T> t, float2* __restrict__ sums, Geometry g, int act) {
@@ -253,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, 3)
             stage<T, kAligned>(ds + at + i * pitch, d, p.count);
         }
     }
+    const float w = kWhole ? 0.0f : own_weight(t.weight, p, g);
     Column<T, kWhole> column;
     float2 db[kPairs<T>], dw[kPairs<T>];
 #pragma unroll
@@ -273,10 +325,12 @@ __global__ void __launch_bounds__(kThreads, 3)
                 make_uint4(__float_as_uint(d[2 * q].x), __float_as_uint(d[2 * q].y),
                            __float_as_uint(d[2 * q + 1].x), __float_as_uint(d[2 * q + 1].y));
     }
-    if (mine > 0) column.finish(dw);
-    add_up<T>(db, dw, part, means,
-                        sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
-                        t.weight, unit_of(act), p, g);
+    float2 weighed = splat2(0.0f);
+    if (mine > 0) {
+        if (kWhole) weighed = column.weigh(db, dw);
+        column.finish(db, dw, act);
+    }
+    add_up<T, kWhole>(db, dw, weighed, w, part, means, sums_of(sums, p, g), t.weight, p, g);
     if (g.blocks > 1) {
         float2* gathered = part;  // [block][group]
         auto cluster = cg::this_cluster();
@@ -322,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 3)
 
 // The two launches of a stream. The first leaves each block's (s1, s2) in `partial` [N, G, parts *
 // blocks]; the second goes through the rows against the order of the first, so that it begins
-// with those that are still in L2, and its last blocks add up the parameters' gradients. It is
+// with those that are still in L2, and its first blocks add up the parameters' gradients. It is
 // launched early (programmatic dependent launch): its rows are on their way by the time the
 // first has ended.
 template <typename T, bool kAligned, bool kWhole>
@@ -339,7 +393,8 @@ __global__ void __launch_bounds__(kThreads, 3)
     rows.from[0] = t.x + from;
     rows.from[1] = t.dout + from;
     rows.start(shared, mine, static_cast<int64_t>(g.step) * g.channels, p.count);
-    float2 db[kPairs<T>], dw[kPairs<T>];
+    const float w = kWhole ? 0.0f : own_weight(t.weight, p, g);
+    float2 db[kPairs<T>], dw[kPairs<T>], weighed = splat2(0.0f);
 #pragma unroll
     for (int e = 0; e < kPairs<T>; ++e) db[e] = dw[e] = splat2(0.0f);
     if (mine > 0) {
@@ -353,12 +408,12 @@ __global__ void __launch_bounds__(kThreads, 3)
             column.through(d, x, act);
             column.add(db, dw, d, x);
         });
-        column.finish(dw);
+        if (kWhole) weighed = column.weigh(db, dw);
+        column.finish(db, dw, act);
     }
     __syncthreads();  // the slots become the threads' sums
-    add_up<T>(db, dw, reinterpret_cast<float2*>(shared), group_sums,
-                        sums + (static_cast<int64_t>(p.n) * g.blocks + p.block) * g.channels,
-                        t.weight, unit_of(act), p, g);
+    add_up<T, kWhole>(db, dw, weighed, w, reinterpret_cast<float2*>(shared), group_sums,
+                      sums_of(sums, p, g), t.weight, p, g);
     if (threadIdx.x < p.groups)
         partial[(static_cast<int64_t>(p.n) * g.groups + p.first_group + threadIdx.x) * g.parts *
                     g.blocks +
@@ -367,18 +422,17 @@ __global__ void __launch_bounds__(kThreads, 3)
 
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 3)
-    group_norm_gradient_kernel(Tensors<T> t, const float2* partial, Parameters<T> out, int streams,
+    group_norm_gradient_kernel(Tensors<T> t, const float2* partial, Parameters<T> out, int adders,
                                Geometry g, int act) {
     extern __shared__ __align__(16) uint4 shared[];
-    if (blockIdx.x >= streams) {
+    if (blockIdx.x < adders) {
         cudaGridDependencySynchronize();
         __shared__ float2 part[kThreads];
-        sum_parameters(out.sums, out.dweight, out.dbias, out.rows, g.channels, blockIdx.x - streams,
-                       part);
+        sum_parameters(out.sums, out.dweight, out.dbias, out.rows, g, blockIdx.x, part);
         return;
     }
     __shared__ float2 means[kMaxSlabGroups];
-    const Place<T> p = Place<T>::make(g, t.lengths, streams - 1 - blockIdx.x);
+    const Place<T> p = Place<T>::make(g, t.lengths, gridDim.x - 1 - blockIdx.x);
     const int mine = p.own_rows();
     const int64_t stride = static_cast<int64_t>(g.step) * g.channels;
     const int64_t from = p.at(g, p.begin + p.row);
@@ -425,10 +479,10 @@ __global__ void __launch_bounds__(kThreads, 3)
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    group_norm_parameters_kernel(Parameters<T> out, int channels) {
+    group_norm_parameters_kernel(Parameters<T> out, Geometry g) {
     __shared__ float2 part[kThreads];
     cudaGridDependencySynchronize();
-    sum_parameters(out.sums, out.dweight, out.dbias, out.rows, channels, blockIdx.x, part);
+    sum_parameters(out.sums, out.dweight, out.dbias, out.rows, g, blockIdx.x, part);
 }
 
 Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
@@ -450,16 +504,12 @@ cudaError_t run(const GroupNormBackwardProblem& p, const Shape& s, cudaStream_t 
     const Geometry& g = s.geo;
     float2* sums = static_cast<float2*>(p.workspace);
     const int64_t rows = sum_rows(s, p.batch);
-    // The sums of a warp's rows of threads, or of each row of threads, and the columns' for more
-    // than one group; in their place, what a cluster gathers.
-    const int columns = g.lanes * kVec<T> * static_cast<int>(sizeof(float2));
-    const int gather = g.blocks * g.slab_groups * static_cast<int>(sizeof(float2));
-    const int part = std::max(columns * ((kWarp % g.lanes == 0 ? kBlockWarps : g.step) +
-                                         (g.slab_groups > 1 ? 1 : 0)),
-                              s.split ? 0 : gather);
+    // What a cluster gathers takes the place of the sums.
+    const int part = static_cast<int>(sizeof(float2)) *
+                     std::max(sum_values<T, kWhole>(g), s.split ? 0 : g.blocks * g.slab_groups);
     const Parameters<T> out{sums, static_cast<T*>(p.grad_weight), static_cast<T*>(p.grad_bias),
                             static_cast<int>(rows)};
-    const int adders = (p.channels + kSumChannels - 1) / kSumChannels;
+    const int adders = static_cast<int>((sum_pitch<T>(g) + kSumColumns - 1) / kSumColumns);
     const int64_t blocks = s.units * g.blocks;
     cudaError_t e;
     if (!s.split) {
@@ -468,18 +518,18 @@ cudaError_t run(const GroupNormBackwardProblem& p, const Shape& s, cudaStream_t 
                     kTileBytes + kThreads * kVectorBytes<T> + kSumBytes<T> + kGatherBytes},
                    stream, t, sums, g, p.activation);
         if (e != cudaSuccess) return e;
-        return launch(second, group_norm_parameters_kernel<T>, {adders, 1, true, 0, 0}, stream, out,
-                      p.channels);
+        return launch(second, group_norm_parameters_kernel<T>, {adders, 1, true, 0, 0}, stream,
+                      out, g);
     }
     constexpr int kSlots = Stream<T, kAligned, 2>::kBytes, kMost = std::max(kSlots, kSumBytes<T>);
-    float2* partial = sums + rows * p.channels;
+    float2* partial = sums + rows * sum_pitch<T>(g);
     e = launch(first, group_norm_sums_kernel<T, kAligned, kWhole>,
                {blocks, 1, false, std::max(kSlots, part), kMost}, stream, t, sums, partial, g,
                p.activation);
     if (e != cudaSuccess) return e;
     return launch(second, group_norm_gradient_kernel<T, kAligned, kWhole>,
                   {blocks + adders, 1, true, kSlots, kSlots}, stream, t,
-                  static_cast<const float2*>(partial), out, static_cast<int>(blocks), g,
+                  static_cast<const float2*>(partial), out, adders, g,
                   p.activation);
 }
 
@@ -495,7 +545,8 @@ size_t group_norm_backward_workspace(const GroupNormBackwardProblem& p) {
     size_t most = 0;
     for (bool aligned : {true, false}) {
         const Shape s = shape_of(p, aligned);
-        size_t values = static_cast<size_t>(sum_rows(s, p.batch)) * p.channels;
+        size_t values = static_cast<size_t>(sum_rows(s, p.batch)) *
+                        (p.dtype == FGA_FLOAT ? sum_pitch<float>(s.geo) : sum_pitch<__half>(s.geo));
         if (s.split)
             values += static_cast<size_t>(p.batch) * p.groups * s.geo.parts * s.geo.blocks;
         most = std::max(most, values * sizeof(float2));
