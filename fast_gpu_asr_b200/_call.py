@@ -116,7 +116,7 @@ class Operator:
         address = None
         if size:
             if workspace is None:
-                workspace = torch.empty(size, dtype=torch.uint8, device=tensors[0].device)
+                workspace = tensors[0].new_empty(size, dtype=torch.uint8)
             elif (not isinstance(workspace, torch.Tensor) or workspace.get_device() != device
                   or not workspace.is_contiguous()):
                 raise ValueError("workspace must be a contiguous CUDA tensor on the current device")
