@@ -507,11 +507,21 @@ int32_t check_buffers(const fga_tensor_desc* in, const void* const* inputs, int 
     return FGA_SUCCESS;
 }
 
-int32_t check_workspace(const void* workspace, size_t bytes, size_t needed) {
+// Present, large enough, aligned and on top of no binding.
+int32_t check_workspace(const void* workspace, size_t bytes, size_t needed,
+                        const fga_tensor_desc* in, const void* const* inputs, int nin,
+                        const fga_tensor_desc* out, void* const* outputs, int nout) {
     if (needed == 0) return FGA_SUCCESS;
-    if (workspace == nullptr || bytes < needed ||
-        (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
-        return FGA_ERROR_WORKSPACE;
+    const uintptr_t ws = reinterpret_cast<uintptr_t>(workspace);
+    if (workspace == nullptr || bytes < needed || (ws & 15u) != 0) return FGA_ERROR_WORKSPACE;
+    auto on_top = [&](const void* p, const fga_tensor_desc& d) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+        return p != nullptr && ws < at + static_cast<uintptr_t>(desc_bytes(d)) && at < ws + needed;
+    };
+    for (int i = 0; i < nin; ++i)
+        if (on_top(inputs[i], in[i])) return FGA_ERROR_WORKSPACE;
+    for (int i = 0; i < nout; ++i)
+        if (on_top(outputs[i], out[i])) return FGA_ERROR_WORKSPACE;
     return FGA_SUCCESS;
 }
 
@@ -806,7 +816,8 @@ int32_t fga_group_norm_activation_enqueue(const fga_tensor_desc* in, const fga_t
     if (st != FGA_SUCCESS) return st;
     st = check_buffers(in, inputs, 4, 0u, out, outputs, 3, 6u, -1, -1);
     if (st != FGA_SUCCESS) return st;
-    st = check_workspace(workspace, workspace_bytes, fga::group_norm_workspace(p));
+    st = check_workspace(workspace, workspace_bytes, fga::group_norm_workspace(p), in,
+                         inputs, 4, out, outputs, 3);
     if (st != FGA_SUCCESS) return st;
     if ((st = prior_error_status()) != FGA_SUCCESS) return st;
     if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
@@ -852,7 +863,8 @@ int32_t fga_group_norm_activation_backward_enqueue(const fga_tensor_desc* in,
     if (st != FGA_SUCCESS) return st;
     st = check_buffers(in, inputs, 7, 0u, out, outputs, 3, 0u, -1, -1);
     if (st != FGA_SUCCESS) return st;
-    st = check_workspace(workspace, workspace_bytes, fga::group_norm_backward_workspace(p));
+    st = check_workspace(workspace, workspace_bytes, fga::group_norm_backward_workspace(p),
+                         in, inputs, 7, out, outputs, 3);
     if (st != FGA_SUCCESS) return st;
     if ((st = prior_error_status()) != FGA_SUCCESS) return st;
     if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
@@ -902,7 +914,8 @@ int32_t fga_gated_linear_recurrence_enqueue(const fga_tensor_desc* in,
     if (st != FGA_SUCCESS) return st;
     st = check_buffers(in, inputs, 4, 8u, out, outputs, 3, 4u, 3, 1);
     if (st != FGA_SUCCESS) return st;
-    st = check_workspace(workspace, workspace_bytes, fga::recurrence_workspace(p));
+    st = check_workspace(workspace, workspace_bytes, fga::recurrence_workspace(p), in,
+                         inputs, 4, out, outputs, 3);
     if (st != FGA_SUCCESS) return st;
     if ((st = prior_error_status()) != FGA_SUCCESS) return st;
     if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;
@@ -945,7 +958,8 @@ int32_t fga_gated_linear_recurrence_backward_enqueue(const fga_tensor_desc* in,
     if (st != FGA_SUCCESS) return st;
     st = check_buffers(in, inputs, 6, 32u, out, outputs, 3, 0u, -1, -1);
     if (st != FGA_SUCCESS) return st;
-    st = check_workspace(workspace, workspace_bytes, fga::recurrence_backward_workspace(p));
+    st = check_workspace(workspace, workspace_bytes, fga::recurrence_backward_workspace(p), in,
+                         inputs, 6, out, outputs, 3);
     if (st != FGA_SUCCESS) return st;
     if ((st = prior_error_status()) != FGA_SUCCESS) return st;
     if (!fga::device_is_sm100()) return FGA_ERROR_NO_DEVICE;

@@ -117,7 +117,7 @@ template <typename T, bool kWhole> struct Column {
     template <bool kAligned>
     __device__ __forceinline__ void read(const T* w, const T* b, const float2* stats,
                                          const Place<T>& p, const Geometry& g, int act) {
-        const float2 unit = splat2(unit_of(act)), origin = splat2(-origin_of(act));
+        const float2 unit = splat2(unit_of(act));
         unpack<T>(load<T, kAligned>(w + p.channel(), p.count), scale);
         unpack<T>(load<T, kAligned>(b + p.channel(), p.count), shift);
 #pragma unroll
@@ -125,7 +125,7 @@ template <typename T, bool kWhole> struct Column {
             const float2 s = stats[p.group_of(kWhole ? 0 : 2 * i, g)];
             const float2 t = kWhole ? s : stats[p.group_of(2 * i + 1, g)];
             scale[i] = mul2(mul2(scale[i], unit), make_float2(s.y, t.y));
-            shift[i] = mul2(add2(shift[i], origin), unit);
+            shift[i] = shift_of(shift[i], act);
             minus[kWhole ? 0 : i] = make_float2(-s.x, -t.x);
         }
     }

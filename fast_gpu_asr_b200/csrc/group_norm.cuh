@@ -108,6 +108,14 @@ __device__ __forceinline__ float unit_of(int act) {
 __device__ __forceinline__ float origin_of(int act) {
     return act == FGA_ACTIVATION_SWOOSH_R ? 1.0f : 0.0f;
 }
+// A column's shift from its bias. Next to the largest number a bias would leave fp32 in the
+// exponent's units, and silu of the lowest be inf * 0: it stops short of that.
+__device__ __forceinline__ float2 shift_of(float2 bias, int act) {
+    if (act == FGA_ACTIVATION_NONE) return bias;
+    constexpr float kMost = 2.3e38f;
+    const float2 s = mul2(add2(bias, splat2(-origin_of(act))), splat2(unit_of(act)));
+    return make_float2(fminf(fmaxf(s.x, -kMost), kMost), fminf(fmaxf(s.y, -kMost), kMost));
+}
 __device__ __forceinline__ float2 exp2_of(float2 y) {
     return make_float2(exp2_approx(y.x), exp2_approx(y.y));
 }

@@ -50,7 +50,7 @@ template <typename T, bool kWhole> struct Column {
     template <bool kAligned>
     __device__ __forceinline__ void read(const Tensors<T>& t, const Place<T>& p, const Geometry& g,
                                          int act) {
-        const float2 unit = splat2(unit_of(act)), origin = splat2(-origin_of(act));
+        const float2 unit = splat2(unit_of(act));
         unpack<T>(load<T, kAligned>(t.weight + p.channel(), p.count), scale);
         unpack<T>(load<T, kAligned>(t.bias + p.channel(), p.count), shift);
         const int64_t group = static_cast<int64_t>(p.n) * g.groups + p.first_group;
@@ -63,7 +63,7 @@ template <typename T, bool kWhole> struct Column {
         }
 #pragma unroll
         for (int e = 0; e < kPairs<T>; ++e) {
-            shift[e] = mul2(add2(shift[e], origin), unit);
+            shift[e] = shift_of(shift[e], act);
             scale[e] = mul2(mul2(scale[e], unit), rstd[kWhole ? 0 : e]);
         }
     }

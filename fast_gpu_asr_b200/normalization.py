@@ -81,7 +81,7 @@ def group_norm_activation(x: torch.Tensor, valid_lengths: torch.Tensor, weight: 
 
     outputs = _FORWARD((x, valid_lengths, weight, bias), (out,), allocate,
                        lambda name: (torch.float32, (x.shape[0], num_groups)),
-                       (num_groups, eps, _activation(activation)), (num_groups,), workspace, stream)
+                       (num_groups, float(eps), _activation(activation)), (num_groups,), workspace, stream)
     return outputs if return_statistics else outputs[0]
 
 

@@ -116,6 +116,24 @@ def test_constant_groups_and_extremes(dtype):
 
 
 @pytest.mark.parametrize("dtype", cases.DTYPES)
+def test_the_lowest_bias_closes_a_channel(dtype):
+    """A bias of the type's lowest value: silu gives zero and so do its gradients."""
+    x, w, b, dout = cases.norm_inputs(2, 9, 8, dtype, 4)
+    lens = lengths_on_gpu([9, 3])
+    args = [cases.to_cuda(v, dtype) for v in (x, w, b, dout)]
+    args[2][5] = torch.finfo(args[2].dtype).min
+    out, mean, rstd = group_norm_activation(args[0], lens, args[1], args[2], 2,
+                                            return_statistics=True)
+    assert torch.isfinite(out).all() and not out[:, :, 5].any() and out[0, :, 4].all()
+    grads = group_norm_activation_backward(args[3], args[0], lens, args[1], args[2], mean, rstd)
+    assert all(torch.isfinite(g).all() for g in grads)
+    assert grads[1][5] == 0 and grads[2][5] == 0
+    for activation in ("none", "swoosh_r"):
+        out = group_norm_activation(args[0], lens, args[1], args[2], 2, activation=activation)
+        assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", cases.DTYPES)
 def test_a_nan_stays_in_its_group(dtype):
     n, t, c, groups = 2, 40, 48, 6
     x, w, b, dout = cases.norm_inputs(n, t, c, dtype, 3)

@@ -156,6 +156,8 @@ def test_buffers_are_checked_before_any_launch(library):
     step = 1 << 30
     i, o = _lib.pointer_array([step * k for k in (1, 2, 3, 4)]), [step * k for k in (5, 6, 7)]
     size = library.fga_group_norm_activation_workspace_size(ins, 4, 1)
+    assert size == 0 or library.fga_group_norm_activation_enqueue(
+        ins, outs, i, _lib.pointer_array(o), 1, 1e-5, 1, o[0] + 64, size, None) == WORKSPACE
     for ws, have in ((None, size), (step * 8, size - 1), (step * 8 + 8, size)):
         if size:
             assert library.fga_group_norm_activation_enqueue(
