@@ -113,13 +113,19 @@ __device__ __forceinline__ void block_moments(const uint4& first, Each each, flo
 template <typename T, bool kWhole> struct Column {
     static constexpr int kMeans = kWhole ? 1 : kPairs<T>;
     float2 scale[kPairs<T>], shift[kPairs<T>], minus[kMeans];  // minus the mean
-    // `stats`: (mean, rstd) of the slab's groups.
+    uint4 weight, bias;
+    // Asked for before the statistics are there.
     template <bool kAligned>
-    __device__ __forceinline__ void read(const T* w, const T* b, const float2* stats,
-                                         const Place<T>& p, const Geometry& g, int act) {
+    __device__ __forceinline__ void read(const T* w, const T* b, const Place<T>& p) {
+        weight = load<T, kAligned>(w + p.channel(), p.count);
+        bias = load<T, kAligned>(b + p.channel(), p.count);
+    }
+    // `stats`: (mean, rstd) of the slab's groups.
+    __device__ __forceinline__ void make(const float2* stats, const Place<T>& p, const Geometry& g,
+                                         int act) {
         const float2 unit = splat2(unit_of(act));
-        unpack<T>(load<T, kAligned>(w + p.channel(), p.count), scale);
-        unpack<T>(load<T, kAligned>(b + p.channel(), p.count), shift);
+        unpack<T>(weight, scale);
+        unpack<T>(bias, shift);
 #pragma unroll
         for (int i = 0; i < kPairs<T>; ++i) {
             const float2 s = stats[p.group_of(kWhole ? 0 : 2 * i, g)];
@@ -170,6 +176,8 @@ __global__ void __launch_bounds__(kThreads, 4)
         for (int i = 0; i < mine; ++i, from += stride)
             stage<T, kAligned>(at + i * pitch, from, p.count);
     }
+    Column<T, kWhole> column;
+    if (mine > 0) column.template read<kAligned>(t.weight, t.bias, p);
     arrived();
     block_moments<T, kWhole>(mine > 0 ? at[0] : uint4{}, [&](auto work) {
 #pragma unroll 4
@@ -208,8 +216,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     __syncthreads();
     if (mine > 0) {
-        Column<T, kWhole> column;
-        column.template read<kAligned>(t.weight, t.bias, moments, p, g, act);
+        column.make(moments, p, g, act);
         T* to = t.out + p.at(g, p.begin + p.row);
 #pragma unroll 2
         for (int i = 0; i < mine; ++i, to += stride)
@@ -257,6 +264,8 @@ __global__ void __launch_bounds__(kThreads, 4)
     Stream<T, kAligned, 1> rows;
     rows.from[0] = t.x + from;
     rows.start(slots, mine, stride, p.count);
+    Column<T, kWhole> column;
+    if (mine > 0) column.template read<kAligned>(t.weight, t.bias, p);
     const int count = g.parts * g.blocks;
     const float total = static_cast<float>(p.m) * static_cast<float>(g.group_channels);
     cudaGridDependencySynchronize();
@@ -282,8 +291,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     __syncthreads();
     if (mine > 0) {
-        Column<T, kWhole> column;
-        column.template read<kAligned>(t.weight, t.bias, stats, p, g, act);
+        column.make(stats, p, g, act);
         T* to = t.out + from;
         rows.each([&](const uint4(&v)[1]) {
             store<T, kAligned>(to, column.apply(v[0], act), p.count);

@@ -440,6 +440,8 @@ __global__ void __launch_bounds__(kThreads, 3)
     rows.from[0] = t.x + from;
     rows.from[1] = t.dout + from;
     rows.start(shared, mine, stride, p.count);
+    Column<T, kWhole> column;
+    if (mine > 0) column.template read<kAligned>(t, p, g, act);
     const int count = g.parts * g.blocks;
     cudaGridDependencySynchronize();
     for (int j = threadIdx.x / kWarp; j < p.groups; j += kBlockWarps) {
@@ -457,8 +459,6 @@ __global__ void __launch_bounds__(kThreads, 3)
     __syncthreads();
     if (mine > 0) {
         const float inv = 1.0f / (static_cast<float>(p.m) * static_cast<float>(g.group_channels));
-        Column<T, kWhole> column;
-        column.template read<kAligned>(t, p, g, act);
         Final<T, kWhole> final_;
         final_.make(column, means, inv, p, g);
         T* to = t.dx + from;
