@@ -88,8 +88,12 @@ __device__ __forceinline__ void gates(float2 g, float2& f, float2& p) {
 // of. `from` and `to` are the first row's slab.
 struct Rows {
     uint32_t pitch;
-    int bytes;  // of the slab's row: less than kRow in the last slab
+    int bytes;            // of the slab's row: less than kRow in the last slab
+    uint32_t lane_bytes;  // of this lane's first 16-byte unit, where there are four rows a warp
+    bool lane_present;    // whether it lies within the row
 };
+constexpr int kHalf = kFrames / 2;
+static_assert(kHalf * kRow == kWarp * 16, "a warp's 16-byte units cover half of its rows");
 
 template <int kUnit>
 using Unit = std::conditional_t<kUnit == 16, uint4, std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
@@ -111,6 +115,16 @@ template <int kUnit>
 __device__ __forceinline__ void fetch(char* to, const void* from, const Rows& at, int rows,
                                       uint32_t fill, int lane) {
     constexpr int kPerRow = kRow / kUnit;
+    if constexpr (kUnit == 16) {
+        if (rows >= kFrames) {  // all but an utterance's last rows
+            if (at.lane_present) {
+                const char* p = static_cast<const char*>(from) + at.lane_bytes;
+                copy_unit<16>(to + lane * 16, p);
+                copy_unit<16>(to + kHalf * kRow + lane * 16, p + kHalf * at.pitch);
+            }
+            return;
+        }
+    }
 #pragma unroll 2
     for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
         const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
@@ -130,6 +144,17 @@ template <int kUnit>
 __device__ __forceinline__ void store(void* to, const char* from, const Rows& at, int rows,
                                       int lane) {
     constexpr int kPerRow = kRow / kUnit;
+    if constexpr (kUnit == 16) {
+        if (rows >= kFrames) {
+            if (at.lane_present) {
+                char* p = static_cast<char*>(to) + at.lane_bytes;
+                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(from + lane * 16);
+                *reinterpret_cast<uint4*>(p + kHalf * at.pitch) =
+                    *reinterpret_cast<const uint4*>(from + kHalf * kRow + lane * 16);
+            }
+            return;
+        }
+    }
 #pragma unroll 2
     for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
         const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
@@ -196,6 +221,8 @@ template <typename T> struct Place {
         first = static_cast<int64_t>(n) * g.length * g.channels + slab;
         state = static_cast<int64_t>(n) * g.channels + channel;
         rows.bytes = min(kRow, (g.channels - slab) * static_cast<int>(sizeof(T)));
+        rows.lane_bytes = lane / (kRow / 16) * rows.pitch + lane % (kRow / 16) * 16;
+        rows.lane_present = lane % (kRow / 16) * 16 < rows.bytes;
     }
     // The block of the last valid frame, or the first where there is none.
     __device__ bool last_valid(const Geometry& g) const {
