@@ -14,9 +14,17 @@
 // rows are on their way to shared memory meanwhile. The backward pass recomputes h from the
 // states that the forward pass saved every 64 frames.
 //
+// Bound by HBM where there are walks enough: 256 x 375 x 1024 ragged, forward bf16 72.7 us (90 %
+// of a plain copy's rate for the bytes it cannot do without), backward f16 130 us (87 %). What
+// is next is instruction issue (64 % busy, 60 instructions a pair of values forward and 103
+// backward), which is why pairs go through the f32x2 instructions.
+//
 // Where utterances and channels are too few to fill the GPU, several blocks divide an
 // utterance's tiles: a first launch leaves the (A, B) of each block's frames in the workspace,
-// and a block of the second starts from what those before it make of the state.
+// and a block of the second starts from what those before it make of the state. That reads the
+// inputs twice, the second time from L2 where they fit: 2 x 12000 x 512, 24000 frames in 16
+// walks: forward f16 with saved states 26.8 us, backward bf16 35.5 us; 168 and 284
+// undivided.
 #include <algorithm>
 #include <cstdint>
 #include <initializer_list>
@@ -96,7 +104,8 @@ constexpr int kHalf = kFrames / 2;
 static_assert(kHalf * kRow == kWarp * 16, "a warp's 16-byte units cover half of its rows");
 
 template <int kUnit>
-using Unit = std::conditional_t<kUnit == 16, uint4, std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
+using Unit = std::conditional_t<kUnit == 16, uint4,
+                                std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
 
 template <int kUnit> __device__ __forceinline__ void copy_unit(char* to, const char* from) {
     if constexpr (kUnit == 2) {
@@ -104,7 +113,8 @@ template <int kUnit> __device__ __forceinline__ void copy_unit(char* to, const c
     } else {
         const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(to));
         if constexpr (kUnit == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from)
+                         : "memory");
         else
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(from) : "memory");
     }
@@ -521,7 +531,9 @@ __global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks)
 // ---- the first launch of a divided walk ----------------------------------------------------
 // Each warp streams an eighth of the block's frames, kFrames at a time through a ring of stages,
 // for their run alone: (A, B) of the state from x and gate, or (kBack) of the carry from dout
-// and gate: c[first] = A c + sum over t of (f[first] .. f[t]) dout[t].
+// and gate: c[first] = A c + sum over t of (f[first] .. f[t]) dout[t]. Three stages let four
+// blocks stand on a multiprocessor (2 x 12000 x 512 f16, both launches: 26.8 us; four stages
+// 30.0).
 constexpr int kDepth = 3;
 constexpr int kRing = kDepth * 2 * kRows;
 template <typename V> constexpr int runs_smem() {
@@ -594,16 +606,18 @@ struct Shape {
     size_t runs_bytes, workspace;
 };
 
-// A walk is divided below three blocks of it for every four multiprocessors: into as many as
-// `resident` blocks on each of them take. (T = 3000, C = 1024, bf16, forward: 4 utterances, 64
-// walks, 30 us divided and 51 not; 8 utterances, 128 walks, 58 and 51; backward 75 and 79.)
+// A walk of more than two tiles is divided below three blocks of it for every four
+// multiprocessors: into as many as `resident` blocks on each of them take. (T = 3000, C = 1024,
+// bf16, forward: 4 utterances, 64 walks, 26 us divided and 45 not; 8 utterances, 128 walks, 52
+// and 46; backward 38 and 73, 71 and 75. C = 512 f16, one utterance: two tiles 4.8 divided and
+// 3.9 not, three 4.8 and 5.0; backward 5.0 and 5.0, 5.2 and 6.6.)
 Shape shape_of(int batch, int length, int channels, int chunks, int element, int resident) {
     const int slab = kRow / element;
     Shape s{};
     s.geo = {length, channels, chunks, (channels + slab - 1) / slab, 1, 0};
     s.units = static_cast<int64_t>(batch) * s.geo.slabs;
     int each = chunks;
-    if (4 * s.units < 3 * sm_count()) {
+    if (chunks > 2 && 4 * s.units < 3 * sm_count()) {
         const int64_t blocks = std::min<int64_t>(chunks, resident * sm_count() / s.units);
         each = static_cast<int>((chunks + blocks - 1) / blocks);
         s.geo.blocks = (chunks + each - 1) / each;

@@ -58,6 +58,15 @@ def group_norm_activation_workspace_size(x: torch.Tensor, valid_lengths: torch.T
         descs([(t.dtype, t.shape) for t in (x, valid_lengths, weight, bias)]), 4, int(num_groups))
 
 
+def group_norm_activation_backward_workspace_size(x: torch.Tensor, valid_lengths: torch.Tensor,
+                                                  weight: torch.Tensor, bias: torch.Tensor,
+                                                  num_groups: int) -> int:
+    """Bytes of device memory that a backward call with these bindings takes as ``workspace``."""
+    stats = (torch.float32, (x.shape[0], int(num_groups)))
+    ins = [(t.dtype, t.shape) for t in (x, x, valid_lengths, weight, bias)] + [stats] * 2
+    return _lib.library().fga_group_norm_activation_backward_workspace_size(descs(ins), 7)
+
+
 def group_norm_activation(x: torch.Tensor, valid_lengths: torch.Tensor, weight: torch.Tensor,
                           bias: torch.Tensor, num_groups: int, *, eps: float = 1e-5,
                           activation: str = "silu", return_statistics: bool = False,
@@ -81,7 +90,8 @@ def group_norm_activation(x: torch.Tensor, valid_lengths: torch.Tensor, weight: 
 
     outputs = _FORWARD((x, valid_lengths, weight, bias), (out,), allocate,
                        lambda name: (torch.float32, (x.shape[0], num_groups)),
-                       (num_groups, float(eps), _activation(activation)), (num_groups,), workspace, stream)
+                       (num_groups, float(eps), _activation(activation)), (num_groups,),
+                       workspace, stream)
     return outputs if return_statistics else outputs[0]
 
 

@@ -263,6 +263,18 @@ def test_a_given_workspace_is_enough():
     assert torch.equal(want, got) and torch.all(ws[size:] == 171)
 
 
+@pytest.mark.parametrize("n,t,c,groups", [(2, 3000, 256, 1), (200, 400, 256, 8), (1, 60, 512, 32)])
+def test_a_given_backward_workspace_is_enough(n, t, c, groups):
+    x, w, b, dout = (cases.to_cuda(v, "float16") for v in cases.norm_inputs(n, t, c, "float16", 6))
+    lens = lengths_on_gpu([t] + [t // 2] * (n - 1))
+    _, mean, rstd = group_norm_activation(x, lens, w, b, groups, return_statistics=True)
+    size = normalization.group_norm_activation_backward_workspace_size(x, lens, w, b, groups)
+    ws = torch.full((size + 256,), 171, dtype=torch.uint8, device="cuda")
+    want = group_norm_activation_backward(dout, x, lens, w, b, mean, rstd)
+    got = group_norm_activation_backward(dout, x, lens, w, b, mean, rstd, workspace=ws[:size])
+    assert all(torch.equal(p, q) for p, q in zip(want, got)) and torch.all(ws[size:] == 171)
+
+
 def test_offsets_past_32_bits():
     """More than 2^31 elements: the last utterance as in a call of its own."""
     n, t, c, groups = 3, 1 << 19, 1408, 11

@@ -13,7 +13,7 @@ import torch
 import sequence_cases as cases
 from fast_gpu_asr_b200 import (_lib, gated_linear_recurrence, gated_linear_recurrence_backward,
                                group_norm_activation, group_norm_activation_backward,
-                               parakeet_conformer_convolution)
+                               parakeet_conformer_convolution, recurrence)
 from oracle import sequence_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -243,6 +243,29 @@ def test_streams_graphs_and_repeats_give_the_same_bits(n, t, c):
     torch.cuda.synchronize()
     for other in (on_side, graphs[0][1], graphs[1][1], both()):
         assert all(torch.equal(p, q) for p, q in zip(first, other))
+
+
+@pytest.mark.parametrize("n,t,c", [(1, 5000, 64), (3, 700, 65), (2, 60, 64), (1, 128, 40)])
+def test_a_given_workspace_is_enough(n, t, c):
+    x, gate, dout, initial, dfinal = cases.recurrence_inputs(n, t, c, "float16", 6)
+    x, gate, dout = (cases.to_cuda(v, "float16") for v in (x, gate, dout))
+    initial, dfinal = (cases.to_cuda(v, "float32") for v in (initial, dfinal))
+    lens = lengths_on_gpu([t] + [t // 3] * (n - 1))
+    size = recurrence.gated_linear_recurrence_workspace_size(x, lens)
+    size_back = recurrence.gated_linear_recurrence_backward_workspace_size(x, lens)
+    assert (size > 0) == (size_back > 0) == (t > 128)
+    ws = torch.full((size + 256,), 171, dtype=torch.uint8, device="cuda")
+    ws_back = torch.full((size_back + 256,), 171, dtype=torch.uint8, device="cuda")
+    want = gated_linear_recurrence(x, gate, lens, initial, return_states=True)
+    got = gated_linear_recurrence(x, gate, lens, initial, return_states=True, workspace=ws[:size])
+    want += gated_linear_recurrence_backward(dout, x, gate, lens, want[2], dfinal)
+    got += gated_linear_recurrence_backward(dout, x, gate, lens, got[2], dfinal,
+                                            workspace=ws_back[:size_back])
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    assert torch.all(ws[size:] == 171) and torch.all(ws_back[size_back:] == 171)
+    if size:
+        with pytest.raises(_lib.AttentionError, match="WORKSPACE"):
+            gated_linear_recurrence(x, gate, lens, initial, workspace=ws[:size - 1])
 
 
 def test_a_decoding_loop_in_a_graph():
