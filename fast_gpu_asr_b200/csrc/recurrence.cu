@@ -42,7 +42,10 @@ namespace {
 constexpr int kChunk = FGA_RECURRENCE_STATE_FRAMES;
 constexpr int kRow = 128;   // bytes of a row that a warp takes
 constexpr int kFrames = 8;  // rows that a warp moves at a time
-constexpr int kRows = kFrames * kRow;
+// In shared memory a row has room for where it starts in its first 16 bytes, unless all rows
+// start at a multiple of 16.
+template <int kUnit> constexpr int kPitch = kUnit == 16 ? kRow : kRow + 16;
+template <int kUnit> constexpr int kRows = kFrames * kPitch<kUnit>;
 
 // ---- a lane's four bytes of a row ----------------------------------------------------------
 using fga::add2;
@@ -92,8 +95,11 @@ __device__ __forceinline__ void gates(float2 g, float2& f, float2& p) {
 }
 
 // ---- rows between global and shared memory -------------------------------------------------
-// A warp moves kFrames rows in units of kUnit bytes, which every row's address is a multiple
-// of. `from` and `to` are the first row's slab.
+// A warp moves kFrames rows of a slab at a time, 16 bytes an access. kUnit bytes, which every
+// row's address is a multiple of, is 16, 4 or an element. Below 16 a row is fetched as the
+// aligned words that hold it, and its values are read from where it starts in the first: the 15
+// accesses that a unit of 4 bytes or the 64 of 2 would take instead are what bounds the kernel
+// then (30 x 2223 x 589 bf16 ragged, backward: 709 us with units of 2 bytes, UNALIGNED_NOW so).
 struct Rows {
     uint32_t pitch;
     int bytes;            // of the slab's row: less than kRow in the last slab
@@ -107,70 +113,85 @@ template <int kUnit>
 using Unit = std::conditional_t<kUnit == 16, uint4,
                                 std::conditional_t<kUnit == 4, uint32_t, uint16_t>>;
 
-template <int kUnit> __device__ __forceinline__ void copy_unit(char* to, const char* from) {
-    if constexpr (kUnit == 2) {
-        *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
-    } else {
-        const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(to));
-        if constexpr (kUnit == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from)
-                         : "memory");
-        else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(from) : "memory");
+// A tensor's rows of one utterance at the slab.
+struct Source {
+    const char* first;       // row 0's slab
+    const char *begin, *end; // the utterance's bytes: nothing outside is read
+    // Where row i of any kFrames rows that start at a multiple of kFrames begins in its first
+    // aligned word.
+    __device__ __forceinline__ uint32_t offset(const Rows& at, int i) const {
+        return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(first)) + i * at.pitch) & 15u;
     }
+};
+static_assert(kFrames * sizeof(uint16_t) % 16 == 0, "every kFrames rows start alike");
+
+__device__ __forceinline__ void copy16(char* to, const char* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
 }
 
-// The first `rows` rows; the others hold `fill`.
+// Rows t and up, `rows` of them at most; the others hold `fill`.
 template <int kUnit>
-__device__ __forceinline__ void fetch(char* to, const void* from, const Rows& at, int rows,
-                                      uint32_t fill, int lane) {
-    constexpr int kPerRow = kRow / kUnit;
+__device__ __forceinline__ void fetch(char* to, const Source& source, int t, const Rows& at,
+                                      int rows, uint32_t fill, int lane) {
+    const char* from = source.first + t * static_cast<int64_t>(at.pitch);
     if constexpr (kUnit == 16) {
         if (rows >= kFrames) {  // all but an utterance's last rows
             if (at.lane_present) {
-                const char* p = static_cast<const char*>(from) + at.lane_bytes;
-                copy_unit<16>(to + lane * 16, p);
-                copy_unit<16>(to + kHalf * kRow + lane * 16, p + kHalf * at.pitch);
+                const char* p = from + at.lane_bytes;
+                copy16(to + lane * 16, p);
+                copy16(to + kHalf * kRow + lane * 16, p + kHalf * at.pitch);
             }
             return;
         }
     }
-#pragma unroll 2
-    for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
-        const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
+    constexpr int kWords = kPitch<kUnit> / 16;  // of a row
+#pragma unroll
+    for (int j = 0; j < (kFrames * kWords + kWarp - 1) / kWarp; ++j) {
+        const int u = j * kWarp + lane, row = u / kWords, k = u % kWords;
+        if (u >= kFrames * kWords) break;
+        char* word = to + u * 16;
         if (row < rows) {
-            if (byte < at.bytes)
-                copy_unit<kUnit>(to + u * kUnit,
-                                 static_cast<const char*>(from) + (row * at.pitch + byte));
-        } else if constexpr (kUnit == 16) {
-            *reinterpret_cast<uint4*>(to + u * kUnit) = make_uint4(fill, fill, fill, fill);
+            const char* p = from + row * at.pitch;
+            const char* w = p + k * 16;
+            if constexpr (kUnit < 16) w -= reinterpret_cast<uintptr_t>(p) & 15u;
+            if (w < p + at.bytes) {
+                if (kUnit == 16 || (w >= source.begin && w + 16 <= source.end)) {
+                    copy16(word, w);
+                } else {
+                    for (int b = 0; b < 16; b += kUnit)
+                        if (w + b >= source.begin && w + b < source.end)
+                            *reinterpret_cast<Unit<kUnit>*>(word + b) =
+                                *reinterpret_cast<const Unit<kUnit>*>(w + b);
+                }
+            }
         } else {
-            *reinterpret_cast<Unit<kUnit>*>(to + u * kUnit) = static_cast<Unit<kUnit>>(fill);
+            *reinterpret_cast<uint4*>(word) = make_uint4(fill, fill, fill, fill);
         }
     }
 }
 
-template <int kUnit>
-__device__ __forceinline__ void store(void* to, const char* from, const Rows& at, int rows,
+// The same rows back, where they start at a multiple of 16 bytes.
+__device__ __forceinline__ void store(char* to, const char* from, const Rows& at, int rows,
                                       int lane) {
-    constexpr int kPerRow = kRow / kUnit;
-    if constexpr (kUnit == 16) {
-        if (rows >= kFrames) {
-            if (at.lane_present) {
-                char* p = static_cast<char*>(to) + at.lane_bytes;
-                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(from + lane * 16);
-                *reinterpret_cast<uint4*>(p + kHalf * at.pitch) =
-                    *reinterpret_cast<const uint4*>(from + kHalf * kRow + lane * 16);
-            }
-            return;
+    if (rows >= kFrames) {
+        if (at.lane_present) {
+            char* p = to + at.lane_bytes;
+            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(from + lane * 16);
+            *reinterpret_cast<uint4*>(p + kHalf * at.pitch) =
+                *reinterpret_cast<const uint4*>(from + kHalf * kRow + lane * 16);
         }
+        return;
     }
-#pragma unroll 2
-    for (int j = 0; j < kFrames * kPerRow / kWarp; ++j) {
-        const int u = j * kWarp + lane, row = u / kPerRow, byte = u % kPerRow * kUnit;
+    constexpr int kWords = kRow / 16;
+#pragma unroll
+    for (int j = 0; j < kFrames * kWords / kWarp; ++j) {
+        const int u = j * kWarp + lane, row = u / kWords, byte = u % kWords * 16;
         if (row < rows && byte < at.bytes)
-            *reinterpret_cast<Unit<kUnit>*>(static_cast<char*>(to) + (row * at.pitch + byte)) =
-                *reinterpret_cast<const Unit<kUnit>*>(from + u * kUnit);
+            *reinterpret_cast<uint4*>(to + (row * at.pitch + byte)) =
+                *reinterpret_cast<const uint4*>(from + u * 16);
     }
 }
 
@@ -294,28 +315,58 @@ template <typename T> struct Backward {
     void* runs;
 };
 
-// Rows [t, end) of a tensor to kRows bytes of shared memory.
-template <int kUnit, typename T>
-__device__ __forceinline__ void fetch_rows(char* to, const T* tensor, const Place<T>& at,
-                                           const Geometry& g, int t, int end, uint32_t fill) {
-    fetch<kUnit>(to, tensor + at.first + t * static_cast<int64_t>(g.channels), at.rows, end - t,
-                 fill, at.lane);
-}
-template <int kUnit, typename T>
-__device__ __forceinline__ void store_rows(T* tensor, const char* from, const Place<T>& at,
-                                           const Geometry& g, int t, int end) {
-    store<kUnit>(tensor + at.first + t * static_cast<int64_t>(g.channels), from, at.rows, end - t,
-                 at.lane);
-}
 template <typename T>
-__device__ __forceinline__ typename Lane<T>::Value value(const char* rows, int i, int lane) {
-    using Raw = typename Lane<T>::Raw;
-    return Lane<T>::unpack(reinterpret_cast<const Raw*>(rows + i * kRow)[lane]);
+__device__ __forceinline__ Source source_of(const T* tensor, const Place<T>& at,
+                                            const Geometry& g) {
+    const T* utterance = tensor + static_cast<int64_t>(at.n) * g.length * g.channels;
+    return {reinterpret_cast<const char*>(tensor + at.first),
+            reinterpret_cast<const char*>(utterance),
+            reinterpret_cast<const char*>(utterance + static_cast<int64_t>(g.length) * g.channels)};
 }
-template <typename T>
-__device__ __forceinline__ void put(char* rows, int i, int lane, typename Lane<T>::Value v) {
+// The lane's values of row i of those that `source` was fetched from.
+template <typename T, int kUnit>
+__device__ __forceinline__ typename Lane<T>::Value value(const char* rows, int i,
+                                                         const Source& source,
+                                                         const Place<T>& at) {
     using Raw = typename Lane<T>::Raw;
-    reinterpret_cast<Raw*>(rows + i * kRow)[lane] = Lane<T>::pack(v);
+    rows += i * kPitch<kUnit> + at.lane * 4;
+    if constexpr (kUnit < 16) rows += source.offset(at.rows, i);
+    if constexpr (kUnit == 2) {
+        // Two aligned words hold them.
+        const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(rows)) & 2u;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(rows - odd);
+        return Lane<T>::unpack(__funnelshift_r(words[0], words[1], 8 * odd));
+    } else {
+        return Lane<T>::unpack(*reinterpret_cast<const Raw*>(rows));
+    }
+}
+// Row i's values of an output: to `rows`, which `store` moves, or from here. `frame`: row 0's.
+template <typename T, int kUnit>
+__device__ __forceinline__ void put(T* tensor, char* rows, int frame, int i, const Place<T>& at,
+                                    const Geometry& g, typename Lane<T>::Value v) {
+    using Raw = typename Lane<T>::Raw;
+    const Raw raw = Lane<T>::pack(v);
+    if constexpr (kUnit == 16) {
+        reinterpret_cast<Raw*>(rows + i * kRow)[at.lane] = raw;
+    } else if (frame + i < at.end && at.present > 0) {
+        T* to = tensor + at.first + (frame + i) * static_cast<int64_t>(g.channels) +
+                at.lane * Lane<T>::kVec;
+        if constexpr (kUnit == 2) {
+            uint16_t* halves = reinterpret_cast<uint16_t*>(to);
+            halves[0] = static_cast<uint16_t>(raw);
+            if (at.present > 1) halves[1] = static_cast<uint16_t>(raw >> 16);
+        } else {
+            *reinterpret_cast<Raw*>(to) = raw;
+        }
+    }
+}
+template <typename T, int kUnit>
+__device__ __forceinline__ void store_rows(T* tensor, const char* rows, int frame,
+                                           const Place<T>& at) {
+    if constexpr (kUnit == 16)
+        store(reinterpret_cast<char*>(tensor + at.first) +
+                  frame * static_cast<int64_t>(at.rows.pitch),
+              rows, at.rows, at.end - frame, at.lane);
 }
 
 // The padding of an output and of the saved states; `index` and `by` number all warps that work
@@ -349,7 +400,8 @@ template <typename V> struct Tile {
     V back[2][kWarps][kWarp];  // B of the carry (backward)
     V behind[2][kWarp];        // the state (forward) or carry (backward) after the tile
 };
-constexpr int kForwardStage = 2 * kRows, kBackwardStage = 3 * kRows;
+template <int kUnit> constexpr int kForwardStage = 2 * kRows<kUnit>;
+template <int kUnit> constexpr int kBackwardStage = 3 * kRows<kUnit>;
 template <typename V> constexpr int tile_smem(int stage) {
     return 2 * kWarps * stage + static_cast<int>(sizeof(Tile<V>));
 }
@@ -379,17 +431,19 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
     using L = Lane<T>;
     using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
-    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kForwardStage);
+    constexpr int kStage = kForwardStage<kUnit>, kGate = kRows<kUnit>;
+    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kStage);
     const Place<T> at(geo, f.lengths);
-    char* stage = smem + at.warp * 2 * kForwardStage;
+    const Source x = source_of(f.x, at, geo), gate = source_of(f.gate, at, geo);
+    char* stage = smem + at.warp * 2 * kStage;
     const int last = at.warps - 1;
 
     auto fetch_tile = [&](int start, int which) {
         const int t = start + at.warp * kFrames;
-        char* to = stage + which * kForwardStage;
-        fetch_rows<kUnit>(to, f.x, at, geo, t, at.end, 0u);
+        char* to = stage + which * kStage;
+        fetch<kUnit>(to, x, t, at.rows, at.end - t, 0u, at.lane);
         // An infinite gate keeps the state.
-        fetch_rows<kUnit>(to + kRows, f.gate, at, geo, t, at.end, L::kInfinity);
+        fetch<kUnit>(to + kGate, gate, t, at.rows, at.end - t, L::kInfinity, at.lane);
     };
     if (at.begin < at.end) fetch_tile(at.begin, 0);
     commit();
@@ -408,13 +462,14 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
         if (start + kTile < at.end) fetch_tile(start + kTile, turn ^ 1);
         commit();
         arrived<1>();
-        char* rows = stage + turn * kForwardStage;
+        char* rows = stage + turn * kStage;
+        const int frame = start + at.warp * kFrames;
         Run<V> run[kFrames];  // from the warp's first frame to each of them
 #pragma unroll
         for (int i = 0; i < kFrames; ++i) {
             V keep, take;
-            gates(value<T>(rows + kRows, i, at.lane), keep, take);
-            const V add = mul2(take, value<T>(rows, i, at.lane));
+            gates(value<T, kUnit>(rows + kGate, i, gate, at), keep, take);
+            const V add = mul2(take, value<T, kUnit>(rows, i, x, at));
             run[i].a = i == 0 ? keep : mul2(run[i - 1].a, keep);
             run[i].b = i == 0 ? add : fma2(keep, run[i - 1].b, add);
         }
@@ -429,39 +484,16 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
 #pragma unroll
         for (int i = 0; i < kFrames; ++i) {
             after = run[i](h);
-            put<T>(rows, i, at.lane, after);
+            put<T, kUnit>(f.out, rows, frame, i, at, geo, after);
         }
         h = after;
         if (at.warp == last) tile.behind[turn][at.lane] = h;
         __syncwarp();
-        store_rows<kUnit>(f.out, rows, at, geo, start + at.warp * kFrames, at.end);
+        store_rows<T, kUnit>(f.out, rows, frame, at);
         __syncwarp();
     }
     if (at.warp == last && at.last_valid(geo)) write_state(f.final_state + at.state, h, at.present);
     finish<kUnit>(f, at, geo);
-}
-
-// The gradients of kFrames frames whose rows are in `rows` (x, gate, dout) from h before them and
-// the carry behind them; dx takes the place of x, dgate that of gate. f and p are the caller's.
-template <typename T, typename V>
-__device__ __forceinline__ void gradients(char* rows, int lane, const V (&keep)[kFrames],
-                                          const V (&take)[kFrames], V h, V& carry) {
-    const V minus = Lane<T>::all(-1.0f);
-    V away[kFrames];  // h[t-1] - x[t]
-#pragma unroll
-    for (int i = 0; i < kFrames; ++i) {
-        const V x = value<T>(rows, i, lane);
-        away[i] = fma2(x, minus, h);
-        h = fma2(keep[i], h, mul2(take[i], x));
-    }
-#pragma unroll
-    for (int i = kFrames - 1; i >= 0; --i) {
-        const V total = add2(value<T>(rows + 2 * kRows, i, lane), carry);
-        const V gx = mul2(take[i], total);
-        carry = mul2(keep[i], total);
-        put<T>(rows, i, lane, gx);
-        put<T>(rows + kRows, i, lane, mul2(mul2(keep[i], gx), away[i]));
-    }
 }
 
 template <typename T, int kUnit>
@@ -470,17 +502,20 @@ __global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks)
     using L = Lane<T>;
     using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
-    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kBackwardStage);
+    constexpr int kStage = kBackwardStage<kUnit>, kGate = kRows<kUnit>, kDout = 2 * kRows<kUnit>;
+    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kStage);
     const Place<T> at(geo, f.lengths);
-    char* stage = smem + at.warp * 2 * kBackwardStage;
+    const Source x = source_of(f.x, at, geo), gate = source_of(f.gate, at, geo),
+                 dout = source_of(f.dout, at, geo);
+    char* stage = smem + at.warp * 2 * kStage;
     const int last = at.warps - 1;
 
     auto fetch_tile = [&](int start, int which) {
         const int t = start + at.warp * kFrames;
-        char* to = stage + which * kBackwardStage;
-        fetch_rows<kUnit>(to, f.x, at, geo, t, at.end, 0u);
-        fetch_rows<kUnit>(to + kRows, f.gate, at, geo, t, at.end, L::kInfinity);
-        fetch_rows<kUnit>(to + 2 * kRows, f.dout, at, geo, t, at.end, 0u);
+        char* to = stage + which * kStage;
+        fetch<kUnit>(to, x, t, at.rows, at.end - t, 0u, at.lane);
+        fetch<kUnit>(to + kGate, gate, t, at.rows, at.end - t, L::kInfinity, at.lane);
+        fetch<kUnit>(to + kDout, dout, t, at.rows, at.end - t, 0u, at.lane);
     };
     const int top = at.begin < at.end ? (at.end - 1) / kTile * kTile : -1;  // the last tile
     if (top >= 0) fetch_tile(top, 0);
@@ -500,15 +535,16 @@ __global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks)
         if (start > at.begin) fetch_tile(start - kTile, turn ^ 1);
         commit();
         arrived<1>();
-        char* rows = stage + turn * kBackwardStage;
+        char* rows = stage + turn * kStage;
+        const int frame = start + at.warp * kFrames;
         V keep[kFrames], take[kFrames], back = L::all(0.0f);
         Run<V> run{L::all(1.0f), L::all(0.0f)};
 #pragma unroll
         for (int i = 0; i < kFrames; ++i) {
-            gates(value<T>(rows + kRows, i, at.lane), keep[i], take[i]);
+            gates(value<T, kUnit>(rows + kGate, i, gate, at), keep[i], take[i]);
             run.a = mul2(run.a, keep[i]);
-            run.b = fma2(keep[i], run.b, mul2(take[i], value<T>(rows, i, at.lane)));
-            back = fma2(run.a, value<T>(rows + 2 * kRows, i, at.lane), back);
+            run.b = fma2(keep[i], run.b, mul2(take[i], value<T, kUnit>(rows, i, x, at)));
+            back = fma2(run.a, value<T, kUnit>(rows + kDout, i, dout, at), back);
         }
         tile.run[turn][at.warp][at.lane] = run;
         tile.back[turn][at.warp][at.lane] = back;
@@ -517,11 +553,27 @@ __global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks)
         carry = tile.behind[turn ^ 1][at.lane];
         for (int w = last; w > at.warp; --w)
             carry = fma2(tile.run[turn][w][at.lane].a, carry, tile.back[turn][w][at.lane]);
-        gradients<T>(rows, at.lane, keep, take, h, carry);
+        V away[kFrames];  // h[t-1] - x[t]
+#pragma unroll
+        for (int i = 0; i < kFrames; ++i) {
+            const V v = value<T, kUnit>(rows, i, x, at);
+            away[i] = fma2(v, L::all(-1.0f), h);
+            h = fma2(keep[i], h, mul2(take[i], v));
+        }
+        // dx takes the place of x, dgate that of the gates.
+#pragma unroll
+        for (int i = kFrames - 1; i >= 0; --i) {
+            const V total = add2(value<T, kUnit>(rows + kDout, i, dout, at), carry);
+            const V gx = mul2(take[i], total);
+            carry = mul2(keep[i], total);
+            put<T, kUnit>(f.dx, rows, frame, i, at, geo, gx);
+            put<T, kUnit>(f.dgate, rows + kGate, frame, i, at, geo,
+                          mul2(mul2(keep[i], gx), away[i]));
+        }
         if (at.warp == 0) tile.behind[turn][at.lane] = carry;
         __syncwarp();
-        store_rows<kUnit>(f.dx, rows, at, geo, start + at.warp * kFrames, at.end);
-        store_rows<kUnit>(f.dgate, rows + kRows, at, geo, start + at.warp * kFrames, at.end);
+        store_rows<T, kUnit>(f.dx, rows, frame, at);
+        store_rows<T, kUnit>(f.dgate, rows + kGate, frame, at);
         __syncwarp();
     }
     if (at.warp == 0 && at.block == 0) write_state(f.dinitial + at.state, carry, at.present);
@@ -535,9 +587,9 @@ __global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks)
 // blocks stand on a multiprocessor (2 x 12000 x 512 f16, both launches: 26.8 us; four stages
 // 30.0).
 constexpr int kDepth = 3;
-constexpr int kRing = kDepth * 2 * kRows;
-template <typename V> constexpr int runs_smem() {
-    return kWarps * (kRing + kWarp * static_cast<int>(sizeof(Run<V>)));
+template <int kUnit> constexpr int kRing = kDepth * 2 * kRows<kUnit>;
+template <typename V, int kUnit> constexpr int runs_smem() {
+    return kWarps * (kRing<kUnit> + kWarp * static_cast<int>(sizeof(Run<V>)));
 }
 
 template <typename T, int kUnit, bool kBack>
@@ -550,16 +602,19 @@ __global__ void __launch_bounds__(kWarps* kWarp, 4)
     extern __shared__ __align__(16) char smem[];
     cudaTriggerProgrammaticLaunchCompletion();
     const Place<T> at(geo, lengths);
-    char* ring = smem + at.warp * kRing;
-    Run<V>* warps = reinterpret_cast<Run<V>*>(smem + kWarps * kRing);
+    const Source from = source_of(input, at, geo), gate_from = source_of(gate, at, geo);
+    constexpr int kGate = kRows<kUnit>;
+    char* ring = smem + at.warp * kRing<kUnit>;
+    Run<V>* warps = reinterpret_cast<Run<V>*>(smem + kWarps * kRing<kUnit>);
     const int part = geo.span / kWarps, begin = at.begin + at.warp * part;
     const int end = min(at.end, begin + part);
     const int steps = begin < end ? (end - begin + kFrames - 1) / kFrames : 0;
     auto request = [&](int i) {
         if (i < steps) {
-            char* to = ring + i % kDepth * 2 * kRows;
-            fetch_rows<kUnit>(to, input, at, geo, begin + i * kFrames, end, 0u);
-            fetch_rows<kUnit>(to + kRows, gate, at, geo, begin + i * kFrames, end, L::kInfinity);
+            char* to = ring + i % kDepth * 2 * kGate;
+            const int t = begin + i * kFrames;
+            fetch<kUnit>(to, from, t, at.rows, end - t, 0u, at.lane);
+            fetch<kUnit>(to + kGate, gate_from, t, at.rows, end - t, L::kInfinity, at.lane);
         }
         commit();
     };
@@ -569,12 +624,12 @@ __global__ void __launch_bounds__(kWarps* kWarp, 4)
     for (int i = 0; i < steps; ++i) {
         request(i + kDepth - 1);
         arrived<kDepth - 1>();
-        const char* rows = ring + i % kDepth * 2 * kRows;
+        const char* rows = ring + i % kDepth * 2 * kGate;
 #pragma unroll
         for (int k = 0; k < kFrames; ++k) {
             V keep, take;
-            gates(value<T>(rows + kRows, k, at.lane), keep, take);
-            const V v = value<T>(rows, k, at.lane);
+            gates(value<T, kUnit>(rows + kGate, k, gate_from, at), keep, take);
+            const V v = value<T, kUnit>(rows, k, from, at);
             run.a = mul2(run.a, keep);
             run.b = kBack ? fma2(run.a, v, run.b) : fma2(keep, run.b, mul2(take, v));
         }
@@ -679,11 +734,11 @@ template <typename T, int kUnit> cudaError_t forward(const RecurrenceProblem& p,
         f.runs = p.workspace;
         f.first = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + shape.runs_bytes);
         const cudaError_t e =
-            launch(runs, recurrence_runs_kernel<T, kUnit, false>, shape, runs_smem<V>(), false, s,
+            launch(runs, recurrence_runs_kernel<T, kUnit, false>, shape, runs_smem<V, kUnit>(), false, s,
                    f.x, f.gate, f.lengths, f.initial, f.runs, f.first, shape.geo);
         if (e != cudaSuccess) return e;
     }
-    return launch(walk, recurrence_kernel<T, kUnit>, shape, tile_smem<V>(kForwardStage), divided, s,
+    return launch(walk, recurrence_kernel<T, kUnit>, shape, tile_smem<V>(kForwardStage<kUnit>), divided, s,
                   f, shape.geo);
 }
 
@@ -700,12 +755,12 @@ cudaError_t backward(const RecurrenceBackwardProblem& p, cudaStream_t s) {
                         divided ? p.workspace : nullptr};
     if (divided) {
         const cudaError_t e =
-            launch(runs, recurrence_runs_kernel<T, kUnit, true>, shape, runs_smem<V>(), false, s,
+            launch(runs, recurrence_runs_kernel<T, kUnit, true>, shape, runs_smem<V, kUnit>(), false, s,
                    f.dout, f.gate, f.lengths, static_cast<const float*>(nullptr), f.runs,
                    static_cast<float*>(nullptr), shape.geo);
         if (e != cudaSuccess) return e;
     }
-    return launch(walk, recurrence_backward_kernel<T, kUnit>, shape, tile_smem<V>(kBackwardStage),
+    return launch(walk, recurrence_backward_kernel<T, kUnit>, shape, tile_smem<V>(kBackwardStage<kUnit>),
                   divided, s, f, shape.geo);
 }
 
