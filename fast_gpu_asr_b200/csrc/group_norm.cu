@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(kThreads, 4)
         const T* from = t.x + p.at(g, p.begin + p.row);
 #pragma unroll 4
         for (int i = 0; i < mine; ++i, from += stride)
-            stage<T, kAligned>(at + i * pitch, from, p.count);
+            stage<T, kAligned>(at + i * pitch, from, p.count,
+                               p.inner(g, p.begin + p.row + i * g.step));
     }
     Column<T, kWhole> column;
     if (mine > 0) column.template read<kAligned>(t.weight, t.bias, p);
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     Stream<T, kAligned, 1> rows;
     rows.from[0] = t.x + p.at(g, p.begin + p.row);
     const uint4 first = p.own_rows() > 0 ? load<T, kAligned>(rows.from[0], p.count) : uint4{};
-    rows.start(slots, p.own_rows(), static_cast<int64_t>(g.step) * g.channels, p.count);
+    rows.start(slots, p, g);
     block_moments<T, kWhole>(first, [&](auto work) {
         rows.each([&](const uint4(&v)[1]) { work(v[0]); });
     }, part, moments, p, g);
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     const int64_t from = p.at(g, p.begin + p.row);
     Stream<T, kAligned, 1> rows;
     rows.from[0] = t.x + from;
-    rows.start(slots, mine, stride, p.count);
+    rows.start(slots, p, g);
     Column<T, kWhole> column;
     if (mine > 0) column.template read<kAligned>(t.weight, t.bias, p);
     const int count = g.parts * g.blocks;

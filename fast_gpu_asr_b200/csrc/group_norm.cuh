@@ -75,6 +75,23 @@ template <typename T, bool kAligned>
 __device__ __forceinline__ void store(T* p, const uint4& r, int count) {
     if constexpr (kAligned) {
         *reinterpret_cast<uint4*>(p) = r;
+    } else if (sizeof(T) == 2 && count == kVec<T>) {
+        // In words, between two halves at an odd element.
+        uint32_t* words = reinterpret_cast<uint32_t*>(p);
+        if (reinterpret_cast<uintptr_t>(p) & 2u) {
+            uint16_t* halves = reinterpret_cast<uint16_t*>(p);
+            words = reinterpret_cast<uint32_t*>(halves + 1);
+            halves[0] = static_cast<uint16_t>(r.x);
+            words[0] = __funnelshift_r(r.x, r.y, 16);
+            words[1] = __funnelshift_r(r.y, r.z, 16);
+            words[2] = __funnelshift_r(r.z, r.w, 16);
+            halves[7] = static_cast<uint16_t>(r.w >> 16);
+        } else {
+            words[0] = r.x;
+            words[1] = r.y;
+            words[2] = r.z;
+            words[3] = r.w;
+        }
     } else {
         const T* v = reinterpret_cast<const T*>(&r);
 #pragma unroll
@@ -82,16 +99,57 @@ __device__ __forceinline__ void store(T* p, const uint4& r, int count) {
             if (e < count) p[e] = v[e];
     }
 }
-// The same into shared memory, to be read by the same thread after `arrived`.
+
+// A vector that starts anywhere, from the one or two aligned words that hold it: 16 bytes an
+// access where its elements one by one would take 8, which is what bounds a kernel then (14 x
+// 4611 x 598 bf16 ragged in 46 groups: 239 us by elements, GN_UNALIGNED_NOW so).
+__device__ __forceinline__ uint32_t start_of(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+}
+// `count` channels from byte `start` of the words; the others are zero.
+template <typename T>
+__device__ __forceinline__ uint4 vector_of(const uint4& a, const uint4& b, uint32_t start, int count) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = start & 8u ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = start & 4u ? w[i + 1] : w[i];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (start & 2u));
+    }
+    if (count < kVec<T>) {
+        T* v = reinterpret_cast<T*>(w);
+#pragma unroll
+        for (int e = 0; e < kVec<T>; ++e)
+            if (e >= count) v[e] = T(0.0f);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Of these two, the second only if the vector reaches into it.
+template <typename T> __device__ __forceinline__ bool in_two(uint32_t start, int count) {
+    return start + static_cast<uint32_t>(count) * sizeof(T) > 16u;
+}
+template <typename T> __device__ __forceinline__ uint4 load_words(const T* p, int count) {
+    const uint32_t start = start_of(p);
+    const uint4* words = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) - start);
+    return vector_of<T>(words[0], in_two<T>(start, count) ? words[1] : uint4{}, start, count);
+}
+
+__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
+}
+// A vector into shared memory, to be read by the same thread after `arrived`. `inner`: its words
+// are the tensor's own.
 template <typename T, bool kAligned>
-__device__ __forceinline__ void stage(uint4* to, const T* p, int count) {
+__device__ __forceinline__ void stage(uint4* to, const T* p, int count, bool inner) {
     if constexpr (kAligned)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-                     "l"(p)
-                     : "memory");
+        copy16(to, p);
     else
-        *to = load<T, false>(p, count);
+        *to = inner ? load_words<T>(p, count) : load<T, false>(p, count);
 }
 __device__ __forceinline__ void arrived() {
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -186,6 +244,7 @@ struct Geometry {
     int blocks;       // that divide the valid rows of an utterance's slab evenly
     int rows;         // most rows of a block
     int lanes, step;  // threads of a row, rows of a block's threads
+    int edge;         // rows at either end of an utterance whose words may be partly another's
     int item_width, item_rows;  // of Items: a group's columns, and rows of 32 of them
     Divisor by_blocks, by_slabs, by_lanes, by_step, by_group, by_item;
 };
@@ -241,6 +300,10 @@ template <typename T> struct Place {
     __device__ __forceinline__ int group_of(int e, const Geometry& g) const {
         return g.parts > 1 ? 0 : min(g.by_group.quotient(lane * kVec<T> + e), groups - 1);
     }
+    // Whether the words that hold row t are this utterance's.
+    __device__ __forceinline__ static bool inner(const Geometry& g, int t) {
+        return t >= g.edge && t < g.length - g.edge;
+    }
     __device__ __forceinline__ int channel() const { return first_channel + lane * kVec<T>; }
     // Element offset of this thread's vector in row t.
     __device__ __forceinline__ int64_t at(const Geometry& g, int t) const {
@@ -276,29 +339,59 @@ struct Items {
 constexpr int kDepth = 4;
 template <typename T, bool kAligned, int kSources> struct Stream {
     const T* from[kSources];
-    uint4* slots;  // [kDepth][kSources][kThreads]
+    uint4* slots;  // [kDepth][kSources][kWords][kThreads]
     int64_t stride;
     int rows, count;
+    // Not kAligned: the next row to request, and where the next to work on starts in its words.
+    int t, t_step, t_low, t_high;
+    uint32_t begins[kSources];
 
-    static constexpr int kBytes = kAligned ? kDepth * kSources * kThreads * 16 : 0;
+    static constexpr int kWords = kAligned ? 1 : 2;
+    static constexpr int kBytes = kDepth * kSources * kWords * kThreads * 16;
 
+    __device__ __forceinline__ uint4* slot_of(int slot, int k) const {
+        return slots + (slot * kSources + k) * kWords * kThreads;
+    }
     __device__ __forceinline__ void request(bool wanted, int slot) {
-        if (wanted)
+        if (wanted) {
 #pragma unroll
             for (int k = 0; k < kSources; ++k) {
-                stage<T, true>(slots + (slot * kSources + k) * kThreads, from[k], count);
+                uint4* to = slot_of(slot, k);
+                if constexpr (kAligned) {
+                    copy16(to, from[k]);
+                } else {
+                    const uint32_t start = start_of(from[k]);
+                    const char* words = reinterpret_cast<const char*>(from[k]) - start;
+                    if (t >= t_low && t < t_high) {
+                        copy16(to, words);
+                        if (in_two<T>(start, count)) copy16(to + kThreads, words + 16);
+                    } else {
+                        for (int e = 0; e < count; ++e) {
+                            const uint32_t at = start + e * static_cast<uint32_t>(sizeof(T));
+                            *reinterpret_cast<T*>(reinterpret_cast<char*>(to + at / 16 * kThreads) +
+                                                  at % 16) = from[k][e];
+                        }
+                    }
+                }
                 from[k] += stride;
             }
+            t += t_step;
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    __device__ __forceinline__ void start(uint4* shared, int rows_, int64_t stride_, int count_) {
+    __device__ __forceinline__ void start(uint4* shared, const Place<T>& p, const Geometry& g) {
         slots = shared + threadIdx.x;
-        rows = rows_;
-        stride = stride_;
-        count = count_;
-        if constexpr (kAligned)
+        rows = p.own_rows();
+        stride = static_cast<int64_t>(g.step) * g.channels;
+        count = p.count;
+        t = p.begin + p.row;
+        t_step = g.step;
+        t_low = g.edge;
+        t_high = g.length - g.edge;
 #pragma unroll
-            for (int i = 0; i < kDepth - 1; ++i) request(i < rows, i);
+        for (int k = 0; k < kSources; ++k) begins[k] = start_of(from[k]);
+#pragma unroll
+        for (int i = 0; i < kDepth - 1; ++i) request(i < rows, i);
     }
     // work(vectors) for every row.
     template <typename Work> __device__ __forceinline__ void each(Work work) {
@@ -307,16 +400,17 @@ template <typename T, bool kAligned, int kSources> struct Stream {
             for (int s = 0; s < kDepth; ++s) {
                 if (i + s >= rows) break;
                 uint4 v[kSources];
-                if constexpr (kAligned) {
-                    request(i + s + kDepth - 1 < rows, (s + kDepth - 1) % kDepth);
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+                request(i + s + kDepth - 1 < rows, (s + kDepth - 1) % kDepth);
+                asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
 #pragma unroll
-                    for (int k = 0; k < kSources; ++k) v[k] = slots[(s * kSources + k) * kThreads];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < kSources; ++k) {
-                        v[k] = load<T, false>(from[k], count);
-                        from[k] += stride;
+                for (int k = 0; k < kSources; ++k) {
+                    const uint4* at = slot_of(s, k);
+                    if constexpr (kAligned) {
+                        v[k] = at[0];
+                    } else {
+                        v[k] = vector_of<T>(at[0], at[kThreads], begins[k], count);
+                        begins[k] = (begins[k] + static_cast<uint32_t>(stride) *
+                                                     static_cast<uint32_t>(sizeof(T))) & 15u;
                     }
                 }
                 work(v);
@@ -386,6 +480,8 @@ inline Shape slabs_of(const Problem& p, int64_t slab_bytes) {
     g.item_width = std::min(width, g.part_channels) / (s.whole ? vec : 1);
     g.lanes = (std::min(width * g.slab_groups, g.part_channels) + vec - 1) / vec;
     g.step = kThreads / g.lanes;
+    const int64_t row_bytes = static_cast<int64_t>(p.channels) * p.element;
+    g.edge = static_cast<int>((15 + row_bytes - 1) / row_bytes);
     return s;
 }
 

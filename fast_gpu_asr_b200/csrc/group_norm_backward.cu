@@ -313,8 +313,9 @@ __global__ void __launch_bounds__(kThreads, 3)
         const T *x = t.x + first, *d = t.dout + first;
 #pragma unroll 4
         for (int i = 0; i < mine; ++i, x += stride, d += stride) {
-            stage<T, kAligned>(xs + at + i * pitch, x, p.count);
-            stage<T, kAligned>(ds + at + i * pitch, d, p.count);
+            const bool inner = p.inner(g, p.begin + p.row + i * g.step);
+            stage<T, kAligned>(xs + at + i * pitch, x, p.count, inner);
+            stage<T, kAligned>(ds + at + i * pitch, d, p.count, inner);
         }
     }
     const float w = kWhole ? 0.0f : own_weight(t.weight, p, g);
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     Stream<T, kAligned, 2> rows;
     rows.from[0] = t.x + from;
     rows.from[1] = t.dout + from;
-    rows.start(shared, mine, static_cast<int64_t>(g.step) * g.channels, p.count);
+    rows.start(shared, p, g);
     const float w = kWhole ? 0.0f : own_weight(t.weight, p, g);
     float2 db[kPairs<T>], dw[kPairs<T>], weighed = splat2(0.0f);
 #pragma unroll
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 3)
     Stream<T, kAligned, 2> rows;
     rows.from[0] = t.x + from;
     rows.from[1] = t.dout + from;
-    rows.start(shared, mine, stride, p.count);
+    rows.start(shared, p, g);
     Column<T, kWhole> column;
     if (mine > 0) column.template read<kAligned>(t, p, g, act);
     const int count = g.parts * g.blocks;

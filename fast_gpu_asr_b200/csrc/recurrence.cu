@@ -105,7 +105,13 @@ struct Rows {
     int bytes;            // of the slab's row: less than kRow in the last slab
     uint32_t lane_bytes;  // of this lane's first 16-byte unit, where there are four rows a warp
     bool lane_present;    // whether it lies within the row
+    // The words of a block of rows that this lane fetches where rows start anywhere: from row 0,
+    // kOutside if there is none. Only if all inputs start alike (`alike`).
+    int word[3];
+    bool alike;
+    int length;  // frames of the utterance
 };
+constexpr int kOutside = INT32_MIN;
 constexpr int kHalf = kFrames / 2;
 static_assert(kHalf * kRow == kWarp * 16, "a warp's 16-byte units cover half of its rows");
 
@@ -144,6 +150,16 @@ __device__ __forceinline__ void fetch(char* to, const Source& source, int t, con
                 copy16(to + lane * 16, p);
                 copy16(to + kHalf * kRow + lane * 16, p + kHalf * at.pitch);
             }
+            return;
+        }
+    }
+    if constexpr (kUnit < 16) {
+        // All but the first and last rows, which may share a word with other memory.
+        if (at.alike && rows >= kFrames && t > 0 && t + 2 * kFrames <= at.length) {
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (at.word[j] != kOutside)
+                    copy16(to + (j * kWarp + lane) * 16, from + at.word[j]);
             return;
         }
     }
@@ -249,6 +265,7 @@ template <typename T> struct Place {
         begin = block * g.span;
         end = max(begin, min(m, begin + g.span));
         rows.pitch = static_cast<uint32_t>(g.channels) * sizeof(T);
+        rows.length = g.length;
         first = static_cast<int64_t>(n) * g.length * g.channels + slab;
         state = static_cast<int64_t>(n) * g.channels + channel;
         rows.bytes = min(kRow, (g.channels - slab) * static_cast<int>(sizeof(T)));
@@ -322,6 +339,24 @@ __device__ __forceinline__ Source source_of(const T* tensor, const Place<T>& at,
     return {reinterpret_cast<const char*>(tensor + at.first),
             reinterpret_cast<const char*>(utterance),
             reinterpret_cast<const char*>(utterance + static_cast<int64_t>(g.length) * g.channels)};
+}
+// The lane's words, if all of `sources` start alike.
+template <int kUnit>
+__device__ __forceinline__ void plan(Rows& at, std::initializer_list<Source> sources, int lane) {
+    if constexpr (kUnit < 16) {
+        at.alike = true;
+        const Source& one = *sources.begin();
+        for (const Source& s : sources) at.alike = at.alike && s.offset(at, 0) == one.offset(at, 0);
+        constexpr int kWords = kPitch<kUnit> / 16;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            const int u = j * kWarp + lane, row = u / kWords;
+            const int in_row = u % kWords * 16 - static_cast<int>(one.offset(at, row));
+            at.word[j] = row < kFrames && in_row < at.bytes
+                             ? static_cast<int>(row * at.pitch) + in_row
+                             : kOutside;
+        }
+    }
 }
 // The lane's values of row i of those that `source` was fetched from.
 template <typename T, int kUnit>
@@ -433,8 +468,9 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
     extern __shared__ __align__(16) char smem[];
     constexpr int kStage = kForwardStage<kUnit>, kGate = kRows<kUnit>;
     Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kStage);
-    const Place<T> at(geo, f.lengths);
+    Place<T> at(geo, f.lengths);
     const Source x = source_of(f.x, at, geo), gate = source_of(f.gate, at, geo);
+    plan<kUnit>(at.rows, {x, gate}, at.lane);
     char* stage = smem + at.warp * 2 * kStage;
     const int last = at.warps - 1;
 
@@ -497,16 +533,17 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
 }
 
 template <typename T, int kUnit>
-__global__ void __launch_bounds__(kWarps* kWarp, kBackwardBlocks)
+__global__ void __launch_bounds__(kWarps* kWarp, kUnit == 2 ? 2 : kBackwardBlocks)
     recurrence_backward_kernel(Backward<T> f, Geometry geo) {
     using L = Lane<T>;
     using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
     constexpr int kStage = kBackwardStage<kUnit>, kGate = kRows<kUnit>, kDout = 2 * kRows<kUnit>;
     Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kStage);
-    const Place<T> at(geo, f.lengths);
+    Place<T> at(geo, f.lengths);
     const Source x = source_of(f.x, at, geo), gate = source_of(f.gate, at, geo),
                  dout = source_of(f.dout, at, geo);
+    plan<kUnit>(at.rows, {x, gate, dout}, at.lane);
     char* stage = smem + at.warp * 2 * kStage;
     const int last = at.warps - 1;
 
@@ -601,8 +638,9 @@ __global__ void __launch_bounds__(kWarps* kWarp, 4)
     using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
     cudaTriggerProgrammaticLaunchCompletion();
-    const Place<T> at(geo, lengths);
+    Place<T> at(geo, lengths);
     const Source from = source_of(input, at, geo), gate_from = source_of(gate, at, geo);
+    plan<kUnit>(at.rows, {from, gate_from}, at.lane);
     constexpr int kGate = kRows<kUnit>;
     char* ring = smem + at.warp * kRing<kUnit>;
     Run<V>* warps = reinterpret_cast<Run<V>*>(smem + kWarps * kRing<kUnit>);
