@@ -334,11 +334,18 @@ cudaError_t run(const GroupNormProblem& p, const Shape& s, cudaStream_t stream) 
 
 // Rows on chip wherever a cluster holds them: as fast as two streams for large batches (256 x 375
 // x 1024 f16 in one group: 105 us against 106), faster for small ones (1 x 3000 x 512: 8 against
-// 14), where the streams' second launch shows.
+// 14), where the streams' second launch shows. Rows that start anywhere are cut into as few
+// slabs as can be, since a slab's ends share their words with its neighbours': streams where it
+// would take a cluster and x is not small (x of 24 MB f16 in 7 groups of 143: 41 us on chip, 32
+// in streams; of 12 MB 22.8 and 23.4, in one group of 514 19.5 and 25.9).
+constexpr int64_t kAnywhereBytes = 16 << 20;
 Shape shape_of(const GroupNormProblem& p, bool aligned) {
     const Problem q{p.batch, p.length, p.channels, p.groups, p.dtype == FGA_FLOAT ? 4 : 2, aligned};
     const Shape s = resident_shape(q, 16, kTileBytes);
-    return s.geo.blocks > 0 ? s : stream_shape(q);
+    const int64_t bytes = static_cast<int64_t>(p.batch) * p.length * p.channels * q.element;
+    const bool resident =
+        s.geo.blocks == 1 || (s.geo.blocks > 1 && (s.aligned || bytes <= kAnywhereBytes));
+    return resident ? s : stream_shape(q);
 }
 
 template <typename T> cudaError_t run(const GroupNormProblem& p, cudaStream_t stream) {

@@ -102,13 +102,14 @@ __device__ __forceinline__ void store(T* p, const uint4& r, int count) {
 
 // A vector that starts anywhere, from the one or two aligned words that hold it: 16 bytes an
 // access where its elements one by one would take 8, which is what bounds a kernel then (14 x
-// 4611 x 598 bf16 ragged in 46 groups: 239 us by elements, GN_UNALIGNED_NOW so).
+// 4611 x 598 bf16 ragged in 46 groups, on chip: 239 us by elements, 130 so).
 __device__ __forceinline__ uint32_t start_of(const void* p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
 }
 // `count` channels from byte `start` of the words; the others are zero.
 template <typename T>
-__device__ __forceinline__ uint4 vector_of(const uint4& a, const uint4& b, uint32_t start, int count) {
+__device__ __forceinline__ uint4 vector_of(const uint4& a, const uint4& b, uint32_t start,
+                                           int count) {
     uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int i = 0; i < 6; ++i) w[i] = start & 8u ? w[i + 2] : w[i];
@@ -368,8 +369,8 @@ template <typename T, bool kAligned, int kSources> struct Stream {
                     } else {
                         for (int e = 0; e < count; ++e) {
                             const uint32_t at = start + e * static_cast<uint32_t>(sizeof(T));
-                            *reinterpret_cast<T*>(reinterpret_cast<char*>(to + at / 16 * kThreads) +
-                                                  at % 16) = from[k][e];
+                            char* word = reinterpret_cast<char*>(to + at / 16 * kThreads);
+                            *reinterpret_cast<T*>(word + at % 16) = from[k][e];
                         }
                     }
                 }

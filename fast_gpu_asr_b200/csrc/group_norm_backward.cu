@@ -502,7 +502,8 @@ __global__ void __launch_bounds__(kThreads)
 // Rows on chip where one block holds a slab's whole length. Where it takes a cluster, that still
 // wins for small batches (x and dout of 18 MB bf16: 13.9 us against 17.5 in two streams) and in
 // fp32, whose streams move twice the bytes for each slope they evaluate again (64 x 375 x 1024:
-// 73 us against 87); larger ones of 16 bits stream (256 x 750 x 192 bf16 ragged: 52 against 65).
+// 73 us against 87); larger ones of 16 bits stream (256 x 750 x 192 bf16 ragged: 52 against 65),
+// and in fp32 those whose rows start anywhere (64 x 375 x 1001: 92 against 163).
 constexpr int64_t kClusterBytes = 64 << 20;
 Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
     const int element = p.dtype == FGA_FLOAT ? 4 : 2;
@@ -511,7 +512,8 @@ Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
                                    kTileBytes);
     const int64_t bytes = 2LL * p.batch * p.length * p.channels * element;
     const bool resident =
-        s.geo.blocks == 1 || (s.geo.blocks > 1 && (element == 4 || bytes <= kClusterBytes));
+        s.geo.blocks == 1 || (s.geo.blocks > 1 &&
+                               ((element == 4 && s.aligned) || bytes <= kClusterBytes));
     return resident ? s : stream_shape(q);
 }
 

@@ -97,9 +97,10 @@ __device__ __forceinline__ void gates(float2 g, float2& f, float2& p) {
 // ---- rows between global and shared memory -------------------------------------------------
 // A warp moves kFrames rows of a slab at a time, 16 bytes an access. kUnit bytes, which every
 // row's address is a multiple of, is 16, 4 or an element. Below 16 a row is fetched as the
-// aligned words that hold it, and its values are read from where it starts in the first: the 15
-// accesses that a unit of 4 bytes or the 64 of 2 would take instead are what bounds the kernel
-// then (30 x 2223 x 589 bf16 ragged, backward: 709 us with units of 2 bytes, UNALIGNED_NOW so).
+// aligned words that hold it, and its values are read from where it starts in the first: the 32
+// and 64 accesses a row that units of 4 and 2 bytes would take are what bounds a kernel then (30
+// x 2223 x 589 bf16 ragged, backward: 709 us by elements, 173 so; 15 x 9490 x 275 f32, forward:
+// 289 and 156).
 struct Rows {
     uint32_t pitch;
     int bytes;            // of the slab's row: less than kRow in the last slab
@@ -532,6 +533,8 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
     finish<kUnit>(f, at, geo);
 }
 
+// (Two blocks a multiprocessor with units of 2 bytes: three would spill registers, 173 us against
+// 196 in the case above.)
 template <typename T, int kUnit>
 __global__ void __launch_bounds__(kWarps* kWarp, kUnit == 2 ? 2 : kBackwardBlocks)
     recurrence_backward_kernel(Backward<T> f, Geometry geo) {
