@@ -14,8 +14,8 @@
 // first of which leaves each block's (mean, squares) in the workspace.
 //
 // So x is read once and out written once: 256 x 375 x 1024 f16 ragged, 32 groups, SiLU, takes
-// 59.7 us, 80 % of a plain copy's rate for those bytes (fp32, 64 x 375 x 1024: 29.5 us, 80 %).
-// In the way of the rest are instruction issue (58 % busy, 42 instructions a pair of values) and
+// 59 us, 81 % of a plain copy's rate for those bytes (fp32, 64 x 375 x 1024: 29.4 us, 81 %). In
+// the way of the rest are instruction issue (56 % busy, 32 instructions a pair of values) and
 // that a block loads, reduces and stores in turn; four on a multiprocessor cover for one another,
 // which is what 48 KB of tile and 64 registers are chosen for.
 #include "fga_kernels.h"

@@ -21,9 +21,9 @@
 // Measured: 256 x 375 x 1024 f16 ragged in 32 groups, SiLU, on chip, 126 us (52 % of a plain
 // copy's rate for reading x and dout and writing dx once); 256 x 750 x 192 bf16 ragged in 6
 // groups, Swoosh-R, streams, 51.3 us (48 %, and 79 % with what is read twice counted twice); 16 x
-// 3000 x 1024 f16 in one group, SiLU, streams, 65.3 us (50 % and 83 %). Issue is about 60 % busy
-// (57 instructions a pair of values in each stream) and the rest is a block's own latency: its
-// parameters, its first rows and its sums across threads.
+// 3000 x 1024 f16 in one group, SiLU, streams, 65 us (50 % and 83 %). Issue is 54 to 65 % busy (65
+// instructions a pair of values on chip, 45 and 42 in the two streams) and the rest is a block's
+// own latency: its parameters, its first rows and its sums across threads.
 #include "fga_kernels.h"
 #include "group_norm.cuh"
 

@@ -16,7 +16,7 @@
 //
 // Bound by HBM where there are walks enough: 256 x 375 x 1024 ragged, forward bf16 72.7 us (90 %
 // of a plain copy's rate for the bytes it cannot do without), backward f16 130 us (87 %). What
-// is next is instruction issue (64 % busy, 60 instructions a pair of values forward and 103
+// is next is instruction issue (68 and 63 % busy, 48 instructions a pair of values forward and 82
 // backward), which is why pairs go through the f32x2 instructions.
 //
 // Where utterances and channels are too few to fill the GPU, several blocks divide an

@@ -183,6 +183,36 @@ def test_unaligned_buffers_and_guards(dtype, shift):
         cases.assert_within(cases.host(got), e, bound)
 
 
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+@pytest.mark.parametrize("n,t,c,groups", [(2, 100, 65, 5), (1, 9, 3, 1), (1, 3000, 129, 3),
+                                          (2, 5000, 1, 1), (3, 70, 130, 130), (40, 900, 258, 2)])
+def test_tensors_that_start_differently(n, t, c, groups, dtype):
+    x, w, b, dout = cases.norm_inputs(n, t, c, dtype, 8)
+    lengths = [t] * n
+    lens = lengths_on_gpu(lengths)
+
+    def starting(v, shift):
+        room = torch.full((v.size + 64,), float("nan"), dtype=getattr(torch, dtype), device="cuda")
+        room[shift:shift + v.size] = cases.to_cuda(v, dtype).flatten()
+        return room[shift:shift + v.size].view(v.shape)
+
+    gx, gw, gb, gd = (starting(v, s) for v, s in ((x, 1), (w, 3), (b, 0), (dout, 6)))
+    out = starting(np.zeros((n, t, c)), 5)
+    _, mean, rstd = group_norm_activation(gx, lens, gw, gb, groups, out=out,
+                                          return_statistics=True)
+    expected = oracle.group_norm_activation(x, lengths, w, b, groups, 1e-5, "silu")
+    bounds = cases.norm_bounds(x, lengths, w, b, groups, expected[1], expected[2], expected[0],
+                               dtype)
+    for v, want, bound in zip((out, mean, rstd), expected, bounds):
+        cases.assert_within(cases.host(v), want, bound)
+    grads = group_norm_activation_backward(gd, gx, lens, gw, gb, mean, rstd)
+    mu, r = cases.host(mean), cases.host(rstd)
+    want = oracle.group_norm_activation_backward(dout, x, lengths, w, b, mu, r, "silu")
+    bounds = cases.norm_gradient_bounds(dout, x, lengths, w, b, mu, r, want, "silu", dtype)
+    for v, e, bound in zip(grads, want, bounds):
+        cases.assert_within(cases.host(v), e, bound)
+
+
 @pytest.mark.parametrize("n,t,c,groups", [(4, 60, 128, 8), (2, 2500, 64, 1), (1, 700, 1040, 1)])
 def test_streams_graphs_and_repeats_give_the_same_bits(n, t, c, groups):
     x, w, b, dout = (cases.to_cuda(v, "bfloat16") for v in cases.norm_inputs(n, t, c, "bfloat16", 5))

@@ -212,6 +212,35 @@ def test_unaligned_buffers_and_guards(dtype, shift):
         cases.assert_within(cases.host(v), e, bound)
 
 
+def starting(v, dtype, shift):
+    """`v` on the GPU, `shift` elements into a storage of NaN."""
+    room = torch.full((v.size + 64,), float("nan"), dtype=getattr(torch, dtype), device="cuda")
+    room[shift:shift + v.size] = cases.to_cuda(v, dtype).flatten()
+    return room[shift:shift + v.size].view(v.shape)
+
+
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+@pytest.mark.parametrize("n,t,c", [(2, 100, 65), (1, 9, 3), (1, 1500, 33), (3, 70, 130), (2, 64, 1)])
+def test_tensors_that_start_differently(n, t, c, dtype):
+    x, gate, dout, initial, dfinal = cases.recurrence_inputs(n, t, c, dtype, 23)
+    lengths = [t] * n
+    lens = lengths_on_gpu(lengths)
+    gx, gg, gd = (starting(v, dtype, s) for v, s in ((x, 1), (gate, 0), (dout, 5)))
+    gi, gf = (cases.to_cuda(v, "float32") for v in (initial, dfinal))
+    out = starting(np.zeros((n, t, c)), dtype, 3)
+    got = gated_linear_recurrence(gx, gg, lens, gi, out=out, return_states=True)
+    expected = oracle.gated_linear_recurrence(x, gate, lengths, initial)
+    bounds = cases.recurrence_bounds(x, gate, lengths, initial, expected, dtype)
+    for v, want, bound in zip(got, expected, bounds):
+        cases.assert_within(cases.host(v), want, bound)
+    grads = gated_linear_recurrence_backward(gd, gx, gg, lens, got[2], gf)
+    want = oracle.gated_linear_recurrence_backward(dout, x, gate, lengths, initial, dfinal)
+    bounds = cases.recurrence_gradient_bounds(dout, x, gate, lengths, initial, dfinal,
+                                              expected[0], want, dtype)
+    for v, e, bound in zip(grads, want, bounds):
+        cases.assert_within(cases.host(v), e, bound)
+
+
 @pytest.mark.parametrize("n,t,c", [(4, 60, 128), (1, 5000, 64), (3, 700, 65)])
 def test_streams_graphs_and_repeats_give_the_same_bits(n, t, c):
     x, gate, dout, initial, dfinal = cases.recurrence_inputs(n, t, c, "float16", 5)
