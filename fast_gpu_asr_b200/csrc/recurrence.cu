@@ -430,16 +430,25 @@ constexpr int kWarps = 8, kTile = kFrames * kWarps;
 constexpr int kForwardBlocks = 4, kBackwardBlocks = 3;  // on a multiprocessor
 static_assert(kTile == kChunk, "a tile starts at a saved state");
 
-// What the warps tell one another, two of each in turn, so that one barrier a tile is enough.
+// What the warps tell one another, two of each in turn, so that one barrier a tile is enough. It
+// starts a block's shared memory and ends with the last warp that the block has.
 template <typename V> struct Tile {
-    Run<V> run[2][kWarps][kWarp];
-    V back[2][kWarps][kWarp];  // B of the carry (backward)
-    V behind[2][kWarp];        // the state (forward) or carry (backward) after the tile
+    V behind[2][kWarp];  // the state (forward) or carry (backward) after the tile
+    struct Warp {
+        Run<V> run[2][kWarp];
+        V back[2][kWarp];  // B of the carry (backward)
+    } warp[kWarps];
+    static constexpr int bytes(int warps) {
+        return static_cast<int>(sizeof(behind) + warps * sizeof(Warp));
+    }
 };
 template <int kUnit> constexpr int kForwardStage = 2 * kRows<kUnit>;
 template <int kUnit> constexpr int kBackwardStage = 3 * kRows<kUnit>;
-template <typename V> constexpr int tile_smem(int stage) {
-    return 2 * kWarps * stage + static_cast<int>(sizeof(Tile<V>));
+// Shared memory of a walk: no more than its warps and tiles need, since a streaming step's blocks
+// are one warp each, and as many as a multiprocessor takes have to fit (20000 x 1 x 512 f16: 97
+// us, 422 with room for eight warps and two tiles; 256 x 16 x 1024: 7 and 11).
+template <typename V> constexpr int tile_smem(int stage, int warps, bool one_tile) {
+    return Tile<V>::bytes(warps) + (one_tile ? 1 : 2) * warps * stage;
 }
 
 // What the blocks before this one make of `v`, or (kBack) those behind it: each warp composes a
@@ -455,9 +464,9 @@ __device__ __forceinline__ V through_blocks(V v, const void* runs, Tile<V>& tile
 #pragma unroll 4
     for (int i = from; i < min(count, from + each); ++i)
         run.then(all[(kBack ? g.blocks - 1 - i : i) * kWarp]);
-    tile.run[1][at.warp][at.lane] = run;
+    tile.warp[at.warp].run[1][at.lane] = run;
     __syncthreads();
-    for (int w = 0; w < kWarps; ++w) v = tile.run[1][w][at.lane](v);
+    for (int w = 0; w < kWarps; ++w) v = tile.warp[w].run[1][at.lane](v);
     return v;
 }
 
@@ -468,11 +477,12 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
     using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
     constexpr int kStage = kForwardStage<kUnit>, kGate = kRows<kUnit>;
-    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kStage);
     Place<T> at(geo, f.lengths);
     const Source x = source_of(f.x, at, geo), gate = source_of(f.gate, at, geo);
     plan<kUnit>(at.rows, {x, gate}, at.lane);
-    char* stage = smem + at.warp * 2 * kStage;
+    const int buffers = geo.length > kTile ? 2 : 1;
+    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem);
+    char* stage = smem + Tile<V>::bytes(at.warps) + at.warp * buffers * kStage;
     const int last = at.warps - 1;
 
     auto fetch_tile = [&](int start, int which) {
@@ -510,12 +520,12 @@ __global__ void __launch_bounds__(kWarps* kWarp, kForwardBlocks)
             run[i].a = i == 0 ? keep : mul2(run[i - 1].a, keep);
             run[i].b = i == 0 ? add : fma2(keep, run[i - 1].b, add);
         }
-        tile.run[turn][at.warp][at.lane] = run[kFrames - 1];
+        tile.warp[at.warp].run[turn][at.lane] = run[kFrames - 1];
         __syncthreads();
         h = tile.behind[turn ^ 1][at.lane];
         if (f.states != nullptr && at.warp == 0)
             write_state(f.states + at.saved(geo, start / kChunk), h, at.present);
-        for (int w = 0; w < at.warp; ++w) h = tile.run[turn][w][at.lane](h);
+        for (int w = 0; w < at.warp; ++w) h = tile.warp[w].run[turn][at.lane](h);
         // The outputs take the place of x.
         V after;
 #pragma unroll
@@ -542,12 +552,13 @@ __global__ void __launch_bounds__(kWarps* kWarp, kUnit == 2 ? 2 : kBackwardBlock
     using V = typename L::Value;
     extern __shared__ __align__(16) char smem[];
     constexpr int kStage = kBackwardStage<kUnit>, kGate = kRows<kUnit>, kDout = 2 * kRows<kUnit>;
-    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem + 2 * kWarps * kStage);
     Place<T> at(geo, f.lengths);
     const Source x = source_of(f.x, at, geo), gate = source_of(f.gate, at, geo),
                  dout = source_of(f.dout, at, geo);
     plan<kUnit>(at.rows, {x, gate, dout}, at.lane);
-    char* stage = smem + at.warp * 2 * kStage;
+    const int buffers = geo.length > kTile ? 2 : 1;
+    Tile<V>& tile = *reinterpret_cast<Tile<V>*>(smem);
+    char* stage = smem + Tile<V>::bytes(at.warps) + at.warp * buffers * kStage;
     const int last = at.warps - 1;
 
     auto fetch_tile = [&](int start, int which) {
@@ -586,13 +597,13 @@ __global__ void __launch_bounds__(kWarps* kWarp, kUnit == 2 ? 2 : kBackwardBlock
             run.b = fma2(keep[i], run.b, mul2(take[i], value<T, kUnit>(rows, i, x, at)));
             back = fma2(run.a, value<T, kUnit>(rows + kDout, i, dout, at), back);
         }
-        tile.run[turn][at.warp][at.lane] = run;
-        tile.back[turn][at.warp][at.lane] = back;
+        tile.warp[at.warp].run[turn][at.lane] = run;
+        tile.warp[at.warp].back[turn][at.lane] = back;
         __syncthreads();
-        for (int w = 0; w < at.warp; ++w) h = tile.run[turn][w][at.lane](h);
+        for (int w = 0; w < at.warp; ++w) h = tile.warp[w].run[turn][at.lane](h);
         carry = tile.behind[turn ^ 1][at.lane];
         for (int w = last; w > at.warp; --w)
-            carry = fma2(tile.run[turn][w][at.lane].a, carry, tile.back[turn][w][at.lane]);
+            carry = fma2(tile.warp[w].run[turn][at.lane].a, carry, tile.warp[w].back[turn][at.lane]);
         V away[kFrames];  // h[t-1] - x[t]
 #pragma unroll
         for (int i = 0; i < kFrames; ++i) {
@@ -730,8 +741,8 @@ Shape shape_of(int batch, int length, int channels, int chunks, int element, int
 
 template <typename... Params, typename... Args>
 cudaError_t launch(SmemAttr& attribute, void (*kernel)(Params...), const Shape& s, int smem,
-                   bool early, cudaStream_t stream, Args... args) {
-    const cudaError_t e = attribute.ensure(reinterpret_cast<const void*>(kernel), smem);
+                   int most_smem, bool early, cudaStream_t stream, Args... args) {
+    const cudaError_t e = attribute.ensure(reinterpret_cast<const void*>(kernel), most_smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(s.units * s.geo.blocks));
@@ -775,12 +786,14 @@ template <typename T, int kUnit> cudaError_t forward(const RecurrenceProblem& p,
         f.runs = p.workspace;
         f.first = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + shape.runs_bytes);
         const cudaError_t e =
-            launch(runs, recurrence_runs_kernel<T, kUnit, false>, shape, runs_smem<V, kUnit>(), false, s,
-                   f.x, f.gate, f.lengths, f.initial, f.runs, f.first, shape.geo);
+            launch(runs, recurrence_runs_kernel<T, kUnit, false>, shape, runs_smem<V, kUnit>(),
+                   runs_smem<V, kUnit>(), false, s, f.x, f.gate, f.lengths, f.initial, f.runs, f.first, shape.geo);
         if (e != cudaSuccess) return e;
     }
-    return launch(walk, recurrence_kernel<T, kUnit>, shape, tile_smem<V>(kForwardStage<kUnit>), divided, s,
-                  f, shape.geo);
+    constexpr int kStage = kForwardStage<kUnit>;
+    return launch(walk, recurrence_kernel<T, kUnit>, shape,
+                  tile_smem<V>(kStage, shape.warps, p.length <= kTile),
+                  tile_smem<V>(kStage, kWarps, false), divided, s, f, shape.geo);
 }
 
 template <typename T, int kUnit>
@@ -796,13 +809,15 @@ cudaError_t backward(const RecurrenceBackwardProblem& p, cudaStream_t s) {
                         divided ? p.workspace : nullptr};
     if (divided) {
         const cudaError_t e =
-            launch(runs, recurrence_runs_kernel<T, kUnit, true>, shape, runs_smem<V, kUnit>(), false, s,
-                   f.dout, f.gate, f.lengths, static_cast<const float*>(nullptr), f.runs,
+            launch(runs, recurrence_runs_kernel<T, kUnit, true>, shape, runs_smem<V, kUnit>(),
+                   runs_smem<V, kUnit>(), false, s, f.dout, f.gate, f.lengths, static_cast<const float*>(nullptr), f.runs,
                    static_cast<float*>(nullptr), shape.geo);
         if (e != cudaSuccess) return e;
     }
-    return launch(walk, recurrence_backward_kernel<T, kUnit>, shape, tile_smem<V>(kBackwardStage<kUnit>),
-                  divided, s, f, shape.geo);
+    constexpr int kStage = kBackwardStage<kUnit>;
+    return launch(walk, recurrence_backward_kernel<T, kUnit>, shape,
+                  tile_smem<V>(kStage, shape.warps, p.length <= kTile),
+                  tile_smem<V>(kStage, kWarps, false), divided, s, f, shape.geo);
 }
 
 template <typename T> cudaError_t forward(const RecurrenceProblem& p, cudaStream_t s) {
