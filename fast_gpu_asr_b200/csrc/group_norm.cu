@@ -18,6 +18,8 @@
 // the way of the rest are instruction issue (56 % busy, 32 instructions a pair of values) and
 // that a block loads, reduces and stores in turn; four on a multiprocessor cover for one another,
 // which is what 48 KB of tile and 64 registers are chosen for.
+#include <type_traits>
+
 #include "fga_kernels.h"
 #include "group_norm.cuh"
 
@@ -127,6 +129,16 @@ template <typename T, bool kWhole> struct Column {
         weight = load<T, kAligned>(w + p.channel(), p.count);
         bias = load<T, kAligned>(b + p.channel(), p.count);
     }
+    // Whether a bias is too far out for its shift (none of fp16 is, but infinities, which stay).
+    __device__ __forceinline__ bool far(int act) const {
+        if (std::is_same_v<T, __half> || act == FGA_ACTIVATION_NONE) return false;
+        float2 v[kPairs<T>];
+        unpack<T>(bias, v);
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPairs<T>; ++i) most = fmaxf(most, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+        return most >= kFarBias;
+    }
     // `stats`: (mean, rstd) of the slab's groups.
     __device__ __forceinline__ void make(const float2* stats, const Place<T>& p, const Geometry& g,
                                          int act) {
@@ -166,6 +178,35 @@ template <typename T> struct Tensors {
     float* mean;  // [N, G] or null
     float* rstd;
 };
+
+// This thread's values where a bias is too far out for its shift, from the formulas in z itself.
+// It stands in place of the rows' loop and finds its place anew, from an index and a thread that
+// the compiler cannot know to be the same, so that nothing is kept for it through the kernel (256
+// x 375 x 1024 bf16 ragged, silu, without such a bias: 57.7 us, 57.9 without this branch, 59.7
+// with the values put right after the loop). `stats`: (mean, rstd) of the slab's groups; `index`
+// as for Place.
+template <typename T>
+__device__ __forceinline__ void far_biases(const Tensors<T>& t, const Geometry& g,
+                                           const float2* stats, int index, int act) {
+    int thread = threadIdx.x;
+    asm volatile("" : "+r"(index), "+r"(thread));
+    const Place<T> p = Place<T>::make(g, t.lengths, index, thread);
+#pragma unroll 1
+    for (int e = 0; e < p.count; ++e) {
+        const int c = p.channel() + e;
+        const float bias = to_f32<T>(t.bias[c]), weight = to_f32<T>(t.weight[c]);
+        const float2 s = stats[p.group_of(e, g)];
+#pragma unroll 1
+        for (int i = 0; i < p.own_rows(); ++i) {
+            const int64_t at = p.at(g, p.begin + p.row + i * g.step) + e;
+            const float z = fmaf((to_f32<T>(t.x[at]) - s.x) * s.y, weight, bias), v = z - 1.0f;
+            const float y = act == FGA_ACTIVATION_SILU
+                                ? z / (1.0f + expf(-z))
+                                : fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))) - 0.08f * z - 0.313261687f;
+            t.out[at] = from_f32<T>(y);
+        }
+    }
+}
 
 template <typename T, bool kAligned, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 4)
@@ -224,11 +265,15 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     __syncthreads();
     if (mine > 0) {
-        column.make(moments, p, g, act);
-        T* to = t.out + p.at(g, p.begin + p.row);
+        if (column.far(act)) {
+            far_biases(t, g, moments, blockIdx.x, act);
+        } else {
+            column.make(moments, p, g, act);
+            T* to = t.out + p.at(g, p.begin + p.row);
 #pragma unroll 2
-        for (int i = 0; i < mine; ++i, to += stride)
-            store<T, kAligned>(to, column.apply(at[i * pitch], act), p.count);
+            for (int i = 0; i < mine; ++i, to += stride)
+                store<T, kAligned>(to, column.apply(at[i * pitch], act), p.count);
+        }
     }
     zero_padding<T, kAligned>(t.out, p, g);
 }
@@ -320,12 +365,17 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
     __syncthreads();
     if (mine > 0) {
-        column.make(stats, p, g, act);
-        T* to = t.out + from;
-        rows.each([&](const uint4(&v)[1]) {
-            store<T, kAligned>(to, column.apply(v[0], act), p.count);
-            to += stride;
-        });
+        if (column.far(act)) {
+            arrived();
+            far_biases(t, g, stats, gridDim.x - 1 - blockIdx.x, act);
+        } else {
+            column.make(stats, p, g, act);
+            T* to = t.out + from;
+            rows.each([&](const uint4(&v)[1]) {
+                store<T, kAligned>(to, column.apply(v[0], act), p.count);
+                to += stride;
+            });
+        }
     }
     zero_padding<T, kAligned>(t.out, p, g);
 }

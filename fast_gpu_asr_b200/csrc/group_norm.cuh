@@ -167,13 +167,11 @@ __device__ __forceinline__ float unit_of(int act) {
 __device__ __forceinline__ float origin_of(int act) {
     return act == FGA_ACTIVATION_SWOOSH_R ? 1.0f : 0.0f;
 }
-// A column's shift from its bias. Next to the largest number a bias would leave fp32 in the
-// exponent's units, and silu of the lowest be inf * 0: it stops short of that.
+// A column's shift from its bias, which has to be below kFarBias for it to stay within fp32 in the
+// exponent's units.
+constexpr float kFarBias = 1.5e38f;
 __device__ __forceinline__ float2 shift_of(float2 bias, int act) {
-    if (act == FGA_ACTIVATION_NONE) return bias;
-    constexpr float kMost = 2.3e38f;
-    const float2 s = mul2(add2(bias, splat2(-origin_of(act))), splat2(unit_of(act)));
-    return make_float2(fminf(fmaxf(s.x, -kMost), kMost), fminf(fmaxf(s.y, -kMost), kMost));
+    return mul2(add2(bias, splat2(-origin_of(act))), splat2(unit_of(act)));
 }
 __device__ __forceinline__ float2 exp2_of(float2 y) {
     return make_float2(exp2_approx(y.x), exp2_approx(y.y));
@@ -261,7 +259,8 @@ template <typename T> struct Place {
     int passes, extra;            // rows of a thread: passes, and one more in the first `extra`
 
     // `index`: of the block in the launch, or against it.
-    __device__ static Place make(const Geometry& g, const int32_t* lengths, int index) {
+    __device__ static Place make(const Geometry& g, const int32_t* lengths, int index,
+                                 int thread = threadIdx.x) {
         Place p;
         const int unit = g.by_blocks.quotient(index);
         p.block = index - unit * g.blocks;
@@ -281,8 +280,8 @@ template <typename T> struct Place {
             p.width = g.group_channels;
             p.channels = p.groups * p.width;
         }
-        p.row = g.by_lanes.quotient(threadIdx.x);
-        p.lane = threadIdx.x - p.row * g.lanes;
+        p.row = g.by_lanes.quotient(thread);
+        p.lane = thread - p.row * g.lanes;
         p.count = p.row < g.step ? min(kVec<T>, p.channels - p.lane * kVec<T>) : 0;
         p.each = g.by_blocks.quotient(p.m + g.blocks - 1);
         p.begin = min(p.m, p.block * p.each);

@@ -53,6 +53,16 @@ template <typename T> struct Tensors {
     T* dx;
 };
 
+// A column's shift, which stops short of where it would leave fp32: the slopes there are what they
+// are further on, and silu's would be inf * 0. Infinities and NaN stay what they are.
+__device__ __forceinline__ float2 bounded_shift_of(float2 bias, int act) {
+    constexpr float kMost = 2.3e38f;
+    const float2 s = shift_of(bias, act);
+    if (act == FGA_ACTIVATION_NONE) return s;
+    return make_float2(isfinite(bias.x) ? fminf(fmaxf(s.x, -kMost), kMost) : s.x,
+                       isfinite(bias.y) ? fminf(fmaxf(s.y, -kMost), kMost) : s.y);
+}
+
 // A column's parameters: d = x - mean, z = d scale + shift (both in the activation's units), xhat
 // = d rstd. What `through` makes of dout is dz / unit: the sums make up for it at their end, dx
 // in its product with scale.
@@ -75,7 +85,7 @@ template <typename T, bool kWhole> struct Column {
         }
 #pragma unroll
         for (int e = 0; e < kPairs<T>; ++e) {
-            shift[e] = shift_of(shift[e], act);
+            shift[e] = bounded_shift_of(shift[e], act);
             scale[e] = mul2(mul2(scale[e], unit), rstd[kWhole ? 0 : e]);
         }
     }

@@ -106,7 +106,9 @@ enum fga_activation {
  * Over the valid frames of an utterance and the C/G channels of a group: mean, biased
  * variance, rstd = (variance + eps)^-1/2; out = act((x - mean) rstd weight + bias). An
  * utterance without valid frames has mean 0 and variance 0. num_groups divides C; eps is
- * finite and > 0.
+ * finite and > 0. Biases may be any number; an infinite or NaN bias and a NaN weight show as
+ * the formulas have it. |weight| rstd and |weight (x - mean) rstd| from 2^126 count as
+ * infinite.
  * -------------------------------------------------------------------------------- */
 FGA_API int32_t fga_group_norm_activation_check(const fga_tensor_desc* input_descs,
     int32_t nb_inputs, const fga_tensor_desc* output_descs, int32_t nb_outputs,
