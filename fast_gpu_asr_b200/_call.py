@@ -98,6 +98,9 @@ class Operator:
             return self._launch(tensors, given, allocate, absent, fields, size_fields, workspace,
                                 device, _current_stream(device))
         stream = _torch_stream(stream)
+        if stream.device.index != device:
+            # torch would make that device the current one for the launch.
+            raise ValueError(f"stream is on {stream.device}, the current device is cuda:{device}")
         with torch.cuda.stream(stream):
             return self._launch(tensors, given, allocate, absent, fields, size_fields, workspace,
                                 device, stream.cuda_stream)

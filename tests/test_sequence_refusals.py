@@ -1,0 +1,37 @@
+"""Calls that the sequence operators refuse before anything is launched, without a device: torch's
+view of the current device and stream is replaced."""
+
+from __future__ import annotations
+
+import types
+
+import pytest
+import torch
+
+from fast_gpu_asr_b200 import (_call, gated_linear_recurrence, gated_linear_recurrence_backward,
+                               group_norm_activation, group_norm_activation_backward)
+
+
+def calls(x, **options):
+    """Each operator on tensors shaped after ``x`` [N, T, C]."""
+    n, t, c = x.shape
+    lens, w = torch.zeros(n, dtype=torch.int32), x.new_ones(c)
+    stats, states = torch.zeros(n, 1), torch.zeros(n, -(-t // 64), c)
+    return (lambda: group_norm_activation(x, lens, w, w, 1, **options),
+            lambda: group_norm_activation_backward(x, x, lens, w, w, stats, stats, **options),
+            lambda: gated_linear_recurrence(x, x, lens, **options),
+            lambda: gated_linear_recurrence_backward(x, x, x, lens, states, **options))
+
+
+def test_a_stream_of_another_device(monkeypatch):
+    """It would make its device the current one, and the kernels read the tensors from there."""
+    def entered(stream):
+        raise AssertionError("the stream's device was made the current one")
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "stream", entered)
+    monkeypatch.setattr(_call, "_torch_stream", lambda s: s)
+    stream = types.SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=0)
+    for call in calls(torch.zeros(2, 3, 4), stream=stream):
+        with pytest.raises(ValueError, match="stream is on cuda:1, the current device is cuda:0"):
+            call()
