@@ -13,6 +13,7 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .attention import _check, _torch_stream, dtype_code
@@ -36,10 +37,22 @@ def require(name: str, t, rank: int) -> None:
                                   f"{name} of rank {t.dim()}")
 
 
+def _dual() -> bool:
+    """Whether tensors may carry forward-mode tangents."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def _has_tangent(t) -> bool:
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
 def _refuse(name: str, t, device: int, grad: bool) -> None:
     """Why a binding cannot be launched on."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor (got {type(t).__name__})")
+    if _dual() and _has_tangent(t):
+        raise ValueError(f"{name} carries a forward-mode tangent, which this operator would lose: "
+                         "call it on forward_ad.unpack_dual(...).primal")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (got {t.device})")
     if t.get_device() != device:
@@ -107,7 +120,7 @@ class Operator:
 
     def _launch(self, tensors, given, allocate, absent, fields, size_fields, workspace, device,
                 handle):
-        grad = torch.is_grad_enabled()
+        grad, dual = torch.is_grad_enabled(), _dual()
         key, sources, i = [device, size_fields], [], 0
         for t in tensors:
             if t is None:
@@ -115,7 +128,8 @@ class Operator:
                 key.append(None)
             else:
                 if (not isinstance(t, torch.Tensor) or t.get_device() != device
-                        or not t.is_contiguous() or (grad and t.requires_grad)):
+                        or not t.is_contiguous() or (grad and t.requires_grad)
+                        or (dual and _has_tangent(t))):
                     _refuse(self.inputs[i], t, device, grad)
                 sources.append(t.data_ptr())
                 key.append(t.dtype)
@@ -127,7 +141,8 @@ class Operator:
                 key.append(None)
             else:
                 if (not isinstance(t, torch.Tensor) or t.get_device() != device
-                        or not t.is_contiguous() or (grad and t.requires_grad)):
+                        or not t.is_contiguous() or (grad and t.requires_grad)
+                        or (dual and _has_tangent(t))):
                     _refuse(self.outputs[i], t, device, grad)
                 key.append(t.dtype)
                 key.append(t.shape)

@@ -10,7 +10,7 @@ and gradients cover the valid frames, padded frames are not read, and padded fra
 ``out`` and ``grad_x`` are zeros. All arithmetic is fp32, with one rounding at the store.
 
 The operators record no autograd graph: a call on tensors that require grad is refused while
-grad mode is on. The two functions are the halves of a ``torch.autograd.Function``.
+grad mode is on, and one on tensors that carry forward-mode tangents. The two functions are the halves of a ``torch.autograd.Function``.
 
 Tensors must be contiguous and live on the current CUDA device. Work is enqueued on
 ``stream`` (default: torch's current stream), outputs and workspace are allocated on it, and

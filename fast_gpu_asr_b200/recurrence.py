@@ -12,7 +12,7 @@ to ``[0, T]``: padded frames are not read and leave the state as it is, and padd
 the outputs are zeros. No reference plugin.
 
 The operators record no autograd graph: a call on tensors that require grad is refused while
-grad mode is on. The two functions are the halves of a ``torch.autograd.Function``.
+grad mode is on, and one on tensors that carry forward-mode tangents. The two functions are the halves of a ``torch.autograd.Function``.
 
 Tensors must be contiguous and live on the current CUDA device. Work is enqueued on
 ``stream`` (default: torch's current stream), outputs and workspace are allocated on it, and

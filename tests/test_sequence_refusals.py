@@ -7,6 +7,7 @@ import types
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from fast_gpu_asr_b200 import (_call, gated_linear_recurrence, gated_linear_recurrence_backward,
                                group_norm_activation, group_norm_activation_backward)
@@ -35,3 +36,27 @@ def test_a_stream_of_another_device(monkeypatch):
     for call in calls(torch.zeros(2, 3, 4), stream=stream):
         with pytest.raises(ValueError, match="stream is on cuda:1, the current device is cuda:0"):
             call()
+
+
+def test_forward_mode_tangents(monkeypatch):
+    """They would be lost. (A tensor on the CPU is on device -1, which stands for the current one
+    here; nothing is launched.)"""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(_call, "_current_stream", lambda device: 0)
+
+    def launched(self, *args):
+        raise AssertionError("the call went on to its launch")
+
+    monkeypatch.setattr(_call.Operator, "_plan", launched)
+    x = torch.zeros(2, 3, 4)
+    with forward_ad.dual_level():
+        for call in calls(forward_ad.make_dual(x, torch.ones_like(x))):
+            with pytest.raises(ValueError, match="carries a forward-mode tangent"):
+                call()
+        with torch.no_grad():
+            for call in calls(forward_ad.make_dual(x, torch.ones_like(x))):
+                with pytest.raises(ValueError, match="carries a forward-mode tangent"):
+                    call()
+        for call in calls(x):
+            with pytest.raises(AssertionError, match="went on"):
+                call()
