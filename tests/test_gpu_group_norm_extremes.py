@@ -18,7 +18,7 @@ ACTIVATIONS = ("none", "silu", "swoosh_r")
 # Vectors of one group, of several, rows that start anywhere, clusters, streams of both kinds, a
 # group wider than a block.
 SHAPES = [(2, 40, 48, 6), (2, 29, 30, 2), (3, 33, 35, 5), (2, 700, 256, 2), (1, 12000, 40, 5),
-          (1, 9000, 67, 1), (1, 300, 4104, 1)]
+          (1, 9000, 67, 1), (1, 300, 4104, 1), (1, 17000, 24, 2)]
 
 
 def inputs(n, t, c, dtype, seed):
