@@ -257,23 +257,24 @@ template <typename T> __device__ __forceinline__ int channel_at(const Geometry& 
 }
 
 // Adds the rows of column sums, in an order that the launch fixes: kSumColumns columns a block, a
-// thread every kSumRows-th row of one of them.
+// thread every kSumRows-th row of one of them. (Unsigned: there may be INT32_MAX rows, and the
+// last step goes past them.)
 constexpr int kSumColumns = 8, kSumRows = kThreads / kSumColumns;
 template <typename T>
 __device__ __forceinline__ void sum_parameters(const float2* sums, T* __restrict__ dweight,
-                                               T* __restrict__ dbias, int rows, const Geometry& g,
-                                               int block, float2* part) {
-    const int row = threadIdx.x / kSumColumns;
+                                               T* __restrict__ dbias, uint32_t rows,
+                                               const Geometry& g, int block, float2* part) {
+    const uint32_t row = threadIdx.x / kSumColumns;
     const int i = block * kSumColumns + threadIdx.x % kSumColumns;
     const int64_t pitch = sum_pitch<T>(g);
     float2 s = splat2(0.0f);
     if (i < pitch) {
 #pragma unroll 8
-        for (int r = row; r < rows; r += kSumRows) s = add2(s, sums[r * pitch + i]);
+        for (uint32_t r = row; r < rows; r += kSumRows) s = add2(s, sums[r * pitch + i]);
     }
     part[threadIdx.x] = s;
 #pragma unroll
-    for (int half = kSumRows / 2; half > 0; half /= 2) {
+    for (uint32_t half = kSumRows / 2; half > 0; half /= 2) {
         __syncthreads();
         if (row < half) {
             s = add2(s, part[threadIdx.x + half * kSumColumns]);
@@ -301,7 +302,7 @@ template <typename T> struct Parameters {
     const float2* sums;
     T* dweight;
     T* dbias;
-    int rows;
+    uint32_t rows;
 };
 
 // `sums`: a row of column sums for each block of each utterance.
@@ -542,7 +543,7 @@ cudaError_t run(const GroupNormBackwardProblem& p, const Shape& s, cudaStream_t 
     const int part = static_cast<int>(sizeof(float2)) *
                      std::max(sum_values<T, kWhole>(g), s.split ? 0 : g.blocks * g.slab_groups);
     const Parameters<T> out{sums, static_cast<T*>(p.grad_weight), static_cast<T*>(p.grad_bias),
-                            static_cast<int>(rows)};
+                            static_cast<uint32_t>(rows)};
     const int adders = static_cast<int>((sum_pitch<T>(g) + kSumColumns - 1) / kSumColumns);
     const int64_t blocks = s.units * g.blocks;
     cudaError_t e;

@@ -9,8 +9,9 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from fast_gpu_asr_b200 import (_call, gated_linear_recurrence, gated_linear_recurrence_backward,
-                               group_norm_activation, group_norm_activation_backward)
+from fast_gpu_asr_b200 import (_call, _lib, gated_linear_recurrence, gated_linear_recurrence_backward,
+                               group_norm_activation, group_norm_activation_backward,
+                               normalization, recurrence)
 
 
 def calls(x, **options):
@@ -60,3 +61,22 @@ def test_forward_mode_tangents(monkeypatch):
         for call in calls(x):
             with pytest.raises(AssertionError, match="went on"):
                 call()
+
+
+@pytest.mark.parametrize("n,t", [(2 ** 31 - 1, 1), (2, 2 ** 30 - 1), (1, 2 ** 30)])
+def test_the_most_frames_of_a_batch(library, n, t):
+    """The kernels' loops over frames, utterances and blocks take what the checks let through: all
+    their counts are below 2^31 and a step past the last one below 2^32."""
+    d, F32 = _lib.TensorDesc.make, _lib.FGA_FLOAT
+    w = d(F32, (1,))
+    for n, status in ((n, 0), (2 ** 31 // t + 1, 4)):
+        a, lens, stats = d(F32, (n, t, 1)), d(_lib.FGA_INT32, (n,)), d(F32, (n, 1))
+        states = d(F32, (n, -(-t // 64), 1))
+        assert normalization.group_norm_activation_check(
+            [a, lens, w, w], [a, stats, stats], 1, 1e-5, "silu") == status
+        assert normalization.group_norm_activation_backward_check(
+            [a, a, lens, w, w, stats, stats], [a, w, w], "silu") == status
+        assert recurrence.gated_linear_recurrence_check(
+            [a, a, lens, stats], [a, stats, states]) == status
+        assert recurrence.gated_linear_recurrence_backward_check(
+            [a, a, a, lens, states, stats], [a, a, stats]) == status
