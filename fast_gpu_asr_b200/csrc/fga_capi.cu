@@ -339,7 +339,8 @@ int32_t check_bindings(const Binding* b, int count, int32_t type) {
 // The kernels count frames and channels of the whole batch in 32 bits, frames a tile past
 // the last one, and the bytes of some thousand rows.
 bool rows_in_range(const fga_tensor_desc& x) {
-    return x.dims[1] <= (1 << 30) && x.dims[2] <= (1 << 18) && x.dims[0] <= kInt32Max / x.dims[1] && x.dims[0] <= kInt32Max / x.dims[2];
+    return x.dims[1] <= (1 << 30) && x.dims[2] <= (1 << 18) &&
+           x.dims[0] <= kInt32Max / x.dims[1] && x.dims[0] <= kInt32Max / x.dims[2];
 }
 
 bool activation_ok(int32_t a) {

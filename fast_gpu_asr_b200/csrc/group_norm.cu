@@ -7,11 +7,12 @@
 // The rows of an utterance's slab stay on chip between the statistics and the output: a block
 // keeps them in shared memory, a cluster of up to 16 blocks where one is not enough. Every
 // thread reads only vectors that it copied itself, so the tile needs no barrier. A thread
-// takes the mean and the sum of squares about it over its own values, and pairs of (mean,
-// squares) merge exactly as the two-pass formula would have it:
-//   mean = sum n_i mean_i / sum n_i, squares = sum (squares_i + n_i (mean_i - mean)^2);
-// no difference of large sums is taken. What no cluster holds is done in two launches, the
-// first of which leaves each block's (mean, squares) in the workspace.
+// takes the mean and the sum of squares about it over its own values, in one pass about a pivot
+// (block_moments says what that costs in rounding), and pairs of (mean, squares) merge exactly
+// as the two-pass formula would have it:
+//   mean = sum n_i mean_i / sum n_i, squares = sum (squares_i + n_i (mean_i - mean)^2),
+// without a difference of large sums. What no cluster holds is done in two launches, the first
+// of which leaves each block's (mean, squares) in the workspace.
 //
 // So x is read once and out written once: 256 x 375 x 1024 f16 ragged, 32 groups, SiLU, takes
 // 59 us, 81 % of a plain copy's rate for those bytes (fp32, 64 x 375 x 1024: 29.4 us, 81 %). In
@@ -52,9 +53,10 @@ template <typename Visit> __device__ __forceinline__ float2 merge(float total, V
 // A thread takes both in one pass, about a pivot: the mean of its own first vector (the first
 // value of each channel). With n values and the first q of them in the pivot, squares about
 // the mean are at least q (pivot - mean)^2, so the n (pivot - mean)^2 taken off the squares
-// about the pivot is at most n / q times what is left, a factor on its rounding error: with 12
-// rows of a tile or 64 of a stream at most, and values that differ like that only where the
-// first vector is an outlier itself.
+// about the pivot is at most n / q times what is left, a factor on its rounding error. n / q is
+// the thread's rows: 12 of a tile where all threads work, 23 at most (129 vectors a row leave
+// 127 of the 256 threads idle), 64 of a stream; and it takes a first vector that is an outlier
+// itself for the factor to be near that.
 template <typename T, bool kWhole, typename Each>
 __device__ __forceinline__ void block_moments(const uint4& first, Each each, float2* part,
                                               float2* moments, const Place<T>& p,
@@ -202,7 +204,8 @@ __device__ __forceinline__ void far_biases(const Tensors<T>& t, const Geometry& 
             const float z = fmaf((to_f32<T>(t.x[at]) - s.x) * s.y, weight, bias), v = z - 1.0f;
             const float y = act == FGA_ACTIVATION_SILU
                                 ? z / (1.0f + expf(-z))
-                                : fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))) - 0.08f * z - 0.313261687f;
+                                : fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))) - 0.08f * z -
+                                      0.313261687f;
             t.out[at] = from_f32<T>(y);
         }
     }

@@ -10,10 +10,12 @@
 // each block, whose rows are added up in an order that the launch fixes.
 //
 // Two ways, chosen by size (shape_of):
-// - Rows on chip: a block keeps its rows of x, and dz in fp32 in the place of dout (which takes
-//   48 bytes for 8 values of a 16-bit type, but evaluating the slope twice would make the kernel
-//   bound by instructions), so x and dout are read once; a cluster adds up (s1, s2) where one
-//   block cannot hold an utterance's slab. A second launch adds the parameters' gradients.
+// - Rows on chip: a block keeps its rows of x, and dz in fp32 in the place of dout, so x and dout
+//   are read once and the slope is evaluated once; that takes 48 bytes for 8 values of a 16-bit
+//   type. (32, with dout as it came and the slope evaluated again as the streams do, would let
+//   one block hold half as much again; it has not been measured.) A cluster adds up (s1, s2)
+//   where one block cannot hold an utterance's slab. A second launch adds the parameters'
+//   gradients.
 // - Streams: one launch for the sums, and one for dx and the parameters' gradients, which
 //   evaluates the slope again. It reads x and dout twice, but none of its blocks waits for
 //   another or holds 72 KB while it does.
@@ -514,7 +516,9 @@ __global__ void __launch_bounds__(kThreads)
 // wins for small batches (x and dout of 18 MB bf16: 13.9 us against 17.5 in two streams) and in
 // fp32, whose streams move twice the bytes for each slope they evaluate again (64 x 375 x 1024:
 // 73 us against 87); larger ones of 16 bits stream (256 x 750 x 192 bf16 ragged: 52 against 65),
-// and in fp32 those whose rows start anywhere (64 x 375 x 1001: 92 against 163).
+// and in fp32 those whose rows start anywhere (64 x 375 x 1001: 92 against 163). Between the 18
+// and the 147 MB that were measured in 16 bits the switch is a guess, and it goes by the padded
+// batch, since the host does not know the lengths.
 constexpr int64_t kClusterBytes = 64 << 20;
 Shape shape_of(const GroupNormBackwardProblem& p, bool aligned) {
     const int element = p.dtype == FGA_FLOAT ? 4 : 2;

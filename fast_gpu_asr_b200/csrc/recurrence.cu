@@ -74,8 +74,12 @@ template <> struct Lane<float> {
     static constexpr uint32_t kInfinity = 0x7f800000u;
 };
 
-// f and p = 1 - f, both with all their bits: e = exp(-gate), f = 1 / (1 + e), p = e f. The
-// exponent stops at 126, where f is the smallest normal number and p is 1; a NaN stays one.
+// f and p = 1 - f: e = exp(-gate), f = 1 / (1 + e), p = e f, so that neither is a difference of
+// numbers next to 1. What is off is e: the product with log2 e rounds, which makes e, and with it
+// the smaller of f and p, relatively off by up to |gate| 2^-24, besides some steps of the
+// exponential and the reciprocal. That is 6 bits of an fp32 p at |gate| = 60, and nothing that
+// 16 bits show. The exponent stops at 126, where f is the smallest normal number and p is 1; a
+// NaN stays one.
 __device__ __forceinline__ float stop(float exponent) {
     float e;
     asm("min.NaN.f32 %0, %1, 0f42fc0000;" : "=f"(e) : "f"(exponent));
@@ -787,7 +791,8 @@ template <typename T, int kUnit> cudaError_t forward(const RecurrenceProblem& p,
         f.first = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + shape.runs_bytes);
         const cudaError_t e =
             launch(runs, recurrence_runs_kernel<T, kUnit, false>, shape, runs_smem<V, kUnit>(),
-                   runs_smem<V, kUnit>(), false, s, f.x, f.gate, f.lengths, f.initial, f.runs, f.first, shape.geo);
+                   runs_smem<V, kUnit>(), false, s, f.x, f.gate, f.lengths, f.initial, f.runs,
+                   f.first, shape.geo);
         if (e != cudaSuccess) return e;
     }
     constexpr int kStage = kForwardStage<kUnit>;
@@ -810,8 +815,9 @@ cudaError_t backward(const RecurrenceBackwardProblem& p, cudaStream_t s) {
     if (divided) {
         const cudaError_t e =
             launch(runs, recurrence_runs_kernel<T, kUnit, true>, shape, runs_smem<V, kUnit>(),
-                   runs_smem<V, kUnit>(), false, s, f.dout, f.gate, f.lengths, static_cast<const float*>(nullptr), f.runs,
-                   static_cast<float*>(nullptr), shape.geo);
+                   runs_smem<V, kUnit>(), false, s, f.dout, f.gate, f.lengths,
+                   static_cast<const float*>(nullptr), f.runs, static_cast<float*>(nullptr),
+                   shape.geo);
         if (e != cudaSuccess) return e;
     }
     constexpr int kStage = kBackwardStage<kUnit>;

@@ -6,11 +6,12 @@ because its statistics come from the utterance itself: group norm, and with one 
 channel per group the layer and instance forms over time. No reference plugin.
 
 ``valid_lengths`` is int32 ``[N]`` as in the convolutions, clamped to ``[0, T]``: statistics
-and gradients cover the valid frames, padded frames are not read, and padded frames of
-``out`` and ``grad_x`` are zeros. All arithmetic is fp32, with one rounding at the store.
+and gradients cover the valid frames, what padded frames hold is not used, and padded frames
+of ``out`` and ``grad_x`` are zeros. All arithmetic is fp32, with one rounding at the store.
 
 The operators record no autograd graph: a call on tensors that require grad is refused while
-grad mode is on, and one on tensors that carry forward-mode tangents. The two functions are the halves of a ``torch.autograd.Function``.
+grad mode is on, and one on tensors that carry forward-mode tangents. The two functions are
+the halves of a ``torch.autograd.Function``.
 
 Tensors must be contiguous and live on the current CUDA device. Work is enqueued on
 ``stream`` (default: torch's current stream), outputs and workspace are allocated on it, and

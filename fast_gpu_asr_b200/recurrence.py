@@ -8,11 +8,12 @@ value per channel::
 
 The state is float32 and passes from call to call, so a recording may be cut anywhere; ``T =
 1`` is the streaming step. ``valid_lengths`` is int32 ``[N]`` as in the convolutions, clamped
-to ``[0, T]``: padded frames are not read and leave the state as it is, and padded frames of
-the outputs are zeros. No reference plugin.
+to ``[0, T]``: what padded frames hold is not used, they leave the state as it is, and padded
+frames of the outputs are zeros. No reference plugin.
 
 The operators record no autograd graph: a call on tensors that require grad is refused while
-grad mode is on, and one on tensors that carry forward-mode tangents. The two functions are the halves of a ``torch.autograd.Function``.
+grad mode is on, and one on tensors that carry forward-mode tangents. The two functions are
+the halves of a ``torch.autograd.Function``.
 
 Tensors must be contiguous and live on the current CUDA device. Work is enqueued on
 ``stream`` (default: torch's current stream), outputs and workspace are allocated on it, and

@@ -71,8 +71,8 @@ FGA_API int32_t fga_zipformer_convolution_enqueue(const fga_tensor_desc* input_d
  * Group norm with activation, and the gated linear recurrence: no reference plugin.
  *
  * Both work on [N, T, C] activations with the convolutions' valid_lengths (clamped to
- * [0, T]): padded frames are never read, and every output's padded frames are written as
- * zeros. Conventions that all four entry points share:
+ * [0, T]): what padded frames hold is never used (a word of memory that one shares with a
+ * valid frame may be read), and every output's padded frames are written as zeros. Conventions that all four entry points share:
  * - "type" is f32, f16 or bf16; arithmetic, statistics, sums and states are fp32, each
  *   output is rounded once.
  * - T is at most 2^30, C at most 2^18, N*T and N*C at most INT32_MAX (N*T*C may be
@@ -162,7 +162,8 @@ FGA_API int32_t fga_group_norm_activation_backward_enqueue(const fga_tensor_desc
  * f = sigmoid(gate), h[t] = f[t] h[t-1] + (1 - f[t]) x[t], h[-1] = initial_state;
  * out[t] = h[t] on valid frames; final_state is h after the last of them (initial_state
  * when there is none). states[n, j] is h before frame 64 j where that frame is valid, else
- * zero. T = 1 is the streaming step.
+ * zero. T = 1 is the streaming step. f is at least 2^-126, which gates below -87.3 reach; the
+ * smaller of f and 1 - f is relatively off by up to |gate| 2^-24 on top of some roundings.
  * -------------------------------------------------------------------------------- */
 FGA_API int32_t fga_gated_linear_recurrence_check(const fga_tensor_desc* input_descs,
     int32_t nb_inputs, const fga_tensor_desc* output_descs, int32_t nb_outputs);
