@@ -168,7 +168,7 @@ __device__ __forceinline__ float origin_of(int act) {
     return act == FGA_ACTIVATION_SWOOSH_R ? 1.0f : 0.0f;
 }
 // A column's shift from its bias, which has to be below kFarBias for it to stay within fp32 in the
-// exponent's units.
+// exponent's units (with 2^126 log2 e of weight xhat on top).
 constexpr float kFarBias = 1.5e38f;
 __device__ __forceinline__ float2 shift_of(float2 bias, int act) {
     return mul2(add2(bias, splat2(-origin_of(act))), splat2(unit_of(act)));

@@ -26,6 +26,8 @@
 // 3000 x 1024 f16 in one group, SiLU, streams, 65 us (50 % and 83 %). Issue is 54 to 65 % busy (65
 // instructions a pair of values on chip, 45 and 42 in the two streams) and the rest is a block's
 // own latency: its parameters, its first rows and its sums across threads.
+#include <type_traits>
+
 #include "fga_kernels.h"
 #include "group_norm.cuh"
 
@@ -56,11 +58,13 @@ template <typename T> struct Tensors {
 };
 
 // A column's shift, which stops short of where it would leave fp32: the slopes there are what they
-// are further on, and silu's would be inf * 0. Infinities and NaN stay what they are.
+// are further on, and silu's would be inf * 0. (2^126 log2 e of weight xhat still fit on top.)
+// Infinities and NaN stay what they are. (No finite bias of fp16 gets there.)
+template <typename T>
 __device__ __forceinline__ float2 bounded_shift_of(float2 bias, int act) {
-    constexpr float kMost = 2.3e38f;
+    constexpr float kMost = 2.1e38f;
     const float2 s = shift_of(bias, act);
-    if (act == FGA_ACTIVATION_NONE) return s;
+    if (std::is_same_v<T, __half> || act == FGA_ACTIVATION_NONE) return s;
     return make_float2(isfinite(bias.x) ? fminf(fmaxf(s.x, -kMost), kMost) : s.x,
                        isfinite(bias.y) ? fminf(fmaxf(s.y, -kMost), kMost) : s.y);
 }
@@ -87,7 +91,7 @@ template <typename T, bool kWhole> struct Column {
         }
 #pragma unroll
         for (int e = 0; e < kPairs<T>; ++e) {
-            shift[e] = bounded_shift_of(shift[e], act);
+            shift[e] = bounded_shift_of<T>(shift[e], act);
             scale[e] = mul2(mul2(scale[e], unit), rstd[kWhole ? 0 : e]);
         }
     }
